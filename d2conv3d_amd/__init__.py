@@ -15,6 +15,7 @@ from .modules import (
 from .grid import offsets_from_size_map
 from .util import add_deformable_conv
 from .depthwise_conv import DepthwiseConv3d, depthwise_separable_conv3d, install_as_fast_depthwise_conv3d
+from .attention import CrossAttention3d, LayerNorm, cross_attention, layer_norm, rotary3d
 
 __all__ = [
     "deform_conv1d", "deform_conv3d", "deform_conv3d_sized", "DeformConv1d", "DeformConv3d", "DeformConvNd",
@@ -25,6 +26,7 @@ __all__ = [
     "XYZSizeConditionedDConv3d", "XYZSizeConditionedMDConv3d",
     "offsets_from_size_map", "add_deformable_conv", "install_as_dconv_native",
     "DepthwiseConv3d", "depthwise_separable_conv3d", "install_as_fast_depthwise_conv3d",
+    "CrossAttention3d", "LayerNorm", "cross_attention", "layer_norm", "rotary3d",
 ]
 
 

@@ -37,6 +37,9 @@ EXPORTS = (
     "d2c_conv3d_forward_stats_workspace_bytes", "d2c_conv3d_forward_stats", "d2c_channel_stats",
     "d2c_group_norm_forward", "d2c_group_norm_backward_workspace_bytes", "d2c_group_norm_backward",
     "d2c_dwconv3d_check", "d2c_dwconv3d_backward_workspace_bytes", "d2c_dwconv3d_forward", "d2c_dwconv3d_backward",
+    "d2c_layer_norm_forward", "d2c_layer_norm_backward_workspace_bytes", "d2c_layer_norm_backward", "d2c_rotary3d",
+    "d2c_attention_forward_workspace_bytes", "d2c_attention_forward",
+    "d2c_attention_backward_workspace_bytes", "d2c_attention_backward",
 )
 
 
@@ -83,6 +86,23 @@ class DwConv3dDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in (
         "N", "C", "Cout", "D", "H", "W", "kd", "kh", "kw", "sd", "sh", "sw",
         "pd", "ph", "pw", "dd", "dh", "dw", "Do", "Ho", "Wo", "dtype")]
+
+
+class LayerNormDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("C", "dtype", "param_dtype")] + [("eps", ctypes.c_float)]
+
+
+class Rotary3dDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("N", "L", "H", "D")] + [
+        ("pairs", ctypes.c_int32 * 3), ("grid", ctypes.c_int32 * 3)] + [
+        (n, ctypes.c_int32) for n in ("interleaved", "direction", "dtype")] + [
+        ("base", ctypes.c_float), ("x_stride", ctypes.c_int64 * 3), ("position_stride", ctypes.c_int64)]
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("N", "Lq", "Lk", "Hq", "Hkv", "D", "dtype")] + [("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
 
 
 class Conv1dDesc(ctypes.Structure):
@@ -184,6 +204,18 @@ def load():
     lib.d2c_dwconv3d_backward_workspace_bytes.restype = sz
     lib.d2c_dwconv3d_forward.argtypes, lib.d2c_dwconv3d_forward.restype = [pdw] + [vp] * 5, ctypes.c_int
     lib.d2c_dwconv3d_backward.argtypes, lib.d2c_dwconv3d_backward.restype = [pdw] + [vp] * 7 + [sz, vp], ctypes.c_int
+    pln = ctypes.POINTER(LayerNormDesc)
+    lib.d2c_layer_norm_forward.argtypes, lib.d2c_layer_norm_forward.restype = [pln] + [vp] * 6, ctypes.c_int
+    lib.d2c_layer_norm_backward_workspace_bytes.argtypes = [pln]
+    lib.d2c_layer_norm_backward_workspace_bytes.restype = sz
+    lib.d2c_layer_norm_backward.argtypes, lib.d2c_layer_norm_backward.restype = [pln] + [vp] * 8 + [sz, vp], ctypes.c_int
+    lib.d2c_rotary3d.argtypes, lib.d2c_rotary3d.restype = [ctypes.POINTER(Rotary3dDesc)] + [vp] * 4, ctypes.c_int
+    pat = ctypes.POINTER(AttentionDesc)
+    for d in ("forward", "backward"):
+        f = getattr(lib, f"d2c_attention_{d}_workspace_bytes")
+        f.argtypes, f.restype = [pat], sz
+    lib.d2c_attention_forward.argtypes, lib.d2c_attention_forward.restype = [pat] + [vp] * 8 + [sz, vp], ctypes.c_int
+    lib.d2c_attention_backward.argtypes, lib.d2c_attention_backward.restype = [pat] + [vp] * 12 + [sz, vp], ctypes.c_int
     lib.d2c_profile_enable.argtypes, lib.d2c_profile_enable.restype = [ctypes.c_int], None
     lib.d2c_profile_reset.argtypes, lib.d2c_profile_reset.restype = [], None
     lib.d2c_profile_read.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int)]

@@ -1,0 +1,218 @@
+// Building blocks of the attention kernels: operand fragments, tiles in LDS, the mapping of rows.
+//
+//   s[i][j] = scale * sum_d q[i][d] k[j][d]   over the keys j that are there
+//   p = exp(s - max_j s) / sum_j exp(s - max_j s),   o[i] = sum_j p[i][j] v[j]           (a row without a key: o = 0)
+//   backward, with L = log sum_j exp s kept from the forward pass and delta = sum_d do[i][d] o[i][d]:
+//     p = exp(s - L),  dv = p^T do,  dp = do v^T,  ds = p (dp - delta),  dq = scale ds k,  dk = scale ds^T q
+//
+// Everything runs on v_mfma_f32_32x32x16_bf16.  The scores are made with the reader's index along the lanes (one column of the
+// accumulator to a lane): row maxima and sums then stay in a lane but for one exchange between its halves, and the
+// accumulator's registers are the next product's operand as they are -- in the order of the reduction that the accumulator has,
+// 4 of 8 keys to a half of the wavefront, in which the other operand is read, too (transposing LDS reads, four at a time).
+//
+// float32 operands travel as three bfloat16 terms, which represent a float exactly, and a product as the six partial products that
+// count (what is left out is below 2^-24 of it): 6/16 of the float instruction's time.
+//
+// The rows of a group of query heads that share a key head are one axis: row = position * group + head in group.
+#pragma once
+#include "d2c_common.hpp"
+#include "d2c_mma.hpp"
+
+namespace d2c_attn {
+
+struct Args {
+    const void *q, *k, *v, *g, *o;      // g: gradient of the output o
+    const int32_t *lengths;             // [N] or NULL
+    const uint8_t *mask;                // [N][Lk], 0: not to be read; or NULL
+    void *out, *gq, *gk, *gv;           // [N][Lq][Hq][D], [N][Lk][Hkv][D]
+    float *lse, *delta;                 // [N * Hkv][rows]: log2 of the sum of a row (+infinity: no key), and sum_d do o
+    float *part, *part_ml;              // partial results of `splits` workgroups: [splits][N * Hkv][rows or Lk][D] and (forward) [..][2]
+    long qs[3], ks[3], vs[3], gs[3];    // strides of sample, position, head
+    int N, Lq, Lk, Hq, Hkv, group, D, rows;
+    int splits;
+    float scale, scale2;                // scale2 = scale * log2(e)
+};
+
+template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 1 : 3;
+
+// 8 reduction elements of a matrix operand's row
+template <int P> struct Frag { uint4 t[P]; };
+
+D2C_DEV f32x16 mma1(f32x16 acc, const uint4 &a, const uint4 &b)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), acc, 0, 0, 0);
+}
+template <int P> D2C_DEV void mma(f32x16 &acc, const Frag<P> &a, const Frag<P> &b)
+{
+    if constexpr (P == 3) {
+        acc = mma1(acc, a.t[2], b.t[0]);
+        acc = mma1(acc, a.t[0], b.t[2]);
+        acc = mma1(acc, a.t[1], b.t[1]);
+        acc = mma1(acc, a.t[1], b.t[0]);
+        acc = mma1(acc, a.t[0], b.t[1]);
+    }
+    acc = mma1(acc, a.t[0], b.t[0]);
+}
+// Two floats -> their terms, each a packed pair
+D2C_DEV void split_pair(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo)
+{
+    hi = pack_bf16x2(x, y);
+    x = bf16_residual(x, hi << 16); y = bf16_residual(y, hi & 0xffff0000u);
+    mid = pack_bf16x2(x, y);
+    lo = pack_bf16x2(x - __uint_as_float(mid << 16), y - __uint_as_float(mid & 0xffff0000u));
+}
+template <int P> D2C_DEV Frag<P> make_frag(const float *v)
+{
+    Frag<P> f;
+    if constexpr (P == 1) {
+        f.t[0] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    } else {
+        uint32_t h[4], m[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) split_pair(v[2 * i], v[2 * i + 1], h[i], m[i], l[i]);
+        f.t[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        f.t[1] = make_uint4(m[0], m[1], m[2], m[3]);
+        f.t[2] = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+    return f;
+}
+
+// 8 elements as they lie in memory, `left` of them there (zeros behind; none: p is not read)
+template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
+template <typename T> D2C_DEV Raw8<T> load8(const T *p, int left)
+{
+    constexpr int VEC = 16 / (int)sizeof(T);
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+        r.v[i] = make_uint4(0, 0, 0, 0);
+        if (left > i * VEC) r.v[i] = load_run<T>(p + i * VEC, left - i * VEC);
+    }
+    return r;
+}
+template <typename T> D2C_DEV Frag<kTerms<T>> terms_of(const Raw8<T> &r)
+{
+    if constexpr (sizeof(T) == 2) return Frag<1>{{r.v[0]}};
+    else {
+        float f[8];
+        *reinterpret_cast<uint4 *>(f) = r.v[0];
+        *reinterpret_cast<uint4 *>(f + 4) = r.v[1];
+        return make_frag<3>(f);
+    }
+}
+template <typename T> D2C_DEV void floats_of(const Raw8<T> &r, float *f)
+{
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else {
+        *reinterpret_cast<uint4 *>(f) = r.v[0];
+        *reinterpret_cast<uint4 *>(f + 4) = r.v[1];
+    }
+}
+
+// A tile of ROWS rows of DP bfloat16 values (per term) in LDS, in pieces of 16 bytes.  A row's pieces change places so that neither 8
+// rows' pieces of one column (operand reads) nor 4 rows' 64 bytes (transposing reads) meet in a bank.
+template <int DP> D2C_DEV int piece_swizzle(int row)
+{
+    if constexpr (DP == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (DP == 64) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return (row >> 2) & 3;
+}
+template <int DP> D2C_DEV int piece_at(int row, int piece) { return row * (DP * 2) + ((piece ^ piece_swizzle<DP>(row)) << 4); }
+
+typedef short v4s_t __attribute__((ext_vector_type(4)));
+
+template <typename T, int DP, int ROWS, int THREADS> struct Tile {
+    static constexpr int P = kTerms<T>, PIECES = DP / 8, PER = (ROWS * PIECES + THREADS - 1) / THREADS;
+    static constexpr int TERM = ROWS * DP * 2, BYTES = P * TERM;
+    Raw8<T> r[PER];
+    // row(i): the address of row i, or NULL where it reads as zeros
+    template <typename Row> D2C_DEV void load(int D, Row row)
+    {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int at = i * THREADS + threadIdx.x;
+            const T *p = ROWS * PIECES % THREADS == 0 || at < ROWS * PIECES ? row(at / PIECES) : nullptr;
+            r[i] = load8<T>(p + at % PIECES * 8, p ? D - at % PIECES * 8 : 0);
+        }
+    }
+    D2C_DEV void store(unsigned char *lds) const
+    {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int at = i * THREADS + threadIdx.x;
+            if (ROWS * PIECES % THREADS != 0 && at >= ROWS * PIECES) continue;
+            const Frag<P> f = terms_of<T>(r[i]);
+#pragma unroll
+            for (int t = 0; t < P; t++)
+                *reinterpret_cast<uint4 *>(lds + t * TERM + piece_at<DP>(at / PIECES, at % PIECES)) = f.t[t];
+        }
+    }
+    // columns 16 ks + 8 half .. of row `row`
+    static D2C_DEV Frag<P> rows(const unsigned char *lds, int row, int ks, int half)
+    {
+        Frag<P> f;
+#pragma unroll
+        for (int t = 0; t < P; t++) f.t[t] = *reinterpret_cast<const uint4 *>(lds + t * TERM + piece_at<DP>(row, ks * 2 + half));
+        return f;
+    }
+    // column c0 + lane % 32 of the rows r0 + {0..3, 8..11} (first half of the wavefront) and r0 + {4..7, 12..15}: the order in which an
+    // accumulator's registers 8 i .. 8 i + 7 hold them.  (Within 16 lanes, lane l element j comes from lane 4j + l/4, element l%4.)
+    static D2C_DEV Frag<P> columns(const unsigned char *lds, int r0, int c0, int lane)
+    {
+        const int row = r0 + (lane >> 5) * 4 + ((lane & 15) >> 2), col = c0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        Frag<P> f;
+#pragma unroll
+        for (int t = 0; t < P; t++) {
+            const unsigned char *p = lds + t * TERM + (col & 7) * 2;
+            const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t *)(p + piece_at<DP>(row, col >> 3))));
+            const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s_t *)(p + piece_at<DP>(row + 8, col >> 3))));
+            f.t[t] = make_uint4(a.x, a.y, b.x, b.y);
+        }
+        return f;
+    }
+};
+
+// Sample and key head of a workgroup: consecutive workgroups take consecutive heads, so that a head's workgroups share an XCD's L2
+// where the heads are a multiple of 8.
+struct Head { int n, h; long nh; };
+D2C_DEV Head head_of(const Args &a)
+{
+    const int nh = (int)blockIdx.x, n = nh / a.Hkv;
+    return {n, nh - n * a.Hkv, nh};
+}
+D2C_DEV int keys_of(const Args &a, int n) { return a.lengths ? min(max(a.lengths[n], 0), a.Lk) : a.Lk; }
+
+// Row `row` of a tensor [N][Lq][Hq][D] with strides s
+template <typename T> D2C_DEV const T *row_at(const void *base, const long *s, const Args &a, const Head &hd, int row)
+{
+    const int pos = row / a.group, g = row - pos * a.group;
+    return reinterpret_cast<const T *>(base) + hd.n * s[0] + pos * s[1] + (long)(hd.h * a.group + g) * s[2];
+}
+
+// Four consecutive values of a row that ends at `left`
+template <typename T> D2C_DEV void store4(T *p, const float *v, int left)
+{
+    typedef uint32_t u32x2_by2 __attribute__((ext_vector_type(2), aligned(2)));
+    typedef float f32x4_by4 __attribute__((ext_vector_type(4), aligned(4)));
+    if (left >= 4) {
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2_by2 *>(p) = u32x2_by2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        else *reinterpret_cast<f32x4_by4 *>(p) = f32x4_by4{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i < left) p[i] = f32_to_elem<T>(v[i]);
+    }
+}
+
+// Both halves of the wavefront: the larger value, the sum
+D2C_DEV float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+D2C_DEV float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+
+Args make_args(const d2c_attention_desc &q);
+
+}  // namespace d2c_attn
+
+int d2c_attention_check(const d2c_attention_desc *q);

@@ -1,0 +1,381 @@
+// Attention of one map's positions to those of another: backward pass.  Formulas and operand orders: d2c_attention.hpp.
+//
+// Two kernels, so that every gradient is a sum in one order and none is added up in memory: attn_bwd_q_kernel (a workgroup keeps 128 rows
+// and walks over the keys; it also leaves delta of its rows), then attn_bwd_kv_kernel (a workgroup keeps 128 keys, 32 to a wavefront, and walks over the
+// rows).  Scores and dp are made in both: 7 products where one kernel would need 5.  Few rows, or few keys: several workgroups share the
+// walk, and attn_bwd_join_kernel adds up their sums.
+#include <algorithm>
+#include "d2c_attention.hpp"
+
+using namespace d2c_attn;
+
+namespace {
+
+template <typename T, int DP> struct QShape {
+    static constexpr int KT = sizeof(T) == 2 ? 64 : 32;
+    using KV = Tile<T, DP, KT, 256>;
+    static constexpr int LDS = 2 * KV::BYTES;
+};
+
+template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_q_kernel(Args a)
+{
+    using KV = typename QShape<T, DP>::KV;
+    constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, KT = QShape<T, DP>::KT;
+    extern __shared__ __align__(16) unsigned char lds[];
+    unsigned char *s_k = lds, *s_v = lds + KV::BYTES;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const Head hd = head_of(a);
+    const int row = (int)blockIdx.y * 128 + wave * 32 + (lane & 31);
+    const bool live = row < a.rows;
+    const int keys = keys_of(a, hd.n), tiles = (keys + KT - 1) / KT;
+    const int split = (int)blockIdx.z, t1 = (int)((long)tiles * (split + 1) / a.splits);
+    int t = (int)((long)tiles * split / a.splits);
+
+    const T *kb = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2];
+    const T *vb = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2];
+    KV k, v;
+    bool b = false;
+    auto ask = [&](int k0) INLINE { const int key = k0 + lane; b = lane < KT && key < keys && (!a.mask || a.mask[(long)hd.n * a.Lk + key]); };
+    uint64_t next = 0;
+    auto request = [&](int tile) INLINE {
+        const int k0 = tile * KT;
+        k.load(a.D, [&](int i) INLINE { return (next >> i) & 1 ? kb + (long)(k0 + i) * a.ks[1] : nullptr; });
+        v.load(a.D, [&](int i) INLINE { return (next >> i) & 1 ? vb + (long)(k0 + i) * a.vs[1] : nullptr; });
+    };
+    if (t < t1) {
+        ask(t * KT);
+        next = __ballot(b);
+        request(t);
+        ask((t + 1) * KT);
+    }
+    Frag<P> q[NK], g[NK];
+    float delta = 0.f;
+    {
+        const int r = min(row, a.rows - 1);
+        const T *qr = row_at<T>(a.q, a.qs, a, hd, r), *gr = row_at<T>(a.g, a.gs, a, hd, r), *orow = row_at<T>(a.o, a.gs, a, hd, r);
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int d = i * 16 + half * 8, left = live ? a.D - d : 0;
+            q[i] = terms_of<T>(load8<T>(qr + d, left));
+            const Raw8<T> x = load8<T>(gr + d, left), y = load8<T>(orow + d, left);
+            g[i] = terms_of<T>(x);
+            float xf[8], yf[8];
+            floats_of<T>(x, xf);
+            floats_of<T>(y, yf);
+#pragma unroll
+            for (int j = 0; j < 8; j++) delta = fmaf(xf[j], yf[j], delta);
+        }
+    }
+    delta = half_sum(delta);
+    const float lse = live ? a.lse[hd.nh * a.rows + row] : INFINITY;
+    if (live && split == 0 && half == 0) a.delta[hd.nh * a.rows + row] = delta;
+    f32x16 dq[ND];
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) dq[i][r] = 0.f;
+    const float c = a.scale2;
+
+    for (; t < t1; t++) {
+        const uint64_t now = next;
+        __syncthreads();
+        k.store(s_k);
+        v.store(s_v);
+        __syncthreads();
+        if (t + 1 < t1) {
+            next = __ballot(b);
+            request(t + 1);
+            ask((t + 2) * KT);
+        }
+        if (now == 0) continue;
+#pragma unroll
+        for (int i = 0; i < KT / 32; i++) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < NK; ks++) {
+                mma<P>(s, KV::rows(s_k, i * 32 + (lane & 31), ks, half), q[ks]);
+                mma<P>(dp, KV::rows(s_v, i * 32 + (lane & 31), ks, half), g[ks]);
+            }
+            const uint32_t there = (uint32_t)(now >> (i * 32));
+            if (there != 0xffffffffu) {
+                const uint32_t w = there >> (half * 4);
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (!((w >> (8 * (r / 4) + r % 4)) & 1)) s[r] = -INFINITY;
+            }
+            float ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; r++) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+                const Frag<P> f = make_frag<P>(ds + kk * 8);
+#pragma unroll
+                for (int d = 0; d < ND; d++) mma<P>(dq[d], KV::columns(s_k, i * 32 + kk * 16, d * 32, lane), f);
+            }
+        }
+    }
+    if (!live) return;
+    if (a.splits > 1) {
+        float *p = a.part + (((long)split * gridDim.x + hd.nh) * a.rows + row) * a.D;
+#pragma unroll
+        for (int i = 0; i < ND; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int d = i * 32 + j * 8 + half * 4;
+                const float x[4] = {dq[i][j * 4], dq[i][j * 4 + 1], dq[i][j * 4 + 2], dq[i][j * 4 + 3]};
+                store4<float>(p + d, x, a.D - d);
+            }
+        return;
+    }
+    T *out = const_cast<T *>(row_at<T>(a.gq, a.gs, a, hd, row));
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int d = i * 32 + j * 8 + half * 4;
+            const float x[4] = {dq[i][j * 4] * a.scale, dq[i][j * 4 + 1] * a.scale, dq[i][j * 4 + 2] * a.scale, dq[i][j * 4 + 3] * a.scale};
+            store4<T>(out + d, x, a.D - d);
+        }
+}
+
+template <typename T, int DP> struct KvShape {
+    static constexpr int RT = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
+    using QG = Tile<T, DP, RT, 256>;
+    static constexpr int LDS = 2 * QG::BYTES + 2 * RT * 4;
+};
+
+template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_kv_kernel(Args a)
+{
+    using QG = typename KvShape<T, DP>::QG;
+    constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, RT = KvShape<T, DP>::RT;
+    extern __shared__ __align__(16) unsigned char lds[];
+    unsigned char *s_q = lds, *s_g = lds + QG::BYTES;
+    float *s_lse = reinterpret_cast<float *>(lds + 2 * QG::BYTES), *s_delta = s_lse + RT;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const Head hd = head_of(a);
+    const int keys = keys_of(a, hd.n), key0 = (int)blockIdx.y * 128, key = key0 + wave * 32 + (lane & 31);
+    const bool live = key < keys && (!a.mask || a.mask[(long)hd.n * a.Lk + key]);
+    const int tiles = (a.rows + RT - 1) / RT;
+    const int split = (int)blockIdx.z, t1 = key0 < keys ? (int)((long)tiles * (split + 1) / a.splits) : 0;
+    int t = (int)((long)tiles * split / a.splits);
+
+    QG q, g;
+    float stat = 0.f;
+    auto request = [&](int tile) INLINE {
+        const int r0 = tile * RT;
+        q.load(a.D, [&](int i) INLINE { return r0 + i < a.rows ? row_at<T>(a.q, a.qs, a, hd, r0 + i) : nullptr; });
+        g.load(a.D, [&](int i) INLINE { return r0 + i < a.rows ? row_at<T>(a.g, a.gs, a, hd, r0 + i) : nullptr; });
+        if (threadIdx.x < 2 * RT) {
+            const bool first = threadIdx.x < RT;
+            const int r = r0 + (first ? threadIdx.x : threadIdx.x - RT);
+            stat = r < a.rows ? (first ? a.lse : a.delta)[hd.nh * a.rows + r] : (first ? INFINITY : 0.f);
+        }
+    };
+    if (t < t1) request(t);
+    Frag<P> k[NK], v[NK];
+    {
+        const T *kr = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2] + (long)key * a.ks[1];
+        const T *vr = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2] + (long)key * a.vs[1];
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int d = i * 16 + half * 8, left = live ? a.D - d : 0;
+            k[i] = terms_of<T>(load8<T>(kr + d, left));
+            v[i] = terms_of<T>(load8<T>(vr + d, left));
+        }
+    }
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) dk[i][r] = dv[i][r] = 0.f;
+    const float c = a.scale2;
+
+    for (; t < t1; t++) {
+        __syncthreads();
+        q.store(s_q);
+        g.store(s_g);
+        if (threadIdx.x < 2 * RT) s_lse[threadIdx.x] = stat;
+        __syncthreads();
+        if (t + 1 < t1) request(t + 1);
+#pragma unroll
+        for (int i = 0; i < RT / 32; i++) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < NK; ks++) {
+                mma<P>(s, QG::rows(s_q, i * 32 + (lane & 31), ks, half), k[ks]);
+                mma<P>(dp, QG::rows(s_g, i * 32 + (lane & 31), ks, half), v[ks]);
+            }
+            float p[16], ds[16];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float4 ls = *reinterpret_cast<const float4 *>(s_lse + i * 32 + j * 8 + half * 4);
+                const float4 de = *reinterpret_cast<const float4 *>(s_delta + i * 32 + j * 8 + half * 4);
+                const float lr[4] = {ls.x, ls.y, ls.z, ls.w}, dr[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    p[j * 4 + r] = __builtin_amdgcn_exp2f(fmaf(s[j * 4 + r], c, -lr[r]));
+                    ds[j * 4 + r] = p[j * 4 + r] * (dp[j * 4 + r] - dr[r]);
+                }
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+                const Frag<P> pf = make_frag<P>(p + kk * 8), df = make_frag<P>(ds + kk * 8);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    mma<P>(dv[d], QG::columns(s_g, i * 32 + kk * 16, d * 32, lane), pf);
+                    mma<P>(dk[d], QG::columns(s_q, i * 32 + kk * 16, d * 32, lane), df);
+                }
+            }
+        }
+    }
+    if (key >= a.Lk) return;
+    // (a key that is not to be read: a column of the accumulators of its own, whatever is in it)
+    const float fk = a.splits > 1 ? 1.f : a.scale;
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int d = i * 32 + j * 8 + half * 4;
+            float x[4], y[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) { x[r] = live ? dk[i][j * 4 + r] * fk : 0.f; y[r] = live ? dv[i][j * 4 + r] : 0.f; }
+            if (a.splits > 1) {
+                const long heads = gridDim.x;
+                store4<float>(a.part + (((2L * split) * heads + hd.nh) * a.Lk + key) * a.D + d, x, a.D - d);
+                store4<float>(a.part + (((2L * split + 1) * heads + hd.nh) * a.Lk + key) * a.D + d, y, a.D - d);
+            } else {
+                const long at = (((long)hd.n * a.Lk + key) * a.Hkv + hd.h) * a.D + d;
+                if (a.gk) store4<T>(reinterpret_cast<T *>(a.gk) + at, x, a.D - d);
+                if (a.gv) store4<T>(reinterpret_cast<T *>(a.gv) + at, y, a.D - d);
+            }
+        }
+}
+
+// Sums of the workgroups that shared a walk: part [splits][1 or 2][N * Hkv][rows or Lk][D]
+template <typename T, bool KV> __global__ void __launch_bounds__(256) attn_bwd_join_kernel(Args a)
+{
+    const int len = KV ? a.Lk : a.rows;
+    const long total = (long)a.N * a.Hkv * len * a.D, at = (long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= total) return;
+    const long which = KV ? blockIdx.y : 0;
+    if (KV && !(which ? a.gv : a.gk)) return;
+    float x = 0.f;
+    for (int s = 0; s < a.splits; s++) x += a.part[(s * (KV ? 2L : 1L) + which) * total + at];
+    if (which == 0) x *= a.scale;
+    const int d = (int)(at % a.D);
+    const long line = at / a.D, nh = line / len;
+    const int i = (int)(line - nh * len), n = (int)(nh / a.Hkv);
+    const Head hd{n, (int)(nh - (long)n * a.Hkv), nh};
+    if constexpr (KV)
+        reinterpret_cast<T *>(which ? a.gv : a.gk)[(((long)n * a.Lk + i) * a.Hkv + hd.h) * a.D + d] = f32_to_elem<T>(x);
+    else
+        const_cast<T *>(row_at<T>(a.gq, a.gs, a, hd, i))[d] = f32_to_elem<T>(x);
+}
+
+// delta alone, where the queries' gradient is not wanted: one wavefront to a row
+template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(Args a)
+{
+    const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6), nh = at / a.rows;
+    if (at >= (long)a.N * a.Hkv * a.rows) return;
+    const int n = (int)(nh / a.Hkv), lane = threadIdx.x & 63;
+    const Head hd{n, (int)(nh - (long)n * a.Hkv), nh};
+    const T *g = row_at<T>(a.g, a.gs, a, hd, (int)(at - nh * a.rows)), *o = row_at<T>(a.o, a.gs, a, hd, (int)(at - nh * a.rows));
+    float x = 0.f;
+    for (int d = lane; d < a.D; d += 64) x = fmaf(elem_to_f32<T>(g[d]), elem_to_f32<T>(o[d]), x);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+    if (lane == 0) a.delta[at] = x;
+}
+
+struct BwdPlan { int row_tiles, key_tiles, q_splits, kv_splits; size_t delta_bytes, bytes; };
+BwdPlan bwd_plan(const d2c_attention_desc &q)
+{
+    BwdPlan p;
+    const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv, want = 2L * std::max(d2c_num_cus(), 1);
+    const bool bf = q.dtype == D2C_BF16;
+    p.row_tiles = (int)((rows + 127) / 128);
+    p.key_tiles = (q.Lk + 127) / 128;
+    const long kt = (q.Lk + (bf ? 63 : 31)) / (bf ? 64 : 32), rt_rows = bf && q.D <= 64 ? 64 : 32, rt = (rows + rt_rows - 1) / rt_rows;
+    // (two workgroups to a compute unit, each with two tiles at least)
+    p.q_splits = (int)std::max(1L, std::min(want / std::max(heads * p.row_tiles, 1L), kt / 2));
+    p.kv_splits = (int)std::max(1L, std::min(want / std::max(heads * p.key_tiles, 1L), rt / 2));
+    p.delta_bytes = d2c_align_up((size_t)heads * rows * 4);
+    const size_t qb = p.q_splits > 1 ? (size_t)p.q_splits * heads * rows * q.D * 4 : 0;
+    const size_t kvb = p.kv_splits > 1 ? (size_t)p.kv_splits * 2 * heads * q.Lk * q.D * 4 : 0;
+    p.bytes = p.delta_bytes + d2c_align_up(std::max(qb, kvb));
+    return p;
+}
+
+template <typename T, int DP> int launch_bwd_d(Args a, const BwdPlan &p, hipStream_t st)
+{
+    const unsigned heads = (unsigned)(a.N * a.Hkv);
+    if (a.Lq > 0 && !a.gq && (a.gk || a.gv)) {
+        hipLaunchKernelGGL(attn_delta_kernel<T>, dim3((unsigned)(((long)heads * a.rows + 3) / 4)), dim3(256), 0, st, a);
+        if (int rc = d2c_check_launch("attn_delta_kernel")) return rc;
+    } else if (a.Lq > 0 && a.gq) {
+        constexpr int lds = QShape<T, DP>::LDS;
+        if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP>), lds, "attn_bwd_q_kernel")) return rc;
+        a.splits = p.q_splits;
+        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP>), dim3(heads, (unsigned)p.row_tiles, (unsigned)p.q_splits), dim3(256), lds, st, a);
+        if (int rc = d2c_check_launch("attn_bwd_q_kernel")) return rc;
+        if (p.q_splits > 1) {
+            const long total = (long)heads * a.rows * a.D;
+            hipLaunchKernelGGL((attn_bwd_join_kernel<T, false>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a);
+            if (int rc = d2c_check_launch("attn_bwd_join_kernel")) return rc;
+        }
+    }
+    if (a.Lk == 0 || !(a.gk || a.gv)) return D2C_OK;
+    constexpr int lds = KvShape<T, DP>::LDS;
+    if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP>), lds, "attn_bwd_kv_kernel")) return rc;
+    a.splits = p.kv_splits;
+    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP>), dim3(heads, (unsigned)p.key_tiles, (unsigned)p.kv_splits), dim3(256), lds, st, a);
+    if (int rc = d2c_check_launch("attn_bwd_kv_kernel")) return rc;
+    if (p.kv_splits > 1) {
+        const long total = (long)heads * a.Lk * a.D;
+        hipLaunchKernelGGL((attn_bwd_join_kernel<T, true>), dim3((unsigned)((total + 255) / 256), 2), dim3(256), 0, st, a);
+        return d2c_check_launch("attn_bwd_join_kernel");
+    }
+    return D2C_OK;
+}
+template <typename T> int launch_bwd(const Args &a, const BwdPlan &p, hipStream_t st)
+{
+    if (a.D <= 32) return launch_bwd_d<T, 32>(a, p, st);
+    if (a.D <= 64) return launch_bwd_d<T, 64>(a, p, st);
+    if (a.D <= 96) return launch_bwd_d<T, 96>(a, p, st);
+    return launch_bwd_d<T, 128>(a, p, st);
+}
+
+}  // namespace
+
+extern "C" size_t d2c_attention_backward_workspace_bytes(const d2c_attention_desc *q)
+{
+    return d2c_attention_check(q) == D2C_OK ? bwd_plan(*q).bytes : 0;
+}
+
+extern "C" int d2c_attention_backward(const d2c_attention_desc *q, const void *grad_out, const void *query, const void *key,
+                                      const void *value, const int32_t *key_lengths, const uint8_t *key_mask, const void *out,
+                                      const float *lse, void *grad_query, void *grad_key, void *grad_value, void *ws,
+                                      size_t ws_bytes, void *stream)
+{
+    if (int rc = d2c_attention_check(q)) return rc;
+    if (q->N == 0 || (q->Lq == 0 && q->Lk == 0)) return D2C_OK;
+    if ((q->Lq > 0 && (!grad_out || !query || !out || !lse)) || (q->Lk > 0 && (!key || !value))) {
+        d2c_set_error("null tensor pointer");
+        return D2C_ERR_SHAPE;
+    }
+    const BwdPlan p = bwd_plan(*q);
+    if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 255u))) {
+        d2c_set_error("workspace of %zu bytes (256-byte aligned) required, got %zu at %p", p.bytes, ws_bytes, ws);
+        return D2C_ERR_WORKSPACE;
+    }
+    Args a = make_args(*q);
+    a.g = grad_out; a.q = query; a.k = key; a.v = value; a.lengths = key_lengths; a.mask = key_mask; a.o = out;
+    a.lse = const_cast<float *>(lse);
+    a.gq = grad_query; a.gk = grad_key; a.gv = grad_value;
+    a.delta = (float *)ws; a.part = (float *)((char *)ws + p.delta_bytes);
+    return q->dtype == D2C_BF16 ? launch_bwd<bf16_t>(a, p, (hipStream_t)stream) : launch_bwd<float>(a, p, (hipStream_t)stream);
+}

@@ -479,6 +479,64 @@ int d2c_dwconv3d_backward(const d2c_dwconv3d_desc *desc, const void *grad_out, c
                           void *grad_x, void *grad_weight, void *grad_bias, void *workspace,
                           size_t workspace_bytes, void *stream);
 
+/* ---- a map's positions read another map's: norm, positions, attention -----------------------------------------
+ * The operators of a block in which a clip's features read those of other frames (no counterpart in the reference).
+ *
+ * Layer norm over the C channels of a row: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps), var the mean of
+ * the squared deviations.  x: `rows` rows of C elements, x_stride elements apart; y, grad_y, grad_x: contiguous.  weight and
+ * bias [C] (may be NULL: 1, 0) and their gradients in `param_dtype`: `dtype`, or D2C_F32 beside D2C_BF16.  `stats` [rows][2]:
+ * mean and rstd of a row, which the backward call reads; the forward call leaves them out where it is NULL.  Gradients of the
+ * parameters are sums in an order that the sizes and the GPU alone determine. */
+typedef struct d2c_layer_norm_desc {
+    int64_t rows, x_stride;
+    int32_t C, dtype, param_dtype;
+    float eps;
+} d2c_layer_norm_desc;
+int d2c_layer_norm_forward(const d2c_layer_norm_desc *desc, const void *x, const void *weight, const void *bias, void *y,
+                           float *stats, void *stream);
+size_t d2c_layer_norm_backward_workspace_bytes(const d2c_layer_norm_desc *desc);
+int d2c_layer_norm_backward(const d2c_layer_norm_desc *desc, const void *grad_y, const void *x, const float *stats,
+                            const void *weight, void *grad_x, void *grad_weight, void *grad_bias, void *workspace,
+                            size_t workspace_bytes, void *stream);
+
+/* Rotary positions along time, height and width.  x [N, L, H, D] with strides x_stride (sample, token, head; channels
+ * adjacent), y contiguous.  The first 2 * (pairs[0] + pairs[1] + pairs[2]) channels of a head turn in pairs, the others pass:
+ * pair j of all is channels (2j, 2j + 1) if `interleaved`, else (j, j + all pairs); pair i of axis a turns by
+ *     direction * position[a] * base^(-i / pairs[a])       radians,
+ * direction 1, or -1 (which is the gradient's way back).  positions: float32 [L][3] for each sample, position_stride elements
+ * from sample to sample (0: the same for all); NULL: token (t * grid[1] + h) * grid[2] + w has the position (t, h, w). */
+#define D2C_ROTARY_MAX_PAIRS 128
+typedef struct d2c_rotary3d_desc {
+    int32_t N, L, H, D;
+    int32_t pairs[3], grid[3];
+    int32_t interleaved, direction, dtype;
+    float base;
+    int64_t x_stride[3], position_stride;
+} d2c_rotary3d_desc;
+int d2c_rotary3d(const d2c_rotary3d_desc *desc, const void *x, const float *positions, void *y, void *stream);
+
+/* Attention: query [N, Lq, Hq, D], key and value [N, Lk, Hkv, D] with strides (sample, position, head; channels adjacent), Hq a
+ * multiple of Hkv (query heads h * Hq / Hkv .. share key head h), D up to 128.
+ *     out[n,i,h] = sum_j softmax_j(scale * <query[n,i,h], key[n,j,h']>) value[n,j,h'],
+ * j over the first key_lengths[n] keys (NULL: all; taken into 0 .. Lk) whose key_mask[n][j] is not 0 (NULL: all).  Keys and
+ * values that are not to be read have no influence whatever they hold; a row without a key is 0, and so are its gradients.
+ * out, grad_out and the gradients are contiguous.  `lse` [N, Hkv, Lq * Hq / Hkv] is for the backward call (NULL: not kept).
+ * Results do not depend on the order in which workgroups run. */
+typedef struct d2c_attention_desc {
+    int32_t N, Lq, Lk, Hq, Hkv, D, dtype;
+    float scale;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+} d2c_attention_desc;
+size_t d2c_attention_forward_workspace_bytes(const d2c_attention_desc *desc);
+int d2c_attention_forward(const d2c_attention_desc *desc, const void *query, const void *key, const void *value,
+                          const int32_t *key_lengths, const uint8_t *key_mask, void *out, float *lse, void *workspace,
+                          size_t workspace_bytes, void *stream);
+size_t d2c_attention_backward_workspace_bytes(const d2c_attention_desc *desc);
+int d2c_attention_backward(const d2c_attention_desc *desc, const void *grad_out, const void *query, const void *key,
+                           const void *value, const int32_t *key_lengths, const uint8_t *key_mask, const void *out,
+                           const float *lse, void *grad_query, void *grad_key, void *grad_value, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
 /* Test hook for the matrix-core backward pass: 1 (default) builds grad_input from
  * per-voxel sample lists, every element written once; 0 scatters with fp32 atomics
  * like the reference (dconv3d_gpu.cu:637).  A value n >= 2 is mode 1 with lists
