@@ -18,7 +18,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._ops import _DT, _ptr, _stream, _workspace
+from ._ops import _DT, _ptr, _stream, _try_native, _workspace
 
 _TYPES = (torch.float32, torch.bfloat16)
 
@@ -89,6 +89,9 @@ def layer_norm(input, weight=None, bias=None, eps=1e-5):
     """`torch.nn.functional.layer_norm(input, input.shape[-1:], weight, bias, eps)`: up to 16384 channels; rows of any
     distance from each other are read in place.  `weight` and `bias` [channels] may be None and may be float32 beside a
     bfloat16 input.  Gradients of all three; statistics and the sums of the gradients are held in float32."""
+    out = _try_native("layer_norm", input, weight, bias, eps)
+    if out is not None:
+        return out
     _check_tensors("layer_norm", input=input, weight=weight, bias=bias)
     _check(input.dim() >= 1 and input.size(-1) > 0, "layer_norm: input needs a last dimension with channels")
     for name, t in (("weight", weight), ("bias", bias)):
@@ -145,6 +148,12 @@ def rotary3d(input, positions, axis_pairs=None, base=10000.0, interleaved=False)
     (default_axis_pairs); pair i of an axis turns by position * base^(-i / pairs of the axis) radians, channels behind the
     last pair pass.  Pair j of all is channels (2j, 2j + 1) with `interleaved`, else (j, j + all pairs).  Angles are exact to
     float32 however far the position."""
+    if isinstance(input, torch.Tensor) and input.dim() == 4:
+        pairs = default_axis_pairs(input.size(3)) if axis_pairs is None else axis_pairs
+        real = isinstance(positions, torch.Tensor)
+        out = _try_native("rotary3d", input, positions if real else None, (0, 0, 0) if real else positions, pairs, base, interleaved)
+        if out is not None:
+            return out
     _check_tensors("rotary3d", input=input)
     _check(input.dim() == 4, f"rotary3d: input must be [N, L, H, D], got {input.dim()} dimensions")
     N, L, H, D = input.shape
@@ -222,6 +231,9 @@ def cross_attention(query, key, value, key_lengths=None, key_mask=None, scale=No
     included); a row without a key is 0 and has gradients of 0.  Any strides with the channels adjacent are read in place, a
     part of a wider projection for instance.  One row or thousands, one key or a long memory: where rows are few the work is
     split over the keys.  Sums in an order that sizes and GPU alone determine."""
+    out = _try_native("cross_attention", query, key, value, key_lengths, key_mask, scale)
+    if out is not None:
+        return out
     _check_tensors("cross_attention", query=query, key=key, value=value, key_lengths=key_lengths, key_mask=key_mask)
     for name, t in (("query", query), ("key", key), ("value", value)):
         _check(t.dim() == 4, f"cross_attention: {name} must be [N, L, H, D], got {t.dim()} dimensions")

@@ -19,6 +19,7 @@
 #include <torch/types.h>
 
 #include <array>
+#include <cmath>
 #include <cstring>
 #include <optional>
 
@@ -44,11 +45,13 @@ void check(int rc, const char *what)
 // (a tensor whose memory the kernels can take as it is: no subclass with its own dispatch, no functorch wrapper, no
 // forward-mode tangent; and no call that torch.jit.trace records: of one it would see the allocation of the result
 // alone, where the Python functions are recorded as operations)
-bool plain(const Tensor &t)
+// (... with strides)
+bool plain_strided(const Tensor &t)
 {
     return t.defined() && !torch::jit::tracer::isTracing() && t.is_cuda() && t.layout() == at::kStrided && t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() &&
-           t.is_contiguous() && !t._fw_grad(0).defined();
+           !t._fw_grad(0).defined();
 }
+bool plain(const Tensor &t) { return plain_strided(t) && t.is_contiguous(); }
 int dtype_code(const Tensor &t)
 {
     switch (t.scalar_type()) {
@@ -566,6 +569,265 @@ py::object dwconv3d(const Tensor &x, const Tensor &w, const opt_tensor &bias, in
     return py::cast(record(out, node));
 }
 
+// ---------------------------------------------------------------- layer_norm
+struct LayerNormBackward : public Node {
+    d2c_layer_norm_desc q;
+    SavedVariable x, w, b, stats;
+    bool has_w = false, has_b = false;
+    std::string name() const override { return "LayerNormBackward"; }
+    void release_variables() override
+    {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        x.reset_data(); w.reset_data(); b.reset_data(); stats.reset_data();
+    }
+    variable_list apply(variable_list &&grads) override
+    {
+        variable_list r(3);
+        const std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) grads[0] = input_metadata(0).zeros_like();
+        {
+            at::NoGradGuard no_grad;
+            const Tensor vx = x.unpack(), vs = stats.unpack();
+            Tensor vw, vb;
+            if (has_w) vw = w.unpack();
+            if (has_b) vb = b.unpack();
+            c10::DeviceGuard guard(vx.device());
+            const hipStream_t st = stream_of(vx);
+            const Tensor g = grads[0].contiguous();
+            if (should_compute_output(0)) r[0] = no_grad_empty_like(vx);
+            if (has_w && should_compute_output(1)) r[1] = no_grad_empty_like(vw);
+            if (has_b && should_compute_output(2)) r[2] = no_grad_empty_like(vb);
+            const size_t nb = r[1].defined() || r[2].defined() ? d2c_layer_norm_backward_workspace_bytes(&q) : 0;
+            const Tensor ws = workspace(nb, vx, st);
+            check(d2c_layer_norm_backward(&q, ptr(g), ptr(vx), (const float *)ptr(vs), ptr(vw), ptr(r[0]), ptr(r[1]), ptr(r[2]), ptr(ws), nb, st),
+                  "layer_norm backward");
+        }
+        once_differentiable(r, grads[0]);
+        return r;
+    }
+};
+
+// The distance of a tensor's rows (all but the last dimension), or -1 where they lie at no single one
+int64_t row_stride(const Tensor &x)
+{
+    const int64_t nd = x.dim(), C = x.size(nd - 1);
+    if (x.stride(nd - 1) != 1 && C > 1) return -1;
+    int64_t step = -1, rows = 1;
+    for (int64_t i = nd - 2; i >= 0; i--) {
+        if (x.size(i) == 1) continue;
+        if (step < 0) step = x.stride(i);
+        else if (x.stride(i) != step * rows) return -1;
+        rows *= x.size(i);
+    }
+    return step < 0 ? C : step;
+}
+
+py::object layer_norm(const Tensor &x, const opt_tensor &weight, const opt_tensor &bias, double eps)
+{
+    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    if (!plain_strided(x) || x.dim() < 1 || x.numel() == 0 || x.size(-1) >= (1ll << 31)) return py::none();
+    const int64_t C = x.size(-1), step = row_stride(x);
+    const int dt = dtype_code(x);
+    if (step < 0 || (dt != D2C_F32 && dt != D2C_BF16)) return py::none();
+    int pdt = -1;
+    for (const Tensor *t : {&w, &b}) {
+        if (!t->defined()) continue;
+        if (!plain(*t) || t->device() != x.device() || t->dim() != 1 || t->size(0) != C) return py::none();
+        const int c = dtype_code(*t);
+        if ((c != dt && c != D2C_F32) || (pdt >= 0 && c != pdt)) return py::none();
+        pdt = c;
+    }
+    d2c_layer_norm_desc q{x.numel() / C, step, (int)C, dt, pdt < 0 ? dt : pdt, (float)eps};
+    const bool grad = wants_grad(x, w, b);
+    std::shared_ptr<LayerNormBackward> node;
+    if (grad) {
+        node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
+    }
+    c10::DeviceGuard guard(x.device());
+    const auto opt = x.options().requires_grad(false);
+    Tensor out = at::empty(x.sizes(), opt), stats;
+    if (grad) stats = at::empty({q.rows, 2}, opt.dtype(at::kFloat));
+    check(d2c_layer_norm_forward(&q, ptr(x), ptr(w), ptr(b), ptr(out), (float *)ptr(stats), stream_of(x)), "layer_norm forward");
+    if (!grad) return py::cast(out);
+    node->q = q;
+    node->x = SavedVariable(x, false); node->stats = SavedVariable(stats, false);
+    node->has_w = w.defined(); node->has_b = b.defined();
+    if (w.defined()) node->w = SavedVariable(w, false);
+    if (b.defined()) node->b = SavedVariable(b, false);
+    return py::cast(record(out, node));
+}
+
+// ---------------------------------------------------------------- rotary3d
+Tensor rotary_call(d2c_rotary3d_desc q, const Tensor &x, const Tensor &pos, int direction)
+{
+    for (int i = 0; i < 3; i++) q.x_stride[i] = x.stride(i);
+    q.direction = direction;
+    Tensor out = at::empty({q.N, q.L, q.H, q.D}, x.options().requires_grad(false));
+    check(d2c_rotary3d(&q, ptr(x), (const float *)ptr(pos), ptr(out), stream_of(x)), "rotary3d");
+    return out;
+}
+bool inner_contiguous(const Tensor &t) { return t.stride(t.dim() - 1) == 1 || t.size(t.dim() - 1) == 1; }
+
+struct Rotary3dBackward : public Node {
+    d2c_rotary3d_desc q;
+    SavedVariable pos;
+    bool has_pos = false;
+    std::string name() const override { return "Rotary3dBackward"; }
+    void release_variables() override
+    {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        pos.reset_data();
+    }
+    variable_list apply(variable_list &&grads) override
+    {
+        variable_list r(1);
+        const std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) grads[0] = input_metadata(0).zeros_like();
+        {
+            at::NoGradGuard no_grad;
+            Tensor vp;
+            if (has_pos) vp = pos.unpack();
+            c10::DeviceGuard guard(grads[0].device());
+            if (should_compute_output(0)) r[0] = rotary_call(q, inner_contiguous(grads[0]) ? grads[0] : grads[0].contiguous(), vp, -1);
+        }
+        once_differentiable(r, grads[0]);
+        return r;
+    }
+};
+
+py::object rotary3d(const Tensor &x, const opt_tensor &positions, int3_t grid, int3_t pairs, double base, bool interleaved)
+{
+    const Tensor pos = positions.value_or(Tensor());
+    if (!plain_strided(x) || x.dim() != 4 || x.numel() == 0 || !inner_contiguous(x)) return py::none();
+    const int dt = dtype_code(x);
+    if (dt != D2C_F32 && dt != D2C_BF16) return py::none();
+    for (int i = 0; i < 4; i++)
+        if (x.size(i) >= (1ll << 31)) return py::none();
+    d2c_rotary3d_desc q;
+    std::memset(&q, 0, sizeof q);
+    q.N = (int)x.size(0); q.L = (int)x.size(1); q.H = (int)x.size(2); q.D = (int)x.size(3);
+    int64_t cells = 1, turned = 0;
+    for (int i = 0; i < 3; i++) {
+        q.pairs[i] = pairs[i]; q.grid[i] = grid[i];
+        if (pairs[i] < 0 || grid[i] < 0) return py::none();
+        turned += pairs[i]; cells *= grid[i];
+    }
+    if (2 * turned > q.D) return py::none();
+    if (pos.defined()) {
+        if (!plain(pos) || pos.device() != x.device() || pos.scalar_type() != at::kFloat || pos.requires_grad() || pos.dim() < 2 || pos.dim() > 3) return py::none();
+        if (pos.size(-1) != 3 || pos.size(-2) != q.L || (pos.dim() == 3 && pos.size(0) != q.N)) return py::none();
+        q.position_stride = pos.dim() == 3 ? 3ll * q.L : 0;
+    } else if (cells != q.L) return py::none();
+    q.interleaved = interleaved; q.dtype = dt; q.base = (float)base;
+    const bool grad = wants_grad(x);
+    std::shared_ptr<Rotary3dBackward> node;
+    if (grad) {
+        node = std::shared_ptr<Rotary3dBackward>(new Rotary3dBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x));
+    }
+    c10::DeviceGuard guard(x.device());
+    Tensor out = rotary_call(q, x, pos, 1);
+    if (!grad) return py::cast(out);
+    node->q = q;
+    node->has_pos = pos.defined();
+    if (pos.defined()) node->pos = SavedVariable(pos, false);
+    return py::cast(record(out, node));
+}
+
+// ---------------------------------------------------------------- cross_attention
+struct CrossAttentionBackward : public Node {
+    d2c_attention_desc q;
+    SavedVariable query, key, value, lengths, mask, out, lse;
+    bool has_lengths = false, has_mask = false;
+    std::string name() const override { return "CrossAttentionBackward"; }
+    void release_variables() override
+    {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *v : {&query, &key, &value, &lengths, &mask, &out, &lse}) v->reset_data();
+    }
+    variable_list apply(variable_list &&grads) override
+    {
+        variable_list r(3);
+        const std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) grads[0] = input_metadata(0).zeros_like();
+        {
+            at::NoGradGuard no_grad;
+            const Tensor vq = query.unpack(), vk = key.unpack(), vv = value.unpack(), vo = out.unpack(shared_from_this()), vl = lse.unpack();
+            Tensor len, msk;
+            if (has_lengths) len = lengths.unpack();
+            if (has_mask) msk = mask.unpack();
+            c10::DeviceGuard guard(vq.device());
+            const hipStream_t st = stream_of(vq);
+            const Tensor g = grads[0].contiguous();
+            if (should_compute_output(0)) r[0] = no_grad_empty_like(vq);
+            if (should_compute_output(1)) r[1] = no_grad_empty_like(vk);
+            if (should_compute_output(2)) r[2] = no_grad_empty_like(vv);
+            const size_t nb = d2c_attention_backward_workspace_bytes(&q);
+            const Tensor ws = workspace(nb, vq, st);
+            check(d2c_attention_backward(&q, ptr(g), ptr(vq), ptr(vk), ptr(vv), (const int32_t *)ptr(len), (const uint8_t *)ptr(msk), ptr(vo),
+                                         (const float *)ptr(vl), ptr(r[0]), ptr(r[1]), ptr(r[2]), ptr(ws), nb, st),
+                  "cross_attention backward");
+        }
+        once_differentiable(r, grads[0]);
+        return r;
+    }
+};
+
+py::object cross_attention(const Tensor &query, const Tensor &key, const Tensor &value, const opt_tensor &key_lengths, const opt_tensor &key_mask,
+                           const std::optional<double> &scale)
+{
+    const Tensor len = key_lengths.value_or(Tensor()), msk = key_mask.value_or(Tensor());
+    for (const Tensor *t : {&query, &key, &value}) {
+        if (!plain_strided(*t) || t->dim() != 4 || t->device() != query.device() || !inner_contiguous(*t) || t->scalar_type() != query.scalar_type())
+            return py::none();
+        for (int i = 0; i < 4; i++)
+            if (t->size(i) == 0 || t->size(i) >= (1ll << 31)) return py::none();
+    }
+    const int dt = dtype_code(query);
+    if ((dt != D2C_F32 && dt != D2C_BF16) || key.sizes() != value.sizes() || key.size(0) != query.size(0) || key.size(3) != query.size(3) ||
+        query.size(2) % key.size(2) != 0 || query.size(3) > 128)
+        return py::none();
+    d2c_attention_desc q;
+    std::memset(&q, 0, sizeof q);
+    q.N = (int)query.size(0); q.Lq = (int)query.size(1); q.Hq = (int)query.size(2); q.D = (int)query.size(3);
+    q.Lk = (int)key.size(1); q.Hkv = (int)key.size(2);
+    q.dtype = dt;
+    const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.D);
+    if (!(s > 0.0) || !((float)s > 0.f) || !((float)s < INFINITY)) return py::none();
+    q.scale = (float)s;
+    for (int i = 0; i < 3; i++) { q.q_stride[i] = query.stride(i); q.k_stride[i] = key.stride(i); q.v_stride[i] = value.stride(i); }
+    if (len.defined() && (!plain(len) || len.device() != query.device() || len.scalar_type() != at::kInt || len.dim() != 1 || len.size(0) != q.N)) return py::none();
+    if (msk.defined() && (!plain(msk) || msk.device() != query.device() || msk.scalar_type() != at::kBool || msk.dim() != 2 || msk.size(0) != q.N || msk.size(1) != q.Lk))
+        return py::none();
+    const bool grad = wants_grad(query, key, value);
+    std::shared_ptr<CrossAttentionBackward> node;
+    if (grad) {
+        node = std::shared_ptr<CrossAttentionBackward>(new CrossAttentionBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(query, key, value));
+    }
+    c10::DeviceGuard guard(query.device());
+    const hipStream_t st = stream_of(query);
+    const auto opt = query.options().requires_grad(false);
+    Tensor out = at::empty(query.sizes(), opt), lse;
+    if (grad) lse = at::empty({q.N, q.Hkv, (int64_t)q.Lq * (q.Hq / q.Hkv)}, opt.dtype(at::kFloat));
+    const size_t nb = d2c_attention_forward_workspace_bytes(&q);
+    const Tensor ws = workspace(nb, query, st);
+    check(d2c_attention_forward(&q, ptr(query), ptr(key), ptr(value), (const int32_t *)ptr(len), (const uint8_t *)ptr(msk), ptr(out), (float *)ptr(lse),
+                                ptr(ws), nb, st),
+          "cross_attention forward");
+    if (!grad) return py::cast(out);
+    node->q = q;
+    node->query = SavedVariable(query, false); node->key = SavedVariable(key, false); node->value = SavedVariable(value, false);
+    node->lse = SavedVariable(lse, false);
+    node->has_lengths = len.defined(); node->has_mask = msk.defined();
+    if (len.defined()) node->lengths = SavedVariable(len, false);
+    if (msk.defined()) node->mask = SavedVariable(msk, false);
+    Tensor recorded = record(out, node);
+    node->out = SavedVariable(recorded, true);
+    return py::cast(recorded);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m)
@@ -579,4 +841,7 @@ PYBIND11_MODULE(_native, m)
     m.def("conv1d", &conv1d);
     m.def("plain_conv3d", &plain_conv3d);
     m.def("dwconv3d", &dwconv3d);
+    m.def("layer_norm", &layer_norm);
+    m.def("rotary3d", &rotary3d);
+    m.def("cross_attention", &cross_attention);
 }
