@@ -28,17 +28,17 @@ template <int WORDS> struct KeyBits {
     }
 };
 
-template <typename T, int DP, int WK> struct FwdShape {
+template <typename T, int DP, int WK, bool WHOLE> struct FwdShape {
     static constexpr int KW = sizeof(T) == 2 && WK == 1 ? 64 : 32, KT = KW * WK, ROWS = 32 * (4 / WK);
-    using KV = Tile<T, DP, KT, 256>;
+    using KV = Tile<T, DP, KT, 256, WHOLE>;
     static constexpr int JOIN = WK > 1 ? 4 * 32 * (DP + 2) * 4 : 0;
     static constexpr int LDS = 2 * KV::BYTES > JOIN ? 2 * KV::BYTES : JOIN;
 };
 
 // WK: wavefronts that share rows and split the keys of a tile
-template <typename T, int DP, int WK> __global__ void __launch_bounds__(256) attn_fwd_kernel(Args a)
+template <typename T, int DP, int WK, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(Args a)
 {
-    using Shape = FwdShape<T, DP, WK>;
+    using Shape = FwdShape<T, DP, WK, WHOLE>;
     using KV = typename Shape::KV;
     constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = (KT + 63) / 64;
     extern __shared__ __align__(16) unsigned char lds[];
@@ -56,10 +56,11 @@ template <typename T, int DP, int WK> __global__ void __launch_bounds__(256) att
     KeyBits<WORDS> bits;
     uint64_t next[WORDS];
     auto request = [&](int tile) INLINE {
-        const int k0 = tile * KT;
-        auto there = [&](int i) INLINE { return (next[WORDS == 1 ? 0 : i >> 6] >> (i & 63)) & 1; };
-        k.load(a.D, [&](int i) INLINE { return there(i) ? kb + (long)(k0 + i) * a.ks[1] : nullptr; });
-        v.load(a.D, [&](int i) INLINE { return there(i) ? vb + (long)(k0 + i) * a.vs[1] : nullptr; });
+        const int any = any_key(next);
+        if (any < 0) return;
+        const T *kt = kb + (long)tile * KT * a.ks[1], *vt = vb + (long)tile * KT * a.vs[1];
+        k.load(a.D, [&](int i) INLINE { return kt + key_to_load(next, i, any) * a.ks[1]; });
+        v.load(a.D, [&](int i) INLINE { return vt + key_to_load(next, i, any) * a.vs[1]; });
     };
     if (t < t1) {
         bits.request(a, hd.n, keys, t * KT);
@@ -73,7 +74,7 @@ template <typename T, int DP, int WK> __global__ void __launch_bounds__(256) att
 #pragma unroll
         for (int i = 0; i < NK; i++) {
             const int d = i * 16 + half * 8;
-            q[i] = terms_of<T>(load8<T>(qr + d, row < a.rows ? a.D - d : 0));
+            q[i] = terms_of<T>(load8_of<WHOLE, T>(qr, d, a.D, row < a.rows));
         }
     }
     f32x16 o[ND];
@@ -81,7 +82,7 @@ template <typename T, int DP, int WK> __global__ void __launch_bounds__(256) att
     for (int i = 0; i < ND; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[i][r] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, lift = -INFINITY, l = 0.f;
     const float c = a.scale2;
 
     for (; t < t1; t++) {
@@ -119,15 +120,20 @@ template <typename T, int DP, int WK> __global__ void __launch_bounds__(256) att
         for (int i = 0; i < NS; i++)
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[i][r]);
-        top = fmaxf(m, half_max(top));
-        if (__any(top > m)) {
-            const float f = top > m ? __builtin_amdgcn_exp2f((m - top) * c) : 1.f;
-            m = top;
-            l *= f;
+        // (a row's maximum follows only where it has grown by a factor of 2^8 of the weights: what is added up stays far from float32's
+        // ends, and the sums are seldom scaled anew)
+        if (__any(top > lift)) {
+            const float grown = half_max(top);
+            if (grown > lift) {
+                const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - grown) * c);
+                m = grown;
+                lift = m + 8.f / c;
+                l *= f;
 #pragma unroll
-            for (int i = 0; i < ND; i++)
+                for (int i = 0; i < ND; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) o[i][r] *= f;
+                    for (int r = 0; r < 16; r++) o[i][r] *= f;
+            }
         }
         const float mc = m == -INFINITY ? 0.f : m * c;
 #pragma unroll
@@ -259,18 +265,19 @@ FwdPlan fwd_plan(const d2c_attention_desc &q)
     return p;
 }
 
-template <typename T, int DP, int WK> int launch_fwd(const Args &a, const FwdPlan &p, hipStream_t st)
+template <typename T, int DP, int WK, bool WHOLE> int launch_fwd(const Args &a, const FwdPlan &p, hipStream_t st)
 {
-    constexpr int lds = FwdShape<T, DP, WK>::LDS;
-    const void *kernel = reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, WK>);
+    constexpr int lds = FwdShape<T, DP, WK, WHOLE>::LDS;
+    const void *kernel = reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, WK, WHOLE>);
     if (int rc = d2c_allow_lds(kernel, lds, "attn_fwd_kernel")) return rc;
-    hipLaunchKernelGGL((attn_fwd_kernel<T, DP, WK>), dim3((unsigned)(a.N * a.Hkv), (unsigned)p.row_tiles, (unsigned)p.splits), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((attn_fwd_kernel<T, DP, WK, WHOLE>), dim3((unsigned)(a.N * a.Hkv), (unsigned)p.row_tiles, (unsigned)p.splits), dim3(256), lds, st, a);
     return d2c_check_launch("attn_fwd_kernel");
 }
 template <typename T, int DP> int launch_fwd_d(const Args &a, const FwdPlan &p, hipStream_t st)
 {
-    if (p.wk > 1) return launch_fwd<T, DP, sizeof(T) == 2 ? 4 : 2>(a, p, st);
-    return launch_fwd<T, DP, 1>(a, p, st);
+    constexpr int WK = sizeof(T) == 2 ? 4 : 2;
+    if (a.D % 8 == 0) return p.wk > 1 ? launch_fwd<T, DP, WK, true>(a, p, st) : launch_fwd<T, DP, 1, true>(a, p, st);
+    return p.wk > 1 ? launch_fwd<T, DP, WK, false>(a, p, st) : launch_fwd<T, DP, 1, false>(a, p, st);
 }
 template <typename T> int launch_fwd_t(const Args &a, const FwdPlan &p, hipStream_t st)
 {

@@ -77,18 +77,34 @@ template <int P> D2C_DEV Frag<P> make_frag(const float *v)
     return f;
 }
 
-// 8 elements as they lie in memory, `left` of them there (zeros behind; none: p is not read)
+// 8 elements as they lie in memory.  WHOLE: all of them there; else `left` of them (zeros behind; none: p is not read)
 template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
-template <typename T> D2C_DEV Raw8<T> load8(const T *p, int left)
+template <bool WHOLE, typename T> D2C_DEV Raw8<T> load8(const T *p, int left)
 {
     constexpr int VEC = 16 / (int)sizeof(T);
     Raw8<T> r;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; i++) {
-        r.v[i] = make_uint4(0, 0, 0, 0);
-        if (left > i * VEC) r.v[i] = load_run<T>(p + i * VEC, left - i * VEC);
+        if constexpr (WHOLE) {
+            const AnyVec<T> v = load_any(p + i * VEC);
+            r.v[i] = make_uint4(v[0], v[1], v[2], v[3]);
+        } else {
+            r.v[i] = make_uint4(0, 0, 0, 0);
+            if (left > i * VEC) r.v[i] = load_run<T>(p + i * VEC, left - i * VEC);
+        }
     }
     return r;
+}
+// ... of a row of D elements, from element d on, zeros behind the row (WHOLE: D is a multiple of 8)
+template <bool WHOLE, typename T> D2C_DEV Raw8<T> load8_of(const T *row, int d, int D, bool live)
+{
+    if constexpr (WHOLE) {
+        Raw8<T> r = load8<true, T>(row + min(d, D - 8), 8);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++)
+            if (d >= D || !live) r.v[i] = make_uint4(0, 0, 0, 0);
+        return r;
+    } else return load8<false, T>(row + d, live ? D - d : 0);
 }
 template <typename T> D2C_DEV Frag<kTerms<T>> terms_of(const Raw8<T> &r)
 {
@@ -124,18 +140,21 @@ template <int DP> D2C_DEV int piece_at(int row, int piece) { return row * (DP * 
 
 typedef short v4s_t __attribute__((ext_vector_type(4)));
 
-template <typename T, int DP, int ROWS, int THREADS> struct Tile {
+// WHOLE (D is a multiple of 8): loads without branches.  Pieces behind a row's end then repeat its last one: they meet zeros of the other operand, or make
+// columns that are not stored.  Else elements behind the end are zeros.
+template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
     static constexpr int P = kTerms<T>, PIECES = DP / 8, PER = (ROWS * PIECES + THREADS - 1) / THREADS;
     static constexpr int TERM = ROWS * DP * 2, BYTES = P * TERM;
     Raw8<T> r[PER];
-    // row(i): the address of row i, or NULL where it reads as zeros
+    // row(i): the address of row i, which is there to be read whatever i
     template <typename Row> D2C_DEV void load(int D, Row row)
     {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            const int at = i * THREADS + threadIdx.x;
-            const T *p = ROWS * PIECES % THREADS == 0 || at < ROWS * PIECES ? row(at / PIECES) : nullptr;
-            r[i] = load8<T>(p + at % PIECES * 8, p ? D - at % PIECES * 8 : 0);
+            const int at = min(i * THREADS + (int)threadIdx.x, ROWS * PIECES - 1), d = at % PIECES * 8;
+            const T *p = row(at / PIECES);
+            if constexpr (WHOLE) r[i] = load8<true, T>(p + min(d, D - 8), 8);
+            else r[i] = load8<false, T>(p + d, D - d);
         }
     }
     D2C_DEV void store(unsigned char *lds) const
@@ -208,8 +227,28 @@ template <typename T> D2C_DEV void store4(T *p, const float *v, int left)
 }
 
 // Both halves of the wavefront: the larger value, the sum
-D2C_DEV float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
-D2C_DEV float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+D2C_DEV void other_half(float v, float &x, float &y)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    x = __uint_as_float(r[0]); y = __uint_as_float(r[1]);
+}
+D2C_DEV float half_max(float v) { float x, y; other_half(v, x, y); return fmaxf(x, y); }
+D2C_DEV float half_sum(float v) { float x, y; other_half(v, x, y); return x + y; }
+
+// The rows of a tile of keys to request: a key that is not to be read is replaced by one of the tile's that is (`any`, a bit of
+// `words`), so that what it holds is nowhere read: its score is put to -infinity, its weight 0 meets that other key's value.
+template <int WORDS> D2C_DEV int key_to_load(const uint64_t (&words)[WORDS], int i, int any)
+{
+    const uint64_t w = WORDS == 1 ? words[0] : words[i >> 6];
+    return (w >> (i & 63)) & 1 ? i : any;
+}
+template <int WORDS> D2C_DEV int any_key(const uint64_t (&words)[WORDS])
+{
+#pragma unroll
+    for (int j = 0; j < WORDS; j++)
+        if (words[j]) return j * 64 + __builtin_ctzll(words[j]);
+    return -1;
+}
 
 Args make_args(const d2c_attention_desc &q);
 

@@ -11,16 +11,16 @@ using namespace d2c_attn;
 
 namespace {
 
-template <typename T, int DP> struct QShape {
+template <typename T, int DP, bool WHOLE> struct QShape {
     static constexpr int KT = sizeof(T) == 2 ? 64 : 32;
-    using KV = Tile<T, DP, KT, 256>;
+    using KV = Tile<T, DP, KT, 256, WHOLE>;
     static constexpr int LDS = 2 * KV::BYTES;
 };
 
-template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_q_kernel(Args a)
+template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_bwd_q_kernel(Args a)
 {
-    using KV = typename QShape<T, DP>::KV;
-    constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, KT = QShape<T, DP>::KT;
+    using KV = typename QShape<T, DP, WHOLE>::KV;
+    constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, KT = QShape<T, DP, WHOLE>::KT;
     extern __shared__ __align__(16) unsigned char lds[];
     unsigned char *s_k = lds, *s_v = lds + KV::BYTES;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -36,15 +36,17 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_q_
     KV k, v;
     bool b = false;
     auto ask = [&](int k0) INLINE { const int key = k0 + lane; b = lane < KT && key < keys && (!a.mask || a.mask[(long)hd.n * a.Lk + key]); };
-    uint64_t next = 0;
+    uint64_t next[1] = {0};
     auto request = [&](int tile) INLINE {
-        const int k0 = tile * KT;
-        k.load(a.D, [&](int i) INLINE { return (next >> i) & 1 ? kb + (long)(k0 + i) * a.ks[1] : nullptr; });
-        v.load(a.D, [&](int i) INLINE { return (next >> i) & 1 ? vb + (long)(k0 + i) * a.vs[1] : nullptr; });
+        const int any = any_key(next);
+        if (any < 0) return;
+        const T *kt = kb + (long)tile * KT * a.ks[1], *vt = vb + (long)tile * KT * a.vs[1];
+        k.load(a.D, [&](int i) INLINE { return kt + key_to_load(next, i, any) * a.ks[1]; });
+        v.load(a.D, [&](int i) INLINE { return vt + key_to_load(next, i, any) * a.vs[1]; });
     };
     if (t < t1) {
         ask(t * KT);
-        next = __ballot(b);
+        next[0] = __ballot(b);
         request(t);
         ask((t + 1) * KT);
     }
@@ -55,9 +57,9 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_q_
         const T *qr = row_at<T>(a.q, a.qs, a, hd, r), *gr = row_at<T>(a.g, a.gs, a, hd, r), *orow = row_at<T>(a.o, a.gs, a, hd, r);
 #pragma unroll
         for (int i = 0; i < NK; i++) {
-            const int d = i * 16 + half * 8, left = live ? a.D - d : 0;
-            q[i] = terms_of<T>(load8<T>(qr + d, left));
-            const Raw8<T> x = load8<T>(gr + d, left), y = load8<T>(orow + d, left);
+            const int d = i * 16 + half * 8;
+            q[i] = terms_of<T>(load8_of<WHOLE, T>(qr, d, a.D, live));
+            const Raw8<T> x = load8_of<WHOLE, T>(gr, d, a.D, live), y = load8_of<WHOLE, T>(orow, d, a.D, live);
             g[i] = terms_of<T>(x);
             float xf[8], yf[8];
             floats_of<T>(x, xf);
@@ -77,13 +79,13 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_q_
     const float c = a.scale2;
 
     for (; t < t1; t++) {
-        const uint64_t now = next;
+        const uint64_t now = next[0];
         __syncthreads();
         k.store(s_k);
         v.store(s_v);
         __syncthreads();
         if (t + 1 < t1) {
-            next = __ballot(b);
+            next[0] = __ballot(b);
             request(t + 1);
             ask((t + 2) * KT);
         }
@@ -140,16 +142,16 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_q_
         }
 }
 
-template <typename T, int DP> struct KvShape {
+template <typename T, int DP, bool WHOLE> struct KvShape {
     static constexpr int RT = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
-    using QG = Tile<T, DP, RT, 256>;
+    using QG = Tile<T, DP, RT, 256, WHOLE>;
     static constexpr int LDS = 2 * QG::BYTES + 2 * RT * 4;
 };
 
-template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_kv_kernel(Args a)
+template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_bwd_kv_kernel(Args a)
 {
-    using QG = typename KvShape<T, DP>::QG;
-    constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, RT = KvShape<T, DP>::RT;
+    using QG = typename KvShape<T, DP, WHOLE>::QG;
+    constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, RT = KvShape<T, DP, WHOLE>::RT;
     extern __shared__ __align__(16) unsigned char lds[];
     unsigned char *s_q = lds, *s_g = lds + QG::BYTES;
     float *s_lse = reinterpret_cast<float *>(lds + 2 * QG::BYTES), *s_delta = s_lse + RT;
@@ -165,8 +167,9 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_kv
     float stat = 0.f;
     auto request = [&](int tile) INLINE {
         const int r0 = tile * RT;
-        q.load(a.D, [&](int i) INLINE { return r0 + i < a.rows ? row_at<T>(a.q, a.qs, a, hd, r0 + i) : nullptr; });
-        g.load(a.D, [&](int i) INLINE { return r0 + i < a.rows ? row_at<T>(a.g, a.gs, a, hd, r0 + i) : nullptr; });
+        // (rows behind the last one repeat it: their weights are 0, by a sum of +infinity)
+        q.load(a.D, [&](int i) INLINE { return row_at<T>(a.q, a.qs, a, hd, min(r0 + i, a.rows - 1)); });
+        g.load(a.D, [&](int i) INLINE { return row_at<T>(a.g, a.gs, a, hd, min(r0 + i, a.rows - 1)); });
         if (threadIdx.x < 2 * RT) {
             const bool first = threadIdx.x < RT;
             const int r = r0 + (first ? threadIdx.x : threadIdx.x - RT);
@@ -176,13 +179,14 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) attn_bwd_kv
     if (t < t1) request(t);
     Frag<P> k[NK], v[NK];
     {
-        const T *kr = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2] + (long)key * a.ks[1];
-        const T *vr = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2] + (long)key * a.vs[1];
+        const long at = min(key, a.Lk - 1);
+        const T *kr = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2] + at * a.ks[1];
+        const T *vr = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2] + at * a.vs[1];
 #pragma unroll
         for (int i = 0; i < NK; i++) {
-            const int d = i * 16 + half * 8, left = live ? a.D - d : 0;
-            k[i] = terms_of<T>(load8<T>(kr + d, left));
-            v[i] = terms_of<T>(load8<T>(vr + d, left));
+            const int d = i * 16 + half * 8;
+            k[i] = terms_of<T>(load8_of<WHOLE, T>(kr, d, a.D, live));
+            v[i] = terms_of<T>(load8_of<WHOLE, T>(vr, d, a.D, live));
         }
     }
     f32x16 dk[ND], dv[ND];
@@ -310,17 +314,17 @@ BwdPlan bwd_plan(const d2c_attention_desc &q)
     return p;
 }
 
-template <typename T, int DP> int launch_bwd_d(Args a, const BwdPlan &p, hipStream_t st)
+template <typename T, int DP, bool WHOLE> int launch_bwd_d(Args a, const BwdPlan &p, hipStream_t st)
 {
     const unsigned heads = (unsigned)(a.N * a.Hkv);
     if (a.Lq > 0 && !a.gq && (a.gk || a.gv)) {
         hipLaunchKernelGGL(attn_delta_kernel<T>, dim3((unsigned)(((long)heads * a.rows + 3) / 4)), dim3(256), 0, st, a);
         if (int rc = d2c_check_launch("attn_delta_kernel")) return rc;
     } else if (a.Lq > 0 && a.gq) {
-        constexpr int lds = QShape<T, DP>::LDS;
-        if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP>), lds, "attn_bwd_q_kernel")) return rc;
+        constexpr int lds = QShape<T, DP, WHOLE>::LDS;
+        if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, WHOLE>), lds, "attn_bwd_q_kernel")) return rc;
         a.splits = p.q_splits;
-        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP>), dim3(heads, (unsigned)p.row_tiles, (unsigned)p.q_splits), dim3(256), lds, st, a);
+        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, WHOLE>), dim3(heads, (unsigned)p.row_tiles, (unsigned)p.q_splits), dim3(256), lds, st, a);
         if (int rc = d2c_check_launch("attn_bwd_q_kernel")) return rc;
         if (p.q_splits > 1) {
             const long total = (long)heads * a.rows * a.D;
@@ -329,10 +333,10 @@ template <typename T, int DP> int launch_bwd_d(Args a, const BwdPlan &p, hipStre
         }
     }
     if (a.Lk == 0 || !(a.gk || a.gv)) return D2C_OK;
-    constexpr int lds = KvShape<T, DP>::LDS;
-    if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP>), lds, "attn_bwd_kv_kernel")) return rc;
+    constexpr int lds = KvShape<T, DP, WHOLE>::LDS;
+    if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, WHOLE>), lds, "attn_bwd_kv_kernel")) return rc;
     a.splits = p.kv_splits;
-    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP>), dim3(heads, (unsigned)p.key_tiles, (unsigned)p.kv_splits), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, WHOLE>), dim3(heads, (unsigned)p.key_tiles, (unsigned)p.kv_splits), dim3(256), lds, st, a);
     if (int rc = d2c_check_launch("attn_bwd_kv_kernel")) return rc;
     if (p.kv_splits > 1) {
         const long total = (long)heads * a.Lk * a.D;
@@ -343,10 +347,11 @@ template <typename T, int DP> int launch_bwd_d(Args a, const BwdPlan &p, hipStre
 }
 template <typename T> int launch_bwd(const Args &a, const BwdPlan &p, hipStream_t st)
 {
-    if (a.D <= 32) return launch_bwd_d<T, 32>(a, p, st);
-    if (a.D <= 64) return launch_bwd_d<T, 64>(a, p, st);
-    if (a.D <= 96) return launch_bwd_d<T, 96>(a, p, st);
-    return launch_bwd_d<T, 128>(a, p, st);
+    const bool whole = a.D % 8 == 0;
+    if (a.D <= 32) return whole ? launch_bwd_d<T, 32, true>(a, p, st) : launch_bwd_d<T, 32, false>(a, p, st);
+    if (a.D <= 64) return whole ? launch_bwd_d<T, 64, true>(a, p, st) : launch_bwd_d<T, 64, false>(a, p, st);
+    if (a.D <= 96) return whole ? launch_bwd_d<T, 96, true>(a, p, st) : launch_bwd_d<T, 96, false>(a, p, st);
+    return whole ? launch_bwd_d<T, 128, true>(a, p, st) : launch_bwd_d<T, 128, false>(a, p, st);
 }
 
 }  // namespace
