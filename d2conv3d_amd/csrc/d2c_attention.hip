@@ -217,24 +217,44 @@ template <typename T, int DP, int WK, bool WHOLE> __global__ void __launch_bound
     if (a.lse && half == 0) a.lse[hd.nh * a.rows + row] = l == 0.f ? INFINITY : mc + log2f(l);
 }
 
-// One wavefront to a row: the partial results of `splits` workgroups
-template <typename T> __global__ void __launch_bounds__(256) attn_join_kernel(Args a)
+// The partial results of `splits` workgroups.  LANES lanes take four of a row's columns each, `groups` (a power of two) of them the splits in turn; their sums
+// meet in LDS.  Latency counts: one row of 102 splits 13.6 us as a wavefront that walks over them, JOIN_FEW as here.
+template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_join_kernel(Args a, int groups)
 {
-    const long total = (long)a.N * a.Hkv * a.rows, at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= total) return;
-    const int lane = threadIdx.x & 63;
-    float all = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) all = fmaxf(all, a.part_ml[(s * total + at) * 2]);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) all = fmaxf(all, __shfl_xor(all, d, 64));
-    const float base = all == -INFINITY ? 0.f : all;
-    float l = 0.f, x[2] = {0.f, 0.f};
-    for (int s = 0; s < a.splits; s++) {
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[(s * total + at) * 2] - base);
-        l = fmaf(a.part_ml[(s * total + at) * 2 + 1], f, l);
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (lane + i * 64 < a.D) x[i] = fmaf(a.part[(s * total + at) * a.D + lane + i * 64], f, x[i]);
+    __shared__ float4 s_x[256];
+    __shared__ float2 s_ml[256];
+    const int per = 256 / (LANES * groups), lane = threadIdx.x % LANES, group = threadIdx.x / LANES % groups;
+    const long total = (long)a.N * a.Hkv * a.rows, at = (long)blockIdx.x * per + threadIdx.x / (LANES * groups);
+    const bool live = at < total;
+    const int d = lane * 4;
+    float all = -INFINITY, l = 0.f;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+#pragma unroll 4
+        for (int s = group; s < a.splits; s += groups) {
+            const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (s * total + at) * 2);
+            const float4 y = __builtin_bit_cast(float4, d < a.D ? load_run<float>(a.part + (s * total + at) * a.D + d, a.D - d) : make_uint4(0, 0, 0, 0));
+            const float top = fmaxf(all, ml.x), base = top == -INFINITY ? 0.f : top;
+            const float f = __builtin_amdgcn_exp2f(all - base), g = __builtin_amdgcn_exp2f(ml.x - base);
+            all = top;
+            l = l * f + ml.y * g;
+            x[0] = x[0] * f + y.x * g; x[1] = x[1] * f + y.y * g; x[2] = x[2] * f + y.z * g; x[3] = x[3] * f + y.w * g;
+        }
+    }
+    s_x[threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
+    s_ml[threadIdx.x] = make_float2(all, l);
+    __syncthreads();
+    if (group != 0 || !live) return;
+    float top = all;
+    for (int g = 1; g < groups; g++) top = fmaxf(top, s_ml[threadIdx.x + g * LANES].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    l = x[0] = x[1] = x[2] = x[3] = 0.f;
+    for (int g = 0; g < groups; g++) {
+        const float2 ml = s_ml[threadIdx.x + g * LANES];
+        const float4 y = s_x[threadIdx.x + g * LANES];
+        const float f = __builtin_amdgcn_exp2f(ml.x - base);
+        l = fmaf(ml.y, f, l);
+        x[0] = fmaf(y.x, f, x[0]); x[1] = fmaf(y.y, f, x[1]); x[2] = fmaf(y.z, f, x[2]); x[3] = fmaf(y.w, f, x[3]);
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     const long nh = at / a.rows;
@@ -242,9 +262,9 @@ template <typename T> __global__ void __launch_bounds__(256) attn_join_kernel(Ar
     const int head = (int)(nh - (long)n * a.Hkv) * a.group + row - pos * a.group;
     T *orow = reinterpret_cast<T *>(a.out) + (((long)n * a.Lq + pos) * a.Hq + head) * a.D;
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-        if (lane + i * 64 < a.D) orow[lane + i * 64] = f32_to_elem<T>(x[i] * inv);
-    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : all + log2f(l);
+    for (int i = 0; i < 4; i++) x[i] *= inv;
+    if (d < a.D) store4<T>(orow + d, x, a.D - d);
+    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : top + log2f(l);
 }
 
 // What a call runs on: rows of 32 or fewer are shared by the wavefronts of a workgroup (WK > 1), and so many workgroups share the keys that there
@@ -279,6 +299,14 @@ template <typename T, int DP> int launch_fwd_d(const Args &a, const FwdPlan &p, 
     if (a.D % 8 == 0) return p.wk > 1 ? launch_fwd<T, DP, WK, true>(a, p, st) : launch_fwd<T, DP, 1, true>(a, p, st);
     return p.wk > 1 ? launch_fwd<T, DP, WK, false>(a, p, st) : launch_fwd<T, DP, 1, false>(a, p, st);
 }
+template <typename T, int LANES> int launch_join(const Args &a, hipStream_t st)
+{
+    int groups = 1;
+    while (groups * 2 <= std::min(a.splits, 256 / LANES)) groups *= 2;
+    const long total = (long)a.N * a.Hkv * a.rows, per = 256 / (LANES * groups);
+    hipLaunchKernelGGL((attn_join_kernel<T, LANES>), dim3((unsigned)((total + per - 1) / per)), dim3(256), 0, st, a, groups);
+    return d2c_check_launch("attn_join_kernel");
+}
 template <typename T> int launch_fwd_t(const Args &a, const FwdPlan &p, hipStream_t st)
 {
     int rc;
@@ -287,9 +315,9 @@ template <typename T> int launch_fwd_t(const Args &a, const FwdPlan &p, hipStrea
     else if (a.D <= 96) rc = launch_fwd_d<T, 96>(a, p, st);
     else rc = launch_fwd_d<T, 128>(a, p, st);
     if (rc || p.splits == 1) return rc;
-    const long total = (long)a.N * a.Hkv * a.rows;
-    hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)((total + 3) / 4)), dim3(256), 0, st, a);
-    return d2c_check_launch("attn_join_kernel");
+    if (a.D <= 32) return launch_join<T, 8>(a, st);
+    if (a.D <= 64) return launch_join<T, 16>(a, st);
+    return launch_join<T, 32>(a, st);
 }
 
 }  // namespace

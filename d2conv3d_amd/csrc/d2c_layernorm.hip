@@ -182,22 +182,38 @@ template <typename T, typename TP, int LANES, int NV> __global__ void __launch_b
     }
 }
 
-// The workgroups' sums: 16 channels and 16 slices of the workgroups to a workgroup here
-template <typename TP> __global__ void __launch_bounds__(256) ln_params_kernel(LnArgs a)
+// The workgroups' sums: 64 channels (16 lanes of four) and 64 slices of the workgroups to a workgroup here.  Bound: latency, a slice's few loads are in flight
+// together (16 slices of 64 loads each, 1024 workgroups: 20 us).
+constexpr int kLnSlices = 64;
+template <typename TP> __global__ void __launch_bounds__(16 * kLnSlices) ln_params_kernel(LnArgs a)
 {
-    __shared__ float s[16][17];
-    const int c = (int)blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4, which = blockIdx.y;
-    float v = 0.f;
-    if (c < a.C)
-        for (int k = slice; k < a.blocks; k += 16) v += a.part[((long)k * 2 + which) * a.C + c];
-    s[slice][threadIdx.x & 15] = v;
-    __syncthreads();
-    if (slice != 0 || c >= a.C) return;
-    v = 0.f;
+    __shared__ float4 s[kLnSlices][16];
+    const int lane = threadIdx.x & 15, c = (int)blockIdx.x * 64 + lane * 4, slice = threadIdx.x >> 4, which = blockIdx.y;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.C) {
+#pragma unroll 8
+        for (int k = slice; k < a.blocks; k += kLnSlices) {
+            const float4 p = __builtin_bit_cast(float4, load_run<float>(a.part + ((long)k * 2 + which) * a.C + c, a.C - c));
+            v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+        }
+    }
+    s[slice][lane] = make_float4(v[0], v[1], v[2], v[3]);
 #pragma unroll
-    for (int k = 0; k < 16; k++) v += s[k][threadIdx.x];
+    for (int n = kLnSlices / 2; n > 0; n >>= 1) {
+        __syncthreads();
+        if (slice < n) {
+            const float4 p = s[slice][lane], q = s[slice + n][lane];
+            s[slice][lane] = make_float4(p.x + q.x, p.y + q.y, p.z + q.z, p.w + q.w);
+        }
+    }
+    if (slice != 0 || c >= a.C) return;
+    const float4 p = s[0][lane];
+    const float r[4] = {p.x, p.y, p.z, p.w};
     TP *out = reinterpret_cast<TP *>(which ? a.gb : a.gw);
-    if (out) out[c] = f32_to_elem<TP>(v);
+    if (!out) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (c + i < a.C) out[c + i] = f32_to_elem<TP>(r[i]);
 }
 
 constexpr int kLnMaxChannels = 16384;
@@ -301,8 +317,8 @@ extern "C" int d2c_layer_norm_backward(const d2c_layer_norm_desc *q, const void 
     if (q->rows > 0 || params)
         if (int rc = launch<true>(*q, a, s, st)) return rc;      // (no rows: sums of nothing)
     if (!params) return D2C_OK;
-    const dim3 grid((unsigned)((q->C + 15) / 16), 2);
-    if (q->param_dtype == D2C_F32) hipLaunchKernelGGL(ln_params_kernel<float>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(ln_params_kernel<bf16_t>, grid, dim3(256), 0, st, a);
+    const dim3 grid((unsigned)((q->C + 63) / 64), 2);
+    if (q->param_dtype == D2C_F32) hipLaunchKernelGGL(ln_params_kernel<float>, grid, dim3(16 * kLnSlices), 0, st, a);
+    else hipLaunchKernelGGL(ln_params_kernel<bf16_t>, grid, dim3(16 * kLnSlices), 0, st, a);
     return d2c_check_launch("ln_params_kernel");
 }
