@@ -3,7 +3,9 @@
 // A workgroup takes one key head, 128 rows (32 to a wavefront) and walks over the keys a tile at a time, K and V through LDS, the
 // next tile requested while this one is worked on.  Few rows: the wavefronts share them and split the keys of a tile, and several workgroups share the keys;
 // their results are joined by attn_join_kernel.
-#include <algorithm>
+#include <mutex>
+#include <type_traits>
+#include <vector>
 #include "d2c_attention.hpp"
 
 using namespace d2c_attn;
@@ -32,7 +34,9 @@ template <typename T, int DP, int WK, bool WHOLE> struct FwdShape {
     static constexpr int KW = sizeof(T) == 2 && WK == 1 ? 64 : 32, KT = KW * WK, ROWS = 32 * (4 / WK);
     using KV = Tile<T, DP, KT, 256, WHOLE>;
     static constexpr int JOIN = WK > 1 ? 4 * 32 * (DP + 2) * 4 : 0;
-    static constexpr int LDS = 2 * KV::BYTES > JOIN ? 2 * KV::BYTES : JOIN;
+    // two tiles of each where three workgroups of a compute unit have room for them: one barrier a tile
+    static constexpr int BUFFERS = 4 * KV::BYTES <= 52 << 10 ? 2 : 1;
+    static constexpr int LDS = 2 * BUFFERS * KV::BYTES > JOIN ? 2 * BUFFERS * KV::BYTES : JOIN;
 };
 
 // WK: wavefronts that share rows and split the keys of a tile
@@ -42,23 +46,33 @@ template <typename T, int DP, int WK, bool WHOLE> __global__ void __launch_bound
     using KV = typename Shape::KV;
     constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = (KT + 63) / 64;
     extern __shared__ __align__(16) unsigned char lds[];
-    unsigned char *s_k = lds, *s_v = lds + KV::BYTES;
+    constexpr int BUFFERS = Shape::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK;
-    const Head hd = head_of(a);
-    const int row = (int)blockIdx.y * Shape::ROWS + (wave / WK) * 32 + (lane & 31);
+    const Unit unit = unit_of(a);
+    const Head hd = unit.head;
+    const int tile_row = (wave / WK) * 32 + (lane & 31), row = unit.tile * Shape::ROWS + tile_row;
     const int keys = keys_of(a, hd.n), tiles = (keys + KT - 1) / KT;
-    const int split = (int)blockIdx.z, t1 = (int)((long)tiles * (split + 1) / a.splits);
-    int t = (int)((long)tiles * split / a.splits);
+    const int t1 = (int)((long)tiles * (unit.split + 1) / unit.splits);
+    int t = (int)((long)tiles * unit.split / unit.splits);
 
     const T *kb = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2];
     const T *vb = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2];
     KV k, v;
+    unsigned koff[KV::PER], voff[KV::PER];
+    k.places(koff, a.D, [&](int i) INLINE { return i * a.ks[1]; });
+    v.places(voff, a.D, [&](int i) INLINE { return i * a.vs[1]; });
     KeyBits<WORDS> bits;
     uint64_t next[WORDS];
     auto request = [&](int tile) INLINE {
         const int any = any_key(next);
         if (any < 0) return;
         const T *kt = kb + (long)tile * KT * a.ks[1], *vt = vb + (long)tile * KT * a.vs[1];
+        if constexpr (WHOLE)
+            if ((a.near & 1) && all_keys<KT>(next)) {
+                k.load_near(kt, koff);
+                v.load_near(vt, voff);
+                return;
+            }
         k.load(a.D, [&](int i) INLINE { return kt + key_to_load(next, i, any) * a.ks[1]; });
         v.load(a.D, [&](int i) INLINE { return vt + key_to_load(next, i, any) * a.vs[1]; });
     };
@@ -84,12 +98,16 @@ template <typename T, int DP, int WK, bool WHOLE> __global__ void __launch_bound
         for (int r = 0; r < 16; r++) o[i][r] = 0.f;
     float m = -INFINITY, lift = -INFINITY, l = 0.f;
     const float c = a.scale2;
+    int buffer = 0;
 
     for (; t < t1; t++) {
         uint64_t now[WORDS];
 #pragma unroll
         for (int j = 0; j < WORDS; j++) now[j] = next[j];
-        __syncthreads();
+        // (with two buffers: who writes one has passed the barrier behind which the other was read, so nobody reads this one any more)
+        unsigned char *s_k = lds + (BUFFERS == 2 ? buffer * 2 * KV::BYTES : 0), *s_v = s_k + KV::BYTES;
+        buffer ^= 1;
+        if constexpr (BUFFERS == 1) __syncthreads();
         k.store(s_k);
         v.store(s_v);
         __syncthreads();
@@ -189,8 +207,8 @@ template <typename T, int DP, int WK, bool WHOLE> __global__ void __launch_bound
             }
     }
     if (row >= a.rows) return;
-    if (a.splits > 1) {
-        const long at = ((long)split * gridDim.x + hd.nh) * a.rows + row;
+    if (unit.splits > 1) {
+        const long at = ((long)unit.split * a.shared + unit.part) * Shape::ROWS + tile_row;
         float *po = a.part + at * a.D;
 #pragma unroll
         for (int i = 0; i < ND; i++)
@@ -218,14 +236,16 @@ template <typename T, int DP, int WK, bool WHOLE> __global__ void __launch_bound
 }
 
 // The partial results of `splits` workgroups.  LANES lanes take four of a row's columns each, `groups` (a power of two) of them the splits in turn; their sums
-// meet in LDS.  Latency counts: one row of 102 splits 13.6 us as a wavefront that walks over them, JOIN_FEW as here.
-template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_join_kernel(Args a, int groups)
+// meet in LDS.  Latency counts: 16 rows of 102 splits 13.6 us as a wavefront each that walks over them, 4.8 as here.
+template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_join_kernel(Args a, int groups, int tile_rows)
 {
     __shared__ float4 s_x[256];
     __shared__ float2 s_ml[256];
     const int per = 256 / (LANES * groups), lane = threadIdx.x % LANES, group = threadIdx.x / LANES % groups;
-    const long total = (long)a.N * a.Hkv * a.rows, at = (long)blockIdx.x * per + threadIdx.x / (LANES * groups);
-    const bool live = at < total;
+    const long total = (long)a.shared * tile_rows, at = (long)blockIdx.x * per + threadIdx.x / (LANES * groups);
+    const int part = (int)(at / tile_rows), unit = a.whole + part, heads = a.N * a.Hkv, tile = unit / heads, nh = unit - tile * heads;
+    const int row = tile * tile_rows + (int)(at - (long)part * tile_rows);
+    const bool live = at < total && row < a.rows;
     const int d = lane * 4;
     float all = -INFINITY, l = 0.f;
     float x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -257,67 +277,86 @@ template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_joi
         x[0] = fmaf(y.x, f, x[0]); x[1] = fmaf(y.y, f, x[1]); x[2] = fmaf(y.z, f, x[2]); x[3] = fmaf(y.w, f, x[3]);
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    const long nh = at / a.rows;
-    const int row = (int)(at - nh * a.rows), n = (int)(nh / a.Hkv), pos = row / a.group;
-    const int head = (int)(nh - (long)n * a.Hkv) * a.group + row - pos * a.group;
+    const int n = nh / a.Hkv, pos = row / a.group, head = (nh - n * a.Hkv) * a.group + row - pos * a.group;
     T *orow = reinterpret_cast<T *>(a.out) + (((long)n * a.Lq + pos) * a.Hq + head) * a.D;
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] *= inv;
     if (d < a.D) store4<T>(orow + d, x, a.D - d);
-    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : top + log2f(l);
+    if (a.lse && lane == 0) a.lse[(long)nh * a.rows + row] = l == 0.f ? INFINITY : top + log2f(l);
 }
 
-// What a call runs on: rows of 32 or fewer are shared by the wavefronts of a workgroup (WK > 1), and so many workgroups share the keys that there
-// are two to a compute unit, each with a tile at least.
-struct FwdPlan { int wk, row_tiles, splits; size_t part_bytes, bytes; };
-FwdPlan fwd_plan(const d2c_attention_desc &q)
+// f(DP, WK, WHOLE) as constants
+template <typename T, typename F> auto for_shape(int D, bool few, F f)
+{
+    constexpr int WK = sizeof(T) == 2 ? 4 : 2;
+    auto pick = [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        using C = std::integral_constant<int, DP>;
+        if (D % 8 == 0) return few ? f(C{}, std::integral_constant<int, WK>{}, std::true_type{}) : f(C{}, std::integral_constant<int, 1>{}, std::true_type{});
+        return few ? f(C{}, std::integral_constant<int, WK>{}, std::false_type{}) : f(C{}, std::integral_constant<int, 1>{}, std::false_type{});
+    };
+    if (D <= 32) return pick(std::integral_constant<int, 32>{});
+    if (D <= 64) return pick(std::integral_constant<int, 64>{});
+    if (D <= 96) return pick(std::integral_constant<int, 96>{});
+    return pick(std::integral_constant<int, 128>{});
+}
+
+// What a call runs on: 32 rows or fewer are shared by the wavefronts of a workgroup, which split the keys of a tile (WK > 1)
+struct FwdPlan { bool few; int tile_rows; Walks walks; size_t part_bytes, bytes; };
+template <typename T> FwdPlan fwd_plan(const d2c_attention_desc &q)
 {
     FwdPlan p;
     const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv;
-    const bool bf = q.dtype == D2C_BF16;
-    p.wk = rows <= 32 ? (bf ? 4 : 2) : 1;
-    const int tile_rows = 32 * (4 / p.wk), tile_keys = p.wk > 1 ? 32 * p.wk : (bf ? 64 : 32);
-    p.row_tiles = (int)((rows + tile_rows - 1) / tile_rows);
-    const long groups = std::max(heads * p.row_tiles, 1L), tiles = (q.Lk + tile_keys - 1) / tile_keys;
-    p.splits = (int)std::max(1L, std::min(2L * std::max(d2c_num_cus(), 1) / groups, tiles));
-    p.part_bytes = p.splits > 1 ? d2c_align_up((size_t)p.splits * heads * rows * q.D * 4) : 0;
-    p.bytes = p.splits > 1 ? p.part_bytes + d2c_align_up((size_t)p.splits * heads * rows * 8) : 0;
+    p.few = rows <= 32;
+    for_shape<T>(q.D, p.few, [&](auto dp, auto wk, auto whole) {
+        using Shape = FwdShape<T, decltype(dp)::value, decltype(wk)::value, decltype(whole)::value>;
+        p.tile_rows = Shape::ROWS;
+        const long units = heads * ((rows + Shape::ROWS - 1) / Shape::ROWS), steps = (q.Lk + Shape::KT - 1) / Shape::KT;
+        const long places = (long)std::max(d2c_num_cus(), 1) *
+            resident(reinterpret_cast<const void *>(&attn_fwd_kernel<T, decltype(dp)::value, decltype(wk)::value, decltype(whole)::value>), Shape::LDS);
+        // (a step: 64 keys of 64 channels take 2 us with every place taken, float32's six products three times as long)
+        p.walks = plan_walks(units, steps, places, 2.0 * Shape::KT / 64 * dp / 64 * (sizeof(T) == 2 ? 1 : 3) / decltype(wk)::value, (double)Shape::ROWS * q.D * 4);
+        return 0;
+    });
+    const size_t lines = (size_t)p.walks.splits * p.walks.shared * p.tile_rows;
+    p.part_bytes = d2c_align_up(lines * q.D * 4);
+    p.bytes = p.part_bytes + d2c_align_up(lines * 8);
     return p;
 }
 
-template <typename T, int DP, int WK, bool WHOLE> int launch_fwd(const Args &a, const FwdPlan &p, hipStream_t st)
-{
-    constexpr int lds = FwdShape<T, DP, WK, WHOLE>::LDS;
-    const void *kernel = reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, WK, WHOLE>);
-    if (int rc = d2c_allow_lds(kernel, lds, "attn_fwd_kernel")) return rc;
-    hipLaunchKernelGGL((attn_fwd_kernel<T, DP, WK, WHOLE>), dim3((unsigned)(a.N * a.Hkv), (unsigned)p.row_tiles, (unsigned)p.splits), dim3(256), lds, st, a);
-    return d2c_check_launch("attn_fwd_kernel");
-}
-template <typename T, int DP> int launch_fwd_d(const Args &a, const FwdPlan &p, hipStream_t st)
-{
-    constexpr int WK = sizeof(T) == 2 ? 4 : 2;
-    if (a.D % 8 == 0) return p.wk > 1 ? launch_fwd<T, DP, WK, true>(a, p, st) : launch_fwd<T, DP, 1, true>(a, p, st);
-    return p.wk > 1 ? launch_fwd<T, DP, WK, false>(a, p, st) : launch_fwd<T, DP, 1, false>(a, p, st);
-}
-template <typename T, int LANES> int launch_join(const Args &a, hipStream_t st)
+template <typename T, int LANES> int launch_join(const Args &a, int tile_rows, hipStream_t st)
 {
     int groups = 1;
     while (groups * 2 <= std::min(a.splits, 256 / LANES)) groups *= 2;
-    const long total = (long)a.N * a.Hkv * a.rows, per = 256 / (LANES * groups);
-    hipLaunchKernelGGL((attn_join_kernel<T, LANES>), dim3((unsigned)((total + per - 1) / per)), dim3(256), 0, st, a, groups);
+    const long total = (long)a.shared * tile_rows, per = 256 / (LANES * groups);
+    hipLaunchKernelGGL((attn_join_kernel<T, LANES>), dim3((unsigned)((total + per - 1) / per)), dim3(256), 0, st, a, groups, tile_rows);
     return d2c_check_launch("attn_join_kernel");
 }
-template <typename T> int launch_fwd_t(const Args &a, const FwdPlan &p, hipStream_t st)
+template <typename T> int launch_fwd(const Args &a, const FwdPlan &p, hipStream_t st)
 {
-    int rc;
-    if (a.D <= 32) rc = launch_fwd_d<T, 32>(a, p, st);
-    else if (a.D <= 64) rc = launch_fwd_d<T, 64>(a, p, st);
-    else if (a.D <= 96) rc = launch_fwd_d<T, 96>(a, p, st);
-    else rc = launch_fwd_d<T, 128>(a, p, st);
-    if (rc || p.splits == 1) return rc;
-    if (a.D <= 32) return launch_join<T, 8>(a, st);
-    if (a.D <= 64) return launch_join<T, 16>(a, st);
-    return launch_join<T, 32>(a, st);
+    const int rc = for_shape<T>(a.D, p.few, [&](auto dp, auto wk, auto whole) {
+        constexpr int DP = decltype(dp)::value, WK = decltype(wk)::value;
+        constexpr bool WHOLE = decltype(whole)::value;
+        constexpr int lds = FwdShape<T, DP, WK, WHOLE>::LDS;
+        if (int e = d2c_allow_lds(reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, WK, WHOLE>), lds, "attn_fwd_kernel")) return e;
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, WK, WHOLE>), dim3(workgroups(p.walks)), dim3(256), lds, st, a);
+        return d2c_check_launch("attn_fwd_kernel");
+    });
+    if (rc || p.walks.shared == 0) return rc;
+    if (a.D <= 32) return launch_join<T, 8>(a, p.tile_rows, st);
+    if (a.D <= 64) return launch_join<T, 16>(a, p.tile_rows, st);
+    return launch_join<T, 32>(a, p.tile_rows, st);
+}
+template <typename T> int forward(Args a, const d2c_attention_desc &q, void *ws, size_t ws_bytes, hipStream_t st)
+{
+    const FwdPlan p = fwd_plan<T>(q);
+    if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 255u))) {
+        d2c_set_error("workspace of %zu bytes (256-byte aligned) required, got %zu at %p", p.bytes, ws_bytes, ws);
+        return D2C_ERR_WORKSPACE;
+    }
+    set_walks(a, p.walks);
+    a.part = (float *)ws; a.part_ml = (float *)((char *)ws + p.part_bytes);
+    return launch_fwd<T>(a, p, st);
 }
 
 }  // namespace
@@ -333,8 +372,9 @@ int d2c_attention_check(const d2c_attention_desc *q)
     if (q->Hq % q->Hkv != 0) { d2c_set_error("attention: %d query heads are no multiple of %d key heads", q->Hq, q->Hkv); return D2C_ERR_SHAPE; }
     if (q->D > 128) { d2c_set_error("attention: heads of up to 128 channels, got %d", q->D); return D2C_ERR_UNSUPPORTED; }
     if (!(q->scale > 0.f) || !(q->scale < INFINITY)) { d2c_set_error("attention: scale must be positive and finite"); return D2C_ERR_SHAPE; }
-    // (a launch's second and third dimension end at 65535)
-    if ((long)q->N * q->Hkv >= (1L << 31) || (long)q->Lq * (q->Hq / q->Hkv) > 65535L * 32 || q->Lk > 65535 * 32) {
+    const long heads = (long)q->N * q->Hkv, rows = (long)q->Lq * (q->Hq / q->Hkv);
+    // (positions and workgroups are counted in 32 bits)
+    if (heads >= (1L << 24) || rows >= (1L << 30) || q->Lk >= (1 << 30) || heads * ((std::max(rows, (long)q->Lk) + 31) / 32) >= (1L << 30)) {
         d2c_set_error("attention: too many samples, positions or heads");
         return D2C_ERR_SHAPE;
     }
@@ -349,13 +389,36 @@ Args d2c_attn::make_args(const d2c_attention_desc &q)
     a.rows = a.Lq * a.group;
     a.gs[0] = (long)q.Lq * q.Hq * q.D; a.gs[1] = (long)q.Hq * q.D; a.gs[2] = q.D;
     a.scale = q.scale; a.scale2 = q.scale * 1.44269504088896340736f;
-    a.splits = 1;
+    // (a tile has 128 rows at most)
+    const long far = (1L << 30) / 128 / 4;
+    auto near = [&](long stride) { return stride >= 0 && stride < far; };
+    a.near = (near(a.ks[1]) && near(a.vs[1]) ? 1 : 0) | (near(a.qs[1]) && near(a.qs[2] * a.group) && near(a.gs[1]) ? 2 : 0);
     return a;
+}
+
+int d2c_attn::resident(const void *kernel, int lds)
+{
+    struct Known { const void *kernel; int dev, n; };
+    static std::mutex mu;
+    static std::vector<Known> known;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) { (void)hipGetLastError(); return 2; }      // (no GPU: sizes are asked for all the same)
+    std::lock_guard<std::mutex> lock(mu);
+    for (const Known &k : known)
+        if (k.kernel == kernel && k.dev == dev) return k.n;
+    int n = 0;
+    if (d2c_allow_lds(kernel, lds, "attention kernel") != D2C_OK || hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, lds) != hipSuccess || n < 1) {
+        (void)hipGetLastError();
+        n = 1;
+    }
+    known.push_back({kernel, dev, n});
+    return n;
 }
 
 extern "C" size_t d2c_attention_forward_workspace_bytes(const d2c_attention_desc *q)
 {
-    return d2c_attention_check(q) == D2C_OK ? fwd_plan(*q).bytes : 0;
+    if (d2c_attention_check(q) != D2C_OK || q->N == 0 || q->Lq == 0) return 0;
+    return q->dtype == D2C_BF16 ? fwd_plan<bf16_t>(*q).bytes : fwd_plan<float>(*q).bytes;
 }
 
 extern "C" int d2c_attention_forward(const d2c_attention_desc *q, const void *query, const void *key, const void *value,
@@ -365,14 +428,7 @@ extern "C" int d2c_attention_forward(const d2c_attention_desc *q, const void *qu
     if (int rc = d2c_attention_check(q)) return rc;
     if (q->N == 0 || q->Lq == 0) return D2C_OK;
     if (!query || !out || (q->Lk > 0 && (!key || !value))) { d2c_set_error("null tensor pointer"); return D2C_ERR_SHAPE; }
-    const FwdPlan p = fwd_plan(*q);
-    if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 255u))) {
-        d2c_set_error("workspace of %zu bytes (256-byte aligned) required, got %zu at %p", p.bytes, ws_bytes, ws);
-        return D2C_ERR_WORKSPACE;
-    }
     Args a = make_args(*q);
     a.q = query; a.k = key; a.v = value; a.lengths = key_lengths; a.mask = key_mask; a.out = out; a.lse = lse;
-    a.splits = p.splits;
-    a.part = (float *)ws; a.part_ml = (float *)((char *)ws + p.part_bytes);
-    return q->dtype == D2C_BF16 ? launch_fwd_t<bf16_t>(a, p, (hipStream_t)stream) : launch_fwd_t<float>(a, p, (hipStream_t)stream);
+    return q->dtype == D2C_BF16 ? forward<bf16_t>(a, *q, ws, ws_bytes, (hipStream_t)stream) : forward<float>(a, *q, ws, ws_bytes, (hipStream_t)stream);
 }

@@ -15,6 +15,7 @@
 //
 // The rows of a group of query heads that share a key head are one axis: row = position * group + head in group.
 #pragma once
+#include <algorithm>
 #include "d2c_common.hpp"
 #include "d2c_mma.hpp"
 
@@ -26,10 +27,11 @@ struct Args {
     const uint8_t *mask;                // [N][Lk], 0: not to be read; or NULL
     void *out, *gq, *gk, *gv;           // [N][Lq][Hq][D], [N][Lk][Hkv][D]
     float *lse, *delta;                 // [N * Hkv][rows]: log2 of the sum of a row (+infinity: no key), and sum_d do o
-    float *part, *part_ml;              // partial results of `splits` workgroups: [splits][N * Hkv][rows or Lk][D] and (forward) [..][2]
+    float *part, *part_ml;              // partial results of the walks that are shared: [splits][shared][rows of a tile][D] and (forward) [..][2]
     long qs[3], ks[3], vs[3], gs[3];    // strides of sample, position, head
     int N, Lq, Lk, Hq, Hkv, group, D, rows;
-    int splits;
+    int whole, shared, splits;          // see Walks
+    int near;                           // offsets inside a tile of keys (bit 0) and of rows (bit 1) fit 32 bits, see Tile
     float scale, scale2;                // scale2 = scale * log2(e)
 };
 
@@ -157,6 +159,20 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
             else r[i] = load8<false, T>(p + d, D - d);
         }
     }
+    // ... by their offsets in bytes from the tile's first row: 32 bits each, the same for every tile
+    template <typename Off> D2C_DEV void places(unsigned (&off)[PER], int D, Off row_offset) const
+    {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int at = min(i * THREADS + (int)threadIdx.x, ROWS * PIECES - 1);
+            off[i] = (unsigned)((row_offset(at / PIECES) + min(at % PIECES * 8, D - 8)) * (long)sizeof(T));
+        }
+    }
+    D2C_DEV void load_near(const T *tile, const unsigned (&off)[PER])
+    {
+#pragma unroll
+        for (int i = 0; i < PER; i++) r[i] = load8<true, T>(reinterpret_cast<const T *>(reinterpret_cast<const char *>(tile) + off[i]), 8);
+    }
     D2C_DEV void store(unsigned char *lds) const
     {
 #pragma unroll
@@ -194,14 +210,46 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
     }
 };
 
-// Sample and key head of a workgroup: consecutive workgroups take consecutive heads, so that a head's workgroups share an XCD's L2
-// where the heads are a multiple of 8.
+// What the workgroups do: units, each the walk of one tile of rows (or keys) of one key head along the other axis.  As many as
+// fill the GPU's places without a remainder are walked by a workgroup each (`whole`); `splits` workgroups share each of the `shared` others, so that the
+// last round is as short as it is empty, and their sums are joined.
+// Consecutive units are of consecutive heads, so that a head's workgroups meet in an XCD's L2 where the heads are a multiple of 8.
+struct Walks { int whole, shared, splits; };
 struct Head { int n, h; long nh; };
-D2C_DEV Head head_of(const Args &a)
+struct Unit { Head head; int tile, split, splits, part; };      // part: which of the shared ones, for split 0
+D2C_DEV Unit unit_of(const Args &a)
 {
-    const int nh = (int)blockIdx.x, n = nh / a.Hkv;
-    return {n, nh - n * a.Hkv, nh};
+    int unit = (int)blockIdx.x, split = 0, splits = 1, part = 0;
+    if (unit >= a.whole) {
+        const int i = unit - a.whole;
+        split = i / a.shared;
+        part = i - split * a.shared;
+        unit = a.whole + part;
+        splits = a.splits;
+    }
+    const int heads = a.N * a.Hkv, tile = unit / heads, nh = unit - tile * heads, n = nh / a.Hkv;
+    return {{n, nh - n * a.Hkv, nh}, tile, split, splits, part};
 }
+// ... of `steps` steps of `step_us` each at the places' full number, `bytes` of partial sums to a unit and split.  Times of the model: 4 us for the launch that
+// joins, its traffic (written and read) at 4 TB/s.
+inline Walks plan_walks(long units, long steps, long places, double step_us, double bytes)
+{
+    Walks w{(int)(units / places * places), 0, 1};
+    w.shared = (int)(units - w.whole);
+    if (w.shared == 0) return w;
+    double best = 0.0;
+    for (long s = 1; s <= std::max(std::min(steps, 256L), 1L); s++) {
+        const double t = (double)((w.shared * s + places - 1) / places) * (double)((steps + s - 1) / s) * step_us +
+                         (s > 1 ? 4.0 + 2.0 * (double)(w.shared * s) * bytes / 4e6 : 0.0);
+        if (s == 1 || t < best) { best = t; w.splits = (int)s; }
+    }
+    if (w.splits == 1) { w.whole += w.shared; w.shared = 0; }
+    return w;
+}
+inline unsigned workgroups(const Walks &w) { return (unsigned)(w.whole + w.shared * w.splits); }
+// Workgroups of a kernel that a compute unit holds
+int resident(const void *kernel, int lds);
+
 D2C_DEV int keys_of(const Args &a, int n) { return a.lengths ? min(max(a.lengths[n], 0), a.Lk) : a.Lk; }
 
 // Row `row` of a tensor [N][Lq][Hq][D] with strides s
@@ -242,6 +290,13 @@ template <int WORDS> D2C_DEV int key_to_load(const uint64_t (&words)[WORDS], int
     const uint64_t w = WORDS == 1 ? words[0] : words[i >> 6];
     return (w >> (i & 63)) & 1 ? i : any;
 }
+template <int KT, int WORDS> D2C_DEV bool all_keys(const uint64_t (&words)[WORDS])
+{
+    bool all = true;
+#pragma unroll
+    for (int j = 0; j < WORDS; j++) all = all && words[j] == (KT < 64 ? (1ull << (KT & 63)) - 1 : ~0ull);
+    return all;
+}
 template <int WORDS> D2C_DEV int any_key(const uint64_t (&words)[WORDS])
 {
 #pragma unroll
@@ -251,6 +306,7 @@ template <int WORDS> D2C_DEV int any_key(const uint64_t (&words)[WORDS])
 }
 
 Args make_args(const d2c_attention_desc &q);
+inline void set_walks(Args &a, const Walks &w) { a.whole = w.whole; a.shared = w.shared; a.splits = w.splits; }
 
 }  // namespace d2c_attn
 

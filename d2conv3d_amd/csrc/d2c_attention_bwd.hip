@@ -4,7 +4,7 @@
 // and walks over the keys; it also leaves delta of its rows), then attn_bwd_kv_kernel (a workgroup keeps 128 keys, 32 to a wavefront, and walks over the
 // rows).  Scores and dp are made in both: 7 products where one kernel would need 5.  Few rows, or few keys: several workgroups share the
 // walk, and attn_bwd_join_kernel adds up their sums.
-#include <algorithm>
+#include <type_traits>
 #include "d2c_attention.hpp"
 
 using namespace d2c_attn;
@@ -14,7 +14,8 @@ namespace {
 template <typename T, int DP, bool WHOLE> struct QShape {
     static constexpr int KT = sizeof(T) == 2 ? 64 : 32;
     using KV = Tile<T, DP, KT, 256, WHOLE>;
-    static constexpr int LDS = 2 * KV::BYTES;
+    static constexpr int BUFFERS = 4 * KV::BYTES <= 52 << 10 ? 2 : 1;
+    static constexpr int LDS = 2 * BUFFERS * KV::BYTES;
 };
 
 template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_bwd_q_kernel(Args a)
@@ -22,18 +23,22 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
     using KV = typename QShape<T, DP, WHOLE>::KV;
     constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, KT = QShape<T, DP, WHOLE>::KT;
     extern __shared__ __align__(16) unsigned char lds[];
-    unsigned char *s_k = lds, *s_v = lds + KV::BYTES;
+    constexpr int BUFFERS = QShape<T, DP, WHOLE>::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const Head hd = head_of(a);
-    const int row = (int)blockIdx.y * 128 + wave * 32 + (lane & 31);
+    const Unit unit = unit_of(a);
+    const Head hd = unit.head;
+    const int tile_row = wave * 32 + (lane & 31), row = unit.tile * 128 + tile_row;
     const bool live = row < a.rows;
     const int keys = keys_of(a, hd.n), tiles = (keys + KT - 1) / KT;
-    const int split = (int)blockIdx.z, t1 = (int)((long)tiles * (split + 1) / a.splits);
-    int t = (int)((long)tiles * split / a.splits);
+    const int t1 = (int)((long)tiles * (unit.split + 1) / unit.splits);
+    int t = (int)((long)tiles * unit.split / unit.splits);
 
     const T *kb = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2];
     const T *vb = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2];
     KV k, v;
+    unsigned koff[KV::PER], voff[KV::PER];
+    k.places(koff, a.D, [&](int i) INLINE { return i * a.ks[1]; });
+    v.places(voff, a.D, [&](int i) INLINE { return i * a.vs[1]; });
     bool b = false;
     auto ask = [&](int k0) INLINE { const int key = k0 + lane; b = lane < KT && key < keys && (!a.mask || a.mask[(long)hd.n * a.Lk + key]); };
     uint64_t next[1] = {0};
@@ -41,6 +46,12 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
         const int any = any_key(next);
         if (any < 0) return;
         const T *kt = kb + (long)tile * KT * a.ks[1], *vt = vb + (long)tile * KT * a.vs[1];
+        if constexpr (WHOLE)
+            if ((a.near & 1) && all_keys<KT>(next)) {
+                k.load_near(kt, koff);
+                v.load_near(vt, voff);
+                return;
+            }
         k.load(a.D, [&](int i) INLINE { return kt + key_to_load(next, i, any) * a.ks[1]; });
         v.load(a.D, [&](int i) INLINE { return vt + key_to_load(next, i, any) * a.vs[1]; });
     };
@@ -70,17 +81,20 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
     }
     delta = half_sum(delta);
     const float lse = live ? a.lse[hd.nh * a.rows + row] : INFINITY;
-    if (live && split == 0 && half == 0) a.delta[hd.nh * a.rows + row] = delta;
+    if (live && unit.split == 0 && half == 0) a.delta[hd.nh * a.rows + row] = delta;
     f32x16 dq[ND];
 #pragma unroll
     for (int i = 0; i < ND; i++)
 #pragma unroll
         for (int r = 0; r < 16; r++) dq[i][r] = 0.f;
     const float c = a.scale2;
+    int buffer = 0;
 
     for (; t < t1; t++) {
         const uint64_t now = next[0];
-        __syncthreads();
+        unsigned char *s_k = lds + (BUFFERS == 2 ? buffer * 2 * KV::BYTES : 0), *s_v = s_k + KV::BYTES;
+        buffer ^= 1;
+        if constexpr (BUFFERS == 1) __syncthreads();
         k.store(s_k);
         v.store(s_v);
         __syncthreads();
@@ -119,8 +133,8 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
         }
     }
     if (!live) return;
-    if (a.splits > 1) {
-        float *p = a.part + (((long)split * gridDim.x + hd.nh) * a.rows + row) * a.D;
+    if (unit.splits > 1) {
+        float *p = a.part + (((long)unit.split * a.shared + unit.part) * 128 + tile_row) * a.D;
 #pragma unroll
         for (int i = 0; i < ND; i++)
 #pragma unroll
@@ -145,7 +159,8 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
 template <typename T, int DP, bool WHOLE> struct KvShape {
     static constexpr int RT = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
     using QG = Tile<T, DP, RT, 256, WHOLE>;
-    static constexpr int LDS = 2 * QG::BYTES + 2 * RT * 4;
+    static constexpr int BYTES = 2 * QG::BYTES + 2 * RT * 4, BUFFERS = 2 * BYTES <= 52 << 10 ? 2 : 1;
+    static constexpr int LDS = BUFFERS * BYTES;
 };
 
 template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_bwd_kv_kernel(Args a)
@@ -153,23 +168,38 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
     using QG = typename KvShape<T, DP, WHOLE>::QG;
     constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, RT = KvShape<T, DP, WHOLE>::RT;
     extern __shared__ __align__(16) unsigned char lds[];
-    unsigned char *s_q = lds, *s_g = lds + QG::BYTES;
-    float *s_lse = reinterpret_cast<float *>(lds + 2 * QG::BYTES), *s_delta = s_lse + RT;
+    constexpr int BUFFERS = KvShape<T, DP, WHOLE>::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const Head hd = head_of(a);
-    const int keys = keys_of(a, hd.n), key0 = (int)blockIdx.y * 128, key = key0 + wave * 32 + (lane & 31);
+    const Unit unit = unit_of(a);
+    const Head hd = unit.head;
+    const int tile_key = wave * 32 + (lane & 31), keys = keys_of(a, hd.n), key0 = unit.tile * 128, key = key0 + tile_key;
     const bool live = key < keys && (!a.mask || a.mask[(long)hd.n * a.Lk + key]);
     const int tiles = (a.rows + RT - 1) / RT;
-    const int split = (int)blockIdx.z, t1 = key0 < keys ? (int)((long)tiles * (split + 1) / a.splits) : 0;
-    int t = (int)((long)tiles * split / a.splits);
+    const int t1 = key0 < keys ? (int)((long)tiles * (unit.split + 1) / unit.splits) : 0;
+    int t = (int)((long)tiles * unit.split / unit.splits);
 
     QG q, g;
+    // (tiles that begin with a position's first head: the places of their rows are the same from tile to tile)
+    const bool uniform = (a.near & 2) && RT % a.group == 0;
+    const T *qb = row_at<T>(a.q, a.qs, a, hd, 0), *gb = row_at<T>(a.g, a.gs, a, hd, 0);
+    unsigned qoff[QG::PER], goff[QG::PER];
+    q.places(qoff, a.D, [&](int i) INLINE { return i / a.group * a.qs[1] + i % a.group * a.qs[2]; });
+    g.places(goff, a.D, [&](int i) INLINE { return i / a.group * a.gs[1] + i % a.group * a.gs[2]; });
     float stat = 0.f;
     auto request = [&](int tile) INLINE {
         const int r0 = tile * RT;
+        bool done = false;
+        if constexpr (WHOLE)
+            if (uniform && r0 + RT <= a.rows) {
+                q.load_near(qb + (r0 / a.group) * a.qs[1], qoff);
+                g.load_near(gb + (r0 / a.group) * a.gs[1], goff);
+                done = true;
+            }
         // (rows behind the last one repeat it: their weights are 0, by a sum of +infinity)
+        if (!done) {
         q.load(a.D, [&](int i) INLINE { return row_at<T>(a.q, a.qs, a, hd, min(r0 + i, a.rows - 1)); });
         g.load(a.D, [&](int i) INLINE { return row_at<T>(a.g, a.gs, a, hd, min(r0 + i, a.rows - 1)); });
+        }
         if (threadIdx.x < 2 * RT) {
             const bool first = threadIdx.x < RT;
             const int r = r0 + (first ? threadIdx.x : threadIdx.x - RT);
@@ -195,9 +225,13 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
 #pragma unroll
         for (int r = 0; r < 16; r++) dk[i][r] = dv[i][r] = 0.f;
     const float c = a.scale2;
+    int buffer = 0;
 
     for (; t < t1; t++) {
-        __syncthreads();
+        unsigned char *s_q = lds + (BUFFERS == 2 ? buffer * KvShape<T, DP, WHOLE>::BYTES : 0), *s_g = s_q + QG::BYTES;
+        float *s_lse = reinterpret_cast<float *>(s_q + 2 * QG::BYTES), *s_delta = s_lse + RT;
+        buffer ^= 1;
+        if constexpr (BUFFERS == 1) __syncthreads();
         q.store(s_q);
         g.store(s_g);
         if (threadIdx.x < 2 * RT) s_lse[threadIdx.x] = stat;
@@ -238,7 +272,7 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
     }
     if (key >= a.Lk) return;
     // (a key that is not to be read: a column of the accumulators of its own, whatever is in it)
-    const float fk = a.splits > 1 ? 1.f : a.scale;
+    const float fk = unit.splits > 1 ? 1.f : a.scale;
 #pragma unroll
     for (int i = 0; i < ND; i++)
 #pragma unroll
@@ -247,10 +281,9 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
             float x[4], y[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) { x[r] = live ? dk[i][j * 4 + r] * fk : 0.f; y[r] = live ? dv[i][j * 4 + r] : 0.f; }
-            if (a.splits > 1) {
-                const long heads = gridDim.x;
-                store4<float>(a.part + (((2L * split) * heads + hd.nh) * a.Lk + key) * a.D + d, x, a.D - d);
-                store4<float>(a.part + (((2L * split + 1) * heads + hd.nh) * a.Lk + key) * a.D + d, y, a.D - d);
+            if (unit.splits > 1) {
+                store4<float>(a.part + (((2L * unit.split) * a.shared + unit.part) * 128 + tile_key) * a.D + d, x, a.D - d);
+                store4<float>(a.part + (((2L * unit.split + 1) * a.shared + unit.part) * 128 + tile_key) * a.D + d, y, a.D - d);
             } else {
                 const long at = (((long)hd.n * a.Lk + key) * a.Hkv + hd.h) * a.D + d;
                 if (a.gk) store4<T>(reinterpret_cast<T *>(a.gk) + at, x, a.D - d);
@@ -259,21 +292,21 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
         }
 }
 
-// Sums of the workgroups that shared a walk: part [splits][1 or 2][N * Hkv][rows or Lk][D]
+// Sums of the workgroups that shared a walk: part [splits][1 or 2][shared][128][D]
 template <typename T, bool KV> __global__ void __launch_bounds__(256) attn_bwd_join_kernel(Args a)
 {
-    const int len = KV ? a.Lk : a.rows;
-    const long total = (long)a.N * a.Hkv * len * a.D, at = (long)blockIdx.x * 256 + threadIdx.x;
+    const long total = (long)a.shared * 128 * a.D, at = (long)blockIdx.x * 256 + threadIdx.x;
     if (at >= total) return;
     const long which = KV ? blockIdx.y : 0;
     if (KV && !(which ? a.gv : a.gk)) return;
+    const int d = (int)(at % a.D), line = (int)(at / a.D), unit = a.whole + line / 128, heads = a.N * a.Hkv, tile = unit / heads, nh = unit - tile * heads;
+    const int i = tile * 128 + line % 128, n = nh / a.Hkv;
+    if (i >= (KV ? a.Lk : a.rows)) return;
     float x = 0.f;
+#pragma unroll 4
     for (int s = 0; s < a.splits; s++) x += a.part[(s * (KV ? 2L : 1L) + which) * total + at];
     if (which == 0) x *= a.scale;
-    const int d = (int)(at % a.D);
-    const long line = at / a.D, nh = line / len;
-    const int i = (int)(line - nh * len), n = (int)(nh / a.Hkv);
-    const Head hd{n, (int)(nh - (long)n * a.Hkv), nh};
+    const Head hd{n, nh - n * a.Hkv, nh};
     if constexpr (KV)
         reinterpret_cast<T *>(which ? a.gv : a.gk)[(((long)n * a.Lk + i) * a.Hkv + hd.h) * a.D + d] = f32_to_elem<T>(x);
     else
@@ -295,70 +328,83 @@ template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(A
     if (lane == 0) a.delta[at] = x;
 }
 
-struct BwdPlan { int row_tiles, key_tiles, q_splits, kv_splits; size_t delta_bytes, bytes; };
-BwdPlan bwd_plan(const d2c_attention_desc &q)
+// f(DP, WHOLE) as constants
+template <typename F> auto for_shape(int D, F f)
+{
+    auto pick = [&](auto dp) { return D % 8 == 0 ? f(dp, std::true_type{}) : f(dp, std::false_type{}); };
+    if (D <= 32) return pick(std::integral_constant<int, 32>{});
+    if (D <= 64) return pick(std::integral_constant<int, 64>{});
+    if (D <= 96) return pick(std::integral_constant<int, 96>{});
+    return pick(std::integral_constant<int, 128>{});
+}
+
+struct BwdPlan { Walks q, kv; size_t delta_bytes, bytes; };
+template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
 {
     BwdPlan p;
-    const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv, want = 2L * std::max(d2c_num_cus(), 1);
-    const bool bf = q.dtype == D2C_BF16;
-    p.row_tiles = (int)((rows + 127) / 128);
-    p.key_tiles = (q.Lk + 127) / 128;
-    const long kt = (q.Lk + (bf ? 63 : 31)) / (bf ? 64 : 32), rt_rows = bf && q.D <= 64 ? 64 : 32, rt = (rows + rt_rows - 1) / rt_rows;
-    // (two workgroups to a compute unit, each with two tiles at least)
-    p.q_splits = (int)std::max(1L, std::min(want / std::max(heads * p.row_tiles, 1L), kt / 2));
-    p.kv_splits = (int)std::max(1L, std::min(want / std::max(heads * p.key_tiles, 1L), rt / 2));
+    const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv, cus = std::max(d2c_num_cus(), 1);
+    const double part = 128.0 * q.D * 4, slow = sizeof(T) == 2 ? 1 : 3;
+    for_shape(q.D, [&](auto dp, auto whole) {
+        constexpr int DP = decltype(dp)::value;
+        constexpr bool WHOLE = decltype(whole)::value;
+        using Q = QShape<T, DP, WHOLE>;
+        using KV = KvShape<T, DP, WHOLE>;
+        // (a step with every place taken, 64 channels: 64 keys 2.4 us, 64 rows 2.8)
+        p.q = plan_walks(heads * ((rows + 127) / 128), (q.Lk + Q::KT - 1) / Q::KT,
+                         cus * resident(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, WHOLE>), Q::LDS), 2.4 * Q::KT / 64 * DP / 64 * slow, part);
+        p.kv = plan_walks(heads * ((q.Lk + 127) / 128), (rows + KV::RT - 1) / KV::RT,
+                          cus * resident(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, WHOLE>), KV::LDS), 2.8 * KV::RT / 64 * DP / 64 * slow, 2 * part);
+        return 0;
+    });
     p.delta_bytes = d2c_align_up((size_t)heads * rows * 4);
-    const size_t qb = p.q_splits > 1 ? (size_t)p.q_splits * heads * rows * q.D * 4 : 0;
-    const size_t kvb = p.kv_splits > 1 ? (size_t)p.kv_splits * 2 * heads * q.Lk * q.D * 4 : 0;
-    p.bytes = p.delta_bytes + d2c_align_up(std::max(qb, kvb));
+    const size_t unit = (size_t)128 * q.D * 4;
+    p.bytes = p.delta_bytes + d2c_align_up(std::max(p.q.shared * p.q.splits * unit, 2 * p.kv.shared * p.kv.splits * unit));
     return p;
 }
 
-template <typename T, int DP, bool WHOLE> int launch_bwd_d(Args a, const BwdPlan &p, hipStream_t st)
+template <typename T, int DP, bool WHOLE> int launch_bwd(Args a, const BwdPlan &p, hipStream_t st)
 {
-    const unsigned heads = (unsigned)(a.N * a.Hkv);
     if (a.Lq > 0 && !a.gq && (a.gk || a.gv)) {
-        hipLaunchKernelGGL(attn_delta_kernel<T>, dim3((unsigned)(((long)heads * a.rows + 3) / 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(attn_delta_kernel<T>, dim3((unsigned)(((long)a.N * a.Hkv * a.rows + 3) / 4)), dim3(256), 0, st, a);
         if (int rc = d2c_check_launch("attn_delta_kernel")) return rc;
     } else if (a.Lq > 0 && a.gq) {
         constexpr int lds = QShape<T, DP, WHOLE>::LDS;
         if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, WHOLE>), lds, "attn_bwd_q_kernel")) return rc;
-        a.splits = p.q_splits;
-        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, WHOLE>), dim3(heads, (unsigned)p.row_tiles, (unsigned)p.q_splits), dim3(256), lds, st, a);
+        set_walks(a, p.q);
+        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, WHOLE>), dim3(workgroups(p.q)), dim3(256), lds, st, a);
         if (int rc = d2c_check_launch("attn_bwd_q_kernel")) return rc;
-        if (p.q_splits > 1) {
-            const long total = (long)heads * a.rows * a.D;
-            hipLaunchKernelGGL((attn_bwd_join_kernel<T, false>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a);
+        if (p.q.shared > 0) {
+            hipLaunchKernelGGL((attn_bwd_join_kernel<T, false>), dim3((unsigned)(((long)p.q.shared * 128 * a.D + 255) / 256)), dim3(256), 0, st, a);
             if (int rc = d2c_check_launch("attn_bwd_join_kernel")) return rc;
         }
     }
     if (a.Lk == 0 || !(a.gk || a.gv)) return D2C_OK;
     constexpr int lds = KvShape<T, DP, WHOLE>::LDS;
     if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, WHOLE>), lds, "attn_bwd_kv_kernel")) return rc;
-    a.splits = p.kv_splits;
-    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, WHOLE>), dim3(heads, (unsigned)p.key_tiles, (unsigned)p.kv_splits), dim3(256), lds, st, a);
+    set_walks(a, p.kv);
+    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, WHOLE>), dim3(workgroups(p.kv)), dim3(256), lds, st, a);
     if (int rc = d2c_check_launch("attn_bwd_kv_kernel")) return rc;
-    if (p.kv_splits > 1) {
-        const long total = (long)heads * a.Lk * a.D;
-        hipLaunchKernelGGL((attn_bwd_join_kernel<T, true>), dim3((unsigned)((total + 255) / 256), 2), dim3(256), 0, st, a);
-        return d2c_check_launch("attn_bwd_join_kernel");
-    }
-    return D2C_OK;
+    if (p.kv.shared == 0) return D2C_OK;
+    hipLaunchKernelGGL((attn_bwd_join_kernel<T, true>), dim3((unsigned)(((long)p.kv.shared * 128 * a.D + 255) / 256), 2), dim3(256), 0, st, a);
+    return d2c_check_launch("attn_bwd_join_kernel");
 }
-template <typename T> int launch_bwd(const Args &a, const BwdPlan &p, hipStream_t st)
+template <typename T> int backward(Args a, const d2c_attention_desc &q, void *ws, size_t ws_bytes, hipStream_t st)
 {
-    const bool whole = a.D % 8 == 0;
-    if (a.D <= 32) return whole ? launch_bwd_d<T, 32, true>(a, p, st) : launch_bwd_d<T, 32, false>(a, p, st);
-    if (a.D <= 64) return whole ? launch_bwd_d<T, 64, true>(a, p, st) : launch_bwd_d<T, 64, false>(a, p, st);
-    if (a.D <= 96) return whole ? launch_bwd_d<T, 96, true>(a, p, st) : launch_bwd_d<T, 96, false>(a, p, st);
-    return whole ? launch_bwd_d<T, 128, true>(a, p, st) : launch_bwd_d<T, 128, false>(a, p, st);
+    const BwdPlan p = bwd_plan<T>(q);
+    if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 255u))) {
+        d2c_set_error("workspace of %zu bytes (256-byte aligned) required, got %zu at %p", p.bytes, ws_bytes, ws);
+        return D2C_ERR_WORKSPACE;
+    }
+    a.delta = (float *)ws; a.part = (float *)((char *)ws + p.delta_bytes);
+    return for_shape(a.D, [&](auto dp, auto whole) { return launch_bwd<T, decltype(dp)::value, decltype(whole)::value>(a, p, st); });
 }
 
 }  // namespace
 
 extern "C" size_t d2c_attention_backward_workspace_bytes(const d2c_attention_desc *q)
 {
-    return d2c_attention_check(q) == D2C_OK ? bwd_plan(*q).bytes : 0;
+    if (d2c_attention_check(q) != D2C_OK || q->N == 0) return 0;
+    return q->dtype == D2C_BF16 ? bwd_plan<bf16_t>(*q).bytes : bwd_plan<float>(*q).bytes;
 }
 
 extern "C" int d2c_attention_backward(const d2c_attention_desc *q, const void *grad_out, const void *query, const void *key,
@@ -372,15 +418,9 @@ extern "C" int d2c_attention_backward(const d2c_attention_desc *q, const void *g
         d2c_set_error("null tensor pointer");
         return D2C_ERR_SHAPE;
     }
-    const BwdPlan p = bwd_plan(*q);
-    if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 255u))) {
-        d2c_set_error("workspace of %zu bytes (256-byte aligned) required, got %zu at %p", p.bytes, ws_bytes, ws);
-        return D2C_ERR_WORKSPACE;
-    }
     Args a = make_args(*q);
     a.g = grad_out; a.q = query; a.k = key; a.v = value; a.lengths = key_lengths; a.mask = key_mask; a.o = out;
     a.lse = const_cast<float *>(lse);
     a.gq = grad_query; a.gk = grad_key; a.gv = grad_value;
-    a.delta = (float *)ws; a.part = (float *)((char *)ws + p.delta_bytes);
-    return q->dtype == D2C_BF16 ? launch_bwd<bf16_t>(a, p, (hipStream_t)stream) : launch_bwd<float>(a, p, (hipStream_t)stream);
+    return q->dtype == D2C_BF16 ? backward<bf16_t>(a, *q, ws, ws_bytes, (hipStream_t)stream) : backward<float>(a, *q, ws, ws_bytes, (hipStream_t)stream);
 }

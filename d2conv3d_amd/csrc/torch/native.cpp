@@ -90,6 +90,13 @@ Tensor workspace(size_t bytes, const Tensor &like, hipStream_t st)
     return THPVariable_Unpack(made.ptr());
 }
 
+// A workspace of a few megabytes at most, asked for from a backward pass: from the allocator, which is quicker than waiting for the
+// interpreter's lock on the engine's thread
+Tensor small_workspace(size_t bytes, const Tensor &like)
+{
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte).requires_grad(false)) : Tensor();
+}
+
 // ... of a forward call that keeps no columns.  What it takes beyond the least it runs with, to hold the columns in, is not
 // kept from call to call, and a call that does not get it runs with the least.
 Tensor forward_workspace(size_t &bytes, const d2c_conv3d_desc &q, const d2c_size_map_desc *sz, const Tensor &like, hipStream_t st)
@@ -598,7 +605,7 @@ struct LayerNormBackward : public Node {
             if (has_w && should_compute_output(1)) r[1] = no_grad_empty_like(vw);
             if (has_b && should_compute_output(2)) r[2] = no_grad_empty_like(vb);
             const size_t nb = r[1].defined() || r[2].defined() ? d2c_layer_norm_backward_workspace_bytes(&q) : 0;
-            const Tensor ws = workspace(nb, vx, st);
+            const Tensor ws = small_workspace(nb, vx);
             check(d2c_layer_norm_backward(&q, ptr(g), ptr(vx), (const float *)ptr(vs), ptr(vw), ptr(r[0]), ptr(r[1]), ptr(r[2]), ptr(ws), nb, st),
                   "layer_norm backward");
         }
@@ -764,7 +771,7 @@ struct CrossAttentionBackward : public Node {
             if (should_compute_output(1)) r[1] = no_grad_empty_like(vk);
             if (should_compute_output(2)) r[2] = no_grad_empty_like(vv);
             const size_t nb = d2c_attention_backward_workspace_bytes(&q);
-            const Tensor ws = workspace(nb, vq, st);
+            const Tensor ws = small_workspace(nb, vq);
             check(d2c_attention_backward(&q, ptr(g), ptr(vq), ptr(vk), ptr(vv), (const int32_t *)ptr(len), (const uint8_t *)ptr(msk), ptr(vo),
                                          (const float *)ptr(vl), ptr(r[0]), ptr(r[1]), ptr(r[2]), ptr(ws), nb, st),
                   "cross_attention backward");
@@ -812,7 +819,7 @@ py::object cross_attention(const Tensor &query, const Tensor &key, const Tensor 
     Tensor out = at::empty(query.sizes(), opt), lse;
     if (grad) lse = at::empty({q.N, q.Hkv, (int64_t)q.Lq * (q.Hq / q.Hkv)}, opt.dtype(at::kFloat));
     const size_t nb = d2c_attention_forward_workspace_bytes(&q);
-    const Tensor ws = workspace(nb, query, st);
+    const Tensor ws = small_workspace(nb, query);
     check(d2c_attention_forward(&q, ptr(query), ptr(key), ptr(value), (const int32_t *)ptr(len), (const uint8_t *)ptr(msk), ptr(out), (float *)ptr(lse),
                                 ptr(ws), nb, st),
           "cross_attention forward");
