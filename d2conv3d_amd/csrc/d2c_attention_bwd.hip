@@ -82,6 +82,9 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
     delta = half_sum(delta);
     const float lse = live ? a.lse[hd.nh * a.rows + row] : INFINITY;
     if (live && unit.split == 0 && half == 0) a.delta[hd.nh * a.rows + row] = delta;
+    f32x16 minus_delta;      // (what the product dp starts from: dp - delta without an instruction)
+#pragma unroll
+    for (int r = 0; r < 16; r++) minus_delta[r] = -delta;
     f32x16 dq[ND];
 #pragma unroll
     for (int i = 0; i < ND; i++)
@@ -106,9 +109,9 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
         if (now == 0) continue;
 #pragma unroll
         for (int i = 0; i < KT / 32; i++) {
-            f32x16 s, dp;
+            f32x16 s, dp = minus_delta;
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
+            for (int r = 0; r < 16; r++) s[r] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < NK; ks++) {
                 mma<P>(s, KV::rows(s_k, i * 32 + (lane & 31), ks, half), q[ks]);
@@ -123,7 +126,7 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
             }
             float ds[16];
 #pragma unroll
-            for (int r = 0; r < 16; r++) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+            for (int r = 0; r < 16; r++) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * dp[r];
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
                 const Frag<P> f = make_frag<P>(ds + kk * 8);
@@ -203,7 +206,7 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
         if (threadIdx.x < 2 * RT) {
             const bool first = threadIdx.x < RT;
             const int r = r0 + (first ? threadIdx.x : threadIdx.x - RT);
-            stat = r < a.rows ? (first ? a.lse : a.delta)[hd.nh * a.rows + r] : (first ? INFINITY : 0.f);
+            stat = r < a.rows ? (first ? a.lse[hd.nh * a.rows + r] : -a.delta[hd.nh * a.rows + r]) : (first ? INFINITY : 0.f);
         }
     };
     if (t < t1) request(t);
@@ -239,9 +242,14 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
         if (t + 1 < t1) request(t + 1);
 #pragma unroll
         for (int i = 0; i < RT / 32; i++) {
-            f32x16 s, dp;
+            f32x16 s, dp;      // (dp starts from -delta of its rows)
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
+            for (int j = 0; j < 4; j++) {
+                const float4 de = *reinterpret_cast<const float4 *>(s_delta + i * 32 + j * 8 + half * 4);
+                dp[j * 4] = de.x; dp[j * 4 + 1] = de.y; dp[j * 4 + 2] = de.z; dp[j * 4 + 3] = de.w;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < NK; ks++) {
                 mma<P>(s, QG::rows(s_q, i * 32 + (lane & 31), ks, half), k[ks]);
@@ -251,12 +259,11 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float4 ls = *reinterpret_cast<const float4 *>(s_lse + i * 32 + j * 8 + half * 4);
-                const float4 de = *reinterpret_cast<const float4 *>(s_delta + i * 32 + j * 8 + half * 4);
-                const float lr[4] = {ls.x, ls.y, ls.z, ls.w}, dr[4] = {de.x, de.y, de.z, de.w};
+                const float lr[4] = {ls.x, ls.y, ls.z, ls.w};
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     p[j * 4 + r] = __builtin_amdgcn_exp2f(fmaf(s[j * 4 + r], c, -lr[r]));
-                    ds[j * 4 + r] = p[j * 4 + r] * (dp[j * 4 + r] - dr[r]);
+                    ds[j * 4 + r] = p[j * 4 + r] * dp[j * 4 + r];
                 }
             }
 #pragma unroll
