@@ -14,11 +14,12 @@ namespace {
 template <typename T, int DP, bool WHOLE> struct QShape {
     static constexpr int KT = sizeof(T) == 2 ? 64 : 32;
     using KV = Tile<T, DP, KT, 256, WHOLE>;
+    static constexpr int WAVES = sizeof(T) == 2 || DP <= 64 ? 2 : 1;      // to a SIMD
     static constexpr int BUFFERS = 4 * KV::BYTES <= 52 << 10 ? 2 : 1;
     static constexpr int LDS = 2 * BUFFERS * KV::BYTES;
 };
 
-template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_bwd_q_kernel(Args a)
+template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, (QShape<T, DP, WHOLE>::WAVES)) attn_bwd_q_kernel(Args a)
 {
     using KV = typename QShape<T, DP, WHOLE>::KV;
     constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, KT = QShape<T, DP, WHOLE>::KT;
@@ -82,9 +83,6 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
     delta = half_sum(delta);
     const float lse = live ? a.lse[hd.nh * a.rows + row] : INFINITY;
     if (live && unit.split == 0 && half == 0) a.delta[hd.nh * a.rows + row] = delta;
-    f32x16 minus_delta;      // (what the product dp starts from: dp - delta without an instruction)
-#pragma unroll
-    for (int r = 0; r < 16; r++) minus_delta[r] = -delta;
     f32x16 dq[ND];
 #pragma unroll
     for (int i = 0; i < ND; i++)
@@ -109,9 +107,9 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
         if (now == 0) continue;
 #pragma unroll
         for (int i = 0; i < KT / 32; i++) {
-            f32x16 s, dp = minus_delta;
+            f32x16 s, dp;
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = 0.f;
+            for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < NK; ks++) {
                 mma<P>(s, KV::rows(s_k, i * 32 + (lane & 31), ks, half), q[ks]);
@@ -126,7 +124,7 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
             }
             float ds[16];
 #pragma unroll
-            for (int r = 0; r < 16; r++) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * dp[r];
+            for (int r = 0; r < 16; r++) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
                 const Frag<P> f = make_frag<P>(ds + kk * 8);
@@ -160,13 +158,18 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
 }
 
 template <typename T, int DP, bool WHOLE> struct KvShape {
+    // V of the workgroup's keys in LDS where registers do not hold it beside the sums
+    static constexpr bool V_LDS = sizeof(T) == 2 && DP == 128;
+    static constexpr int WAVES = sizeof(T) == 2 || DP <= 64 ? 2 : 1;      // to a SIMD
+    using V = Tile<T, DP, 128, 256, WHOLE>;
+    static constexpr int V_BYTES = V_LDS ? V::BYTES : 0;
     static constexpr int RT = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
     using QG = Tile<T, DP, RT, 256, WHOLE>;
-    static constexpr int BYTES = 2 * QG::BYTES + 2 * RT * 4, BUFFERS = 2 * BYTES <= 52 << 10 ? 2 : 1;
-    static constexpr int LDS = BUFFERS * BYTES;
+    static constexpr int BYTES = 2 * QG::BYTES + 2 * RT * 4, BUFFERS = 2 * BYTES <= 52 << 10 && !V_LDS ? 2 : 1;
+    static constexpr int LDS = BUFFERS * BYTES + V_BYTES;
 };
 
-template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_bwd_kv_kernel(Args a)
+template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, (KvShape<T, DP, WHOLE>::WAVES)) attn_bwd_kv_kernel(Args a)
 {
     using QG = typename KvShape<T, DP, WHOLE>::QG;
     constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, RT = KvShape<T, DP, WHOLE>::RT;
@@ -210,7 +213,15 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
         }
     };
     if (t < t1) request(t);
-    Frag<P> k[NK], v[NK];
+    using Shape = KvShape<T, DP, WHOLE>;
+    Frag<P> k[NK], v[Shape::V_LDS ? 1 : NK];
+    unsigned char *s_v = lds + BUFFERS * Shape::BYTES;
+    if constexpr (Shape::V_LDS) {
+        typename Shape::V tile;
+        const T *vb = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2];
+        tile.load(a.D, [&](int i) INLINE { return vb + (long)min(key0 + i, a.Lk - 1) * a.vs[1]; });
+        tile.store(s_v);      // (a key that is not to be read: a column of its own, see below)
+    }
     {
         const long at = min(key, a.Lk - 1);
         const T *kr = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2] + at * a.ks[1];
@@ -219,7 +230,7 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
         for (int i = 0; i < NK; i++) {
             const int d = i * 16 + half * 8;
             k[i] = terms_of<T>(load8_of<WHOLE, T>(kr, d, a.D, live));
-            v[i] = terms_of<T>(load8_of<WHOLE, T>(vr, d, a.D, live));
+            if constexpr (!Shape::V_LDS) v[i] = terms_of<T>(load8_of<WHOLE, T>(vr, d, a.D, live));
         }
     }
     f32x16 dk[ND], dv[ND];
@@ -253,7 +264,8 @@ template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256,
 #pragma unroll
             for (int ks = 0; ks < NK; ks++) {
                 mma<P>(s, QG::rows(s_q, i * 32 + (lane & 31), ks, half), k[ks]);
-                mma<P>(dp, QG::rows(s_g, i * 32 + (lane & 31), ks, half), v[ks]);
+                if constexpr (Shape::V_LDS) mma<P>(dp, QG::rows(s_g, i * 32 + (lane & 31), ks, half), Shape::V::rows(s_v, tile_key, ks, half));
+                else mma<P>(dp, QG::rows(s_g, i * 32 + (lane & 31), ks, half), v[ks]);
             }
             float p[16], ds[16];
 #pragma unroll
