@@ -161,7 +161,7 @@ template <typename T, int DP, bool WHOLE> struct KvShape {
     // V of the workgroup's keys in LDS where registers do not hold it beside the sums
     static constexpr bool V_LDS = sizeof(T) == 2 && DP == 128;
     static constexpr int WAVES = sizeof(T) == 2 || DP <= 64 ? 2 : 1;      // to a SIMD
-    using V = Tile<T, DP, 128, 256, WHOLE>;
+    using V = Tile<T, DP, 128, 256, false>;      // (zeros behind a row's end: the other operand has its last piece again there)
     static constexpr int V_BYTES = V_LDS ? V::BYTES : 0;
     static constexpr int RT = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
     using QG = Tile<T, DP, RT, 256, WHOLE>;

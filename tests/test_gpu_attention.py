@@ -129,6 +129,11 @@ CASES = [
     (1, 40, 3000, 1, 1, 64, "mask"),
     (2, 1500, 40, 2, 1, 64, "lengths"),     # few keys, rows shared by workgroups
     (1, 300, 700, 12, 3, 32, "both"),
+    (2, 70, 150, 2, 1, 104, "lengths"),     # heads that fill the widest kernels in part, in whole pieces of 16 bytes
+    (1, 40, 260, 2, 2, 120, "mask"),
+    (1, 130, 90, 3, 1, 88, "none"),
+    (1, 20, 50, 1, 1, 8, "none"),
+    (1, 50, 140, 2, 1, 16, "none"),
 ]
 
 
