@@ -40,11 +40,11 @@ template <typename T, int DP, int WK, bool WHOLE> struct FwdShape {
 };
 
 // WK: wavefronts that share rows and split the keys of a tile
-template <typename T, int DP, int WK, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(Args a)
+template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(Args a)
 {
     using Shape = FwdShape<T, DP, WK, WHOLE>;
     using KV = typename Shape::KV;
-    constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = (KT + 63) / 64;
+    constexpr int P = kTerms<T>, ND = DP / 32, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = (KT + 63) / 64;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = Shape::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK;
@@ -235,6 +235,205 @@ template <typename T, int DP, int WK, bool WHOLE> __global__ void __launch_bound
     if (a.lse && half == 0) a.lse[hd.nh * a.rows + row] = l == 0.f ? INFINITY : mc + log2f(l);
 }
 
+// One to eight rows (a token, or a few that share a key head): no matrix instructions, whose 32 columns would be empty, but one pass over the memory by
+// lanes.  LANES lanes hold a key's row, 16 bytes each, so that a load of the wavefront takes 64 / LANES whole rows; scores are summed over these lanes, and
+// every group of lanes keeps its own maximum, sum and output of each of the R rows until the end.  No LDS and no barrier on the way, the next keys requested
+// while these are worked on.  Bound: memory, latency where the memory is short.
+template <int LANES, typename Op> D2C_DEV float over_groups(float v, Op op)      // over the lanes that lie a multiple of LANES apart
+{
+    if constexpr (LANES <= 4) v = op(v, dpp_f32<0x124>(v));    // lanes of sixteen, turned by 4
+    if constexpr (LANES <= 8) v = op(v, dpp_f32<0x128>(v));    // ... by 8
+    if constexpr (LANES <= 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    float x, y;
+    other_half(v, x, y);
+    return op(x, y);
+}
+
+// x + the products of two pairs
+D2C_DEV float dot_pair(uint32_t a, uint32_t b, float x)
+{
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, a), __builtin_bit_cast(bf16x2_t, b), x, false);
+}
+// 16 bytes against 16 bytes
+template <typename T> D2C_DEV float dot_words(const uint4 &a, const uint4 &b)
+{
+    if constexpr (sizeof(T) == 2) return dot_pair(a.w, b.w, dot_pair(a.z, b.z, dot_pair(a.y, b.y, dot_pair(a.x, b.x, 0.f))));
+    else return fmaf(__uint_as_float(a.w), __uint_as_float(b.w), fmaf(__uint_as_float(a.z), __uint_as_float(b.z),
+                fmaf(__uint_as_float(a.y), __uint_as_float(b.y), __uint_as_float(a.x) * __uint_as_float(b.x))));
+}
+
+template <typename T, int LANES, int R> struct TokenShape {
+    static constexpr int VEC = 16 / (int)sizeof(T), DP = LANES * VEC, LOADS = R <= 4 ? 4 : 2, KEYS = 64 / LANES, STEP = 4 * LOADS * KEYS;
+};
+
+template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bounds__(256) attn_token_kernel(Args a)
+{
+    using Shape = TokenShape<T, LANES, R>;
+    constexpr int VEC = Shape::VEC, DP = Shape::DP, LOADS = Shape::LOADS, KEYS = Shape::KEYS, STEP = Shape::STEP;
+    __shared__ __align__(16) float s_o[4][R][DP];
+    __shared__ float2 s_ml[4][R];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = lane % LANES * VEC;
+    const Unit unit = unit_of(a);
+    const Head hd = unit.head;
+    const int keys = keys_of(a, hd.n), steps = (keys + STEP - 1) / STEP;
+    const int t1 = (int)((long)steps * (unit.split + 1) / unit.splits);
+    int t = (int)((long)steps * unit.split / unit.splits);
+    const T *kb = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2];
+    const T *vb = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2];
+
+    auto load = [&](const T *row) INLINE {      // this lane's 16 bytes; zeros behind the row's end
+        if constexpr (WHOLE) {
+            const AnyVec<T> v = load_any(row + min(d0, a.D - VEC));
+            return make_uint4(v[0], v[1], v[2], v[3]);
+        } else return d0 < a.D ? load_run<T>(row + d0, a.D - d0) : make_uint4(0, 0, 0, 0);
+    };
+    uint4 k[LOADS], v[LOADS];
+    bool there[LOADS];
+    auto request = [&](int step) INLINE {
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) {
+            const int key = step * STEP + (u * 4 + wave) * KEYS + lane / LANES;
+            const long at = min(key, keys - 1);
+            there[u] = key < keys && (!a.mask || a.mask[(long)hd.n * a.Lk + at]);
+            k[u] = load(kb + at * a.ks[1]);
+            v[u] = load(vb + at * a.vs[1]);
+        }
+    };
+    if (t < t1) request(t);
+    uint4 q[R];
+    float o[R][VEC], m[R], l[R];      // (m: of the scores in units of scale * log2(e))
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const bool live = d0 < a.D && r < a.rows;      // (zeros against what a load behind a row's end repeats)
+        const uint4 w = load(row_at<T>(a.q, a.qs, a, hd, min(r, a.rows - 1)));
+        q[r] = live ? w : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) o[r][i] = 0.f;
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+    }
+    for (; t < t1; t++) {
+        uint4 vw[LOADS];
+        float s[LOADS][R];
+#pragma unroll
+        for (int u = 0; u < LOADS; u++) {
+            vw[u] = there[u] ? v[u] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const float x = lanes_sum<LANES>(dot_words<T>(q[r], k[u])) * a.scale2;
+                s[u][r] = there[u] ? x : -INFINITY;
+            }
+        }
+        if (t + 1 < t1) request(t + 1);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float top = s[0][r];
+#pragma unroll
+            for (int u = 1; u < LOADS; u++) top = fmaxf(top, s[u][r]);
+            // (the maximum follows where it has grown by more than 8, as in attn_fwd_kernel)
+            if (__any(top > m[r] + 8.f)) {
+                const float grown = fmaxf(top, m[r]), f = grown == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[r] - grown);
+                m[r] = grown;
+                l[r] *= f;
+#pragma unroll
+                for (int i = 0; i < VEC; i++) o[r][i] *= f;
+            }
+            const float base = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - base);
+                l[r] += s[u][r];
+            }
+        }
+        if constexpr (sizeof(T) == 2) {      // two keys to an instruction, weights as bfloat16 (as the matrix kernels take them)
+#pragma unroll
+            for (int u = 0; u < LOADS; u += 2) {
+                const uint32_t x[4] = {vw[u].x, vw[u].y, vw[u].z, vw[u].w}, y[4] = {vw[u + 1].x, vw[u + 1].y, vw[u + 1].z, vw[u + 1].w};
+                uint32_t pair[8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    pair[2 * i] = __builtin_amdgcn_perm(y[i], x[i], 0x05040100u);
+                    pair[2 * i + 1] = __builtin_amdgcn_perm(y[i], x[i], 0x07060302u);
+                }
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const uint32_t p = pack_bf16x2(s[u][r], s[u + 1][r]);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) o[r][i] = dot_pair(p, pair[i], o[r][i]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                float vf[VEC];
+                *reinterpret_cast<uint4 *>(vf) = vw[u];
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) o[r][i] = fmaf(s[u][r], vf[i], o[r][i]);
+            }
+        }
+    }
+    // the groups of a wavefront, two values to a step where half the wavefront can go on with either (32 sums of 8 lanes: 56 instructions for 256), then the
+    // wavefronts
+    float x[R * VEC];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const float top = over_groups<LANES>(m[r], [](float x, float y) INLINE { return fmaxf(x, y); });
+        const float f = m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[r] - top);
+        l[r] = over_groups<LANES>(l[r] * f, [](float x, float y) INLINE { return x + y; });
+#pragma unroll
+        for (int i = 0; i < VEC; i++) x[r * VEC + i] = o[r][i] * f;
+        if (lane == 0) s_ml[wave][r] = make_float2(top, l[r]);
+    }
+    constexpr int HALVINGS = LANES <= 16 ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < R * VEC / 2; i++) {
+        const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1]), false, false);
+        x[i] = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+    }
+    if constexpr (HALVINGS == 2) {
+#pragma unroll
+        for (int i = 0; i < R * VEC / 4; i++) {
+            const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1]), false, false);
+            x[i] = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < (R * VEC >> HALVINGS); i++) {
+        if constexpr (LANES <= 4) x[i] += dpp_f32<0x124>(x[i]);
+        if constexpr (LANES <= 8) x[i] += dpp_f32<0x128>(x[i]);
+        const int at = HALVINGS == 2 ? 4 * i + (lane >> 4 & 1) * 2 + (lane >> 5) : 2 * i + (lane >> 5);
+        if (LANES >= 16 || (lane & 15) < LANES) s_o[wave][at / VEC][d0 + at % VEC] = x[i];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(R, a.rows) * DP; i += 256) {
+        const int r = i / DP, d = i - r * DP;
+        if (d >= a.D) continue;
+        float top = s_ml[0][r].x, sum = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 1; w < 4; w++) top = fmaxf(top, s_ml[w][r].x);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = __builtin_amdgcn_exp2f(s_ml[w][r].x - base);
+            sum = fmaf(s_ml[w][r].y, f, sum);
+            x = fmaf(s_o[w][r][d], f, x);
+        }
+        if (unit.splits > 1) {
+            const long at = ((long)unit.split * a.shared + unit.part) * R + r;
+            a.part[at * a.D + d] = x;
+            if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(top, sum);
+        } else {
+            const_cast<T *>(row_at<T>(a.out, a.gs, a, hd, r))[d] = f32_to_elem<T>(sum == 0.f ? 0.f : x / sum);
+            if (a.lse && d == 0) a.lse[hd.nh * a.rows + r] = sum == 0.f ? INFINITY : top + log2f(sum);
+        }
+    }
+}
+
 // The partial results of `splits` workgroups.  LANES lanes take four of a row's columns each, `groups` (a power of two) of them the splits in turn; their sums
 // meet in LDS.  Latency counts: 16 rows of 102 splits 13.6 us as a wavefront each that walks over them, 4.8 as here.
 template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_join_kernel(Args a, int groups, int tile_rows)
@@ -285,37 +484,59 @@ template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_joi
     if (a.lse && lane == 0) a.lse[(long)nh * a.rows + row] = l == 0.f ? INFINITY : top + log2f(l);
 }
 
-// f(DP, WK, WHOLE) as constants
+// f(Width, WK, WHOLE) as constants
 template <typename T, typename F> auto for_shape(int D, bool few, F f)
 {
     constexpr int WK = sizeof(T) == 2 ? 4 : 2;
-    auto pick = [&](auto dp) {
-        constexpr int DP = decltype(dp)::value;
-        using C = std::integral_constant<int, DP>;
-        if (D % 8 == 0) return few ? f(C{}, std::integral_constant<int, WK>{}, std::true_type{}) : f(C{}, std::integral_constant<int, 1>{}, std::true_type{});
-        return few ? f(C{}, std::integral_constant<int, WK>{}, std::false_type{}) : f(C{}, std::integral_constant<int, 1>{}, std::false_type{});
-    };
-    if (D <= 32) return pick(std::integral_constant<int, 32>{});
-    if (D <= 64) return pick(std::integral_constant<int, 64>{});
-    if (D <= 96) return pick(std::integral_constant<int, 96>{});
-    return pick(std::integral_constant<int, 128>{});
+    return for_width<T>(D, [&](auto width, auto whole) {
+        return few ? f(width, std::integral_constant<int, WK>{}, whole) : f(width, std::integral_constant<int, 1>{}, whole);
+    });
 }
 
-// What a call runs on: 32 rows or fewer are shared by the wavefronts of a workgroup, which split the keys of a tile (WK > 1)
-struct FwdPlan { bool few; int tile_rows; Walks walks; size_t part_bytes, bytes; };
+// f(LANES, R, WHOLE) of attn_token_kernel as constants
+template <typename T, typename F> auto for_token(int D, long rows, F f)
+{
+    auto with_rows = [&](auto lanes, auto whole) {
+        if (rows <= 1) return f(lanes, std::integral_constant<int, 1>{}, whole);
+        if (rows <= 2) return f(lanes, std::integral_constant<int, 2>{}, whole);
+        if (rows <= 4) return f(lanes, std::integral_constant<int, 4>{}, whole);
+        return f(lanes, std::integral_constant<int, 8>{}, whole);
+    };
+    auto pick = [&](auto lanes) { return D % 8 == 0 ? with_rows(lanes, std::true_type{}) : with_rows(lanes, std::false_type{}); };
+    constexpr int L32 = 32 * (int)sizeof(T) / 16;
+    if (D <= 32) return pick(std::integral_constant<int, L32>{});
+    if (D <= 64) return pick(std::integral_constant<int, 2 * L32>{});
+    return pick(std::integral_constant<int, 4 * L32>{});
+}
+
+// What a call runs on: up to 8 rows on attn_token_kernel; up to 32 are shared by the wavefronts of a workgroup, which split the keys of a tile (WK > 1)
+struct FwdPlan { bool token, few; int tile_rows; Walks walks; size_t part_bytes, bytes; };
 template <typename T> FwdPlan fwd_plan(const d2c_attention_desc &q)
 {
     FwdPlan p;
     const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv;
+    p.token = rows <= 8;
     p.few = rows <= 32;
-    for_shape<T>(q.D, p.few, [&](auto dp, auto wk, auto whole) {
-        using Shape = FwdShape<T, decltype(dp)::value, decltype(wk)::value, decltype(whole)::value>;
+    if (p.token) for_token<T>(q.D, rows, [&](auto lanes, auto r, auto whole) {
+        constexpr int LANES = decltype(lanes)::value, R = decltype(r)::value;
+        constexpr bool WHOLE = decltype(whole)::value;
+        using Shape = TokenShape<T, LANES, R>;
+        p.tile_rows = R;
+        const long places = 2L * std::max(d2c_num_cus(), 1);
+        // (a step's bytes, from every place, at 5 TB/s)
+        p.walks = plan_walks(heads, (q.Lk + Shape::STEP - 1) / Shape::STEP, places, 2.0 * Shape::STEP * q.D * sizeof(T) * places / 5e6, (double)R * q.D * 4);
+        return 0;
+    });
+    else for_shape<T>(q.D, p.few, [&](auto width, auto wk, auto whole) {
+        constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK, WK = decltype(wk)::value;
+        constexpr bool WHOLE = decltype(whole)::value;
+        using Shape = FwdShape<T, DP, WK, WHOLE>;
         p.tile_rows = Shape::ROWS;
         const long units = heads * ((rows + Shape::ROWS - 1) / Shape::ROWS), steps = (q.Lk + Shape::KT - 1) / Shape::KT;
         const long places = (long)std::max(d2c_num_cus(), 1) *
-            resident(reinterpret_cast<const void *>(&attn_fwd_kernel<T, decltype(dp)::value, decltype(wk)::value, decltype(whole)::value>), Shape::LDS);
+            resident(reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, NK, WK, WHOLE>), Shape::LDS);
         // (a step: 64 keys of 64 channels take 2 us with every place taken, float32's six products three times as long)
-        p.walks = plan_walks(units, steps, places, 2.0 * Shape::KT / 64 * dp / 64 * (sizeof(T) == 2 ? 1 : 3) / decltype(wk)::value, (double)Shape::ROWS * q.D * 4);
+        p.walks = plan_walks(units, steps, places, 2.0 * Shape::KT / 64 * DP / 64 * (sizeof(T) == 2 ? 1 : 3) / WK, (double)Shape::ROWS * q.D * 4);
         return 0;
     });
     const size_t lines = (size_t)p.walks.splits * p.walks.shared * p.tile_rows;
@@ -334,12 +555,15 @@ template <typename T, int LANES> int launch_join(const Args &a, int tile_rows, h
 }
 template <typename T> int launch_fwd(const Args &a, const FwdPlan &p, hipStream_t st)
 {
-    const int rc = for_shape<T>(a.D, p.few, [&](auto dp, auto wk, auto whole) {
-        constexpr int DP = decltype(dp)::value, WK = decltype(wk)::value;
+    const int rc = p.token ? for_token<T>(a.D, a.rows, [&](auto lanes, auto r, auto whole) {
+        hipLaunchKernelGGL((attn_token_kernel<T, decltype(lanes)::value, decltype(r)::value, decltype(whole)::value>), dim3(workgroups(p.walks)), dim3(256), 0, st, a);
+        return d2c_check_launch("attn_token_kernel");
+    }) : for_shape<T>(a.D, p.few, [&](auto width, auto wk, auto whole) {
+        constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK, WK = decltype(wk)::value;
         constexpr bool WHOLE = decltype(whole)::value;
         constexpr int lds = FwdShape<T, DP, WK, WHOLE>::LDS;
-        if (int e = d2c_allow_lds(reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, WK, WHOLE>), lds, "attn_fwd_kernel")) return e;
-        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, WK, WHOLE>), dim3(workgroups(p.walks)), dim3(256), lds, st, a);
+        if (int e = d2c_allow_lds(reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, NK, WK, WHOLE>), lds, "attn_fwd_kernel")) return e;
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NK, WK, WHOLE>), dim3(workgroups(p.walks)), dim3(256), lds, st, a);
         return d2c_check_launch("attn_fwd_kernel");
     });
     if (rc || p.walks.shared == 0) return rc;

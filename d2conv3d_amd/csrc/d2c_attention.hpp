@@ -16,6 +16,7 @@
 // The rows of a group of query heads that share a key head are one axis: row = position * group + head in group.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 #include "d2c_common.hpp"
 #include "d2c_mma.hpp"
 
@@ -209,6 +210,25 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
         return f;
     }
 };
+
+// Widths that kernels are made for: channels of a tile, a multiple of 32 (the products' columns), and steps of 16 of the products over channels.
+// float32, whose steps are six instructions each, leaves out a last one that heads do not reach (1417 on 3001 positions of 6 heads of 40 channels: the three
+// kernels 210, 181 us).
+template <int DP_, int NK_> struct Width { static constexpr int DP = DP_, NK = NK_; };
+template <typename T, typename F> auto for_width(int D, F f)      // f(Width, whether D is a multiple of 8)
+{
+    auto pick = [&](auto width) {
+        using W = decltype(width);
+        if (D % 8 != 0) return f(width, std::false_type{});
+        if constexpr (sizeof(T) == 4)
+            if (D <= W::DP - 16) return f(Width<W::DP, W::NK - 1>{}, std::true_type{});
+        return f(width, std::true_type{});
+    };
+    if (D <= 32) return pick(Width<32, 2>{});
+    if (D <= 64) return pick(Width<64, 4>{});
+    if (D <= 96) return pick(Width<96, 6>{});
+    return pick(Width<128, 8>{});
+}
 
 // What the workgroups do: units, each the walk of one tile of rows (or keys) of one key head along the other axis.  As many as
 // fill the GPU's places without a remainder are walked by a workgroup each (`whole`); `splits` workgroups share each of the `shared` others, so that the

@@ -19,10 +19,10 @@ template <typename T, int DP, bool WHOLE> struct QShape {
     static constexpr int LDS = 2 * BUFFERS * KV::BYTES;
 };
 
-template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, (QShape<T, DP, WHOLE>::WAVES)) attn_bwd_q_kernel(Args a)
+template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bounds__(256, (QShape<T, DP, WHOLE>::WAVES)) attn_bwd_q_kernel(Args a)
 {
     using KV = typename QShape<T, DP, WHOLE>::KV;
-    constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, KT = QShape<T, DP, WHOLE>::KT;
+    constexpr int P = kTerms<T>, ND = DP / 32, KT = QShape<T, DP, WHOLE>::KT;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = QShape<T, DP, WHOLE>::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -169,10 +169,10 @@ template <typename T, int DP, bool WHOLE> struct KvShape {
     static constexpr int LDS = BUFFERS * BYTES + V_BYTES;
 };
 
-template <typename T, int DP, bool WHOLE> __global__ void __launch_bounds__(256, (KvShape<T, DP, WHOLE>::WAVES)) attn_bwd_kv_kernel(Args a)
+template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bounds__(256, (KvShape<T, DP, WHOLE>::WAVES)) attn_bwd_kv_kernel(Args a)
 {
     using QG = typename KvShape<T, DP, WHOLE>::QG;
-    constexpr int P = kTerms<T>, NK = DP / 16, ND = DP / 32, RT = KvShape<T, DP, WHOLE>::RT;
+    constexpr int P = kTerms<T>, ND = DP / 32, RT = KvShape<T, DP, WHOLE>::RT;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = KvShape<T, DP, WHOLE>::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -347,32 +347,22 @@ template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(A
     if (lane == 0) a.delta[at] = x;
 }
 
-// f(DP, WHOLE) as constants
-template <typename F> auto for_shape(int D, F f)
-{
-    auto pick = [&](auto dp) { return D % 8 == 0 ? f(dp, std::true_type{}) : f(dp, std::false_type{}); };
-    if (D <= 32) return pick(std::integral_constant<int, 32>{});
-    if (D <= 64) return pick(std::integral_constant<int, 64>{});
-    if (D <= 96) return pick(std::integral_constant<int, 96>{});
-    return pick(std::integral_constant<int, 128>{});
-}
-
 struct BwdPlan { Walks q, kv; size_t delta_bytes, bytes; };
 template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
 {
     BwdPlan p;
     const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv, cus = std::max(d2c_num_cus(), 1);
     const double part = 128.0 * q.D * 4, slow = sizeof(T) == 2 ? 1 : 3;
-    for_shape(q.D, [&](auto dp, auto whole) {
-        constexpr int DP = decltype(dp)::value;
+    for_width<T>(q.D, [&](auto width, auto whole) {
+        constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK;
         constexpr bool WHOLE = decltype(whole)::value;
         using Q = QShape<T, DP, WHOLE>;
         using KV = KvShape<T, DP, WHOLE>;
         // (a step with every place taken, 64 channels: 64 keys 2.4 us, 64 rows 2.8)
         p.q = plan_walks(heads * ((rows + 127) / 128), (q.Lk + Q::KT - 1) / Q::KT,
-                         cus * resident(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, WHOLE>), Q::LDS), 2.4 * Q::KT / 64 * DP / 64 * slow, part);
+                         cus * resident(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, NK, WHOLE>), Q::LDS), 2.4 * Q::KT / 64 * DP / 64 * slow, part);
         p.kv = plan_walks(heads * ((q.Lk + 127) / 128), (rows + KV::RT - 1) / KV::RT,
-                          cus * resident(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, WHOLE>), KV::LDS), 2.8 * KV::RT / 64 * DP / 64 * slow, 2 * part);
+                          cus * resident(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, NK, WHOLE>), KV::LDS), 2.8 * KV::RT / 64 * DP / 64 * slow, 2 * part);
         return 0;
     });
     p.delta_bytes = d2c_align_up((size_t)heads * rows * 4);
@@ -381,16 +371,16 @@ template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
     return p;
 }
 
-template <typename T, int DP, bool WHOLE> int launch_bwd(Args a, const BwdPlan &p, hipStream_t st)
+template <typename T, int DP, int NK, bool WHOLE> int launch_bwd(Args a, const BwdPlan &p, hipStream_t st)
 {
     if (a.Lq > 0 && !a.gq && (a.gk || a.gv)) {
         hipLaunchKernelGGL(attn_delta_kernel<T>, dim3((unsigned)(((long)a.N * a.Hkv * a.rows + 3) / 4)), dim3(256), 0, st, a);
         if (int rc = d2c_check_launch("attn_delta_kernel")) return rc;
     } else if (a.Lq > 0 && a.gq) {
         constexpr int lds = QShape<T, DP, WHOLE>::LDS;
-        if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, WHOLE>), lds, "attn_bwd_q_kernel")) return rc;
+        if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, NK, WHOLE>), lds, "attn_bwd_q_kernel")) return rc;
         set_walks(a, p.q);
-        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, WHOLE>), dim3(workgroups(p.q)), dim3(256), lds, st, a);
+        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NK, WHOLE>), dim3(workgroups(p.q)), dim3(256), lds, st, a);
         if (int rc = d2c_check_launch("attn_bwd_q_kernel")) return rc;
         if (p.q.shared > 0) {
             hipLaunchKernelGGL((attn_bwd_join_kernel<T, false>), dim3((unsigned)(((long)p.q.shared * 128 * a.D + 255) / 256)), dim3(256), 0, st, a);
@@ -399,9 +389,9 @@ template <typename T, int DP, bool WHOLE> int launch_bwd(Args a, const BwdPlan &
     }
     if (a.Lk == 0 || !(a.gk || a.gv)) return D2C_OK;
     constexpr int lds = KvShape<T, DP, WHOLE>::LDS;
-    if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, WHOLE>), lds, "attn_bwd_kv_kernel")) return rc;
+    if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, NK, WHOLE>), lds, "attn_bwd_kv_kernel")) return rc;
     set_walks(a, p.kv);
-    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, WHOLE>), dim3(workgroups(p.kv)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, NK, WHOLE>), dim3(workgroups(p.kv)), dim3(256), lds, st, a);
     if (int rc = d2c_check_launch("attn_bwd_kv_kernel")) return rc;
     if (p.kv.shared == 0) return D2C_OK;
     hipLaunchKernelGGL((attn_bwd_join_kernel<T, true>), dim3((unsigned)(((long)p.kv.shared * 128 * a.D + 255) / 256), 2), dim3(256), 0, st, a);
@@ -415,7 +405,7 @@ template <typename T> int backward(Args a, const d2c_attention_desc &q, void *ws
         return D2C_ERR_WORKSPACE;
     }
     a.delta = (float *)ws; a.part = (float *)((char *)ws + p.delta_bytes);
-    return for_shape(a.D, [&](auto dp, auto whole) { return launch_bwd<T, decltype(dp)::value, decltype(whole)::value>(a, p, st); });
+    return for_width<T>(a.D, [&](auto width, auto whole) { return launch_bwd<T, decltype(width)::DP, decltype(width)::NK, decltype(whole)::value>(a, p, st); });
 }
 
 }  // namespace

@@ -26,23 +26,47 @@ struct LnArgs {
     float eps;
 };
 
-// VEC values from p on, `left` of them there
-template <typename T, int VEC> D2C_DEV void load_vals(const T *p, int left, float *v)
+// A lane's vectors of a row: NV pieces of 16 bytes, LANES pieces apart, zeros behind the row's end
+template <typename T, int LANES, int NV> struct RowPart {
+    static constexpr int VEC = 16 / (int)sizeof(T);
+    uint4 v[NV];
+    D2C_DEV void load(const T *row, int lane, int C)
+    {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * LANES + lane) * VEC;
+            v[i] = c < C ? load_run<T>(row + c, C - c) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    D2C_DEV void floats(int i, float *f) const
+    {
+        alignas(16) T e[VEC];
+        *reinterpret_cast<uint4 *>(e) = v[i];
+#pragma unroll
+        for (int j = 0; j < VEC; j++) f[j] = elem_to_f32<T>(e[j]);
+    }
+};
+// VEC parameters from channel c on (NULL: `none`)
+template <typename TP, int VEC> D2C_DEV void load_params(const void *p, int c, int C, float none, float *f)
 {
-    constexpr int E = 16 / (int)sizeof(T);
+    constexpr int E = 16 / (int)sizeof(TP);
 #pragma unroll
     for (int i = 0; i < VEC; i += E) {
-        alignas(16) T e[E];
-        *reinterpret_cast<uint4 *>(e) = left > i ? load_run<T>(p + i, left - i) : make_uint4(0, 0, 0, 0);
+        alignas(16) TP e[E];
+        if (p && c + i < C) *reinterpret_cast<uint4 *>(e) = load_run<TP>(reinterpret_cast<const TP *>(p) + c + i, C - c - i);
+        else {
 #pragma unroll
-        for (int j = 0; j < E && i + j < VEC; j++) v[i + j] = elem_to_f32<T>(e[j]);
+            for (int j = 0; j < E; j++) e[j] = f32_to_elem<TP>(none);
+        }
+#pragma unroll
+        for (int j = 0; j < E; j++) f[i + j] = elem_to_f32<TP>(e[j]);
     }
 }
+
 // Sum over the LANES lanes of a row
 template <int LANES> D2C_DEV float row_sum(float v, float *red)
 {
-#pragma unroll
-    for (int d = (LANES < 64 ? LANES : 64) / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+    v = lanes_sum<LANES < 64 ? LANES : 64>(v);
     if constexpr (LANES > 64) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -52,21 +76,36 @@ template <int LANES> D2C_DEV float row_sum(float v, float *red)
     return v;
 }
 
+// Rows are requested one ahead, and parameters stay in registers where they are few: what a wavefront has in flight while it sums bounds it (a row at a
+// time, sums by shuffles, parameters read for each row, and so; us, bfloat16: 207360 rows of 256 52, 40.6 forward (5.2 TB/s), 61, 57 backward (5.6); 25920 of
+// 512 15.4, 14.8 and 19.5, 18.0).
 template <typename T, typename TP, int LANES, int NV> __global__ void __launch_bounds__(kLnThreads) ln_fwd_kernel(LnArgs a)
 {
     constexpr int VEC = 16 / (int)sizeof(T), PER = kLnThreads / LANES;
+    constexpr bool KEEP = NV * VEC <= 16;
     __shared__ float red[4];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const float C = (float)a.C;
-    for (long r0 = (long)blockIdx.x * PER; r0 < a.rows; r0 += (long)gridDim.x * PER) {
-        const long row = r0 + sub;
-        const bool live = row < a.rows;
-        const T *x = reinterpret_cast<const T *>(a.x) + (live ? row : 0) * a.xs;
+    const long step = (long)gridDim.x * PER;
+    const T *xb = reinterpret_cast<const T *>(a.x);
+    float w[KEEP ? NV : 1][VEC], b[KEEP ? NV : 1][VEC];
+    RowPart<T, LANES, NV> next;
+    long row = (long)blockIdx.x * PER + sub;
+    next.load(xb + min(row, a.rows - 1) * a.xs, lane, a.C);
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            load_params<TP, VEC>(a.w, (i * LANES + lane) * VEC, a.C, 1.f, w[i]);
+            load_params<TP, VEC>(a.b, (i * LANES + lane) * VEC, a.C, 0.f, b[i]);
+        }
+    }
+    for (; row - sub < a.rows; row += step) {
+        const RowPart<T, LANES, NV> now = next;
+        if (row - sub + step < a.rows) next.load(xb + min(row + step, a.rows - 1) * a.xs, lane, a.C);
         float v[NV][VEC], s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int c = (i * LANES + lane) * VEC;
-            load_vals<T, VEC>(x + c, live ? a.C - c : 0, v[i]);
+            now.floats(i, v[i]);
 #pragma unroll
             for (int j = 0; j < VEC; j++) s += v[i][j];
         }
@@ -82,20 +121,19 @@ template <typename T, typename TP, int LANES, int NV> __global__ void __launch_b
             }
         }
         const float rstd = 1.f / sqrtf(row_sum<LANES>(q, red) / C + a.eps);
-        if (!live) continue;
+        if (row >= a.rows) continue;
         T *y = reinterpret_cast<T *>(a.y) + row * a.C;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * LANES + lane) * VEC;
             if (c >= a.C) continue;
-            float w[VEC], b[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; j++) { w[j] = 1.f; b[j] = 0.f; }
-            if (a.w) load_vals<TP, VEC>(reinterpret_cast<const TP *>(a.w) + c, a.C - c, w);
-            if (a.b) load_vals<TP, VEC>(reinterpret_cast<const TP *>(a.b) + c, a.C - c, b);
+            if constexpr (!KEEP) {
+                load_params<TP, VEC>(a.w, c, a.C, 1.f, w[0]);
+                load_params<TP, VEC>(a.b, c, a.C, 0.f, b[0]);
+            }
             alignas(16) T e[VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; j++) e[j] = f32_to_elem<T>(fmaf(v[i][j] * rstd, w[j], b[j]));
+            for (int j = 0; j < VEC; j++) e[j] = f32_to_elem<T>(fmaf(v[i][j] * rstd, w[KEEP ? i : 0][j], b[KEEP ? i : 0][j]));
             store_run<T>(y + c, *reinterpret_cast<const uint4 *>(e), a.C - c);
         }
         if (a.stats && lane == 0) *reinterpret_cast<float2 *>(a.stats + row * 2) = make_float2(mean, rstd);
@@ -105,37 +143,49 @@ template <typename T, typename TP, int LANES, int NV> __global__ void __launch_b
 template <typename T, typename TP, int LANES, int NV> __global__ void __launch_bounds__(kLnThreads) ln_bwd_kernel(LnArgs a)
 {
     constexpr int VEC = 16 / (int)sizeof(T), PER = kLnThreads / LANES;
+    constexpr bool KEEP = NV * VEC <= 16;
     __shared__ float red[4];
     extern __shared__ float s_part[];      // [PER][C], where PER > 1
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const float inv = 1.f / (float)a.C;
-    float gw[NV][VEC], gb[NV][VEC];
+    const long step = (long)gridDim.x * PER;
+    const T *xb = reinterpret_cast<const T *>(a.x), *gyb = reinterpret_cast<const T *>(a.gy);
+    float gw[NV][VEC], gb[NV][VEC], w[KEEP ? NV : 1][VEC];
 #pragma unroll
-    for (int i = 0; i < NV; i++)
+    for (int i = 0; i < NV; i++) {
 #pragma unroll
         for (int j = 0; j < VEC; j++) gw[i][j] = gb[i][j] = 0.f;
-    for (long r0 = (long)blockIdx.x * PER; r0 < a.rows; r0 += (long)gridDim.x * PER) {
-        const long row = r0 + sub;
+        if constexpr (KEEP) load_params<TP, VEC>(a.w, (i * LANES + lane) * VEC, a.C, 1.f, w[i]);
+    }
+    RowPart<T, LANES, NV> nx, ng;
+    float2 nst = make_float2(0.f, 0.f);
+    auto request = [&](long row) INLINE {      // (rows behind the last repeat it: not added up, not stored)
+        const long at = min(row, a.rows - 1);
+        nx.load(xb + at * a.xs, lane, a.C);
+        ng.load(gyb + at * a.C, lane, a.C);
+        nst = *reinterpret_cast<const float2 *>(a.stats + at * 2);
+    };
+    long row = (long)blockIdx.x * PER + sub;
+    if (row - sub < a.rows) request(row);
+    for (; row - sub < a.rows; row += step) {
+        const RowPart<T, LANES, NV> x = nx, g = ng;
+        const float2 st = nst;
         const bool live = row < a.rows;
-        const T *x = reinterpret_cast<const T *>(a.x) + (live ? row : 0) * a.xs, *g = reinterpret_cast<const T *>(a.gy) + (live ? row : 0) * a.C;
-        float2 st = make_float2(0.f, 0.f);
-        if (live) st = *reinterpret_cast<const float2 *>(a.stats + row * 2);
+        if (row - sub + step < a.rows) request(row + step);
         float h[NV][VEC], t[NV][VEC], A = 0.f, B = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int c = (i * LANES + lane) * VEC, left = live ? a.C - c : 0;
-            load_vals<T, VEC>(x + c, left, h[i]);
-            load_vals<T, VEC>(g + c, left, t[i]);
-            float w[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; j++) w[j] = 1.f;
-            if (a.w) load_vals<TP, VEC>(reinterpret_cast<const TP *>(a.w) + c, a.C - c, w);
+            const int c = (i * LANES + lane) * VEC;
+            x.floats(i, h[i]);
+            g.floats(i, t[i]);
+            if constexpr (!KEEP) load_params<TP, VEC>(a.w, c, a.C, 1.f, w[0]);
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
                 h[i][j] = (h[i][j] - st.x) * st.y;
+                if (!live) t[i][j] = 0.f;
                 gw[i][j] = fmaf(t[i][j], h[i][j], gw[i][j]);
                 gb[i][j] += t[i][j];
-                t[i][j] *= w[j];
+                t[i][j] *= w[KEEP ? i : 0][j];
                 A += t[i][j];
                 B = fmaf(t[i][j], h[i][j], B);
             }
@@ -246,7 +296,7 @@ int blocks_of(const d2c_layer_norm_desc &q, const LnShape &s, int per_cu)
     const long per = kLnThreads / s.lanes;
     return (int)std::max(1L, std::min((q.rows + per - 1) / per, (long)per_cu * std::max(d2c_num_cus(), 1)));
 }
-constexpr int kFwdPerCu = 16, kBwdPerCu = 4;
+constexpr int kFwdPerCu = 16, kBwdPerCu = 4;      // (8 and 16: 43.8, 40.6 us forward on 207360 rows of 256; 2, 4, 8: 66, 57, 61 us backward)
 
 template <bool BWD, typename T, typename TP, int LANES, int NV> int launch_shape(const LnArgs &a, hipStream_t st)
 {

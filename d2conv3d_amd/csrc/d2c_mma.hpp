@@ -225,6 +225,25 @@ template <> struct VecAcc<float> {
     D2C_DEV uint4 pack() const { return operand_vec<float, kF32SplitFwd>(a); }
 };
 
+// The sum over LANES (4 .. 64, a power of two) adjacent lanes, in all of them: no LDS (a shuffle is an LDS access and its latency)
+template <int CTRL> D2C_DEV float dpp_f32(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)); }
+template <int LANES> D2C_DEV float lanes_sum(float v)
+{
+    v += dpp_f32<0xb1>(v);                                 // lanes 1 0 3 2 of four
+    v += dpp_f32<0x4e>(v);                                 // lanes 2 3 0 1
+    if constexpr (LANES >= 8) v += dpp_f32<0x141>(v);      // eight, backwards
+    if constexpr (LANES >= 16) v += dpp_f32<0x140>(v);     // sixteen, backwards
+    if constexpr (LANES >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (LANES >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
 template <typename T> D2C_DEV float elem_to_f32(T v);
 template <> D2C_DEV float elem_to_f32<bf16_t>(bf16_t v) { return bf16_to_f32(v); }
 template <> D2C_DEV float elem_to_f32<float>(float v) { return v; }

@@ -134,6 +134,13 @@ CASES = [
     (1, 130, 90, 3, 1, 88, "none"),
     (1, 20, 50, 1, 1, 8, "none"),
     (1, 50, 140, 2, 1, 16, "none"),
+    (2, 1, 700, 8, 1, 64, "both"),          # up to 8 rows of a key head: one, two, four, eight, some not there
+    (1, 2, 333, 4, 1, 40, "mask"),
+    (3, 1, 1300, 6, 2, 96, "lengths"),
+    (1, 1, 900, 1, 1, 7, "mask"),
+    (1, 4, 257, 2, 1, 33, "none"),
+    (2, 2, 64, 1, 1, 128, "lengths"),
+    (1, 5, 2000, 1, 1, 24, "mask"),
 ]
 
 
