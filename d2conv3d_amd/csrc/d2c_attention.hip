@@ -44,7 +44,7 @@ template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __laun
 {
     using Shape = FwdShape<T, DP, WK, WHOLE>;
     using KV = typename Shape::KV;
-    constexpr int P = kTerms<T>, ND = DP / 32, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = (KT + 63) / 64;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = (KT + 63) / 64;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = Shape::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK;
@@ -55,27 +55,11 @@ template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __laun
     const int t1 = (int)((long)tiles * (unit.split + 1) / unit.splits);
     int t = (int)((long)tiles * unit.split / unit.splits);
 
-    const T *kb = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2];
-    const T *vb = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2];
     KV k, v;
-    unsigned koff[KV::PER], voff[KV::PER];
-    k.places(koff, a.D, [&](int i) INLINE { return i * a.ks[1]; });
-    v.places(voff, a.D, [&](int i) INLINE { return i * a.vs[1]; });
+    const KeyTiles<T, KV, KT, WORDS, WHOLE> source(a, hd);
     KeyBits<WORDS> bits;
     uint64_t next[WORDS];
-    auto request = [&](int tile) INLINE {
-        const int any = any_key(next);
-        if (any < 0) return;
-        const T *kt = kb + (long)tile * KT * a.ks[1], *vt = vb + (long)tile * KT * a.vs[1];
-        if constexpr (WHOLE)
-            if ((a.near & 1) && all_keys<KT>(next)) {
-                k.load_near(kt, koff);
-                v.load_near(vt, voff);
-                return;
-            }
-        k.load(a.D, [&](int i) INLINE { return kt + key_to_load(next, i, any) * a.ks[1]; });
-        v.load(a.D, [&](int i) INLINE { return vt + key_to_load(next, i, any) * a.vs[1]; });
-    };
+    auto request = [&](int tile) INLINE { source.request(a, k, v, tile, next); };
     if (t < t1) {
         bits.request(a, hd.n, keys, t * KT);
         bits.words(next);
@@ -124,7 +108,7 @@ template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __laun
 #pragma unroll
             for (int r = 0; r < 16; r++) s[i][r] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < NK; ks++) mma<P>(s[i], KV::rows(s_k, wk * KW + i * 32 + (lane & 31), ks, half), q[ks]);
+            for (int ks = 0; ks < NK; ks++) mma(s[i], KV::rows(s_k, wk * KW + i * 32 + (lane & 31), ks, half), q[ks]);
             const uint32_t there = (uint32_t)(mine >> (i * 32));
             if (there != 0xffffffffu) {
                 const uint32_t b = there >> (half * 4);
@@ -164,9 +148,9 @@ template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __laun
             }
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
-                const Frag<P> pf = make_frag<P>(p + kk * 8);
+                const Frag<PW> pf = make_frag<PW>(p + kk * 8);
 #pragma unroll
-                for (int d = 0; d < ND; d++) mma<P>(o[d], KV::columns(s_v, wk * KW + i * 32 + kk * 16, d * 32, lane), pf);
+                for (int d = 0; d < ND; d++) mma(o[d], KV::columns(s_v, wk * KW + i * 32 + kk * 16, d * 32, lane), pf);
             }
         }
     }
@@ -348,7 +332,7 @@ template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bou
                 l[r] += s[u][r];
             }
         }
-        if constexpr (sizeof(T) == 2) {      // two keys to an instruction, weights as bfloat16 (as the matrix kernels take them)
+        if constexpr (sizeof(T) == 2 && WHOLE) {      // two keys to an instruction, weights as bfloat16 (as the matrix kernels take them)
 #pragma unroll
             for (int u = 0; u < LOADS; u += 2) {
                 const uint32_t x[4] = {vw[u].x, vw[u].y, vw[u].z, vw[u].w}, y[4] = {vw[u + 1].x, vw[u + 1].y, vw[u + 1].z, vw[u + 1].w};
@@ -368,8 +352,11 @@ template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bou
         } else {
 #pragma unroll
             for (int u = 0; u < LOADS; u++) {
+                alignas(16) T e[VEC];
                 float vf[VEC];
-                *reinterpret_cast<uint4 *>(vf) = vw[u];
+                *reinterpret_cast<uint4 *>(e) = vw[u];
+#pragma unroll
+                for (int i = 0; i < VEC; i++) vf[i] = elem_to_f32<T>(e[i]);
 #pragma unroll
                 for (int r = 0; r < R; r++)
 #pragma unroll
@@ -485,24 +472,25 @@ template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_joi
 }
 
 // f(Width, WK, WHOLE) as constants
-template <typename T, typename F> auto for_shape(int D, bool few, F f)
+template <typename T, typename F> auto for_shape(const d2c_attention_desc &q, bool few, F f)
 {
     constexpr int WK = sizeof(T) == 2 ? 4 : 2;
-    return for_width<T>(D, [&](auto width, auto whole) {
+    return for_width<T>(q, [&](auto width, auto whole) {
         return few ? f(width, std::integral_constant<int, WK>{}, whole) : f(width, std::integral_constant<int, 1>{}, whole);
     });
 }
 
 // f(LANES, R, WHOLE) of attn_token_kernel as constants
-template <typename T, typename F> auto for_token(int D, long rows, F f)
+template <typename T, typename F> auto for_token(const d2c_attention_desc &q, long rows, F f)
 {
+    const int D = q.D;
     auto with_rows = [&](auto lanes, auto whole) {
         if (rows <= 1) return f(lanes, std::integral_constant<int, 1>{}, whole);
         if (rows <= 2) return f(lanes, std::integral_constant<int, 2>{}, whole);
         if (rows <= 4) return f(lanes, std::integral_constant<int, 4>{}, whole);
         return f(lanes, std::integral_constant<int, 8>{}, whole);
     };
-    auto pick = [&](auto lanes) { return D % 8 == 0 ? with_rows(lanes, std::true_type{}) : with_rows(lanes, std::false_type{}); };
+    auto pick = [&](auto lanes) { return fast_kernels(q) ? with_rows(lanes, std::true_type{}) : with_rows(lanes, std::false_type{}); };
     constexpr int L32 = 32 * (int)sizeof(T) / 16;
     if (D <= 32) return pick(std::integral_constant<int, L32>{});
     if (D <= 64) return pick(std::integral_constant<int, 2 * L32>{});
@@ -517,7 +505,7 @@ template <typename T> FwdPlan fwd_plan(const d2c_attention_desc &q)
     const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv;
     p.token = rows <= 8;
     p.few = rows <= 32;
-    if (p.token) for_token<T>(q.D, rows, [&](auto lanes, auto r, auto whole) {
+    if (p.token) for_token<T>(q, rows, [&](auto lanes, auto r, auto whole) {
         constexpr int LANES = decltype(lanes)::value, R = decltype(r)::value;
         constexpr bool WHOLE = decltype(whole)::value;
         using Shape = TokenShape<T, LANES, R>;
@@ -527,7 +515,7 @@ template <typename T> FwdPlan fwd_plan(const d2c_attention_desc &q)
         p.walks = plan_walks(heads, (q.Lk + Shape::STEP - 1) / Shape::STEP, places, 2.0 * Shape::STEP * q.D * sizeof(T) * places / 5e6, (double)R * q.D * 4);
         return 0;
     });
-    else for_shape<T>(q.D, p.few, [&](auto width, auto wk, auto whole) {
+    else for_shape<T>(q, p.few, [&](auto width, auto wk, auto whole) {
         constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK, WK = decltype(wk)::value;
         constexpr bool WHOLE = decltype(whole)::value;
         using Shape = FwdShape<T, DP, WK, WHOLE>;
@@ -553,12 +541,12 @@ template <typename T, int LANES> int launch_join(const Args &a, int tile_rows, h
     hipLaunchKernelGGL((attn_join_kernel<T, LANES>), dim3((unsigned)((total + per - 1) / per)), dim3(256), 0, st, a, groups, tile_rows);
     return d2c_check_launch("attn_join_kernel");
 }
-template <typename T> int launch_fwd(const Args &a, const FwdPlan &p, hipStream_t st)
+template <typename T> int launch_fwd(const d2c_attention_desc &q, const Args &a, const FwdPlan &p, hipStream_t st)
 {
-    const int rc = p.token ? for_token<T>(a.D, a.rows, [&](auto lanes, auto r, auto whole) {
+    const int rc = p.token ? for_token<T>(q, a.rows, [&](auto lanes, auto r, auto whole) {
         hipLaunchKernelGGL((attn_token_kernel<T, decltype(lanes)::value, decltype(r)::value, decltype(whole)::value>), dim3(workgroups(p.walks)), dim3(256), 0, st, a);
         return d2c_check_launch("attn_token_kernel");
-    }) : for_shape<T>(a.D, p.few, [&](auto width, auto wk, auto whole) {
+    }) : for_shape<T>(q, p.few, [&](auto width, auto wk, auto whole) {
         constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK, WK = decltype(wk)::value;
         constexpr bool WHOLE = decltype(whole)::value;
         constexpr int lds = FwdShape<T, DP, WK, WHOLE>::LDS;
@@ -580,7 +568,7 @@ template <typename T> int forward(Args a, const d2c_attention_desc &q, void *ws,
     }
     set_walks(a, p.walks);
     a.part = (float *)ws; a.part_ml = (float *)((char *)ws + p.part_bytes);
-    return launch_fwd<T>(a, p, st);
+    return launch_fwd<T>(q, a, p, st);
 }
 
 }  // namespace
@@ -613,10 +601,6 @@ Args d2c_attn::make_args(const d2c_attention_desc &q)
     a.rows = a.Lq * a.group;
     a.gs[0] = (long)q.Lq * q.Hq * q.D; a.gs[1] = (long)q.Hq * q.D; a.gs[2] = q.D;
     a.scale = q.scale; a.scale2 = q.scale * 1.44269504088896340736f;
-    // (a tile has 128 rows at most)
-    const long far = (1L << 30) / 128 / 4;
-    auto near = [&](long stride) { return stride >= 0 && stride < far; };
-    a.near = (near(a.ks[1]) && near(a.vs[1]) ? 1 : 0) | (near(a.qs[1]) && near(a.qs[2] * a.group) && near(a.gs[1]) ? 2 : 0);
     return a;
 }
 

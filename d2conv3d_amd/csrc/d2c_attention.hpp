@@ -32,11 +32,15 @@ struct Args {
     long qs[3], ks[3], vs[3], gs[3];    // strides of sample, position, head
     int N, Lq, Lk, Hq, Hkv, group, D, rows;
     int whole, shared, splits;          // see Walks
-    int near;                           // offsets inside a tile of keys (bit 0) and of rows (bit 1) fit 32 bits, see Tile
     float scale, scale2;                // scale2 = scale * log2(e)
 };
 
 template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 1 : 3;
+// Terms of the weights p and of ds, which are rounded to the matrix instruction's operands: bfloat16 problems take one, whose errors are as large as the
+// rounding of the result and average out over many keys.  Where there are 64 keys or fewer, they do not (two keys: weights just above 1/2, where the
+// spacing is widest), and a second term costs nothing that counts.  (Heads of an odd size run on the same kernels and have it, too.)
+template <typename T, bool FAST> constexpr int kWeightTerms = sizeof(T) == 4 ? 3 : FAST ? 1 : 2;
+constexpr int kExactKeys = 64;
 
 // 8 reduction elements of a matrix operand's row
 template <int P> struct Frag { uint4 t[P]; };
@@ -45,8 +49,10 @@ D2C_DEV f32x16 mma1(f32x16 acc, const uint4 &a, const uint4 &b)
 {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), acc, 0, 0, 0);
 }
-template <int P> D2C_DEV void mma(f32x16 &acc, const Frag<P> &a, const Frag<P> &b)
+template <int P, int PB> D2C_DEV void mma(f32x16 &acc, const Frag<P> &a, const Frag<PB> &b)
 {
+    static_assert(P == 1 || PB == 3, "");
+    if constexpr (P == 1 && PB == 2) acc = mma1(acc, a.t[0], b.t[1]);
     if constexpr (P == 3) {
         acc = mma1(acc, a.t[2], b.t[0]);
         acc = mma1(acc, a.t[0], b.t[2]);
@@ -69,6 +75,12 @@ template <int P> D2C_DEV Frag<P> make_frag(const float *v)
     Frag<P> f;
     if constexpr (P == 1) {
         f.t[0] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    } else if constexpr (P == 2) {
+        uint32_t h[4], m[4], none;
+#pragma unroll
+        for (int i = 0; i < 4; i++) split_pair(v[2 * i], v[2 * i + 1], h[i], m[i], none);
+        f.t[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        f.t[1] = make_uint4(m[0], m[1], m[2], m[3]);
     } else {
         uint32_t h[4], m[4], l[4];
 #pragma unroll
@@ -143,36 +155,31 @@ template <int DP> D2C_DEV int piece_at(int row, int piece) { return row * (DP * 
 
 typedef short v4s_t __attribute__((ext_vector_type(4)));
 
-// WHOLE (D is a multiple of 8): loads without branches.  Pieces behind a row's end then repeat its last one: they meet zeros of the other operand, or make
-// columns that are not stored.  Else elements behind the end are zeros.
+// WHOLE (heads are whole pieces, rows near enough for offsets of 32 bits): loads without branches.  Pieces behind a row's end then repeat its last one: they meet
+// zeros of the other operand, or make columns that are not stored.  Else elements behind the end are zeros.
 template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
     static constexpr int P = kTerms<T>, PIECES = DP / 8, PER = (ROWS * PIECES + THREADS - 1) / THREADS;
     static constexpr int TERM = ROWS * DP * 2, BYTES = P * TERM;
     Raw8<T> r[PER];
+    // this thread's piece i: its row and first column
+    static D2C_DEV int place(int i) { return min(i * THREADS + (int)threadIdx.x, ROWS * PIECES - 1); }
+    static D2C_DEV int row_of(int i) { return place(i) / PIECES; }
+    static D2C_DEV int column_of(int i, int D) { return WHOLE ? min(place(i) % PIECES * 8, D - 8) : place(i) % PIECES * 8; }
     // row(i): the address of row i, which is there to be read whatever i
     template <typename Row> D2C_DEV void load(int D, Row row)
     {
+        static_assert(!WHOLE, "");
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            const int at = min(i * THREADS + (int)threadIdx.x, ROWS * PIECES - 1), d = at % PIECES * 8;
-            const T *p = row(at / PIECES);
-            if constexpr (WHOLE) r[i] = load8<true, T>(p + min(d, D - 8), 8);
-            else r[i] = load8<false, T>(p + d, D - d);
+            const int d = column_of(i, D);
+            r[i] = load8<false, T>(row(row_of(i)) + d, D - d);
         }
     }
-    // ... by their offsets in bytes from the tile's first row: 32 bits each, the same for every tile
-    template <typename Off> D2C_DEV void places(unsigned (&off)[PER], int D, Off row_offset) const
+    // WHOLE: by offsets in bytes from one address
+    D2C_DEV void load_at(const T *base, const unsigned (&off)[PER])
     {
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int at = min(i * THREADS + (int)threadIdx.x, ROWS * PIECES - 1);
-            off[i] = (unsigned)((row_offset(at / PIECES) + min(at % PIECES * 8, D - 8)) * (long)sizeof(T));
-        }
-    }
-    D2C_DEV void load_near(const T *tile, const unsigned (&off)[PER])
-    {
-#pragma unroll
-        for (int i = 0; i < PER; i++) r[i] = load8<true, T>(reinterpret_cast<const T *>(reinterpret_cast<const char *>(tile) + off[i]), 8);
+        for (int i = 0; i < PER; i++) r[i] = load8<true, T>(reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + off[i]), 8);
     }
     D2C_DEV void store(unsigned char *lds) const
     {
@@ -215,11 +222,22 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
 // float32, whose steps are six instructions each, leaves out a last one that heads do not reach (1417 on 3001 positions of 6 heads of 40 channels: the three
 // kernels 210, 181 us).
 template <int DP_, int NK_> struct Width { static constexpr int DP = DP_, NK = NK_; };
-template <typename T, typename F> auto for_width(int D, F f)      // f(Width, whether D is a multiple of 8)
+// Whether a problem runs on the kernels that load whole pieces by offsets of 32 bits: of a tile of 128 keys at most, of all rows (and, bfloat16, take one term of
+// the weights)
+inline bool fast_kernels(const d2c_attention_desc &q)
 {
+    const long size = (long)d2c_elem_size(q.dtype), limit = 1L << 31;
+    auto keys_near = [&](long stride) { return stride >= 0 && 128 * stride * size < limit; };
+    auto rows_near = [&](const int64_t *s) { return s[1] >= 0 && s[2] >= 0 && (q.Lq * s[1] + q.Hq / q.Hkv * s[2] + q.D) * size < limit; };
+    const int64_t g[3] = {0, (int64_t)q.Hq * q.D, q.D};
+    return q.D % 8 == 0 && (q.dtype == D2C_F32 || q.Lk > kExactKeys) && keys_near(q.k_stride[1]) && keys_near(q.v_stride[1]) && rows_near(q.q_stride) && rows_near(g);
+}
+template <typename T, typename F> auto for_width(const d2c_attention_desc &q, F f)      // f(Width, fast_kernels)
+{
+    const int D = q.D;
     auto pick = [&](auto width) {
         using W = decltype(width);
-        if (D % 8 != 0) return f(width, std::false_type{});
+        if (!fast_kernels(q)) return f(width, std::false_type{});
         if constexpr (sizeof(T) == 4)
             if (D <= W::DP - 16) return f(Width<W::DP, W::NK - 1>{}, std::true_type{});
         return f(width, std::true_type{});
@@ -303,12 +321,12 @@ D2C_DEV void other_half(float v, float &x, float &y)
 D2C_DEV float half_max(float v) { float x, y; other_half(v, x, y); return fmaxf(x, y); }
 D2C_DEV float half_sum(float v) { float x, y; other_half(v, x, y); return x + y; }
 
-// The rows of a tile of keys to request: a key that is not to be read is replaced by one of the tile's that is (`any`, a bit of
-// `words`), so that what it holds is nowhere read: its score is put to -infinity, its weight 0 meets that other key's value.
-template <int WORDS> D2C_DEV int key_to_load(const uint64_t (&words)[WORDS], int i, int any)
+// The rows of a tile of keys to request: a key that is not to be read is replaced by one of the tile's that is (any_key, of `words`), so that
+// what it holds is nowhere read: its score is put to -infinity, its weight 0 meets that other key's value.
+template <int WORDS> D2C_DEV bool has_key(const uint64_t (&words)[WORDS], int i)
 {
     const uint64_t w = WORDS == 1 ? words[0] : words[i >> 6];
-    return (w >> (i & 63)) & 1 ? i : any;
+    return (w >> (i & 63)) & 1;
 }
 template <int KT, int WORDS> D2C_DEV bool all_keys(const uint64_t (&words)[WORDS])
 {
@@ -326,6 +344,53 @@ template <int WORDS> D2C_DEV int any_key(const uint64_t (&words)[WORDS])
 }
 
 Args make_args(const d2c_attention_desc &q);
+
+// The keys and values of one key head, a tile of KT keys at a time
+template <typename T, typename KV, int KT, int WORDS, bool WHOLE> struct KeyTiles {
+    const T *kb, *vb;
+    long ks, vs;
+    unsigned koff[WHOLE ? KV::PER : 1], voff[WHOLE ? KV::PER : 1];
+    D2C_DEV KeyTiles(const Args &a, const Head &hd)
+    {
+        kb = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2];
+        vb = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2];
+        ks = a.ks[1]; vs = a.vs[1];
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int i = 0; i < KV::PER; i++) {
+                const unsigned row = KV::row_of(i), d = KV::column_of(i, a.D);
+                koff[i] = (row * (unsigned)ks + d) * (unsigned)sizeof(T);
+                voff[i] = (row * (unsigned)vs + d) * (unsigned)sizeof(T);
+            }
+        }
+    }
+    // `words`: the tile's keys that are to be read (none: nothing is requested)
+    D2C_DEV void request(const Args &a, KV &k, KV &v, int tile, const uint64_t (&words)[WORDS]) const
+    {
+        const int any = any_key(words);
+        if (any < 0) return;
+        const T *kt = kb + (long)tile * KT * ks, *vt = vb + (long)tile * KT * vs;
+        if constexpr (WHOLE) {
+            unsigned ko[KV::PER], vo[KV::PER];
+            const bool all = all_keys<KT>(words);
+#pragma unroll
+            for (int i = 0; i < KV::PER; i++) { ko[i] = koff[i]; vo[i] = voff[i]; }
+            if (!all) {
+#pragma unroll
+                for (int i = 0; i < KV::PER; i++) {
+                    const unsigned step = has_key(words, KV::row_of(i)) ? 0u : (unsigned)(any - KV::row_of(i)) * (unsigned)sizeof(T);
+                    ko[i] += step * (unsigned)ks;
+                    vo[i] += step * (unsigned)vs;
+                }
+            }
+            k.load_at(kt, ko);
+            v.load_at(vt, vo);
+        } else {
+            k.load(a.D, [&](int i) INLINE { return kt + (has_key(words, i) ? i : any) * ks; });
+            v.load(a.D, [&](int i) INLINE { return vt + (has_key(words, i) ? i : any) * vs; });
+        }
+    }
+};
 inline void set_walks(Args &a, const Walks &w) { a.whole = w.whole; a.shared = w.shared; a.splits = w.splits; }
 
 }  // namespace d2c_attn

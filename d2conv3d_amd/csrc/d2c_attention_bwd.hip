@@ -22,7 +22,7 @@ template <typename T, int DP, bool WHOLE> struct QShape {
 template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bounds__(256, (QShape<T, DP, WHOLE>::WAVES)) attn_bwd_q_kernel(Args a)
 {
     using KV = typename QShape<T, DP, WHOLE>::KV;
-    constexpr int P = kTerms<T>, ND = DP / 32, KT = QShape<T, DP, WHOLE>::KT;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, KT = QShape<T, DP, WHOLE>::KT;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = QShape<T, DP, WHOLE>::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -34,28 +34,12 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
     const int t1 = (int)((long)tiles * (unit.split + 1) / unit.splits);
     int t = (int)((long)tiles * unit.split / unit.splits);
 
-    const T *kb = reinterpret_cast<const T *>(a.k) + hd.n * a.ks[0] + hd.h * a.ks[2];
-    const T *vb = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2];
     KV k, v;
-    unsigned koff[KV::PER], voff[KV::PER];
-    k.places(koff, a.D, [&](int i) INLINE { return i * a.ks[1]; });
-    v.places(voff, a.D, [&](int i) INLINE { return i * a.vs[1]; });
+    const KeyTiles<T, KV, KT, 1, WHOLE> source(a, hd);
     bool b = false;
     auto ask = [&](int k0) INLINE { const int key = k0 + lane; b = lane < KT && key < keys && (!a.mask || a.mask[(long)hd.n * a.Lk + key]); };
     uint64_t next[1] = {0};
-    auto request = [&](int tile) INLINE {
-        const int any = any_key(next);
-        if (any < 0) return;
-        const T *kt = kb + (long)tile * KT * a.ks[1], *vt = vb + (long)tile * KT * a.vs[1];
-        if constexpr (WHOLE)
-            if ((a.near & 1) && all_keys<KT>(next)) {
-                k.load_near(kt, koff);
-                v.load_near(vt, voff);
-                return;
-            }
-        k.load(a.D, [&](int i) INLINE { return kt + key_to_load(next, i, any) * a.ks[1]; });
-        v.load(a.D, [&](int i) INLINE { return vt + key_to_load(next, i, any) * a.vs[1]; });
-    };
+    auto request = [&](int tile) INLINE { source.request(a, k, v, tile, next); };
     if (t < t1) {
         ask(t * KT);
         next[0] = __ballot(b);
@@ -112,8 +96,8 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
             for (int r = 0; r < 16; r++) s[r] = dp[r] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < NK; ks++) {
-                mma<P>(s, KV::rows(s_k, i * 32 + (lane & 31), ks, half), q[ks]);
-                mma<P>(dp, KV::rows(s_v, i * 32 + (lane & 31), ks, half), g[ks]);
+                mma(s, KV::rows(s_k, i * 32 + (lane & 31), ks, half), q[ks]);
+                mma(dp, KV::rows(s_v, i * 32 + (lane & 31), ks, half), g[ks]);
             }
             const uint32_t there = (uint32_t)(now >> (i * 32));
             if (there != 0xffffffffu) {
@@ -127,9 +111,9 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
             for (int r = 0; r < 16; r++) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
-                const Frag<P> f = make_frag<P>(ds + kk * 8);
+                const Frag<PW> f = make_frag<PW>(ds + kk * 8);
 #pragma unroll
-                for (int d = 0; d < ND; d++) mma<P>(dq[d], KV::columns(s_k, i * 32 + kk * 16, d * 32, lane), f);
+                for (int d = 0; d < ND; d++) mma(dq[d], KV::columns(s_k, i * 32 + kk * 16, d * 32, lane), f);
             }
         }
     }
@@ -172,7 +156,7 @@ template <typename T, int DP, bool WHOLE> struct KvShape {
 template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bounds__(256, (KvShape<T, DP, WHOLE>::WAVES)) attn_bwd_kv_kernel(Args a)
 {
     using QG = typename KvShape<T, DP, WHOLE>::QG;
-    constexpr int P = kTerms<T>, ND = DP / 32, RT = KvShape<T, DP, WHOLE>::RT;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, RT = KvShape<T, DP, WHOLE>::RT;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = KvShape<T, DP, WHOLE>::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -185,26 +169,38 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
     int t = (int)((long)tiles * unit.split / unit.splits);
 
     QG q, g;
-    // (tiles that begin with a position's first head: the places of their rows are the same from tile to tile)
-    const bool uniform = (a.near & 2) && RT % a.group == 0;
     const T *qb = row_at<T>(a.q, a.qs, a, hd, 0), *gb = row_at<T>(a.g, a.gs, a, hd, 0);
-    unsigned qoff[QG::PER], goff[QG::PER];
-    q.places(qoff, a.D, [&](int i) INLINE { return i / a.group * a.qs[1] + i % a.group * a.qs[2]; });
-    g.places(goff, a.D, [&](int i) INLINE { return i / a.group * a.gs[1] + i % a.group * a.gs[2]; });
+    // (tiles that begin with a position's first head: the places of their rows are the same from tile to tile)
+    const bool uniform = RT % a.group == 0;
+    unsigned qoff[WHOLE ? QG::PER : 1], goff[WHOLE ? QG::PER : 1];
+    auto places = [&](unsigned (&qo)[WHOLE ? QG::PER : 1], unsigned (&go)[WHOLE ? QG::PER : 1], int r0) INLINE {
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int i = 0; i < QG::PER; i++) {
+                const unsigned row = min(r0 + QG::row_of(i), a.rows - 1), pos = row / (unsigned)a.group, head = row - pos * a.group, d = QG::column_of(i, a.D);
+                qo[i] = (pos * (unsigned)a.qs[1] + head * (unsigned)a.qs[2] + d) * (unsigned)sizeof(T);
+                go[i] = (pos * (unsigned)a.gs[1] + head * (unsigned)a.gs[2] + d) * (unsigned)sizeof(T);
+            }
+        }
+    };
+    places(qoff, goff, 0);
     float stat = 0.f;
     auto request = [&](int tile) INLINE {
         const int r0 = tile * RT;
-        bool done = false;
-        if constexpr (WHOLE)
-            if (uniform && r0 + RT <= a.rows) {
-                q.load_near(qb + (r0 / a.group) * a.qs[1], qoff);
-                g.load_near(gb + (r0 / a.group) * a.gs[1], goff);
-                done = true;
-            }
         // (rows behind the last one repeat it: their weights are 0, by a sum of +infinity)
-        if (!done) {
-        q.load(a.D, [&](int i) INLINE { return row_at<T>(a.q, a.qs, a, hd, min(r0 + i, a.rows - 1)); });
-        g.load(a.D, [&](int i) INLINE { return row_at<T>(a.g, a.gs, a, hd, min(r0 + i, a.rows - 1)); });
+        if constexpr (WHOLE) {
+            if (uniform && r0 + RT <= a.rows) {
+                q.load_at(qb + (long)(r0 / a.group) * a.qs[1], qoff);
+                g.load_at(gb + (long)(r0 / a.group) * a.gs[1], goff);
+            } else {
+                unsigned qo[QG::PER], go[QG::PER];
+                places(qo, go, r0);
+                q.load_at(qb, qo);
+                g.load_at(gb, go);
+            }
+        } else {
+            q.load(a.D, [&](int i) INLINE { return row_at<T>(a.q, a.qs, a, hd, min(r0 + i, a.rows - 1)); });
+            g.load(a.D, [&](int i) INLINE { return row_at<T>(a.g, a.gs, a, hd, min(r0 + i, a.rows - 1)); });
         }
         if (threadIdx.x < 2 * RT) {
             const bool first = threadIdx.x < RT;
@@ -263,9 +259,9 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
             for (int r = 0; r < 16; r++) s[r] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < NK; ks++) {
-                mma<P>(s, QG::rows(s_q, i * 32 + (lane & 31), ks, half), k[ks]);
-                if constexpr (Shape::V_LDS) mma<P>(dp, QG::rows(s_g, i * 32 + (lane & 31), ks, half), Shape::V::rows(s_v, tile_key, ks, half));
-                else mma<P>(dp, QG::rows(s_g, i * 32 + (lane & 31), ks, half), v[ks]);
+                mma(s, QG::rows(s_q, i * 32 + (lane & 31), ks, half), k[ks]);
+                if constexpr (Shape::V_LDS) mma(dp, QG::rows(s_g, i * 32 + (lane & 31), ks, half), Shape::V::rows(s_v, tile_key, ks, half));
+                else mma(dp, QG::rows(s_g, i * 32 + (lane & 31), ks, half), v[ks]);
             }
             float p[16], ds[16];
 #pragma unroll
@@ -280,11 +276,11 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
             }
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
-                const Frag<P> pf = make_frag<P>(p + kk * 8), df = make_frag<P>(ds + kk * 8);
+                const Frag<PW> pf = make_frag<PW>(p + kk * 8), df = make_frag<PW>(ds + kk * 8);
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
-                    mma<P>(dv[d], QG::columns(s_g, i * 32 + kk * 16, d * 32, lane), pf);
-                    mma<P>(dk[d], QG::columns(s_q, i * 32 + kk * 16, d * 32, lane), df);
+                    mma(dv[d], QG::columns(s_g, i * 32 + kk * 16, d * 32, lane), pf);
+                    mma(dk[d], QG::columns(s_q, i * 32 + kk * 16, d * 32, lane), df);
                 }
             }
         }
@@ -353,7 +349,7 @@ template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
     BwdPlan p;
     const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv, cus = std::max(d2c_num_cus(), 1);
     const double part = 128.0 * q.D * 4, slow = sizeof(T) == 2 ? 1 : 3;
-    for_width<T>(q.D, [&](auto width, auto whole) {
+    for_width<T>(q, [&](auto width, auto whole) {
         constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK;
         constexpr bool WHOLE = decltype(whole)::value;
         using Q = QShape<T, DP, WHOLE>;
@@ -405,7 +401,7 @@ template <typename T> int backward(Args a, const d2c_attention_desc &q, void *ws
         return D2C_ERR_WORKSPACE;
     }
     a.delta = (float *)ws; a.part = (float *)((char *)ws + p.delta_bytes);
-    return for_width<T>(a.D, [&](auto width, auto whole) { return launch_bwd<T, decltype(width)::DP, decltype(width)::NK, decltype(whole)::value>(a, p, st); });
+    return for_width<T>(q, [&](auto width, auto whole) { return launch_bwd<T, decltype(width)::DP, decltype(width)::NK, decltype(whole)::value>(a, p, st); });
 }
 
 }  // namespace

@@ -141,6 +141,9 @@ CASES = [
     (1, 4, 257, 2, 1, 33, "none"),
     (2, 2, 64, 1, 1, 128, "lengths"),
     (1, 5, 2000, 1, 1, 24, "mask"),
+    (1, 526, 984, 8, 8, 128, "none"),       # the widest heads, tiles that end inside and walks that are shared
+    (2, 300, 1000, 4, 2, 104, "both"),
+    (1, 150, 1100, 3, 1, 64, "mask"),
 ]
 
 
@@ -216,6 +219,38 @@ def test_strides_and_alignment(dtype, dev):
         out = d2c.cross_attention(*args)
         grads = torch.autograd.grad(out, args, view(g, how))
         check((out, *grads), want, bounds, how)
+
+
+def outputs_of(args, g, lengths, mask):
+    out = d2c.cross_attention(*args, key_lengths=lengths, key_mask=mask)
+    return (out, *torch.autograd.grad(out, args, g))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [8, 20, 24, 33, 40, 64, 70, 72, 80, 96, 100, 104, 120, 128])
+def test_nothing_behind_the_tensors_is_read(D, dtype, dev):
+    """Ends inside a tile, walks shared by workgroups, keys that are not to be read among those that are: what lies behind the
+    last row of an input, or between its heads and rows, changes nothing."""
+    print("cross_attention: NaN around the inputs", D, dtype, flush=True)
+    for N, Lq, Lk, Hq, Hkv, kind in ((1, 526, 984, 8, 8, "none"), (2, 300, 2000, 4, 2, "both"), (3, 4, 1900, 3, 3, "lengths"),
+                                     (1, 1500, 130, 2, 2, "none"), (1, 33, 700, 6, 2, "mask"), (2, 2, 400, 2, 2, "mask")):
+        plain = make(N, Lq, Lk, Hq, Hkv, D, dtype, 91 + D)
+        lengths, mask = make_masks(kind, N, Lk, 91)
+        lengths, mask = (None if t is None else t.to(dev) for t in (lengths, mask))
+
+        def inside(t, rows, gap):       # a part of a buffer of NaN
+            n, l, h, d = t.shape
+            buf = torch.full((n, l + rows, h, d + gap), math.nan, dtype=dtype, device=dev)
+            buf[:, :l, :, :d] = t.to(dev)
+            return buf[:, :l, :, :d]
+        want = outputs_of([t.to(dev).requires_grad_() for t in plain[:3]], plain[3].to(dev), lengths, mask)
+        assert not any(bool(t.isnan().any()) for t in want)
+        for rows, gap in ((200, 0), (0, 8)):
+            args = [inside(t, rows, gap).requires_grad_() for t in plain[:3]]
+            for _ in range(3):
+                got = outputs_of(args, inside(plain[3], rows, gap), lengths, mask)
+                for a, b in zip(got, want):
+                    assert torch.equal(a, b), (N, Lq, Lk, Hq, Hkv, kind, rows, gap)
 
 
 def test_shared_and_broadcast_inputs(dev):
