@@ -214,8 +214,8 @@ def load():
     for d in ("forward", "backward"):
         f = getattr(lib, f"d2c_attention_{d}_workspace_bytes")
         f.argtypes, f.restype = [pat], sz
-    lib.d2c_attention_forward.argtypes, lib.d2c_attention_forward.restype = [pat] + [vp] * 8 + [sz, vp], ctypes.c_int
-    lib.d2c_attention_backward.argtypes, lib.d2c_attention_backward.restype = [pat] + [vp] * 12 + [sz, vp], ctypes.c_int
+    lib.d2c_attention_forward.argtypes, lib.d2c_attention_forward.restype = [pat] + [vp] * 9 + [sz, vp], ctypes.c_int
+    lib.d2c_attention_backward.argtypes, lib.d2c_attention_backward.restype = [pat] + [vp] * 13 + [sz, vp], ctypes.c_int
     lib.d2c_profile_enable.argtypes, lib.d2c_profile_enable.restype = [ctypes.c_int], None
     lib.d2c_profile_reset.argtypes, lib.d2c_profile_reset.restype = [], None
     lib.d2c_profile_read.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int)]

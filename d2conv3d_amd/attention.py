@@ -193,14 +193,16 @@ class _CrossAttentionFunction(torch.autograd.Function):
         desc = _lib.AttentionDesc(N, Lq, Lk, Hq, Hkv, D, _DT[q.dtype], scale, _long3(*q.stride()[:3]), _long3(*k.stride()[:3]),
                                   _long3(*v.stride()[:3]))
         out = torch.empty((N, Lq, Hq, D), dtype=q.dtype, device=dev)
-        lse = torch.empty((N, Hkv, Lq * (Hq // Hkv)), dtype=torch.float32, device=dev) if any(ctx.needs_input_grad) else None
+        grad = any(ctx.needs_input_grad)
+        lse = torch.empty((N, Hkv, Lq * (Hq // Hkv)), dtype=torch.float32, device=dev) if grad else None
+        low = torch.empty_like(out) if grad and out.dtype == torch.bfloat16 else None
         with torch.cuda.device(dev):
             nb = lib.d2c_attention_forward_workspace_bytes(ctypes.byref(desc))
             ws = _workspace(nb, dev)
             rc = lib.d2c_attention_forward(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(key_lengths), _ptr(key_mask),
-                                           _ptr(out), _ptr(lse), _ptr(ws), nb, _stream(dev))
+                                           _ptr(out), _ptr(low), _ptr(lse), _ptr(ws), nb, _stream(dev))
         _lib.check(rc, "cross_attention forward")
-        ctx.save_for_backward(q, k, v, key_lengths, key_mask, out, lse)
+        ctx.save_for_backward(q, k, v, key_lengths, key_mask, out, low, lse)
         ctx.desc = desc
         return out
 
@@ -208,7 +210,7 @@ class _CrossAttentionFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         lib = _lib.load()
-        q, k, v, key_lengths, key_mask, out, lse = ctx.saved_tensors
+        q, k, v, key_lengths, key_mask, out, low, lse = ctx.saved_tensors
         desc, dev, need = ctx.desc, q.device, ctx.needs_input_grad
         g = grad_out.to(q.dtype).contiguous()
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((q, k, v), need))
@@ -216,8 +218,8 @@ class _CrossAttentionFunction(torch.autograd.Function):
             nb = lib.d2c_attention_backward_workspace_bytes(ctypes.byref(desc))
             ws = _workspace(nb, dev)
             rc = lib.d2c_attention_backward(ctypes.byref(desc), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(key_lengths),
-                                            _ptr(key_mask), _ptr(out), _ptr(lse), _ptr(gq), _ptr(gk), _ptr(gv), _ptr(ws), nb,
-                                            _stream(dev))
+                                            _ptr(key_mask), _ptr(out), _ptr(low), _ptr(lse), _ptr(gq), _ptr(gk), _ptr(gv),
+                                            _ptr(ws), nb, _stream(dev))
         _lib.check(rc, "cross_attention backward")
         return gq, gk, gv, None, None, None
 

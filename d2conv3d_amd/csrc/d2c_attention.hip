@@ -72,7 +72,15 @@ template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __laun
 #pragma unroll
         for (int i = 0; i < NK; i++) {
             const int d = i * 16 + half * 8;
-            q[i] = terms_of<T>(load8_of<WHOLE, T>(qr, d, a.D, row < a.rows));
+            const Raw8<T> raw = load8_of<WHOLE, T>(qr, d, a.D, row < a.rows);
+            if constexpr (sizeof(T) == 2) q[i] = terms_of<T>(raw);
+            else {
+                float x[8];
+                floats_of<T>(raw, x);
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] *= a.scale2;
+                q[i] = make_frag<3>(x);
+            }
         }
     }
     f32x16 o[ND];
@@ -81,7 +89,8 @@ template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __laun
 #pragma unroll
         for (int r = 0; r < 16; r++) o[i][r] = 0.f;
     float m = -INFINITY, lift = -INFINITY, l = 0.f;
-    const float c = a.scale2;
+    // (float32 has its scale in the rows already: the largest score's weight is 1 to the last bit, and a row with one key takes its value as it is)
+    const float c = sizeof(T) == 4 ? 1.f : a.scale2;
     int buffer = 0;
 
     for (; t < t1; t++) {
@@ -215,6 +224,7 @@ template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __laun
             const int d = i * 32 + j * 8 + half * 4;
             const float x[4] = {o[i][j * 4] * inv, o[i][j * 4 + 1] * inv, o[i][j * 4 + 2] * inv, o[i][j * 4 + 3] * inv};
             store4<T>(orow + d, x, a.D - d);
+            if (a.out_low) store4_low<T>(reinterpret_cast<T *>(a.out_low) + (orow - reinterpret_cast<T *>(a.out)) + d, x, a.D - d);
         }
     if (a.lse && half == 0) a.lse[hd.nh * a.rows + row] = l == 0.f ? INFINITY : mc + log2f(l);
 }
@@ -415,7 +425,10 @@ template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bou
             a.part[at * a.D + d] = x;
             if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(top, sum);
         } else {
-            const_cast<T *>(row_at<T>(a.out, a.gs, a, hd, r))[d] = f32_to_elem<T>(sum == 0.f ? 0.f : x / sum);
+            const float y = sum == 0.f ? 0.f : x / sum;
+            const T rounded = f32_to_elem<T>(y);
+            const_cast<T *>(row_at<T>(a.out, a.gs, a, hd, r))[d] = rounded;
+            if (a.out_low) const_cast<T *>(row_at<T>(a.out_low, a.gs, a, hd, r))[d] = f32_to_elem<T>(y - elem_to_f32<T>(rounded));
             if (a.lse && d == 0) a.lse[hd.nh * a.rows + r] = sum == 0.f ? INFINITY : top + log2f(sum);
         }
     }
@@ -467,7 +480,10 @@ template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_joi
     T *orow = reinterpret_cast<T *>(a.out) + (((long)n * a.Lq + pos) * a.Hq + head) * a.D;
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] *= inv;
-    if (d < a.D) store4<T>(orow + d, x, a.D - d);
+    if (d < a.D) {
+        store4<T>(orow + d, x, a.D - d);
+        if (a.out_low) store4_low<T>(reinterpret_cast<T *>(a.out_low) + (orow - reinterpret_cast<T *>(a.out)) + d, x, a.D - d);
+    }
     if (a.lse && lane == 0) a.lse[(long)nh * a.rows + row] = l == 0.f ? INFINITY : top + log2f(l);
 }
 
@@ -475,7 +491,7 @@ template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_joi
 template <typename T, typename F> auto for_shape(const d2c_attention_desc &q, bool few, F f)
 {
     constexpr int WK = sizeof(T) == 2 ? 4 : 2;
-    return for_width<T>(q, [&](auto width, auto whole) {
+    return for_width<T, false>(q, [&](auto width, auto whole) {
         return few ? f(width, std::integral_constant<int, WK>{}, whole) : f(width, std::integral_constant<int, 1>{}, whole);
     });
 }
@@ -490,7 +506,7 @@ template <typename T, typename F> auto for_token(const d2c_attention_desc &q, lo
         if (rows <= 4) return f(lanes, std::integral_constant<int, 4>{}, whole);
         return f(lanes, std::integral_constant<int, 8>{}, whole);
     };
-    auto pick = [&](auto lanes) { return fast_kernels(q) ? with_rows(lanes, std::true_type{}) : with_rows(lanes, std::false_type{}); };
+    auto pick = [&](auto lanes) { return fast_kernels(q, false) ? with_rows(lanes, std::true_type{}) : with_rows(lanes, std::false_type{}); };
     constexpr int L32 = 32 * (int)sizeof(T) / 16;
     if (D <= 32) return pick(std::integral_constant<int, L32>{});
     if (D <= 64) return pick(std::integral_constant<int, 2 * L32>{});
@@ -630,13 +646,14 @@ extern "C" size_t d2c_attention_forward_workspace_bytes(const d2c_attention_desc
 }
 
 extern "C" int d2c_attention_forward(const d2c_attention_desc *q, const void *query, const void *key, const void *value,
-                                     const int32_t *key_lengths, const uint8_t *key_mask, void *out, float *lse, void *ws,
-                                     size_t ws_bytes, void *stream)
+                                     const int32_t *key_lengths, const uint8_t *key_mask, void *out, void *out_low,
+                                     float *lse, void *ws, size_t ws_bytes, void *stream)
 {
     if (int rc = d2c_attention_check(q)) return rc;
     if (q->N == 0 || q->Lq == 0) return D2C_OK;
     if (!query || !out || (q->Lk > 0 && (!key || !value))) { d2c_set_error("null tensor pointer"); return D2C_ERR_SHAPE; }
     Args a = make_args(*q);
     a.q = query; a.k = key; a.v = value; a.lengths = key_lengths; a.mask = key_mask; a.out = out; a.lse = lse;
+    a.out_low = q->dtype == D2C_BF16 ? out_low : nullptr;
     return q->dtype == D2C_BF16 ? forward<bf16_t>(a, *q, ws, ws_bytes, (hipStream_t)stream) : forward<float>(a, *q, ws, ws_bytes, (hipStream_t)stream);
 }

@@ -24,9 +24,11 @@ namespace d2c_attn {
 
 struct Args {
     const void *q, *k, *v, *g, *o;      // g: gradient of the output o
+    const void *o_low;                  // what rounding took off o (bfloat16, or NULL)
     const int32_t *lengths;             // [N] or NULL
     const uint8_t *mask;                // [N][Lk], 0: not to be read; or NULL
     void *out, *gq, *gk, *gv;           // [N][Lq][Hq][D], [N][Lk][Hkv][D]
+    void *out_low;                      // NULL, or where the forward pass leaves o_low
     float *lse, *delta;                 // [N * Hkv][rows]: log2 of the sum of a row (+infinity: no key), and sum_d do o
     float *part, *part_ml;              // partial results of the walks that are shared: [splits][shared][rows of a tile][D] and (forward) [..][2]
     long qs[3], ks[3], vs[3], gs[3];    // strides of sample, position, head
@@ -38,9 +40,11 @@ struct Args {
 template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 1 : 3;
 // Terms of the weights p and of ds, which are rounded to the matrix instruction's operands: bfloat16 problems take one, whose errors are as large as the
 // rounding of the result and average out over many keys.  Where there are 64 keys or fewer, they do not (two keys: weights just above 1/2, where the
-// spacing is widest), and a second term costs nothing that counts.  (Heads of an odd size run on the same kernels and have it, too.)
+// spacing is widest), nor in the gradients of a small problem, and a second term costs nothing there that counts.  (Heads of an odd size run on the same
+// kernels and have it, too.)
 template <typename T, bool FAST> constexpr int kWeightTerms = sizeof(T) == 4 ? 3 : FAST ? 1 : 2;
 constexpr int kExactKeys = 64;
+constexpr long kExactScores = 1L << 22;
 
 // 8 reduction elements of a matrix operand's row
 template <int P> struct Frag { uint4 t[P]; };
@@ -224,20 +228,21 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
 template <int DP_, int NK_> struct Width { static constexpr int DP = DP_, NK = NK_; };
 // Whether a problem runs on the kernels that load whole pieces by offsets of 32 bits: of a tile of 128 keys at most, of all rows (and, bfloat16, take one term of
 // the weights)
-inline bool fast_kernels(const d2c_attention_desc &q)
+inline bool fast_kernels(const d2c_attention_desc &q, bool gradients)
 {
+    if (q.dtype == D2C_BF16 && (q.Lk <= kExactKeys || (gradients && (long)q.N * q.Hq * q.Lq <= kExactScores / q.Lk))) return false;
     const long size = (long)d2c_elem_size(q.dtype), limit = 1L << 31;
     auto keys_near = [&](long stride) { return stride >= 0 && 128 * stride * size < limit; };
     auto rows_near = [&](const int64_t *s) { return s[1] >= 0 && s[2] >= 0 && (q.Lq * s[1] + q.Hq / q.Hkv * s[2] + q.D) * size < limit; };
     const int64_t g[3] = {0, (int64_t)q.Hq * q.D, q.D};
-    return q.D % 8 == 0 && (q.dtype == D2C_F32 || q.Lk > kExactKeys) && keys_near(q.k_stride[1]) && keys_near(q.v_stride[1]) && rows_near(q.q_stride) && rows_near(g);
+    return q.D % 8 == 0 && keys_near(q.k_stride[1]) && keys_near(q.v_stride[1]) && rows_near(q.q_stride) && rows_near(g);
 }
-template <typename T, typename F> auto for_width(const d2c_attention_desc &q, F f)      // f(Width, fast_kernels)
+template <typename T, bool GRADIENTS, typename F> auto for_width(const d2c_attention_desc &q, F f)      // f(Width, fast_kernels)
 {
     const int D = q.D;
     auto pick = [&](auto width) {
         using W = decltype(width);
-        if (!fast_kernels(q)) return f(width, std::false_type{});
+        if (!fast_kernels(q, GRADIENTS)) return f(width, std::false_type{});
         if constexpr (sizeof(T) == 4)
             if (D <= W::DP - 16) return f(Width<W::DP, W::NK - 1>{}, std::true_type{});
         return f(width, std::true_type{});
@@ -290,6 +295,15 @@ int resident(const void *kernel, int lds);
 
 D2C_DEV int keys_of(const Args &a, int n) { return a.lengths ? min(max(a.lengths[n], 0), a.Lk) : a.Lk; }
 
+// A sample with one key to read (asked of few keys): its weight is 1 whatever the scores, and their gradients are 0, not what two sums of the same terms in
+// different orders leave.
+D2C_DEV bool one_key(const Args &a, int n, int keys)
+{
+    if (a.Lk > kExactKeys) return false;
+    const int key = threadIdx.x & 63;
+    return __popcll(__ballot(key < keys && (!a.mask || a.mask[(long)n * a.Lk + key]))) == 1;
+}
+
 // Row `row` of a tensor [N][Lq][Hq][D] with strides s
 template <typename T> D2C_DEV const T *row_at(const void *base, const long *s, const Args &a, const Head &hd, int row)
 {
@@ -310,6 +324,15 @@ template <typename T> D2C_DEV void store4(T *p, const float *v, int left)
         for (int i = 0; i < 4; i++)
             if (i < left) p[i] = f32_to_elem<T>(v[i]);
     }
+}
+
+// ... what storing them as T takes off
+template <typename T> D2C_DEV void store4_low(T *p, const float *v, int left)
+{
+    float low[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) low[i] = v[i] - elem_to_f32<T>(f32_to_elem<T>(v[i]));
+    store4<T>(p, low, left);
 }
 
 // Both halves of the wavefront: the larger value, the sum

@@ -31,7 +31,7 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
     const int tile_row = wave * 32 + (lane & 31), row = unit.tile * 128 + tile_row;
     const bool live = row < a.rows;
     const int keys = keys_of(a, hd.n), tiles = (keys + KT - 1) / KT;
-    const int t1 = (int)((long)tiles * (unit.split + 1) / unit.splits);
+    const int t1 = one_key(a, hd.n, keys) ? 0 : (int)((long)tiles * (unit.split + 1) / unit.splits);
     int t = (int)((long)tiles * unit.split / unit.splits);
 
     KV k, v;
@@ -60,6 +60,12 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
             float xf[8], yf[8];
             floats_of<T>(x, xf);
             floats_of<T>(y, yf);
+            if (a.o_low) {
+                float lf[8];
+                floats_of<T>(load8_of<WHOLE, T>(row_at<T>(a.o_low, a.gs, a, hd, r), d, a.D, live), lf);
+#pragma unroll
+                for (int j = 0; j < 8; j++) yf[j] += lf[j];
+            }
 #pragma unroll
             for (int j = 0; j < 8; j++) delta = fmaf(xf[j], yf[j], delta);
         }
@@ -163,7 +169,7 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
     const Unit unit = unit_of(a);
     const Head hd = unit.head;
     const int tile_key = wave * 32 + (lane & 31), keys = keys_of(a, hd.n), key0 = unit.tile * 128, key = key0 + tile_key;
-    const bool live = key < keys && (!a.mask || a.mask[(long)hd.n * a.Lk + key]);
+    const bool live = key < keys && (!a.mask || a.mask[(long)hd.n * a.Lk + key]), alone = one_key(a, hd.n, keys);
     const int tiles = (a.rows + RT - 1) / RT;
     const int t1 = key0 < keys ? (int)((long)tiles * (unit.split + 1) / unit.splits) : 0;
     int t = (int)((long)tiles * unit.split / unit.splits);
@@ -295,7 +301,7 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
             const int d = i * 32 + j * 8 + half * 4;
             float x[4], y[4];
 #pragma unroll
-            for (int r = 0; r < 4; r++) { x[r] = live ? dk[i][j * 4 + r] * fk : 0.f; y[r] = live ? dv[i][j * 4 + r] : 0.f; }
+            for (int r = 0; r < 4; r++) { x[r] = live && !alone ? dk[i][j * 4 + r] * fk : 0.f; y[r] = live ? dv[i][j * 4 + r] : 0.f; }
             if (unit.splits > 1) {
                 store4<float>(a.part + (((2L * unit.split) * a.shared + unit.part) * 128 + tile_key) * a.D + d, x, a.D - d);
                 store4<float>(a.part + (((2L * unit.split + 1) * a.shared + unit.part) * 128 + tile_key) * a.D + d, y, a.D - d);
@@ -336,8 +342,9 @@ template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(A
     const int n = (int)(nh / a.Hkv), lane = threadIdx.x & 63;
     const Head hd{n, (int)(nh - (long)n * a.Hkv), nh};
     const T *g = row_at<T>(a.g, a.gs, a, hd, (int)(at - nh * a.rows)), *o = row_at<T>(a.o, a.gs, a, hd, (int)(at - nh * a.rows));
+    const T *low = a.o_low ? row_at<T>(a.o_low, a.gs, a, hd, (int)(at - nh * a.rows)) : nullptr;
     float x = 0.f;
-    for (int d = lane; d < a.D; d += 64) x = fmaf(elem_to_f32<T>(g[d]), elem_to_f32<T>(o[d]), x);
+    for (int d = lane; d < a.D; d += 64) x = fmaf(elem_to_f32<T>(g[d]), elem_to_f32<T>(o[d]) + (low ? elem_to_f32<T>(low[d]) : 0.f), x);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
     if (lane == 0) a.delta[at] = x;
@@ -349,7 +356,7 @@ template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
     BwdPlan p;
     const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv, cus = std::max(d2c_num_cus(), 1);
     const double part = 128.0 * q.D * 4, slow = sizeof(T) == 2 ? 1 : 3;
-    for_width<T>(q, [&](auto width, auto whole) {
+    for_width<T, true>(q, [&](auto width, auto whole) {
         constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK;
         constexpr bool WHOLE = decltype(whole)::value;
         using Q = QShape<T, DP, WHOLE>;
@@ -401,7 +408,7 @@ template <typename T> int backward(Args a, const d2c_attention_desc &q, void *ws
         return D2C_ERR_WORKSPACE;
     }
     a.delta = (float *)ws; a.part = (float *)((char *)ws + p.delta_bytes);
-    return for_width<T>(q, [&](auto width, auto whole) { return launch_bwd<T, decltype(width)::DP, decltype(width)::NK, decltype(whole)::value>(a, p, st); });
+    return for_width<T, true>(q, [&](auto width, auto whole) { return launch_bwd<T, decltype(width)::DP, decltype(width)::NK, decltype(whole)::value>(a, p, st); });
 }
 
 }  // namespace
@@ -414,7 +421,7 @@ extern "C" size_t d2c_attention_backward_workspace_bytes(const d2c_attention_des
 
 extern "C" int d2c_attention_backward(const d2c_attention_desc *q, const void *grad_out, const void *query, const void *key,
                                       const void *value, const int32_t *key_lengths, const uint8_t *key_mask, const void *out,
-                                      const float *lse, void *grad_query, void *grad_key, void *grad_value, void *ws,
+                                      const void *out_low, const float *lse, void *grad_query, void *grad_key, void *grad_value, void *ws,
                                       size_t ws_bytes, void *stream)
 {
     if (int rc = d2c_attention_check(q)) return rc;
@@ -425,6 +432,7 @@ extern "C" int d2c_attention_backward(const d2c_attention_desc *q, const void *g
     }
     Args a = make_args(*q);
     a.g = grad_out; a.q = query; a.k = key; a.v = value; a.lengths = key_lengths; a.mask = key_mask; a.o = out;
+    a.o_low = q->dtype == D2C_BF16 ? out_low : nullptr;
     a.lse = const_cast<float *>(lse);
     a.gq = grad_query; a.gk = grad_key; a.gv = grad_value;
     return q->dtype == D2C_BF16 ? backward<bf16_t>(a, *q, ws, ws_bytes, (hipStream_t)stream) : backward<float>(a, *q, ws, ws_bytes, (hipStream_t)stream);

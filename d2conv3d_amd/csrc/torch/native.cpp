@@ -745,13 +745,13 @@ py::object rotary3d(const Tensor &x, const opt_tensor &positions, int3_t grid, i
 // ---------------------------------------------------------------- cross_attention
 struct CrossAttentionBackward : public Node {
     d2c_attention_desc q;
-    SavedVariable query, key, value, lengths, mask, out, lse;
-    bool has_lengths = false, has_mask = false;
+    SavedVariable query, key, value, lengths, mask, out, low, lse;
+    bool has_lengths = false, has_mask = false, has_low = false;
     std::string name() const override { return "CrossAttentionBackward"; }
     void release_variables() override
     {
         const std::lock_guard<std::mutex> lock(mutex_);
-        for (SavedVariable *v : {&query, &key, &value, &lengths, &mask, &out, &lse}) v->reset_data();
+        for (SavedVariable *v : {&query, &key, &value, &lengths, &mask, &out, &low, &lse}) v->reset_data();
     }
     variable_list apply(variable_list &&grads) override
     {
@@ -761,7 +761,8 @@ struct CrossAttentionBackward : public Node {
         {
             at::NoGradGuard no_grad;
             const Tensor vq = query.unpack(), vk = key.unpack(), vv = value.unpack(), vo = out.unpack(shared_from_this()), vl = lse.unpack();
-            Tensor len, msk;
+            Tensor len, msk, vlow;
+            if (has_low) vlow = low.unpack();
             if (has_lengths) len = lengths.unpack();
             if (has_mask) msk = mask.unpack();
             c10::DeviceGuard guard(vq.device());
@@ -773,7 +774,7 @@ struct CrossAttentionBackward : public Node {
             const size_t nb = d2c_attention_backward_workspace_bytes(&q);
             const Tensor ws = small_workspace(nb, vq);
             check(d2c_attention_backward(&q, ptr(g), ptr(vq), ptr(vk), ptr(vv), (const int32_t *)ptr(len), (const uint8_t *)ptr(msk), ptr(vo),
-                                         (const float *)ptr(vl), ptr(r[0]), ptr(r[1]), ptr(r[2]), ptr(ws), nb, st),
+                                         ptr(vlow), (const float *)ptr(vl), ptr(r[0]), ptr(r[1]), ptr(r[2]), ptr(ws), nb, st),
                   "cross_attention backward");
         }
         once_differentiable(r, grads[0]);
@@ -816,17 +817,20 @@ py::object cross_attention(const Tensor &query, const Tensor &key, const Tensor 
     c10::DeviceGuard guard(query.device());
     const hipStream_t st = stream_of(query);
     const auto opt = query.options().requires_grad(false);
-    Tensor out = at::empty(query.sizes(), opt), lse;
+    Tensor out = at::empty(query.sizes(), opt), low, lse;
+    if (grad && dt == D2C_BF16) low = at::empty(query.sizes(), opt);
     if (grad) lse = at::empty({q.N, q.Hkv, (int64_t)q.Lq * (q.Hq / q.Hkv)}, opt.dtype(at::kFloat));
     const size_t nb = d2c_attention_forward_workspace_bytes(&q);
     const Tensor ws = small_workspace(nb, query);
-    check(d2c_attention_forward(&q, ptr(query), ptr(key), ptr(value), (const int32_t *)ptr(len), (const uint8_t *)ptr(msk), ptr(out), (float *)ptr(lse),
+    check(d2c_attention_forward(&q, ptr(query), ptr(key), ptr(value), (const int32_t *)ptr(len), (const uint8_t *)ptr(msk), ptr(out), ptr(low), (float *)ptr(lse),
                                 ptr(ws), nb, st),
           "cross_attention forward");
     if (!grad) return py::cast(out);
     node->q = q;
     node->query = SavedVariable(query, false); node->key = SavedVariable(key, false); node->value = SavedVariable(value, false);
     node->lse = SavedVariable(lse, false);
+    node->has_low = low.defined();
+    if (low.defined()) node->low = SavedVariable(low, false);
     node->has_lengths = len.defined(); node->has_mask = msk.defined();
     if (len.defined()) node->lengths = SavedVariable(len, false);
     if (msk.defined()) node->mask = SavedVariable(msk, false);

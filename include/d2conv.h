@@ -520,7 +520,9 @@ int d2c_rotary3d(const d2c_rotary3d_desc *desc, const void *x, const float *posi
  *     out[n,i,h] = sum_j softmax_j(scale * <query[n,i,h], key[n,j,h']>) value[n,j,h'],
  * j over the first key_lengths[n] keys (NULL: all; taken into 0 .. Lk) whose key_mask[n][j] is not 0 (NULL: all).  Keys and
  * values that are not to be read have no influence whatever they hold; a row without a key is 0, and so are its gradients.
- * out, grad_out and the gradients are contiguous.  `lse` [N, Hkv, Lq * Hq / Hkv] is for the backward call (NULL: not kept).
+ * out, grad_out and the gradients are contiguous.  `lse` [N, Hkv, Lq * Hq / Hkv] and, bfloat16, `out_low` (as out: what
+ * rounding took off it, which the gradients of queries and keys would miss) are for the backward call (NULL: not kept, and
+ * the backward call takes out_low as 0).
  * Results do not depend on the order in which workgroups run. */
 typedef struct d2c_attention_desc {
     int32_t N, Lq, Lk, Hq, Hkv, D, dtype;
@@ -529,12 +531,12 @@ typedef struct d2c_attention_desc {
 } d2c_attention_desc;
 size_t d2c_attention_forward_workspace_bytes(const d2c_attention_desc *desc);
 int d2c_attention_forward(const d2c_attention_desc *desc, const void *query, const void *key, const void *value,
-                          const int32_t *key_lengths, const uint8_t *key_mask, void *out, float *lse, void *workspace,
-                          size_t workspace_bytes, void *stream);
+                          const int32_t *key_lengths, const uint8_t *key_mask, void *out, void *out_low, float *lse,
+                          void *workspace, size_t workspace_bytes, void *stream);
 size_t d2c_attention_backward_workspace_bytes(const d2c_attention_desc *desc);
 int d2c_attention_backward(const d2c_attention_desc *desc, const void *grad_out, const void *query, const void *key,
                            const void *value, const int32_t *key_lengths, const uint8_t *key_mask, const void *out,
-                           const float *lse, void *grad_query, void *grad_key, void *grad_value, void *workspace,
+                           const void *out_low, const float *lse, void *grad_query, void *grad_key, void *grad_value, void *workspace,
                            size_t workspace_bytes, void *stream);
 
 /* Test hook for the matrix-core backward pass: 1 (default) builds grad_input from

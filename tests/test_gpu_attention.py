@@ -279,6 +279,20 @@ def test_no_rows_or_no_keys(Lq, Lk, dev):
             assert not bool(t.any())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_key(dtype, dev):
+    """Its weight is 1 whatever the scores: the values' gradient is the sum of the rows', the others are 0 and nothing near it."""
+    for Lk, lengths, mask in ((1, None, None), (50, torch.tensor([1, 1]), None), (64, None, torch.arange(64).expand(2, 64) == torch.tensor([[63], [5]]))):
+        q, k, v, g = make(2, 70, Lk, 4, 2, 40, dtype, 37)
+        out, gq, gk, gv = run(dev, q, k, v, g, lengths, mask)
+        which = (0, 0) if mask is None else (63, 5)
+        for n in range(2):
+            assert torch.equal(out[n].cpu(), v[n, which[n]].repeat_interleave(2, 0).expand(70, 4, 40))
+        assert not bool(gq.any()) and not bool(gk.any())
+        want, bounds = reference(q, k, v, g, lengths, mask, 1.0 / math.sqrt(40))
+        check((out, gq, gk, gv), want, bounds, str(Lk))
+
+
 def test_only_some_gradients(dev):
     q, k, v, g = (t.to(dev) for t in make(1, 40, 90, 2, 2, 64, torch.bfloat16, 41))
     full = run(dev, q, k, v, g, None, None)[1:]
