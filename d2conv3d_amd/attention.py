@@ -46,15 +46,21 @@ def _long3(*v):
 
 
 # ---------------------------------------------------------------- layer norm
+def _rows(x):
+    """[rows, channels], in place where the rows lie at one distance, and that distance."""
+    x = x.reshape(-1, x.size(-1))
+    if x.stride(1) != 1 and x.size(1) > 1:
+        x = x.contiguous()
+    return x, x.stride(0)
+
+
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input, weight, bias, eps):
         lib, dev, C = _lib.load(), input.device, input.size(-1)
-        x = input.reshape(-1, C)           # (rows at one distance stay where they are)
-        if x.stride(1) != 1 and C > 1:
-            x = x.contiguous()
+        x, stride = _rows(input)
         params = weight if weight is not None else bias
-        desc = _lib.LayerNormDesc(x.size(0), x.stride(0), C, _DT[x.dtype], _DT[(x if params is None else params).dtype], eps)
+        desc = _lib.LayerNormDesc(x.size(0), stride, C, _DT[x.dtype], _DT[(x if params is None else params).dtype], eps)
         out = torch.empty(input.shape, dtype=x.dtype, device=dev)
         w = None if weight is None else weight.contiguous()
         b = None if bias is None else bias.contiguous()
@@ -62,7 +68,8 @@ class _LayerNormFunction(torch.autograd.Function):
         with torch.cuda.device(dev):
             rc = lib.d2c_layer_norm_forward(ctypes.byref(desc), _ptr(x), _ptr(w), _ptr(b), _ptr(out), _ptr(stats), _stream(dev))
         _lib.check(rc, "layer_norm forward")
-        ctx.save_for_backward(x, w, b, stats)
+        # (the input itself where its rows are read in place: a view made here would hide the input's version from autograd)
+        ctx.save_for_backward(input if x.data_ptr() == input.data_ptr() else x, w, b, stats)
         ctx.desc, ctx.shape = desc, input.shape
         return out
 
@@ -72,6 +79,7 @@ class _LayerNormFunction(torch.autograd.Function):
         lib = _lib.load()
         x, w, b, stats = ctx.saved_tensors
         desc, dev, need = ctx.desc, x.device, ctx.needs_input_grad
+        x, desc.x_stride = _rows(x)      # (strides of what came back: hooks of the caller may have put it elsewhere in the meantime)
         g = grad_out.to(x.dtype).contiguous()
         gx = torch.empty(ctx.shape, dtype=x.dtype, device=dev) if need[0] else None
         gw = torch.empty_like(w) if w is not None and need[1] else None
@@ -212,6 +220,8 @@ class _CrossAttentionFunction(torch.autograd.Function):
         lib = _lib.load()
         q, k, v, key_lengths, key_mask, out, low, lse = ctx.saved_tensors
         desc, dev, need = ctx.desc, q.device, ctx.needs_input_grad
+        q, k, v = (_inner_contiguous(t) for t in (q, k, v))
+        desc.q_stride, desc.k_stride, desc.v_stride = (_long3(*t.stride()[:3]) for t in (q, k, v))
         g = grad_out.to(q.dtype).contiguous()
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((q, k, v), need))
         with torch.cuda.device(dev):

@@ -5,7 +5,6 @@
 // their results are joined by attn_join_kernel.
 #include <mutex>
 #include <type_traits>
-#include <vector>
 #include "d2c_attention.hpp"
 
 using namespace d2c_attn;
@@ -624,18 +623,19 @@ int d2c_attn::resident(const void *kernel, int lds)
 {
     struct Known { const void *kernel; int dev, n; };
     static std::mutex mu;
-    static std::vector<Known> known;
+    static Known known[512];      // (fewer kernels than this on a device; what finds no place is asked for every time)
+    static int count = 0;
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) { (void)hipGetLastError(); return 2; }      // (no GPU: sizes are asked for all the same)
     std::lock_guard<std::mutex> lock(mu);
-    for (const Known &k : known)
-        if (k.kernel == kernel && k.dev == dev) return k.n;
+    for (int i = 0; i < count; i++)
+        if (known[i].kernel == kernel && known[i].dev == dev) return known[i].n;
     int n = 0;
     if (d2c_allow_lds(kernel, lds, "attention kernel") != D2C_OK || hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, lds) != hipSuccess || n < 1) {
         (void)hipGetLastError();
         n = 1;
     }
-    known.push_back({kernel, dev, n});
+    if (count < (int)(sizeof known / sizeof *known)) known[count++] = {kernel, dev, n};
     return n;
 }
 

@@ -299,7 +299,7 @@ D2C_DEV int keys_of(const Args &a, int n) { return a.lengths ? min(max(a.lengths
 // different orders leave.
 D2C_DEV bool one_key(const Args &a, int n, int keys)
 {
-    if (a.Lk > kExactKeys) return false;
+    if (keys > kExactKeys) return false;
     const int key = threadIdx.x & 63;
     return __popcll(__ballot(key < keys && (!a.mask || a.mask[(long)n * a.Lk + key]))) == 1;
 }

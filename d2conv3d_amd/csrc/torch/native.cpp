@@ -577,6 +577,25 @@ py::object dwconv3d(const Tensor &x, const Tensor &w, const opt_tensor &bias, in
 }
 
 // ---------------------------------------------------------------- layer_norm
+// (What a node has kept comes back with the strides that it was given, or with others where the caller's hooks put it elsewhere in the
+// meantime: strides are taken from what came back.)
+bool inner_contiguous(const Tensor &t) { return t.stride(t.dim() - 1) == 1 || t.size(t.dim() - 1) == 1; }
+Tensor with_inner_contiguous(const Tensor &t) { return inner_contiguous(t) ? t : t.contiguous(); }
+// The distance of a tensor's rows (all but the last dimension), or -1 where they lie at no single one
+int64_t row_stride(const Tensor &x)
+{
+    const int64_t nd = x.dim(), C = x.size(nd - 1);
+    if (x.stride(nd - 1) != 1 && C > 1) return -1;
+    int64_t step = -1, rows = 1;
+    for (int64_t i = nd - 2; i >= 0; i--) {
+        if (x.size(i) == 1) continue;
+        if (step < 0) step = x.stride(i);
+        else if (x.stride(i) != step * rows) return -1;
+        rows *= x.size(i);
+    }
+    return step < 0 ? C : step;
+}
+
 struct LayerNormBackward : public Node {
     d2c_layer_norm_desc q;
     SavedVariable x, w, b, stats;
@@ -594,10 +613,12 @@ struct LayerNormBackward : public Node {
         if (!grads[0].defined()) grads[0] = input_metadata(0).zeros_like();
         {
             at::NoGradGuard no_grad;
-            const Tensor vx = x.unpack(), vs = stats.unpack();
-            Tensor vw, vb;
-            if (has_w) vw = w.unpack();
-            if (has_b) vb = b.unpack();
+            Tensor vx = x.unpack(), vw, vb;
+            const Tensor vs = stats.unpack().contiguous();
+            if (has_w) vw = w.unpack().contiguous();
+            if (has_b) vb = b.unpack().contiguous();
+            if (row_stride(vx) < 0) vx = vx.contiguous();
+            q.x_stride = row_stride(vx);
             c10::DeviceGuard guard(vx.device());
             const hipStream_t st = stream_of(vx);
             const Tensor g = grads[0].contiguous();
@@ -613,21 +634,6 @@ struct LayerNormBackward : public Node {
         return r;
     }
 };
-
-// The distance of a tensor's rows (all but the last dimension), or -1 where they lie at no single one
-int64_t row_stride(const Tensor &x)
-{
-    const int64_t nd = x.dim(), C = x.size(nd - 1);
-    if (x.stride(nd - 1) != 1 && C > 1) return -1;
-    int64_t step = -1, rows = 1;
-    for (int64_t i = nd - 2; i >= 0; i--) {
-        if (x.size(i) == 1) continue;
-        if (step < 0) step = x.stride(i);
-        else if (x.stride(i) != step * rows) return -1;
-        rows *= x.size(i);
-    }
-    return step < 0 ? C : step;
-}
 
 py::object layer_norm(const Tensor &x, const opt_tensor &weight, const opt_tensor &bias, double eps)
 {
@@ -674,7 +680,6 @@ Tensor rotary_call(d2c_rotary3d_desc q, const Tensor &x, const Tensor &pos, int 
     check(d2c_rotary3d(&q, ptr(x), (const float *)ptr(pos), ptr(out), stream_of(x)), "rotary3d");
     return out;
 }
-bool inner_contiguous(const Tensor &t) { return t.stride(t.dim() - 1) == 1 || t.size(t.dim() - 1) == 1; }
 
 struct Rotary3dBackward : public Node {
     d2c_rotary3d_desc q;
@@ -694,9 +699,9 @@ struct Rotary3dBackward : public Node {
         {
             at::NoGradGuard no_grad;
             Tensor vp;
-            if (has_pos) vp = pos.unpack();
+            if (has_pos) vp = pos.unpack().contiguous();
             c10::DeviceGuard guard(grads[0].device());
-            if (should_compute_output(0)) r[0] = rotary_call(q, inner_contiguous(grads[0]) ? grads[0] : grads[0].contiguous(), vp, -1);
+            if (should_compute_output(0)) r[0] = rotary_call(q, with_inner_contiguous(grads[0]), vp, -1);
         }
         once_differentiable(r, grads[0]);
         return r;
@@ -743,6 +748,11 @@ py::object rotary3d(const Tensor &x, const opt_tensor &positions, int3_t grid, i
 }
 
 // ---------------------------------------------------------------- cross_attention
+void strides(d2c_attention_desc &q, const Tensor &query, const Tensor &key, const Tensor &value)
+{
+    for (int i = 0; i < 3; i++) { q.q_stride[i] = query.stride(i); q.k_stride[i] = key.stride(i); q.v_stride[i] = value.stride(i); }
+}
+
 struct CrossAttentionBackward : public Node {
     d2c_attention_desc q;
     SavedVariable query, key, value, lengths, mask, out, low, lse;
@@ -760,11 +770,13 @@ struct CrossAttentionBackward : public Node {
         if (!grads[0].defined()) grads[0] = input_metadata(0).zeros_like();
         {
             at::NoGradGuard no_grad;
-            const Tensor vq = query.unpack(), vk = key.unpack(), vv = value.unpack(), vo = out.unpack(shared_from_this()), vl = lse.unpack();
+            const Tensor vq = with_inner_contiguous(query.unpack()), vk = with_inner_contiguous(key.unpack()), vv = with_inner_contiguous(value.unpack());
+            const Tensor vo = out.unpack(shared_from_this()).contiguous(), vl = lse.unpack().contiguous();
             Tensor len, msk, vlow;
-            if (has_low) vlow = low.unpack();
-            if (has_lengths) len = lengths.unpack();
-            if (has_mask) msk = mask.unpack();
+            if (has_low) vlow = low.unpack().contiguous();
+            if (has_lengths) len = lengths.unpack().contiguous();
+            if (has_mask) msk = mask.unpack().contiguous();
+            strides(q, vq, vk, vv);
             c10::DeviceGuard guard(vq.device());
             const hipStream_t st = stream_of(vq);
             const Tensor g = grads[0].contiguous();
@@ -804,7 +816,7 @@ py::object cross_attention(const Tensor &query, const Tensor &key, const Tensor 
     const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.D);
     if (!(s > 0.0) || !((float)s > 0.f) || !((float)s < INFINITY)) return py::none();
     q.scale = (float)s;
-    for (int i = 0; i < 3; i++) { q.q_stride[i] = query.stride(i); q.k_stride[i] = key.stride(i); q.v_stride[i] = value.stride(i); }
+    strides(q, query, key, value);
     if (len.defined() && (!plain(len) || len.device() != query.device() || len.scalar_type() != at::kInt || len.dim() != 1 || len.size(0) != q.N)) return py::none();
     if (msk.defined() && (!plain(msk) || msk.device() != query.device() || msk.scalar_type() != at::kBool || msk.dim() != 2 || msk.size(0) != q.N || msk.size(1) != q.Lk))
         return py::none();

@@ -282,7 +282,7 @@ def test_no_rows_or_no_keys(Lq, Lk, dev):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_one_key(dtype, dev):
     """Its weight is 1 whatever the scores: the values' gradient is the sum of the rows', the others are 0 and nothing near it."""
-    for Lk, lengths, mask in ((1, None, None), (50, torch.tensor([1, 1]), None), (64, None, torch.arange(64).expand(2, 64) == torch.tensor([[63], [5]]))):
+    for Lk, lengths, mask in ((1, None, None), (50, torch.tensor([1, 1]), None), (300, torch.tensor([1, 1]), None), (64, None, torch.arange(64).expand(2, 64) == torch.tensor([[63], [5]]))):
         q, k, v, g = make(2, 70, Lk, 4, 2, 40, dtype, 37)
         out, gq, gk, gv = run(dev, q, k, v, g, lengths, mask)
         which = (0, 0) if mask is None else (63, 5)
