@@ -201,7 +201,7 @@ template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __laun
     if (row >= a.rows) return;
     if (unit.splits > 1) {
         const long at = ((long)unit.split * a.shared + unit.part) * Shape::ROWS + tile_row;
-        float *po = a.part + at * a.D;
+        float *po = a.part + at * part_width(a.D);
 #pragma unroll
         for (int i = 0; i < ND; i++)
 #pragma unroll
@@ -421,7 +421,7 @@ template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bou
         }
         if (unit.splits > 1) {
             const long at = ((long)unit.split * a.shared + unit.part) * R + r;
-            a.part[at * a.D + d] = x;
+            a.part[at * part_width(a.D) + d] = x;
             if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(top, sum);
         } else {
             const float y = sum == 0.f ? 0.f : x / sum;
@@ -433,30 +433,49 @@ template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bou
     }
 }
 
-// The partial results of `splits` workgroups.  LANES lanes take four of a row's columns each, `groups` (a power of two) of them the splits in turn; their sums
-// meet in LDS.  Latency counts: 16 rows of 102 splits 13.6 us as a wavefront each that walks over them, 4.8 as here.
+// The partial results of `splits` workgroups.  LANES lanes take four of a row's columns each, `groups` (a power of two) of them the splits in turn, four
+// requested at a time (eight are no quicker); their sums meet in LDS.  Latency counts: 16 rows of 102 splits 13.6 us as a wavefront each that walks over them, 4.6
+// as here; 26624 rows of 7 splits of 64 columns 11.5 us (4.1 TB/s of the 48 MB), 22 with as many groups as there are splits for.
 template <typename T, int LANES> __global__ void __launch_bounds__(256) attn_join_kernel(Args a, int groups, int tile_rows)
 {
     __shared__ float4 s_x[256];
     __shared__ float2 s_ml[256];
     const int per = 256 / (LANES * groups), lane = threadIdx.x % LANES, group = threadIdx.x / LANES % groups;
-    const long total = (long)a.shared * tile_rows, at = (long)blockIdx.x * per + threadIdx.x / (LANES * groups);
-    const int part = (int)(at / tile_rows), unit = a.whole + part, heads = a.N * a.Hkv, tile = unit / heads, nh = unit - tile * heads;
-    const int row = tile * tile_rows + (int)(at - (long)part * tile_rows);
+    const int total = a.shared * tile_rows, at = (int)blockIdx.x * per + threadIdx.x / (LANES * groups);
+    const int part = at / tile_rows, unit = a.whole + part, heads = a.N * a.Hkv, tile = unit / heads, nh = unit - tile * heads;
+    const int row = tile * tile_rows + at - part * tile_rows;
     const bool live = at < total && row < a.rows;
     const int d = lane * 4;
     float all = -INFINITY, l = 0.f;
     float x[4] = {0.f, 0.f, 0.f, 0.f};
     if (live) {
-#pragma unroll 4
-        for (int s = group; s < a.splits; s += groups) {
-            const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (s * total + at) * 2);
-            const float4 y = __builtin_bit_cast(float4, d < a.D ? load_run<float>(a.part + (s * total + at) * a.D + d, a.D - d) : make_uint4(0, 0, 0, 0));
-            const float top = fmaxf(all, ml.x), base = top == -INFINITY ? 0.f : top;
-            const float f = __builtin_amdgcn_exp2f(all - base), g = __builtin_amdgcn_exp2f(ml.x - base);
+        for (int s0 = group; s0 < a.splits; s0 += 4 * groups) {
+            float2 ml[4];
+            float4 y[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const long from = (long)min(s0 + u * groups, a.splits - 1) * total + at;
+                ml[u] = *reinterpret_cast<const float2 *>(a.part_ml + from * 2);
+                y[u] = *reinterpret_cast<const float4 *>(a.part + from * part_width(a.D) + min(d, part_width(a.D) - 4));
+            }
+            float top = all;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (s0 + u * groups >= a.splits) ml[u] = make_float2(-INFINITY, 0.f);
+                top = fmaxf(top, ml[u].x);
+            }
+            const float base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(all - base);
             all = top;
-            l = l * f + ml.y * g;
-            x[0] = x[0] * f + y.x * g; x[1] = x[1] * f + y.y * g; x[2] = x[2] * f + y.z * g; x[3] = x[3] * f + y.w * g;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] *= f;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (s0 + u * groups >= a.splits) continue;
+                const float g = __builtin_amdgcn_exp2f(ml[u].x - base);
+                l = fmaf(ml[u].y, g, l);
+                x[0] = fmaf(y[u].x, g, x[0]); x[1] = fmaf(y[u].y, g, x[1]); x[2] = fmaf(y[u].z, g, x[2]); x[3] = fmaf(y[u].w, g, x[3]);
+            }
         }
     }
     s_x[threadIdx.x] = make_float4(x[0], x[1], x[2], x[3]);
@@ -543,16 +562,18 @@ template <typename T> FwdPlan fwd_plan(const d2c_attention_desc &q)
         return 0;
     });
     const size_t lines = (size_t)p.walks.splits * p.walks.shared * p.tile_rows;
-    p.part_bytes = d2c_align_up(lines * q.D * 4);
+    p.part_bytes = d2c_align_up(lines * part_width(q.D) * 4);
     p.bytes = p.part_bytes + d2c_align_up(lines * 8);
     return p;
 }
 
 template <typename T, int LANES> int launch_join(const Args &a, int tile_rows, hipStream_t st)
 {
+    // (more lanes to a row only while all of them have a place at once)
+    const long total = (long)a.shared * tile_rows, places = 2048L * std::max(d2c_num_cus(), 1);
     int groups = 1;
-    while (groups * 2 <= std::min(a.splits, 256 / LANES)) groups *= 2;
-    const long total = (long)a.shared * tile_rows, per = 256 / (LANES * groups);
+    while (groups * 2 <= std::min(a.splits, 256 / LANES) && total * LANES * groups * 2 <= places) groups *= 2;
+    const long per = 256 / (LANES * groups);
     hipLaunchKernelGGL((attn_join_kernel<T, LANES>), dim3((unsigned)((total + per - 1) / per)), dim3(256), 0, st, a, groups, tile_rows);
     return d2c_check_launch("attn_join_kernel");
 }

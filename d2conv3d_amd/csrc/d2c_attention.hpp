@@ -326,6 +326,9 @@ template <typename T> D2C_DEV void store4(T *p, const float *v, int left)
     }
 }
 
+// Floats to a row of partial sums: whole pieces of 16 bytes (what is behind a row's end is read and dropped)
+inline __host__ __device__ int part_width(int D) { return (D + 3) & ~3; }
+
 // ... what storing them as T takes off
 template <typename T> D2C_DEV void store4_low(T *p, const float *v, int left)
 {

@@ -125,7 +125,7 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
     }
     if (!live) return;
     if (unit.splits > 1) {
-        float *p = a.part + (((long)unit.split * a.shared + unit.part) * 128 + tile_row) * a.D;
+        float *p = a.part + (((long)unit.split * a.shared + unit.part) * 128 + tile_row) * part_width(a.D);
 #pragma unroll
         for (int i = 0; i < ND; i++)
 #pragma unroll
@@ -303,8 +303,8 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
 #pragma unroll
             for (int r = 0; r < 4; r++) { x[r] = live && !alone ? dk[i][j * 4 + r] * fk : 0.f; y[r] = live ? dv[i][j * 4 + r] : 0.f; }
             if (unit.splits > 1) {
-                store4<float>(a.part + (((2L * unit.split) * a.shared + unit.part) * 128 + tile_key) * a.D + d, x, a.D - d);
-                store4<float>(a.part + (((2L * unit.split + 1) * a.shared + unit.part) * 128 + tile_key) * a.D + d, y, a.D - d);
+                store4<float>(a.part + (((2L * unit.split) * a.shared + unit.part) * 128 + tile_key) * part_width(a.D) + d, x, a.D - d);
+                store4<float>(a.part + (((2L * unit.split + 1) * a.shared + unit.part) * 128 + tile_key) * part_width(a.D) + d, y, a.D - d);
             } else {
                 const long at = (((long)hd.n * a.Lk + key) * a.Hkv + hd.h) * a.D + d;
                 if (a.gk) store4<T>(reinterpret_cast<T *>(a.gk) + at, x, a.D - d);
@@ -313,25 +313,39 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
         }
 }
 
-// Sums of the workgroups that shared a walk: part [splits][1 or 2][shared][128][D]
+// Sums of the workgroups that shared a walk: part [splits][1 or 2][shared][128][D].  A thread takes four of a row's columns, four splits requested at a time.
 template <typename T, bool KV> __global__ void __launch_bounds__(256) attn_bwd_join_kernel(Args a)
 {
-    const long total = (long)a.shared * 128 * a.D, at = (long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= total) return;
-    const long which = KV ? blockIdx.y : 0;
+    const int total = a.shared * 128, pieces = part_width(a.D) / 4;
+    const long index = (long)blockIdx.x * 256 + threadIdx.x;
+    const int line = (int)(index / pieces), d = (int)(index - (long)line * pieces) * 4;
+    if (line >= total) return;
+    const int which = KV ? blockIdx.y : 0;
     if (KV && !(which ? a.gv : a.gk)) return;
-    const int d = (int)(at % a.D), line = (int)(at / a.D), unit = a.whole + line / 128, heads = a.N * a.Hkv, tile = unit / heads, nh = unit - tile * heads;
+    const int unit = a.whole + line / 128, heads = a.N * a.Hkv, tile = unit / heads, nh = unit - tile * heads;
     const int i = tile * 128 + line % 128, n = nh / a.Hkv;
     if (i >= (KV ? a.Lk : a.rows)) return;
-    float x = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < a.splits; s++) x += a.part[(s * (KV ? 2L : 1L) + which) * total + at];
-    if (which == 0) x *= a.scale;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < a.splits; s0 += 4) {
+        float4 y[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            y[u] = *reinterpret_cast<const float4 *>(a.part + (((long)min(s0 + u, a.splits - 1) * (KV ? 2 : 1) + which) * total + line) * part_width(a.D) + d);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (s0 + u >= a.splits) continue;
+            x[0] += y[u].x; x[1] += y[u].y; x[2] += y[u].z; x[3] += y[u].w;
+        }
+    }
+    if (which == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] *= a.scale;
+    }
     const Head hd{n, nh - n * a.Hkv, nh};
     if constexpr (KV)
-        reinterpret_cast<T *>(which ? a.gv : a.gk)[(((long)n * a.Lk + i) * a.Hkv + hd.h) * a.D + d] = f32_to_elem<T>(x);
+        store4<T>(reinterpret_cast<T *>(which ? a.gv : a.gk) + (((long)n * a.Lk + i) * a.Hkv + hd.h) * a.D + d, x, a.D - d);
     else
-        const_cast<T *>(row_at<T>(a.gq, a.gs, a, hd, i))[d] = f32_to_elem<T>(x);
+        store4<T>(const_cast<T *>(row_at<T>(a.gq, a.gs, a, hd, i)) + d, x, a.D - d);
 }
 
 // delta alone, where the queries' gradient is not wanted: one wavefront to a row
@@ -369,7 +383,7 @@ template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
         return 0;
     });
     p.delta_bytes = d2c_align_up((size_t)heads * rows * 4);
-    const size_t unit = (size_t)128 * q.D * 4;
+    const size_t unit = (size_t)128 * part_width(q.D) * 4;
     p.bytes = p.delta_bytes + d2c_align_up(std::max(p.q.shared * p.q.splits * unit, 2 * p.kv.shared * p.kv.splits * unit));
     return p;
 }
@@ -386,7 +400,7 @@ template <typename T, int DP, int NK, bool WHOLE> int launch_bwd(Args a, const B
         hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NK, WHOLE>), dim3(workgroups(p.q)), dim3(256), lds, st, a);
         if (int rc = d2c_check_launch("attn_bwd_q_kernel")) return rc;
         if (p.q.shared > 0) {
-            hipLaunchKernelGGL((attn_bwd_join_kernel<T, false>), dim3((unsigned)(((long)p.q.shared * 128 * a.D + 255) / 256)), dim3(256), 0, st, a);
+            hipLaunchKernelGGL((attn_bwd_join_kernel<T, false>), dim3((unsigned)(((long)p.q.shared * 128 * (part_width(a.D) / 4) + 255) / 256)), dim3(256), 0, st, a);
             if (int rc = d2c_check_launch("attn_bwd_join_kernel")) return rc;
         }
     }
@@ -397,7 +411,7 @@ template <typename T, int DP, int NK, bool WHOLE> int launch_bwd(Args a, const B
     hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, NK, WHOLE>), dim3(workgroups(p.kv)), dim3(256), lds, st, a);
     if (int rc = d2c_check_launch("attn_bwd_kv_kernel")) return rc;
     if (p.kv.shared == 0) return D2C_OK;
-    hipLaunchKernelGGL((attn_bwd_join_kernel<T, true>), dim3((unsigned)(((long)p.kv.shared * 128 * a.D + 255) / 256), 2), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_bwd_join_kernel<T, true>), dim3((unsigned)(((long)p.kv.shared * 128 * (part_width(a.D) / 4) + 255) / 256), 2), dim3(256), 0, st, a);
     return d2c_check_launch("attn_bwd_join_kernel");
 }
 template <typename T> int backward(Args a, const d2c_attention_desc &q, void *ws, size_t ws_bytes, hipStream_t st)
