@@ -552,7 +552,6 @@ template <typename T> FwdPlan fwd_plan(const d2c_attention_desc &q)
     p.few = rows <= 32;
     if (p.token) for_token<T>(q, rows, [&](auto lanes, auto r, auto whole) {
         constexpr int LANES = decltype(lanes)::value, R = decltype(r)::value;
-        constexpr bool WHOLE = decltype(whole)::value;
         using Shape = TokenShape<T, LANES, R>;
         p.tile_rows = R;
         const long places = 2L * std::max(d2c_num_cus(), 1);

@@ -635,13 +635,14 @@ struct LayerNormBackward : public Node {
     }
 };
 
-py::object layer_norm(const Tensor &x, const opt_tensor &weight, const opt_tensor &bias, double eps)
+py::object layer_norm(const Tensor &input, const opt_tensor &weight, const opt_tensor &bias, double eps)
 {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-    if (!plain_strided(x) || x.dim() < 1 || x.numel() == 0 || x.size(-1) >= (1ll << 31)) return py::none();
+    if (!plain_strided(input) || input.dim() < 1 || input.numel() == 0 || input.size(-1) >= (1ll << 31)) return py::none();
+    const int dt = dtype_code(input);
+    if (dt != D2C_F32 && dt != D2C_BF16) return py::none();
+    const Tensor x = row_stride(input) < 0 ? input.detach().contiguous() : input;
     const int64_t C = x.size(-1), step = row_stride(x);
-    const int dt = dtype_code(x);
-    if (step < 0 || (dt != D2C_F32 && dt != D2C_BF16)) return py::none();
     int pdt = -1;
     for (const Tensor *t : {&w, &b}) {
         if (!t->defined()) continue;
@@ -651,11 +652,11 @@ py::object layer_norm(const Tensor &x, const opt_tensor &weight, const opt_tenso
         pdt = c;
     }
     d2c_layer_norm_desc q{x.numel() / C, step, (int)C, dt, pdt < 0 ? dt : pdt, (float)eps};
-    const bool grad = wants_grad(x, w, b);
+    const bool grad = wants_grad(input, w, b);
     std::shared_ptr<LayerNormBackward> node;
     if (grad) {
         node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
-        node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
+        node->set_next_edges(torch::autograd::collect_next_edges(input, w, b));
     }
     c10::DeviceGuard guard(x.device());
     const auto opt = x.options().requires_grad(false);
@@ -711,7 +712,7 @@ struct Rotary3dBackward : public Node {
 py::object rotary3d(const Tensor &x, const opt_tensor &positions, int3_t grid, int3_t pairs, double base, bool interleaved)
 {
     const Tensor pos = positions.value_or(Tensor());
-    if (!plain_strided(x) || x.dim() != 4 || x.numel() == 0 || !inner_contiguous(x)) return py::none();
+    if (!plain_strided(x) || x.dim() != 4 || x.numel() == 0) return py::none();
     const int dt = dtype_code(x);
     if (dt != D2C_F32 && dt != D2C_BF16) return py::none();
     for (int i = 0; i < 4; i++)
@@ -739,7 +740,7 @@ py::object rotary3d(const Tensor &x, const opt_tensor &positions, int3_t grid, i
         node->set_next_edges(torch::autograd::collect_next_edges(x));
     }
     c10::DeviceGuard guard(x.device());
-    Tensor out = rotary_call(q, x, pos, 1);
+    Tensor out = rotary_call(q, inner_contiguous(x) ? x : x.detach().contiguous(), pos, 1);
     if (!grad) return py::cast(out);
     node->q = q;
     node->has_pos = pos.defined();

@@ -127,6 +127,23 @@ def test_kept_tensors_that_come_back_with_other_strides(dtype, dev):
                     assert torch.equal(a, c)
 
 
+def test_tokens_of_a_feature_map(dev):
+    """Channels far apart (a map [N, C, T, H, W] as tokens): read as they are or copied, the results are the dense tensor's."""
+    (x, g, w, b, turn, tg) = (t.to(dev) for t in _rn(6, (2, 72, 41), (2, 41, 72), (72,), (72,), (2, 40, 42, 3), (2, 42, 3, 40)))
+    for fn, dense, grad in ((lambda t: d2c.layer_norm(t, w, b), lambda t: t.transpose(1, 2), g),
+                            (lambda t: d2c.rotary3d(t, (2, 3, 7)), lambda t: t.permute(0, 2, 3, 1), tg)):
+        base = x if grad is g else turn
+        for route in (contextlib.nullcontext, python_route):
+            with route():
+                far = base.clone().requires_grad_()
+                out = fn(dense(far))
+                out.backward(grad)
+                near = dense(base).contiguous().requires_grad_()
+                want = fn(near)
+                want.backward(grad)
+                assert torch.equal(out, want) and torch.equal(dense(far.grad), near.grad)
+
+
 @pytest.mark.parametrize("entry", ENTRIES)
 def test_a_changed_input_is_noticed(entry, dev):
     fn, tensors = ENTRIES[entry]
