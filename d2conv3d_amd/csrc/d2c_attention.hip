@@ -33,6 +33,9 @@ template <int WORDS> struct KeyBits {
 template <typename T, int DP, int WK, bool WHOLE> struct FwdShape {
     static constexpr int KW = sizeof(T) == 2 && WK == 1 ? 64 : 32, KT = KW * WK, ROWS = 32 * (4 / WK);
     using KV = Tile<T, DP, KT, 256, WHOLE>;
+    // wavefronts to a SIMD: one where three terms of wide rows and the sums of split keys do not fit half of the registers (20 rows of 8 heads of 128 reading
+    // 30000: 158 us spilled, 87.5 so; whole tiles of rows spill less, and one to a SIMD takes longer: 2048 reading 4096 227 us, 265)
+    static constexpr int WAVES = sizeof(T) == 4 && DP == 128 && WK > 1 ? 1 : 2;
     static constexpr int JOIN = WK > 1 ? 4 * 32 * (DP + 2) * 4 : 0;
     // two tiles of each where three workgroups of a compute unit have room for them: one barrier a tile
     static constexpr int BUFFERS = 4 * KV::BYTES <= 52 << 10 ? 2 : 1;
@@ -48,7 +51,7 @@ template <typename T, int DP, int WK, bool WHOLE> struct FwdShape {
 // exponentials 0.80 of the time, without the second product 0.80, without either's loads 0.95 each.
 // Measured, bfloat16: 12960 positions reading 25920, 8 heads of 64, 0.82 ms (0.84 PFLOP/s; a library product of 8192 cubed 1.27); 1620 reading 64800, 8 heads of
 // 128 that share 2 key heads, 0.46 ms with the join (0.94 PFLOP/s).  float32: 1417 reading 3001, 6 heads of 40, 44 us.
-template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __launch_bounds__(256, 2) attn_fwd_kernel(Args a)
+template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __launch_bounds__(256, (FwdShape<T, DP, WK, WHOLE>::WAVES)) attn_fwd_kernel(Args a)
 {
     using Shape = FwdShape<T, DP, WK, WHOLE>;
     using KV = typename Shape::KV;
