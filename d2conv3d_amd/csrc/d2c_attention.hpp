@@ -223,8 +223,8 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
 };
 
 // Widths that kernels are made for: channels of a tile, a multiple of 32 (the products' columns), and steps of 16 of the products over channels.
-// float32, whose steps are six instructions each, leaves out a last one that heads do not reach (1417 on 3001 positions of 6 heads of 40 channels: the three
-// kernels 210, 181 us).
+// A last step that heads do not reach is left out (8000 on 8000 positions of 8 heads, bfloat16, forward and backward, us: 40 channels 203 + 586, 191 + 557; 104
+// channels 274 + 981, 266 + 856; 1417 on 3001 of 6 heads of 40, float32: the three kernels 210, 181).
 template <int DP_, int NK_> struct Width { static constexpr int DP = DP_, NK = NK_; };
 // Whether a problem runs on the kernels that load whole pieces by offsets of 32 bits: of a tile of 128 keys at most, of all rows (and, bfloat16, take one term of
 // the weights)
@@ -243,8 +243,7 @@ template <typename T, bool GRADIENTS, typename F> auto for_width(const d2c_atten
     auto pick = [&](auto width) {
         using W = decltype(width);
         if (!fast_kernels(q, GRADIENTS)) return f(width, std::false_type{});
-        if constexpr (sizeof(T) == 4)
-            if (D <= W::DP - 16) return f(Width<W::DP, W::NK - 1>{}, std::true_type{});
+        if (D <= W::DP - 16) return f(Width<W::DP, W::NK - 1>{}, std::true_type{});
         return f(width, std::true_type{});
     };
     if (D <= 32) return pick(Width<32, 2>{});
