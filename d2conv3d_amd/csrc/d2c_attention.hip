@@ -51,13 +51,14 @@ template <typename T, int DP, int WK, bool WHOLE> struct FwdShape {
 // exponentials 0.80 of the time, without the second product 0.80, without either's loads 0.95 each.
 // Measured, bfloat16: 12960 positions reading 25920, 8 heads of 64, 0.82 ms (0.84 PFLOP/s; a library product of 8192 cubed 1.27); 1620 reading 64800, 8 heads of
 // 128 that share 2 key heads, 0.46 ms with the join (0.94 PFLOP/s).  float32: 1417 reading 3001, 6 heads of 40, 44 us.
-template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __launch_bounds__(256, (FwdShape<T, DP, WK, WHOLE>::WAVES)) attn_fwd_kernel(Args a)
+template <typename T, int DP, int NP, int WK, bool WHOLE> __global__ void __launch_bounds__(256, (FwdShape<T, DP, WK, WHOLE>::WAVES)) attn_fwd_kernel(Args a)
 {
     using Shape = FwdShape<T, DP, WK, WHOLE>;
     using KV = typename Shape::KV;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = (KT + 63) / 64;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = (KT + 63) / 64;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = Shape::BUFFERS;
+    constexpr bool END = WHOLE && NP % 2 == 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK;
     const Unit unit = unit_of(a);
     const Head hd = unit.head;
@@ -112,8 +113,8 @@ template <typename T, int DP, int NK, int WK, bool WHOLE> __global__ void __laun
         unsigned char *s_k = lds + (BUFFERS == 2 ? buffer * 2 * KV::BYTES : 0), *s_v = s_k + KV::BYTES;
         buffer ^= 1;
         if constexpr (BUFFERS == 1) __syncthreads();
-        k.store(s_k);
-        v.store(s_v);
+        k.template store<END>(s_k, a.D);
+        v.template store<false>(s_v, a.D);      // (its piece behind the end makes columns of o that are not stored)
         __syncthreads();
         if (t + 1 < t1) {
             bits.words(next);
@@ -314,9 +315,8 @@ template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bou
     float o[R][VEC], m[R], l[R];      // (m: of the scores in units of scale * log2(e))
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        const bool live = d0 < a.D && r < a.rows;      // (zeros against what a load behind a row's end repeats)
         const uint4 w = load(row_at<T>(a.q, a.qs, a, hd, min(r, a.rows - 1)));
-        q[r] = live ? w : make_uint4(0, 0, 0, 0);
+        q[r] = r < a.rows ? w : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < VEC; i++) o[r][i] = 0.f;
         m[r] = -INFINITY;
@@ -328,9 +328,12 @@ template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bou
 #pragma unroll
         for (int u = 0; u < LOADS; u++) {
             vw[u] = there[u] ? v[u] : make_uint4(0, 0, 0, 0);
+            // (a lane behind a row's end has its last piece again, which is no part of the score)
+            uint4 kw = k[u];
+            if (WHOLE && a.D < DP && d0 >= a.D) kw = make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                const float x = lanes_sum<LANES>(dot_words<T>(q[r], k[u])) * a.scale2;
+                const float x = lanes_sum<LANES>(dot_words<T>(q[r], kw)) * a.scale2;
                 s[u][r] = there[u] ? x : -INFINITY;
             }
         }
@@ -563,13 +566,13 @@ template <typename T> FwdPlan fwd_plan(const d2c_attention_desc &q)
         return 0;
     });
     else for_shape<T>(q, p.few, [&](auto width, auto wk, auto whole) {
-        constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK, WK = decltype(wk)::value;
+        constexpr int DP = decltype(width)::DP, NP = decltype(width)::NP, WK = decltype(wk)::value;
         constexpr bool WHOLE = decltype(whole)::value;
         using Shape = FwdShape<T, DP, WK, WHOLE>;
         p.tile_rows = Shape::ROWS;
         const long units = heads * ((rows + Shape::ROWS - 1) / Shape::ROWS), steps = (q.Lk + Shape::KT - 1) / Shape::KT;
         const long places = (long)std::max(d2c_num_cus(), 1) *
-            resident(reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, NK, WK, WHOLE>), Shape::LDS);
+            resident(reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, NP, WK, WHOLE>), Shape::LDS);
         // (a step: 64 keys of 64 channels take 2 us with every place taken, float32's six products three times as long)
         p.walks = plan_walks(units, steps, places, 2.0 * Shape::KT / 64 * DP / 64 * (sizeof(T) == 2 ? 1 : 3) / WK, (double)Shape::ROWS * q.D * 4);
         return 0;
@@ -596,11 +599,11 @@ template <typename T> int launch_fwd(const d2c_attention_desc &q, const Args &a,
         hipLaunchKernelGGL((attn_token_kernel<T, decltype(lanes)::value, decltype(r)::value, decltype(whole)::value>), dim3(workgroups(p.walks)), dim3(256), 0, st, a);
         return d2c_check_launch("attn_token_kernel");
     }) : for_shape<T>(q, p.few, [&](auto width, auto wk, auto whole) {
-        constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK, WK = decltype(wk)::value;
+        constexpr int DP = decltype(width)::DP, NP = decltype(width)::NP, WK = decltype(wk)::value;
         constexpr bool WHOLE = decltype(whole)::value;
         constexpr int lds = FwdShape<T, DP, WK, WHOLE>::LDS;
-        if (int e = d2c_allow_lds(reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, NK, WK, WHOLE>), lds, "attn_fwd_kernel")) return e;
-        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NK, WK, WHOLE>), dim3(workgroups(p.walks)), dim3(256), lds, st, a);
+        if (int e = d2c_allow_lds(reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, NP, WK, WHOLE>), lds, "attn_fwd_kernel")) return e;
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, NP, WK, WHOLE>), dim3(workgroups(p.walks)), dim3(256), lds, st, a);
         return d2c_check_launch("attn_fwd_kernel");
     });
     if (rc || p.walks.shared == 0) return rc;

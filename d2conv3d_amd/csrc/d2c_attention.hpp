@@ -159,8 +159,8 @@ template <int DP> D2C_DEV int piece_at(int row, int piece) { return row * (DP * 
 
 typedef short v4s_t __attribute__((ext_vector_type(4)));
 
-// WHOLE (heads are whole pieces, rows near enough for offsets of 32 bits): loads without branches.  Pieces behind a row's end then repeat its last one: they meet
-// zeros of the other operand, or make columns that are not stored.  Else elements behind the end are zeros.
+// WHOLE (heads are whole pieces, rows near enough for offsets of 32 bits): loads without branches.  Pieces behind a row's end then repeat its last one and make
+// columns that are not stored.  Else elements behind the end are zeros.
 template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
     static constexpr int P = kTerms<T>, PIECES = DP / 8, PER = (ROWS * PIECES + THREADS - 1) / THREADS;
     static constexpr int TERM = ROWS * DP * 2, BYTES = P * TERM;
@@ -185,13 +185,20 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
 #pragma unroll
         for (int i = 0; i < PER; i++) r[i] = load8<true, T>(reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + off[i]), 8);
     }
-    D2C_DEV void store(unsigned char *lds) const
+    // END: the piece at column D, which a product's last step takes in, as zeros (those of the other operand do not undo an infinity that is repeated)
+    template <bool END> D2C_DEV void store(unsigned char *lds, int D) const
     {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int at = i * THREADS + threadIdx.x;
             if (ROWS * PIECES % THREADS != 0 && at >= ROWS * PIECES) continue;
-            const Frag<P> f = terms_of<T>(r[i]);
+            Raw8<T> x = r[i];
+            if constexpr (END) {
+#pragma unroll
+                for (int j = 0; j < (int)sizeof(T) / 2; j++)
+                    if (at % PIECES * 8 == D) x.v[j] = make_uint4(0, 0, 0, 0);
+            }
+            const Frag<P> f = terms_of<T>(x);
 #pragma unroll
             for (int t = 0; t < P; t++)
                 *reinterpret_cast<uint4 *>(lds + t * TERM + piece_at<DP>(at / PIECES, at % PIECES)) = f.t[t];
@@ -222,10 +229,12 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
     }
 };
 
-// Widths that kernels are made for: channels of a tile, a multiple of 32 (the products' columns), and steps of 16 of the products over channels.
+// Widths that kernels are made for: channels of a tile, a multiple of 32 (the products' columns), and pieces of 8 that heads have (the widest's where they are no
+// whole pieces).  The products over channels take NK steps of 16, the last of which may have one piece alone (END).
 // A last step that heads do not reach is left out (8000 on 8000 positions of 8 heads, bfloat16, forward and backward, us: 40 channels 203 + 586, 191 + 557; 104
 // channels 274 + 981, 266 + 856; 1417 on 3001 of 6 heads of 40, float32: the three kernels 210, 181).
-template <int DP_, int NK_> struct Width { static constexpr int DP = DP_, NK = NK_; };
+template <int DP_, int NP_> struct Width { static constexpr int DP = DP_, NP = NP_; };
+template <int NP> constexpr int kSteps = (NP + 1) / 2;
 // Whether a problem runs on the kernels that load whole pieces by offsets of 32 bits: of a tile of 128 keys at most, of all rows (and, bfloat16, take one term of
 // the weights)
 inline bool fast_kernels(const d2c_attention_desc &q, bool gradients)
@@ -239,17 +248,19 @@ inline bool fast_kernels(const d2c_attention_desc &q, bool gradients)
 }
 template <typename T, bool GRADIENTS, typename F> auto for_width(const d2c_attention_desc &q, F f)      // f(Width, fast_kernels)
 {
-    const int D = q.D;
-    auto pick = [&](auto width) {
-        using W = decltype(width);
-        if (!fast_kernels(q, GRADIENTS)) return f(width, std::false_type{});
-        if (D <= W::DP - 16) return f(Width<W::DP, W::NK - 1>{}, std::true_type{});
-        return f(width, std::true_type{});
+    const int pieces = (q.D + 7) / 8;
+    auto pick = [&](auto width) {      // (of the four widths with as many channels)
+        constexpr int DP = decltype(width)::DP, NP = DP / 8;
+        if (!fast_kernels(q, GRADIENTS)) return f(Width<DP, NP>{}, std::false_type{});
+        if (pieces == NP - 3) return f(Width<DP, NP - 3>{}, std::true_type{});
+        if (pieces == NP - 2) return f(Width<DP, NP - 2>{}, std::true_type{});
+        if (pieces == NP - 1) return f(Width<DP, NP - 1>{}, std::true_type{});
+        return f(Width<DP, NP>{}, std::true_type{});
     };
-    if (D <= 32) return pick(Width<32, 2>{});
-    if (D <= 64) return pick(Width<64, 4>{});
-    if (D <= 96) return pick(Width<96, 6>{});
-    return pick(Width<128, 8>{});
+    if (pieces <= 4) return pick(Width<32, 4>{});
+    if (pieces <= 8) return pick(Width<64, 8>{});
+    if (pieces <= 12) return pick(Width<96, 12>{});
+    return pick(Width<128, 16>{});
 }
 
 // What the workgroups do: units, each the walk of one tile of rows (or keys) of one key head along the other axis.  As many as

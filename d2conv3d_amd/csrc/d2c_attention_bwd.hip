@@ -23,12 +23,13 @@ template <typename T, int DP, bool WHOLE> struct QShape {
 // (K read twice, by rows and by columns).  Bound: as there, matrix instructions first (3 products to one exponential).
 // Measured, bfloat16: 12960 rows, 25920 keys, 8 heads of 64, 1.04 ms (0.99 PFLOP/s); 1620 rows, 12960 keys (3/4 of them read), 2 samples, 0.13 ms.
 // float32: 1417 rows, 3001 keys, 6 heads of 40, 62 us.
-template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bounds__(256, (QShape<T, DP, WHOLE>::WAVES)) attn_bwd_q_kernel(Args a)
+template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, (QShape<T, DP, WHOLE>::WAVES)) attn_bwd_q_kernel(Args a)
 {
     using KV = typename QShape<T, DP, WHOLE>::KV;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, KT = QShape<T, DP, WHOLE>::KT;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, KT = QShape<T, DP, WHOLE>::KT;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = QShape<T, DP, WHOLE>::BUFFERS;
+    constexpr bool END = WHOLE && NP % 2 == 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const Unit unit = unit_of(a);
     const Head hd = unit.head;
@@ -90,8 +91,8 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
         unsigned char *s_k = lds + (BUFFERS == 2 ? buffer * 2 * KV::BYTES : 0), *s_v = s_k + KV::BYTES;
         buffer ^= 1;
         if constexpr (BUFFERS == 1) __syncthreads();
-        k.store(s_k);
-        v.store(s_v);
+        k.template store<END>(s_k, a.D);
+        v.template store<false>(s_v, a.D);      // (an infinite value leaves no gradient of its row defined, whatever it meets)
         __syncthreads();
         if (t + 1 < t1) {
             next[0] = __ballot(b);
@@ -168,10 +169,10 @@ template <typename T, int DP, bool WHOLE> struct KvShape {
 // 1.5 times as long at 64 channels: the LDS is read six times a tile then.  Bound: matrix instructions (4 products to one exponential), behind them LDS.
 // Measured, bfloat16: 12960 rows, 25920 keys, 8 heads of 64, 1.38 ms (1.0 PFLOP/s); 1620 rows, 12960 keys (3/4 of them read), 2 samples, 0.21 ms.
 // float32: 1417 rows, 3001 keys, 6 heads of 40, 75 us.
-template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bounds__(256, (KvShape<T, DP, WHOLE>::WAVES)) attn_bwd_kv_kernel(Args a)
+template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, (KvShape<T, DP, WHOLE>::WAVES)) attn_bwd_kv_kernel(Args a)
 {
     using QG = typename KvShape<T, DP, WHOLE>::QG;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, RT = KvShape<T, DP, WHOLE>::RT;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, RT = KvShape<T, DP, WHOLE>::RT;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = KvShape<T, DP, WHOLE>::BUFFERS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -231,7 +232,7 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
         typename Shape::V tile;
         const T *vb = reinterpret_cast<const T *>(a.v) + hd.n * a.vs[0] + hd.h * a.vs[2];
         tile.load(a.D, [&](int i) INLINE { return vb + (long)min(key0 + i, a.Lk - 1) * a.vs[1]; });
-        tile.store(s_v);      // (a key that is not to be read: a column of its own, see below)
+        tile.template store<false>(s_v, a.D);      // (a key that is not to be read: a column of its own, see below)
     }
     {
         const long at = min(key, a.Lk - 1);
@@ -257,8 +258,8 @@ template <typename T, int DP, int NK, bool WHOLE> __global__ void __launch_bound
         float *s_lse = reinterpret_cast<float *>(s_q + 2 * QG::BYTES), *s_delta = s_lse + RT;
         buffer ^= 1;
         if constexpr (BUFFERS == 1) __syncthreads();
-        q.store(s_q);
-        g.store(s_g);
+        q.template store<false>(s_q, a.D);      // (an infinite query has no defined weights, an infinite gradient no defined ds)
+        g.template store<false>(s_g, a.D);
         if (threadIdx.x < 2 * RT) s_lse[threadIdx.x] = stat;
         __syncthreads();
         if (t + 1 < t1) request(t + 1);
@@ -381,15 +382,15 @@ template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
     const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv, cus = std::max(d2c_num_cus(), 1);
     const double part = 128.0 * q.D * 4, slow = sizeof(T) == 2 ? 1 : 3;
     for_width<T, true>(q, [&](auto width, auto whole) {
-        constexpr int DP = decltype(width)::DP, NK = decltype(width)::NK;
+        constexpr int DP = decltype(width)::DP, NP = decltype(width)::NP;
         constexpr bool WHOLE = decltype(whole)::value;
         using Q = QShape<T, DP, WHOLE>;
         using KV = KvShape<T, DP, WHOLE>;
         // (a step with every place taken, 64 channels: 64 keys 2.4 us, 64 rows 2.8)
         p.q = plan_walks(heads * ((rows + 127) / 128), (q.Lk + Q::KT - 1) / Q::KT,
-                         cus * resident(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, NK, WHOLE>), Q::LDS), 2.4 * Q::KT / 64 * DP / 64 * slow, part);
+                         cus * resident(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, NP, WHOLE>), Q::LDS), 2.4 * Q::KT / 64 * DP / 64 * slow, part);
         p.kv = plan_walks(heads * ((q.Lk + 127) / 128), (rows + KV::RT - 1) / KV::RT,
-                          cus * resident(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, NK, WHOLE>), KV::LDS), 2.8 * KV::RT / 64 * DP / 64 * slow, 2 * part);
+                          cus * resident(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, NP, WHOLE>), KV::LDS), 2.8 * KV::RT / 64 * DP / 64 * slow, 2 * part);
         return 0;
     });
     p.delta_bytes = d2c_align_up((size_t)heads * rows * 4);
@@ -398,16 +399,16 @@ template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
     return p;
 }
 
-template <typename T, int DP, int NK, bool WHOLE> int launch_bwd(Args a, const BwdPlan &p, hipStream_t st)
+template <typename T, int DP, int NP, bool WHOLE> int launch_bwd(Args a, const BwdPlan &p, hipStream_t st)
 {
     if (a.Lq > 0 && !a.gq && (a.gk || a.gv)) {
         hipLaunchKernelGGL(attn_delta_kernel<T>, dim3((unsigned)(((long)a.N * a.Hkv * a.rows + 3) / 4)), dim3(256), 0, st, a);
         if (int rc = d2c_check_launch("attn_delta_kernel")) return rc;
     } else if (a.Lq > 0 && a.gq) {
         constexpr int lds = QShape<T, DP, WHOLE>::LDS;
-        if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, NK, WHOLE>), lds, "attn_bwd_q_kernel")) return rc;
+        if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, NP, WHOLE>), lds, "attn_bwd_q_kernel")) return rc;
         set_walks(a, p.q);
-        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NK, WHOLE>), dim3(workgroups(p.q)), dim3(256), lds, st, a);
+        hipLaunchKernelGGL((attn_bwd_q_kernel<T, DP, NP, WHOLE>), dim3(workgroups(p.q)), dim3(256), lds, st, a);
         if (int rc = d2c_check_launch("attn_bwd_q_kernel")) return rc;
         if (p.q.shared > 0) {
             hipLaunchKernelGGL((attn_bwd_join_kernel<T, false>), dim3((unsigned)(((long)p.q.shared * 128 * (part_width(a.D) / 4) + 255) / 256)), dim3(256), 0, st, a);
@@ -416,9 +417,9 @@ template <typename T, int DP, int NK, bool WHOLE> int launch_bwd(Args a, const B
     }
     if (a.Lk == 0 || !(a.gk || a.gv)) return D2C_OK;
     constexpr int lds = KvShape<T, DP, WHOLE>::LDS;
-    if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, NK, WHOLE>), lds, "attn_bwd_kv_kernel")) return rc;
+    if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, NP, WHOLE>), lds, "attn_bwd_kv_kernel")) return rc;
     set_walks(a, p.kv);
-    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, NK, WHOLE>), dim3(workgroups(p.kv)), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((attn_bwd_kv_kernel<T, DP, NP, WHOLE>), dim3(workgroups(p.kv)), dim3(256), lds, st, a);
     if (int rc = d2c_check_launch("attn_bwd_kv_kernel")) return rc;
     if (p.kv.shared == 0) return D2C_OK;
     hipLaunchKernelGGL((attn_bwd_join_kernel<T, true>), dim3((unsigned)(((long)p.kv.shared * 128 * (part_width(a.D) / 4) + 255) / 256), 2), dim3(256), 0, st, a);
@@ -432,7 +433,7 @@ template <typename T> int backward(Args a, const d2c_attention_desc &q, void *ws
         return D2C_ERR_WORKSPACE;
     }
     a.delta = (float *)ws; a.part = (float *)((char *)ws + p.delta_bytes);
-    return for_width<T, true>(q, [&](auto width, auto whole) { return launch_bwd<T, decltype(width)::DP, decltype(width)::NK, decltype(whole)::value>(a, p, st); });
+    return for_width<T, true>(q, [&](auto width, auto whole) { return launch_bwd<T, decltype(width)::DP, decltype(width)::NP, decltype(whole)::value>(a, p, st); });
 }
 
 }  // namespace

@@ -1,0 +1,41 @@
+"""Infinite values among what cross_attention reads, where the definition has a finite result all the same.  A key with a channel of -infinity that meets
+positive queries has scores of -infinity: its weight is 0, as if it were not to be read.  Outputs and gradients are those of the call without it, but for the
+queries' gradient in that channel, where 0 times infinity is no number.  Bounds: test_gpu_attention.py."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_attention import check, make, reference, run
+
+pytestmark = pytest.mark.gpu
+
+
+def without_weight(sizes, D, dtype, channel, masked, dev):
+    N, Lq, Lk, Hq, Hkv = sizes
+    q, k, v, g = make(*sizes, D, dtype, seed=sum(sizes) + D)
+    q[..., channel] = q[..., channel].abs() + 0.125
+    gen = torch.Generator().manual_seed(11)
+    mask = torch.rand(N, Lk, generator=gen) < 0.7 if masked else torch.ones(N, Lk, dtype=torch.bool)
+    gone = mask & (torch.rand(N, Lk, generator=gen) < 0.2)
+    assert bool(gone.any()) and bool((mask & ~gone).any(1).all())
+    want, bounds = reference(q, k, v, g, None, mask & ~gone, 1.0 / math.sqrt(D))
+    k[..., channel][gone] = -math.inf
+    got = run(dev, q, k, v, g, None, mask if masked else None)
+    assert bool(got[1][..., channel].isnan().all())
+    rest = [c for c in range(D) if c != channel]
+    got, want, bounds = ([t if i != 1 else t[..., rest] for i, t in enumerate(ts)] for ts in (got, want, bounds))
+    check(got, want, bounds, f"{sizes} {D} {channel} {masked}")
+    for i in (2, 3):
+        assert not bool(got[i].cpu()[gone].any())
+
+
+# (rows of a key head: up to 8, up to 32, more; few keys; more than 2^22 scores)
+SIZES = [(2, 1, 300, 2, 1), (2, 20, 300, 2, 2), (1, 200, 333, 2, 1), (2, 40, 60, 2, 1), (1, 1100, 2000, 2, 2)]
+
+
+@pytest.mark.parametrize("D", [8, 24, 33, 40, 56, 64, 72, 88, 104, 120, 128])
+def test_keys_at_minus_infinity_bfloat16(D, dev):
+    for sizes in SIZES:
+        for channel, masked in ((D - 1, False), (max(D - 6, 0), True), (0, False)):
+            without_weight(sizes, D, torch.bfloat16, channel, masked, dev)
