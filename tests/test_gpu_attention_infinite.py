@@ -1,11 +1,13 @@
 """Infinite values among what cross_attention reads, where the definition has a finite result all the same.  A key with a channel of -infinity that meets
 positive queries has scores of -infinity: its weight is 0, as if it were not to be read.  Outputs and gradients are those of the call without it, but for the
-queries' gradient in that channel, where 0 times infinity is no number.  Bounds: test_gpu_attention.py."""
+queries' gradient in that channel, where 0 times infinity is no number.  An infinite value makes its channel of the outputs infinite, and no
+other.  Bounds: test_gpu_attention.py."""
 import math
 
 import pytest
 import torch
 
+import d2conv3d_amd as d2c
 from test_gpu_attention import check, make, reference, run
 
 pytestmark = pytest.mark.gpu
@@ -39,3 +41,35 @@ def test_keys_at_minus_infinity_bfloat16(D, dev):
     for sizes in SIZES:
         for channel, masked in ((D - 1, False), (max(D - 6, 0), True), (0, False)):
             without_weight(sizes, D, torch.bfloat16, channel, masked, dev)
+
+
+@pytest.mark.parametrize("D", [8, 24, 33, 40, 64, 72, 96, 104, 128])
+def test_keys_at_minus_infinity_float32(D, dev):
+    for sizes in SIZES[:4]:
+        for channel, masked in ((D - 1, False), (max(D - 6, 0), True), (0, False)):
+            without_weight(sizes, D, torch.float32, channel, masked, dev)
+
+
+def infinite_value(sizes, D, dtype, mask, gone, dev):
+    """`gone` [N, Lk]: the keys whose value is infinite in one channel, of which a sample has no two of opposite sign"""
+    N, Lq, Lk, Hq, Hkv = sizes
+    q, k, v, g = make(*sizes, D, dtype, seed=sum(sizes) + D)
+    want, bounds = reference(q, k, v, g, None, mask, 1.0 / math.sqrt(D))
+    out, bound = want[0], bounds[0]
+    channel, sign = D - 3, 1 - 2 * (torch.arange(N) % 2)
+    v[..., channel] = torch.where(gone[..., None], (sign * math.inf)[:, None, None].to(dtype), v[..., channel])
+    with torch.no_grad():
+        got = d2c.cross_attention(q.to(dev), k.to(dev), v.to(dev), key_mask=None if mask is None else mask.to(dev)).double().cpu()
+    infinite = (sign * math.inf)[:, None, None].expand(N, Lq, Hq).double()
+    assert torch.equal(got[..., channel], infinite), (sizes, D, got[..., channel].isnan().sum())
+    rest = [c for c in range(D) if c != channel]
+    check((got[..., rest],), (out[..., rest],), (bound[..., rest],), f"{sizes} {D}")
+
+
+@pytest.mark.parametrize("D", [8, 24, 33, 40, 64, 96, 104, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinite_values(dtype, D, dev):
+    for sizes in ((2, 1, 384, 2, 1), (2, 20, 384, 2, 2), (2, 200, 384, 2, 1), (2, 200, 64, 2, 1)):
+        gone = torch.zeros(sizes[0], sizes[2], dtype=torch.bool)
+        gone[:, 17], gone[1, 60] = True, True
+        infinite_value(sizes, D, dtype, None, gone, dev)
