@@ -113,6 +113,7 @@ template <typename T, int DP, int NP, int WK, bool WHOLE> __global__ void __laun
         unsigned char *s_k = lds + (BUFFERS == 2 ? buffer * 2 * KV::BYTES : 0), *s_v = s_k + KV::BYTES;
         buffer ^= 1;
         if constexpr (BUFFERS == 1) __syncthreads();
+        if (!all_keys<KT>(now)) v.zero_rows([&](int i) INLINE { return !has_key(now, i); });
         k.template store<END>(s_k, a.D);
         v.template store<false>(s_v, a.D);      // (its piece behind the end makes columns of o that are not stored)
         __syncthreads();

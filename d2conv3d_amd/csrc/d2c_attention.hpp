@@ -207,6 +207,17 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
 #pragma unroll
         for (int i = 0; i < PER; i++) r[i] = load8<true, T>(reinterpret_cast<const T *>(reinterpret_cast<const char *>(base) + off[i]), 8);
     }
+    // zeros in the rows that drop(row) says
+    template <typename Drop> D2C_DEV void zero_rows(Drop drop)
+    {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const bool gone = drop(row_of(i));
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; j++)
+                if (gone) r[i].v[j] = make_uint4(0, 0, 0, 0);
+        }
+    }
     // END: the piece at column D, which a product's last step takes in, as zeros (those of the other operand do not undo an infinity that is repeated)
     template <bool END, bool AGREEING = false> D2C_DEV void store(unsigned char *lds, int D) const
     {
@@ -380,7 +391,8 @@ D2C_DEV float half_max(float v) { float x, y; other_half(v, x, y); return fmaxf(
 D2C_DEV float half_sum(float v) { float x, y; other_half(v, x, y); return x + y; }
 
 // The rows of a tile of keys to request: a key that is not to be read is replaced by one of the tile's that is (any_key, of `words`), so that
-// what it holds is nowhere read: its score is put to -infinity, its weight 0 meets that other key's value.
+// what it holds is nowhere read: its score is put to -infinity, and its weight 0 meets zeros that are put in the place of that other key's value (which
+// may be infinite).
 template <int WORDS> D2C_DEV bool has_key(const uint64_t (&words)[WORDS], int i)
 {
     const uint64_t w = WORDS == 1 ? words[0] : words[i >> 6];

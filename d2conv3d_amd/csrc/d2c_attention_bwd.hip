@@ -203,7 +203,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
     float stat = 0.f;
     auto request = [&](int tile) INLINE {
         const int r0 = tile * RT;
-        // (rows behind the last one repeat it: their weights are 0, by a sum of +infinity)
+        // (rows behind the last one repeat it: their weights are 0, by a sum of +infinity, and their gradients are made 0 on the way to LDS)
         if constexpr (WHOLE) {
             if (uniform && r0 + RT <= a.rows) {
                 q.load_at(qb + (long)(r0 / a.group) * a.qs[1], qoff);
@@ -258,6 +258,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
         float *s_lse = reinterpret_cast<float *>(s_q + 2 * QG::BYTES), *s_delta = s_lse + RT;
         buffer ^= 1;
         if constexpr (BUFFERS == 1) __syncthreads();
+        if (t * RT + RT > a.rows) g.zero_rows([&](int i) INLINE { return t * RT + i >= a.rows; });
         q.template store<false, true>(s_q, a.D);      // (an infinite query has no defined weights, an infinite gradient no defined ds)
         g.template store<false>(s_g, a.D);
         if (threadIdx.x < 2 * RT) s_lse[threadIdx.x] = stat;

@@ -73,3 +73,30 @@ def test_infinite_values(dtype, D, dev):
         gone = torch.zeros(sizes[0], sizes[2], dtype=torch.bool)
         gone[:, 17], gone[1, 60] = True, True
         infinite_value(sizes, D, dtype, None, gone, dev)
+
+
+@pytest.mark.parametrize("D", [8, 24, 33, 40, 64, 96, 104, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinite_values_beside_keys_that_are_not_read(dtype, D, dev):
+    """... in tiles that are not whole, by their end or by the mask; every key that is read is one of those whose value is infinite in turn"""
+    for sizes in ((2, 1, 333, 2, 1), (2, 20, 333, 2, 2), (2, 200, 333, 2, 1), (2, 200, 50, 2, 1), (2, 20, 50, 2, 1), (1, 1100, 2000, 2, 2)):
+        N, Lk = sizes[0], sizes[2]
+        mask = torch.rand(N, Lk, generator=torch.Generator().manual_seed(5)) < 0.5
+        infinite_value(sizes, D, dtype, mask, mask, dev)                          # (weights above 0 all: the scores are near each other)
+        gone = torch.zeros(N, Lk, dtype=torch.bool)
+        gone[:, Lk - 1] = True
+        infinite_value(sizes, D, dtype, None, gone, dev)
+
+
+@pytest.mark.parametrize("D", [8, 33, 40, 64, 104, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinite_gradients(dtype, D, dev):
+    """grad_out of the last row infinite in a channel: that channel of the values' gradients is infinite, the others are as they were."""
+    for sizes in ((2, 3, 333, 2, 1), (1, 70, 300, 3, 1), (2, 20, 50, 2, 2), (1, 1111, 2000, 2, 2)):
+        q, k, v, g = make(*sizes, D, dtype, seed=sum(sizes) + D)
+        want, bounds = reference(q, k, v, g, None, None, 1.0 / math.sqrt(D))
+        g[:, -1, :, D - 2] = math.inf
+        got = run(dev, q, k, v, g, None, None)[3].double().cpu()
+        assert bool((got[..., D - 2] == math.inf).all()), (sizes, D)
+        rest = [c for c in range(D) if c != D - 2]
+        check((got[..., rest],), (want[3][..., rest],), (bounds[3][..., rest],), f"{sizes} {D}")
