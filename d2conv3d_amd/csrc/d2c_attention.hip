@@ -91,7 +91,7 @@ template <typename T, int DP, int NP, int WK, bool WHOLE> __global__ void __laun
                 floats_of<T>(raw, x);
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[e] *= a.scale2;
-                q[i] = make_frag<3, true>(x);
+                q[i] = make_frag<3, READ>(x);
             }
         }
     }
@@ -170,7 +170,7 @@ template <typename T, int DP, int NP, int WK, bool WHOLE> __global__ void __laun
             }
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
-                const Frag<PW> pf = make_frag<PW, true>(p + kk * 8);
+                const Frag<PW> pf = make_frag<PW, WEIGHTS>(p + kk * 8);
 #pragma unroll
                 for (int d = 0; d < ND; d++) mma(o[d], KV::columns(s_v, wk * KW + i * 32 + kk * 16, d * 32, lane), pf);
             }

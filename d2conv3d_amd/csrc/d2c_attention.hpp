@@ -11,7 +11,7 @@
 // 4 of 8 keys to a half of the wavefront, in which the other operand is read, too (transposing LDS reads, four at a time).
 //
 // float32 operands travel as three bfloat16 terms, which represent a float exactly, and a product as the six partial products that
-// count (what is left out is below 2^-24 of it, 2^-23 where one operand's terms are cut off, see split_pair_agreeing): 6/16 of the float instruction's time.
+// count (what is left out is below 2^-24 of it): 6/16 of the float instruction's time.
 //
 // The rows of a group of query heads that share a key head are one axis: row = position * group + head in group.
 #pragma once
@@ -66,51 +66,56 @@ template <int P, int PB> D2C_DEV void mma(f32x16 &acc, const Frag<P> &a, const F
     }
     acc = mma1(acc, a.t[0], b.t[0]);
 }
-// Two floats -> their terms, each a packed pair
-D2C_DEV void split_pair(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo)
+// Two floats -> their three terms, each a packed pair.  INFINITIES (operands that come from memory): one, or a value that rounds to one, is the last term alone.  It
+// meets the other operand's first term only, which is 0 where the value is and has its sign, and so makes the infinity that the product is; against lower
+// terms, which are 0 or of either sign, it would make no number.
+template <bool INFINITIES> D2C_DEV void split_pair(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo)
+{
+    const bool ix = INFINITIES && fabsf(x) > 0x1.fefffep127f, iy = INFINITIES && fabsf(y) > 0x1.fefffep127f;
+    const float x0 = ix ? 0.f : x, y0 = iy ? 0.f : y;
+    hi = pack_bf16x2(x0, y0);
+    const float x1 = x0 - __uint_as_float(hi << 16), y1 = y0 - __uint_as_float(hi & 0xffff0000u);
+    mid = pack_bf16x2(x1, y1);
+    const float x2 = x1 - __uint_as_float(mid << 16), y2 = y1 - __uint_as_float(mid & 0xffff0000u);
+    lo = pack_bf16x2(ix ? x : x2, iy ? y : y2);
+}
+// ... their two terms
+D2C_DEV void split_pair(float x, float y, uint32_t &hi, uint32_t &lo)
 {
     hi = pack_bf16x2(x, y);
-    x = bf16_residual(x, hi << 16); y = bf16_residual(y, hi & 0xffff0000u);
-    mid = pack_bf16x2(x, y);
-    lo = pack_bf16x2(x - __uint_as_float(mid << 16), y - __uint_as_float(mid & 0xffff0000u));
+    lo = pack_bf16x2(bf16_residual(x, hi << 16), bf16_residual(y, hi & 0xffff0000u));
 }
-// ... whose terms agree in sign and of which none is 0 where the value is not (down to 2^-86 of it: the float that a term of 0 would be is 2^-40 of the value).
-// Of what meets an infinity, which is a single term of its operand, all partial products then are the infinity that the product is; terms that are
-// rounded would make it no number, by 0 or by the opposite sign.  Terms are cut off, not rounded: what the six partial products leave out is below 2^-23 of
-// the product then.
-template <int P> D2C_DEV void split_pair_agreeing(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo)
+// ... which agree in sign and neither of which is 0 where the value is not (down to 2^-86: what a second term of 0 would be is 2^-40 of the value).  The other
+// operand is one term: an infinite one makes the infinity that the product is of both.
+D2C_DEV void split_pair_agreeing(float x, float y, uint32_t &hi, uint32_t &lo)
 {
-    auto heads = [](float x, float y) INLINE { return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u); };
-    auto behind = [](float v, float whole) INLINE { return fmaf(whole, 0x1p-40f, v - __uint_as_float(__float_as_uint(v) & 0xffff0000u)); };
-    hi = heads(x, y);
-    const float x1 = behind(x, x), y1 = behind(y, y);
-    if constexpr (P == 2) mid = pack_bf16x2(x1, y1);
-    else {
-        mid = heads(x1, y1);
-        lo = heads(behind(x1, x), behind(y1, y));
-    }
+    auto behind = [](float v) INLINE { return fmaf(v, 0x1p-40f, v - __uint_as_float(__float_as_uint(v) & 0xffff0000u)); };
+    hi = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+    lo = pack_bf16x2(behind(x), behind(y));
 }
-template <int P, bool AGREEING = false> D2C_DEV Frag<P> make_frag(const float *v)
+// Operands that the kernels make (WEIGHTS: those, whose other operand may be infinite; never infinite themselves) or that come from memory
+enum Operand { MADE, WEIGHTS, READ };
+template <int P, Operand KIND> D2C_DEV Frag<P> make_frag(const float *v)
 {
     Frag<P> f;
-    if constexpr (P > 1 && AGREEING) {
-        uint32_t t[3][4];
+    if constexpr (P == 2 && KIND == WEIGHTS) {
+        uint32_t h[4], m[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) split_pair_agreeing<P>(v[2 * i], v[2 * i + 1], t[0][i], t[1][i], t[2][i]);
-#pragma unroll
-        for (int i = 0; i < P; i++) f.t[i] = make_uint4(t[i][0], t[i][1], t[i][2], t[i][3]);
+        for (int i = 0; i < 4; i++) split_pair_agreeing(v[2 * i], v[2 * i + 1], h[i], m[i]);
+        f.t[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        f.t[1] = make_uint4(m[0], m[1], m[2], m[3]);
     } else if constexpr (P == 1) {
         f.t[0] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
     } else if constexpr (P == 2) {
-        uint32_t h[4], m[4], none;
+        uint32_t h[4], m[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) split_pair(v[2 * i], v[2 * i + 1], h[i], m[i], none);
+        for (int i = 0; i < 4; i++) split_pair(v[2 * i], v[2 * i + 1], h[i], m[i]);
         f.t[0] = make_uint4(h[0], h[1], h[2], h[3]);
         f.t[1] = make_uint4(m[0], m[1], m[2], m[3]);
     } else {
         uint32_t h[4], m[4], l[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) split_pair(v[2 * i], v[2 * i + 1], h[i], m[i], l[i]);
+        for (int i = 0; i < 4; i++) split_pair<KIND == READ>(v[2 * i], v[2 * i + 1], h[i], m[i], l[i]);
         f.t[0] = make_uint4(h[0], h[1], h[2], h[3]);
         f.t[1] = make_uint4(m[0], m[1], m[2], m[3]);
         f.t[2] = make_uint4(l[0], l[1], l[2], l[3]);
@@ -147,14 +152,14 @@ template <bool WHOLE, typename T> D2C_DEV Raw8<T> load8_of(const T *row, int d, 
         return r;
     } else return load8<false, T>(row + d, live ? D - d : 0);
 }
-template <typename T, bool AGREEING = false> D2C_DEV Frag<kTerms<T>> terms_of(const Raw8<T> &r)
+template <typename T> D2C_DEV Frag<kTerms<T>> terms_of(const Raw8<T> &r)
 {
     if constexpr (sizeof(T) == 2) return Frag<1>{{r.v[0]}};
     else {
         float f[8];
         *reinterpret_cast<uint4 *>(f) = r.v[0];
         *reinterpret_cast<uint4 *>(f + 4) = r.v[1];
-        return make_frag<3, AGREEING>(f);
+        return make_frag<3, READ>(f);
     }
 }
 template <typename T> D2C_DEV void floats_of(const Raw8<T> &r, float *f)
@@ -219,7 +224,7 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
         }
     }
     // END: the piece at column D, which a product's last step takes in, as zeros (those of the other operand do not undo an infinity that is repeated)
-    template <bool END, bool AGREEING = false> D2C_DEV void store(unsigned char *lds, int D) const
+    template <bool END> D2C_DEV void store(unsigned char *lds, int D) const
     {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
@@ -231,7 +236,7 @@ template <typename T, int DP, int ROWS, int THREADS, bool WHOLE> struct Tile {
                 for (int j = 0; j < (int)sizeof(T) / 2; j++)
                     if (at % PIECES * 8 == D) x.v[j] = make_uint4(0, 0, 0, 0);
             }
-            const Frag<P> f = terms_of<T, AGREEING>(x);
+            const Frag<P> f = terms_of<T>(x);
 #pragma unroll
             for (int t = 0; t < P; t++)
                 *reinterpret_cast<uint4 *>(lds + t * TERM + piece_at<DP>(at / PIECES, at % PIECES)) = f.t[t];

@@ -59,7 +59,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
 #pragma unroll
         for (int i = 0; i < NK; i++) {
             const int d = i * 16 + half * 8;
-            q[i] = terms_of<T, true>(load8_of<WHOLE, T>(qr, d, a.D, live));
+            q[i] = terms_of<T>(load8_of<WHOLE, T>(qr, d, a.D, live));
             const Raw8<T> x = load8_of<WHOLE, T>(gr, d, a.D, live), y = load8_of<WHOLE, T>(orow, d, a.D, live);
             g[i] = terms_of<T>(x);
             float xf[8], yf[8];
@@ -122,7 +122,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
             for (int r = 0; r < 16; r++) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
-                const Frag<PW> f = make_frag<PW>(ds + kk * 8);
+                const Frag<PW> f = make_frag<PW, MADE>(ds + kk * 8);
 #pragma unroll
                 for (int d = 0; d < ND; d++) mma(dq[d], KV::columns(s_k, i * 32 + kk * 16, d * 32, lane), f);
             }
@@ -259,7 +259,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
         buffer ^= 1;
         if constexpr (BUFFERS == 1) __syncthreads();
         if (t * RT + RT > a.rows) g.zero_rows([&](int i) INLINE { return t * RT + i >= a.rows; });
-        q.template store<false, true>(s_q, a.D);      // (an infinite query has no defined weights, an infinite gradient no defined ds)
+        q.template store<false>(s_q, a.D);      // (an infinite query has no defined weights, an infinite gradient no defined ds)
         g.template store<false>(s_g, a.D);
         if (threadIdx.x < 2 * RT) s_lse[threadIdx.x] = stat;
         __syncthreads();
@@ -293,7 +293,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
             }
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
-                const Frag<PW> pf = make_frag<PW, true>(p + kk * 8), df = make_frag<PW>(ds + kk * 8);
+                const Frag<PW> pf = make_frag<PW, WEIGHTS>(p + kk * 8), df = make_frag<PW, MADE>(ds + kk * 8);
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
                     mma(dv[d], QG::columns(s_g, i * 32 + kk * 16, d * 32, lane), pf);
