@@ -343,8 +343,8 @@ int resident(const void *kernel, int lds);
 
 D2C_DEV int keys_of(const Args &a, int n) { return a.lengths ? min(max(a.lengths[n], 0), a.Lk) : a.Lk; }
 
-// A sample with one key to read (asked of few keys): its weight is 1 whatever the scores, and their gradients are 0, not what two sums of the same terms in
-// different orders leave.
+// A sample of up to 64 keys (by its length) of which one is to be read: its weight is 1 whatever its score, and the score's gradients are 0, not what two sums of
+// the same terms in different orders leave (as they do where a mask leaves one of more keys: 2^-24 of the terms for each channel).
 D2C_DEV bool one_key(const Args &a, int n, int keys)
 {
     if (keys > kExactKeys) return false;

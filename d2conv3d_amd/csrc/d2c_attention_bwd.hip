@@ -36,7 +36,8 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
     const int tile_row = wave * 32 + (lane & 31), row = unit.tile * 128 + tile_row;
     const bool live = row < a.rows;
     const int keys = keys_of(a, hd.n), tiles = (keys + KT - 1) / KT;
-    const int t1 = one_key(a, hd.n, keys) ? 0 : (int)((long)tiles * (unit.split + 1) / unit.splits);
+    const bool alone = one_key(a, hd.n, keys);
+    const int t1 = alone ? 0 : (int)((long)tiles * (unit.split + 1) / unit.splits);
     int t = (int)((long)tiles * unit.split / unit.splits);
 
     KV k, v;
@@ -78,11 +79,13 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
     delta = half_sum(delta);
     const float lse = live ? a.lse[hd.nh * a.rows + row] : INFINITY;
     if (live && unit.split == 0 && half == 0) a.delta[hd.nh * a.rows + row] = delta;
+    // (a row with one key has gradients of 0, but none where its weight, its output or the output's gradient is no finite number)
+    const float none = alone && !(lse == lse && fabsf(delta) < INFINITY) ? NAN : 0.f;
     f32x16 dq[ND];
 #pragma unroll
     for (int i = 0; i < ND; i++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) dq[i][r] = 0.f;
+        for (int r = 0; r < 16; r++) dq[i][r] = none;
     const float c = a.scale2;
     int buffer = 0;
 
@@ -312,7 +315,11 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
             const int d = i * 32 + j * 8 + half * 4;
             float x[4], y[4];
 #pragma unroll
-            for (int r = 0; r < 4; r++) { x[r] = live && !alone ? dk[i][j * 4 + r] * fk : 0.f; y[r] = live ? dv[i][j * 4 + r] : 0.f; }
+            for (int r = 0; r < 4; r++) {
+                x[r] = live ? dk[i][j * 4 + r] * fk : 0.f;
+                if (alone && x[r] == x[r]) x[r] = 0.f;
+                y[r] = live ? dv[i][j * 4 + r] : 0.f;
+            }
             if (unit.splits > 1) {
                 store4<float>(a.part + (((2L * unit.split) * a.shared + unit.part) * 128 + tile_key) * part_width(a.D) + d, x, a.D - d);
                 store4<float>(a.part + (((2L * unit.split + 1) * a.shared + unit.part) * 128 + tile_key) * part_width(a.D) + d, y, a.D - d);
