@@ -12,15 +12,16 @@ using namespace d2c_attn;
 
 namespace {
 
-// The keys of a tile that are to be read: bit i of word j is key k0 + 64 j + i.  Requested as bytes two tiles ahead.
-template <int WORDS> struct KeyBits {
+// The keys of a tile of KT that are to be read: bit i of word j is key k0 + 64 j + i.  Requested as bytes two tiles ahead.
+template <int KT> struct KeyBits {
+    static constexpr int WORDS = (KT + 63) / 64;
     bool b[WORDS];
     D2C_DEV void request(const Args &a, int n, int keys, int k0)
     {
 #pragma unroll
         for (int j = 0; j < WORDS; j++) {
-            const int key = k0 + j * 64 + (int)(threadIdx.x & 63);
-            b[j] = key < keys && (!a.mask || a.mask[(long)n * a.Lk + key]);
+            const int i = j * 64 + (int)(threadIdx.x & 63), key = k0 + i;
+            b[j] = i < KT && key < keys && (!a.mask || a.mask[(long)n * a.Lk + key]);
         }
     }
     D2C_DEV void words(uint64_t (&w)[WORDS]) const
@@ -55,7 +56,7 @@ template <typename T, int DP, int NP, int WK, bool WHOLE> __global__ void __laun
 {
     using Shape = FwdShape<T, DP, WK, WHOLE>;
     using KV = typename Shape::KV;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = (KT + 63) / 64;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, KW = Shape::KW, KT = Shape::KT, NS = KW / 32, WORDS = KeyBits<KT>::WORDS;
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int BUFFERS = Shape::BUFFERS;
     constexpr bool END = WHOLE && NP % 2 == 1;
@@ -69,7 +70,7 @@ template <typename T, int DP, int NP, int WK, bool WHOLE> __global__ void __laun
 
     KV k, v;
     const KeyTiles<T, KV, KT, WORDS, WHOLE> source(a, hd);
-    KeyBits<WORDS> bits;
+    KeyBits<KT> bits;
     uint64_t next[WORDS];
     auto request = [&](int tile) INLINE { source.request(a, k, v, tile, next); };
     if (t < t1) {
