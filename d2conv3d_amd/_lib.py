@@ -97,7 +97,7 @@ class Rotary3dDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("N", "L", "H", "D")] + [
         ("pairs", ctypes.c_int32 * 3), ("grid", ctypes.c_int32 * 3)] + [
         (n, ctypes.c_int32) for n in ("interleaved", "direction", "dtype")] + [
-        ("base", ctypes.c_float), ("x_stride", ctypes.c_int64 * 3), ("position_stride", ctypes.c_int64)]
+        ("base", ctypes.c_double), ("x_stride", ctypes.c_int64 * 3), ("position_stride", ctypes.c_int64)]
 
 
 class AttentionDesc(ctypes.Structure):

@@ -155,7 +155,7 @@ def rotary3d(input, positions, axis_pairs=None, base=10000.0, interleaved=False)
     [N, L, 3] of real or whole positions (taken as float32; no gradient).  `axis_pairs`: how many pairs turn with each axis
     (default_axis_pairs); pair i of an axis turns by position * base^(-i / pairs of the axis) radians, channels behind the
     last pair pass.  Pair j of all is channels (2j, 2j + 1) with `interleaved`, else (j, j + all pairs).  Angles are exact to
-    float32 however far the position."""
+    float32 for positions of up to 2^24 either way, and beyond off by 2^-48 turns a position."""
     if isinstance(input, torch.Tensor) and input.dim() == 4:
         pairs = default_axis_pairs(input.size(3)) if axis_pairs is None else axis_pairs
         real = isinstance(positions, torch.Tensor)

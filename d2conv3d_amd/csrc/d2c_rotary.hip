@@ -4,9 +4,9 @@
 // Bound: memory (each value read and written once): 207360 tokens of 8 heads of 64, bfloat16, 78 us (5.4 TB/s, a large copy 5.15); 25920 of 4 heads of 80, float32,
 // tensor of positions, 17.5 us (3.8 TB/s, much of it the way to and from a kernel); a single frame's 350, 3.7 us.  A workgroup takes some tokens, works out their cosines and sines once for all
 // heads (LDS), then moves the tokens' channels in 16-byte vectors.
-// An angle is made in turns, position * rate / 2 pi, with the rate as the sum of two floats, so that what remains after
-// whole turns are taken off is exact to float32 however far away the position is; a product in float32 of a position of 10^4 would be off by
-// 5e-4 radians.
+// An angle is made in turns, position * rate / 2 pi, with the rate as the sum of two floats (48 bits, made from a base in 64), so that what remains after
+// whole turns are taken off is exact to float32 for positions of up to 2^24, where float32 stops to tell whole ones apart; beyond, it is off by position * rate *
+// 2^-48 turns.  A product in float32 of a position of 10^4 would be off by 5e-4 radians.
 #include <algorithm>
 #include <cmath>
 #include "d2c_common.hpp"
@@ -106,7 +106,10 @@ int check(const d2c_rotary3d_desc *q)
     if (2 * pairs > q->D) { d2c_set_error("rotary: %ld pairs do not fit a head of %d channels", pairs, q->D); return D2C_ERR_SHAPE; }
     if (pairs > D2C_ROTARY_MAX_PAIRS) { d2c_set_error("rotary: up to %d pairs", D2C_ROTARY_MAX_PAIRS); return D2C_ERR_UNSUPPORTED; }
     if (q->direction != 1 && q->direction != -1) { d2c_set_error("rotary: direction must be 1 or -1"); return D2C_ERR_SHAPE; }
-    if (!(q->base > 0.f) || !(q->base < INFINITY)) { d2c_set_error("rotary: base must be positive and finite"); return D2C_ERR_SHAPE; }
+    if (!((float)q->base > 0.f) || !((float)q->base < INFINITY)) {      // (rates have to be floats)
+        d2c_set_error("rotary: base must be positive and finite");
+        return D2C_ERR_SHAPE;
+    }
     return D2C_OK;
 }
 
@@ -132,7 +135,7 @@ extern "C" int d2c_rotary3d(const d2c_rotary3d_desc *q, const void *x, const flo
     int j = 0;
     for (int p : q->pairs)
         for (int i = 0; i < p; i++, j++) {
-            const double rate = std::pow((double)q->base, -(double)i / p) * 0.15915494309189533577;
+            const double rate = std::pow(q->base, -(double)i / p) * 0.15915494309189533577;
             a.hi[j] = (float)rate;
             a.lo[j] = (float)(rate - (double)a.hi[j]);
         }

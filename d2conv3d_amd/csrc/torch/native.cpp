@@ -732,7 +732,7 @@ py::object rotary3d(const Tensor &x, const opt_tensor &positions, int3_t grid, i
         if (pos.size(-1) != 3 || pos.size(-2) != q.L || (pos.dim() == 3 && pos.size(0) != q.N)) return py::none();
         q.position_stride = pos.dim() == 3 ? 3ll * q.L : 0;
     } else if (cells != q.L) return py::none();
-    q.interleaved = interleaved; q.dtype = dt; q.base = (float)base;
+    q.interleaved = interleaved; q.dtype = dt; q.base = base;
     const bool grad = wants_grad(x);
     std::shared_ptr<Rotary3dBackward> node;
     if (grad) {

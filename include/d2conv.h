@@ -502,15 +502,15 @@ int d2c_layer_norm_backward(const d2c_layer_norm_desc *desc, const void *grad_y,
 /* Rotary positions along time, height and width.  x [N, L, H, D] with strides x_stride (sample, token, head; channels
  * adjacent), y contiguous.  The first 2 * (pairs[0] + pairs[1] + pairs[2]) channels of a head turn in pairs, the others pass:
  * pair j of all is channels (2j, 2j + 1) if `interleaved`, else (j, j + all pairs); pair i of axis a turns by
- *     direction * position[a] * base^(-i / pairs[a])       radians,
- * direction 1, or -1 (which is the gradient's way back).  positions: float32 [L][3] for each sample, position_stride elements
+ *     direction * position[a] * base^(-i / pairs[a])       radians
+ * (an angle is exact to float32 for positions of up to 2^24, and off by 2^-48 turns a position beyond), direction 1, or -1 (which is the gradient's way back).  positions: float32 [L][3] for each sample, position_stride elements
  * from sample to sample (0: the same for all); NULL: token (t * grid[1] + h) * grid[2] + w has the position (t, h, w). */
 #define D2C_ROTARY_MAX_PAIRS 128
 typedef struct d2c_rotary3d_desc {
     int32_t N, L, H, D;
     int32_t pairs[3], grid[3];
     int32_t interleaved, direction, dtype;
-    float base;
+    double base;
     int64_t x_stride[3], position_stride;
 } d2c_rotary3d_desc;
 int d2c_rotary3d(const d2c_rotary3d_desc *desc, const void *x, const float *positions, void *y, void *stream);
