@@ -16,6 +16,7 @@ import math
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
+from torch.utils._pytree import register_pytree_node
 
 from . import _lib
 from ._ops import _DT, _ptr, _stream, _try_native, _workspace
@@ -287,6 +288,23 @@ class LayerNorm(nn.LayerNorm):
         return layer_norm(input, self.weight, self.bias, self.eps)
 
 
+class Memory(tuple):
+    """(keys, values) of a feature map as `CrossAttention3d.remember` makes them, and the map's extents (T', H', W'), which
+    masks of frames or cells are checked against."""
+
+    def __new__(cls, key, value, dims):
+        self = super().__new__(cls, (key, value))
+        self.dims = tuple(dims)
+        return self
+
+    def __getnewargs__(self):      # (copies and pickles)
+        return (*self, self.dims)
+
+
+# (what walks over tuples of tensors, graphed callables for instance, walks over these, too)
+register_pytree_node(Memory, lambda m: (list(m), m.dims), lambda pair, dims: Memory(*pair, dims))
+
+
 class CrossAttention3d(nn.Module):
     """A clip's feature map reads the feature map of remembered frames, and adds what it read:
 
@@ -327,23 +345,37 @@ class CrossAttention3d(nn.Module):
 
     def remember(self, memory, positions=None):
         """Keys and values of `memory`, to be handed to any number of forward calls: the memory of a stream of frames is
-        projected and turned once.  `positions` as rotary3d's; the memory's own grid by default."""
+        projected and turned once.  `positions` as rotary3d's; the memory's own grid by default.  A pair that knows the map's extents
+        (Memory)."""
         N, _, *dims = memory.shape
         both = self.key_value(self.memory_norm(self._tokens(memory)))
         both = both.view(N, both.size(1), 2, self.kv_heads, self.head_channels)
-        return self._rotate(both[:, :, 0], tuple(dims) if positions is None else positions), both[:, :, 1]
+        return Memory(self._rotate(both[:, :, 0], tuple(dims) if positions is None else positions), both[:, :, 1], dims)
+
+    @staticmethod
+    def _cells(mask, memory):
+        """[N, cells] of a mask of frames or cells"""
+        key, dims = memory[0], getattr(memory, "dims", None)
+        cells = key.size(1)
+        given = mask.flatten(1).size(1)
+        if mask.dim() == 4 and given == cells and dims is not None:
+            _check(tuple(mask.shape[1:]) == dims, f"CrossAttention3d: a mask of {tuple(mask.shape)} does not fit a memory of {dims}")
+        mask = mask.flatten(1)
+        # (of a pair that is no Memory the number of frames is not known: any that divides its cells)
+        frames = dims is None and given > 0 and cells % given == 0 or dims is not None and given == dims[0]
+        _check(given == cells or frames, f"CrossAttention3d: a mask of {given} does not fit {cells} cells"
+               + ("" if dims is None else f" in {dims[0]} frames"))
+        return mask if given == cells else mask.repeat_interleave(cells // given, 1)
 
     def forward(self, x, memory, positions=None, memory_positions=None, memory_lengths=None, memory_mask=None):
         """`memory`: a feature map, or what `remember` made of one.  `memory_lengths` [N]: how many of the memory's cells
         (frame after frame) are there; `memory_mask`: bool [N, T'] (frames) or [N, T', H', W'] or [N, cells]."""
         N, C, *dims = x.shape
-        key, value = memory if isinstance(memory, (tuple, list)) else self.remember(memory, memory_positions)
+        if not isinstance(memory, (tuple, list)):
+            memory = self.remember(memory, memory_positions)
+        key, value = memory
         if memory_mask is not None:
-            memory_mask = memory_mask.flatten(1)
-            if memory_mask.size(1) != key.size(1):
-                _check(memory_mask.size(1) > 0 and key.size(1) % memory_mask.size(1) == 0,
-                       f"CrossAttention3d: a mask of {memory_mask.size(1)} does not fit {key.size(1)} cells")
-                memory_mask = memory_mask.repeat_interleave(key.size(1) // memory_mask.size(1), 1)
+            memory_mask = self._cells(memory_mask, memory)
         q = self.query(self.norm(self._tokens(x))).view(N, -1, self.heads, self.head_channels)
         q = self._rotate(q, tuple(dims) if positions is None else positions)
         read = cross_attention(q, key, value, memory_lengths, memory_mask)
