@@ -376,7 +376,8 @@ class CrossAttention3d(nn.Module):
         key, value = memory
         if memory_mask is not None:
             memory_mask = self._cells(memory_mask, memory)
-        q = self.query(self.norm(self._tokens(x))).view(N, -1, self.heads, self.head_channels)
+        q = self.query(self.norm(self._tokens(x)))
+        q = q.view(N, q.size(1), self.heads, self.head_channels)
         q = self._rotate(q, tuple(dims) if positions is None else positions)
         read = cross_attention(q, key, value, memory_lengths, memory_mask)
         read = self.out(read.flatten(2))
