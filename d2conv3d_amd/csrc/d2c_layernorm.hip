@@ -291,10 +291,13 @@ LnShape shape_of(const d2c_layer_norm_desc &q)
     if (n <= 1024) return {256, 4};
     return {256, 16};
 }
-int blocks_of(const d2c_layer_norm_desc &q, const LnShape &s, int per_cu)
+// `most`: no more than so many (backward: workgroups' sums of up to 64 MB)
+constexpr long kLnPartBytes = 64L << 20;
+long most_blocks(const d2c_layer_norm_desc &q) { return kLnPartBytes / (2L * q.C * (long)sizeof(float)); }
+int blocks_of(const d2c_layer_norm_desc &q, const LnShape &s, int per_cu, long most = 1L << 30)
 {
     const long per = kLnThreads / s.lanes;
-    return (int)std::max(1L, std::min((q.rows + per - 1) / per, (long)per_cu * std::max(d2c_num_cus(), 1)));
+    return (int)std::max(1L, std::min((q.rows + per - 1) / per, std::min((long)per_cu * std::max(d2c_num_cus(), 1), most)));
 }
 constexpr int kFwdPerCu = 16, kBwdPerCu = 4;      // (8 and 16: 43.8, 40.6 us forward on 207360 rows of 256; 2, 4, 8: 66, 57, 61 us backward)
 
@@ -345,7 +348,7 @@ extern "C" int d2c_layer_norm_forward(const d2c_layer_norm_desc *q, const void *
 extern "C" size_t d2c_layer_norm_backward_workspace_bytes(const d2c_layer_norm_desc *q)
 {
     if (check(q) != D2C_OK) return 0;
-    return d2c_align_up((size_t)blocks_of(*q, shape_of(*q), kBwdPerCu) * 2 * q->C * sizeof(float));
+    return d2c_align_up((size_t)blocks_of(*q, shape_of(*q), kBwdPerCu, most_blocks(*q)) * 2 * q->C * sizeof(float));
 }
 
 extern "C" int d2c_layer_norm_backward(const d2c_layer_norm_desc *q, const void *grad_y, const void *x, const float *stats,
@@ -362,7 +365,7 @@ extern "C" int d2c_layer_norm_backward(const d2c_layer_norm_desc *q, const void 
     }
     const LnShape s = shape_of(*q);
     const LnArgs a{x, grad_y, weight, nullptr, grad_x, const_cast<float *>(stats), params ? (float *)ws : nullptr, grad_weight, grad_bias, q->rows,
-                   q->x_stride, q->C, blocks_of(*q, s, kBwdPerCu), q->eps};
+                   q->x_stride, q->C, blocks_of(*q, s, kBwdPerCu, most_blocks(*q)), q->eps};
     hipStream_t st = (hipStream_t)stream;
     if (q->rows > 0 || params)
         if (int rc = launch<true>(*q, a, s, st)) return rc;      // (no rows: sums of nothing)
