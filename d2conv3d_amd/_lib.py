@@ -102,7 +102,7 @@ class Rotary3dDesc(ctypes.Structure):
 
 class AttentionDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("N", "Lq", "Lk", "Hq", "Hkv", "D", "dtype")] + [("scale", ctypes.c_float)] + [
-        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")] + [("part_limit", ctypes.c_int64)]
 
 
 class Conv1dDesc(ctypes.Structure):

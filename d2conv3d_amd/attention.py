@@ -192,6 +192,17 @@ def _inner_contiguous(t):
     return t if t.stride(3) == 1 or t.size(3) == 1 else t.contiguous()
 
 
+def _part_workspace(desc, size, dev):
+    """The workspace of a call, and its size: without room for partial sums where there is none."""
+    nb = size(ctypes.byref(desc))
+    try:
+        return _workspace(nb, dev), nb
+    except torch.cuda.OutOfMemoryError:
+        desc.part_limit = -1
+        nb = size(ctypes.byref(desc))
+        return _workspace(nb, dev), nb
+
+
 class _CrossAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, key_lengths, key_mask, scale):
@@ -206,8 +217,7 @@ class _CrossAttentionFunction(torch.autograd.Function):
         lse = torch.empty((N, Hkv, Lq * (Hq // Hkv)), dtype=torch.float32, device=dev) if grad else None
         low = torch.empty_like(out) if grad and out.dtype == torch.bfloat16 else None
         with torch.cuda.device(dev):
-            nb = lib.d2c_attention_forward_workspace_bytes(ctypes.byref(desc))
-            ws = _workspace(nb, dev)
+            ws, nb = _part_workspace(desc, lib.d2c_attention_forward_workspace_bytes, dev)
             rc = lib.d2c_attention_forward(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(key_lengths), _ptr(key_mask),
                                            _ptr(out), _ptr(low), _ptr(lse), _ptr(ws), nb, _stream(dev))
         _lib.check(rc, "cross_attention forward")
@@ -221,13 +231,13 @@ class _CrossAttentionFunction(torch.autograd.Function):
         lib = _lib.load()
         q, k, v, key_lengths, key_mask, out, low, lse = ctx.saved_tensors
         desc, dev, need = ctx.desc, q.device, ctx.needs_input_grad
+        desc.part_limit = 0
         q, k, v = (_inner_contiguous(t) for t in (q, k, v))
         desc.q_stride, desc.k_stride, desc.v_stride = (_long3(*t.stride()[:3]) for t in (q, k, v))
         g = grad_out.to(q.dtype).contiguous()
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((q, k, v), need))
         with torch.cuda.device(dev):
-            nb = lib.d2c_attention_backward_workspace_bytes(ctypes.byref(desc))
-            ws = _workspace(nb, dev)
+            ws, nb = _part_workspace(desc, lib.d2c_attention_backward_workspace_bytes, dev)
             rc = lib.d2c_attention_backward(ctypes.byref(desc), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(key_lengths),
                                             _ptr(key_mask), _ptr(out), _ptr(low), _ptr(lse), _ptr(gq), _ptr(gk), _ptr(gv),
                                             _ptr(ws), nb, _stream(dev))
@@ -243,7 +253,8 @@ def cross_attention(query, key, value, key_lengths=None, key_mask=None, scale=No
     (bool): keys that may be read.  Keys and values that are not to be read have no influence whatever they hold (NaN
     included); a row without a key is 0 and has gradients of 0.  Any strides with the channels adjacent are read in place, a
     part of a wider projection for instance.  One row or thousands, one key or a long memory: where rows are few the work is
-    split over the keys.  Sums in an order that sizes and GPU alone determine."""
+    split over the keys.  Sums in an order that sizes, strides and GPU alone determine, unless
+    the GPU's memory has no room for the partial sums of split work (256 MB at most), which then is not split."""
     out = _try_native("cross_attention", query, key, value, key_lengths, key_mask, scale)
     if out is not None:
         return out

@@ -564,7 +564,8 @@ template <typename T> FwdPlan fwd_plan(const d2c_attention_desc &q)
         p.tile_rows = R;
         const long places = 2L * std::max(d2c_num_cus(), 1);
         // (a step's bytes, from every place, at 5 TB/s)
-        p.walks = plan_walks(heads, (q.Lk + Shape::STEP - 1) / Shape::STEP, places, 2.0 * Shape::STEP * q.D * sizeof(T) * places / 5e6, (double)R * q.D * 4);
+        p.walks = plan_walks(heads, (q.Lk + Shape::STEP - 1) / Shape::STEP, places, 2.0 * Shape::STEP * q.D * sizeof(T) * places / 5e6, (double)R * (part_width(q.D) * 4 + 8),
+                             part_limit(q));
         return 0;
     });
     else for_shape<T>(q, p.few, [&](auto width, auto wk, auto whole) {
@@ -576,7 +577,7 @@ template <typename T> FwdPlan fwd_plan(const d2c_attention_desc &q)
         const long places = (long)std::max(d2c_num_cus(), 1) *
             resident(reinterpret_cast<const void *>(&attn_fwd_kernel<T, DP, NP, WK, WHOLE>), Shape::LDS);
         // (a step: 64 keys of 64 channels take 2 us with every place taken, float32's six products three times as long)
-        p.walks = plan_walks(units, steps, places, 2.0 * Shape::KT / 64 * DP / 64 * (sizeof(T) == 2 ? 1 : 3) / WK, (double)Shape::ROWS * q.D * 4);
+        p.walks = plan_walks(units, steps, places, 2.0 * Shape::KT / 64 * DP / 64 * (sizeof(T) == 2 ? 1 : 3) / WK, (double)Shape::ROWS * (part_width(q.D) * 4 + 8), part_limit(q));
         return 0;
     });
     const size_t lines = (size_t)p.walks.splits * p.walks.shared * p.tile_rows;

@@ -301,6 +301,9 @@ template <typename T, bool GRADIENTS, typename F> auto for_width(const d2c_atten
     return pick(Width<128, 16>{});
 }
 
+// Floats to a row of partial sums: whole pieces of 16 bytes (what is behind a row's end is read and dropped)
+inline __host__ __device__ int part_width(int D) { return (D + 3) & ~3; }
+
 // What the workgroups do: units, each the walk of one tile of rows (or keys) of one key head along the other axis.  As many as
 // fill the GPU's places without a remainder are walked by a workgroup each (`whole`); `splits` workgroups share each of the `shared` others, so that the
 // last round is as short as it is empty, and their sums are joined.
@@ -321,15 +324,17 @@ D2C_DEV Unit unit_of(const Args &a)
     const int heads = a.N * a.Hkv, tile = unit / heads, nh = unit - tile * heads, n = nh / a.Hkv;
     return {{n, nh - n * a.Hkv, nh}, tile, split, splits, part};
 }
-// ... of `steps` steps of `step_us` each at the places' full number, `bytes` of partial sums to a unit and split.  Times of the model: 4 us for the launch that
-// joins, its traffic (written and read) at 4 TB/s.
-inline Walks plan_walks(long units, long steps, long places, double step_us, double bytes)
+// ... of `steps` steps of `step_us` each at the places' full number, `bytes` of partial sums to a unit and split, `limit` bytes in all.  Times of the model: 4 us
+// for the launch that joins, its traffic (written and read) at 4 TB/s.  (Without a limit 20000 rows of one head of 128 reading 2^24 keys would ask for 770
+// MB, to fill a last round's idle places.  Of 10000 calls of up to 12960 rows and 64800 keys, drawn at random, two would ask for more than 256 MB.)
+inline Walks plan_walks(long units, long steps, long places, double step_us, double bytes, double limit)
 {
     Walks w{(int)(units / places * places), 0, 1};
     w.shared = (int)(units - w.whole);
     if (w.shared == 0) return w;
     double best = 0.0;
     for (long s = 1; s <= std::max(std::min(steps, 256L), 1L); s++) {
+        if (s > 1 && (double)(w.shared * s) * bytes > limit) break;
         const double t = (double)((w.shared * s + places - 1) / places) * (double)((steps + s - 1) / s) * step_us +
                          (s > 1 ? 4.0 + 2.0 * (double)(w.shared * s) * bytes / 4e6 : 0.0);
         if (s == 1 || t < best) { best = t; w.splits = (int)s; }
@@ -337,6 +342,7 @@ inline Walks plan_walks(long units, long steps, long places, double step_us, dou
     if (w.splits == 1) { w.whole += w.shared; w.shared = 0; }
     return w;
 }
+inline double part_limit(const d2c_attention_desc &q) { return q.part_limit == 0 ? (double)D2C_ATTENTION_PART_BYTES : (double)q.part_limit; }
 inline unsigned workgroups(const Walks &w) { return (unsigned)(w.whole + w.shared * w.splits); }
 // Workgroups of a kernel that a compute unit holds
 int resident(const void *kernel, int lds);
@@ -373,9 +379,6 @@ template <typename T> D2C_DEV void store4(T *p, const float *v, int left)
             if (i < left) p[i] = f32_to_elem<T>(v[i]);
     }
 }
-
-// Floats to a row of partial sums: whole pieces of 16 bytes (what is behind a row's end is read and dropped)
-inline __host__ __device__ int part_width(int D) { return (D + 3) & ~3; }
 
 // ... what storing them as T takes off
 template <typename T> D2C_DEV void store4_low(T *p, const float *v, int left)

@@ -388,7 +388,7 @@ template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
 {
     BwdPlan p;
     const long rows = (long)q.Lq * (q.Hq / q.Hkv), heads = (long)q.N * q.Hkv, cus = std::max(d2c_num_cus(), 1);
-    const double part = 128.0 * q.D * 4, slow = sizeof(T) == 2 ? 1 : 3;
+    const double part = 128.0 * part_width(q.D) * 4, limit = part_limit(q), slow = sizeof(T) == 2 ? 1 : 3;
     for_width<T, true>(q, [&](auto width, auto whole) {
         constexpr int DP = decltype(width)::DP, NP = decltype(width)::NP;
         constexpr bool WHOLE = decltype(whole)::value;
@@ -396,9 +396,9 @@ template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
         using KV = KvShape<T, DP, WHOLE>;
         // (a step with every place taken, 64 channels: 64 keys 2.4 us, 64 rows 2.8)
         p.q = plan_walks(heads * ((rows + 127) / 128), (q.Lk + Q::KT - 1) / Q::KT,
-                         cus * resident(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, NP, WHOLE>), Q::LDS), 2.4 * Q::KT / 64 * DP / 64 * slow, part);
+                         cus * resident(reinterpret_cast<const void *>(&attn_bwd_q_kernel<T, DP, NP, WHOLE>), Q::LDS), 2.4 * Q::KT / 64 * DP / 64 * slow, part, limit);
         p.kv = plan_walks(heads * ((q.Lk + 127) / 128), (rows + KV::RT - 1) / KV::RT,
-                          cus * resident(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, NP, WHOLE>), KV::LDS), 2.8 * KV::RT / 64 * DP / 64 * slow, 2 * part);
+                          cus * resident(reinterpret_cast<const void *>(&attn_bwd_kv_kernel<T, DP, NP, WHOLE>), KV::LDS), 2.8 * KV::RT / 64 * DP / 64 * slow, 2 * part, limit);
         return 0;
     });
     p.delta_bytes = d2c_align_up((size_t)heads * rows * 4);

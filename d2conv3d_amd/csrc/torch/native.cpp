@@ -90,8 +90,8 @@ Tensor workspace(size_t bytes, const Tensor &like, hipStream_t st)
     return THPVariable_Unpack(made.ptr());
 }
 
-// A workspace of a few megabytes at most, asked for from a backward pass: from the allocator, which is quicker than waiting for the
-// interpreter's lock on the engine's thread
+// A workspace of up to some tens of megabytes (layer norm: 64 at most) that is not kept from call to call: from the allocator, which is quicker than
+// waiting for the interpreter's lock on the engine's thread
 Tensor small_workspace(size_t bytes, const Tensor &like)
 {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte).requires_grad(false)) : Tensor();
@@ -754,6 +754,20 @@ void strides(d2c_attention_desc &q, const Tensor &query, const Tensor &key, cons
     for (int i = 0; i < 3; i++) { q.q_stride[i] = query.stride(i); q.k_stride[i] = key.stride(i); q.v_stride[i] = value.stride(i); }
 }
 
+// The workspace of an attention call, from the allocator, and its size: without room for partial sums (D2C_ATTENTION_PART_BYTES at most, tens of megabytes as a
+// rule) where there is none
+Tensor part_workspace(d2c_attention_desc &q, size_t (*size)(const d2c_attention_desc *), size_t &bytes, const Tensor &like)
+{
+    bytes = size(&q);
+    try {
+        return small_workspace(bytes, like);
+    } catch (const c10::OutOfMemoryError &) {
+        q.part_limit = -1;
+        bytes = size(&q);
+    }
+    return small_workspace(bytes, like);
+}
+
 struct CrossAttentionBackward : public Node {
     d2c_attention_desc q;
     SavedVariable query, key, value, lengths, mask, out, low, lse;
@@ -784,8 +798,9 @@ struct CrossAttentionBackward : public Node {
             if (should_compute_output(0)) r[0] = no_grad_empty_like(vq);
             if (should_compute_output(1)) r[1] = no_grad_empty_like(vk);
             if (should_compute_output(2)) r[2] = no_grad_empty_like(vv);
-            const size_t nb = d2c_attention_backward_workspace_bytes(&q);
-            const Tensor ws = small_workspace(nb, vq);
+            size_t nb = 0;
+            q.part_limit = 0;
+            const Tensor ws = part_workspace(q, d2c_attention_backward_workspace_bytes, nb, vq);
             check(d2c_attention_backward(&q, ptr(g), ptr(vq), ptr(vk), ptr(vv), (const int32_t *)ptr(len), (const uint8_t *)ptr(msk), ptr(vo),
                                          ptr(vlow), (const float *)ptr(vl), ptr(r[0]), ptr(r[1]), ptr(r[2]), ptr(ws), nb, st),
                   "cross_attention backward");
@@ -833,8 +848,8 @@ py::object cross_attention(const Tensor &query, const Tensor &key, const Tensor 
     Tensor out = at::empty(query.sizes(), opt), low, lse;
     if (grad && dt == D2C_BF16) low = at::empty(query.sizes(), opt);
     if (grad) lse = at::empty({q.N, q.Hkv, (int64_t)q.Lq * (q.Hq / q.Hkv)}, opt.dtype(at::kFloat));
-    const size_t nb = d2c_attention_forward_workspace_bytes(&q);
-    const Tensor ws = small_workspace(nb, query);
+    size_t nb = 0;
+    const Tensor ws = part_workspace(q, d2c_attention_forward_workspace_bytes, nb, query);
     check(d2c_attention_forward(&q, ptr(query), ptr(key), ptr(value), (const int32_t *)ptr(len), (const uint8_t *)ptr(msk), ptr(out), ptr(low), (float *)ptr(lse),
                                 ptr(ws), nb, st),
           "cross_attention forward");

@@ -503,8 +503,9 @@ int d2c_layer_norm_backward(const d2c_layer_norm_desc *desc, const void *grad_y,
  * adjacent), y contiguous.  The first 2 * (pairs[0] + pairs[1] + pairs[2]) channels of a head turn in pairs, the others pass:
  * pair j of all is channels (2j, 2j + 1) if `interleaved`, else (j, j + all pairs); pair i of axis a turns by
  *     direction * position[a] * base^(-i / pairs[a])       radians
- * (an angle is exact to float32 for positions of up to 2^24, and off by 2^-48 turns a position beyond), direction 1, or -1 (which is the gradient's way back).  positions: float32 [L][3] for each sample, position_stride elements
- * from sample to sample (0: the same for all); NULL: token (t * grid[1] + h) * grid[2] + w has the position (t, h, w). */
+ * (an angle is exact to float32 for positions of up to 2^24, and off by 2^-48 turns a position beyond), direction 1, or -1 (which
+ * is the gradient's way back).  positions: float32 [L][3] for each sample, position_stride elements from sample to sample (0: the
+ * same for all); NULL: token (t * grid[1] + h) * grid[2] + w has the position (t, h, w). */
 #define D2C_ROTARY_MAX_PAIRS 128
 typedef struct d2c_rotary3d_desc {
     int32_t N, L, H, D;
@@ -523,11 +524,15 @@ int d2c_rotary3d(const d2c_rotary3d_desc *desc, const void *x, const float *posi
  * out, grad_out and the gradients are contiguous.  `lse` [N, Hkv, Lq * Hq / Hkv] and, bfloat16, `out_low` (as out: what
  * rounding took off it, which the gradients of queries and keys would miss) are for the backward call (NULL: not kept, and
  * the backward call takes out_low as 0).
- * Results do not depend on the order in which workgroups run. */
+ * Results do not depend on the order in which workgroups run.  Sums are made in an order that sizes, strides, GPU and part_limit
+ * determine.  Workgroups that share a row's keys (or a key's rows) leave partial sums in the workspace, of `part_limit` bytes at most: 0 is
+ * D2C_ATTENTION_PART_BYTES, a negative number none, with which a call runs in the least memory and takes longer where rows, or keys, are few. */
+#define D2C_ATTENTION_PART_BYTES (256L << 20)
 typedef struct d2c_attention_desc {
     int32_t N, Lq, Lk, Hq, Hkv, D, dtype;
     float scale;
     int64_t q_stride[3], k_stride[3], v_stride[3];
+    int64_t part_limit;
 } d2c_attention_desc;
 size_t d2c_attention_forward_workspace_bytes(const d2c_attention_desc *desc);
 int d2c_attention_forward(const d2c_attention_desc *desc, const void *query, const void *key, const void *value,
