@@ -367,20 +367,25 @@ template <typename T, bool KV> __global__ void __launch_bounds__(256) attn_bwd_j
         store4<T>(const_cast<T *>(row_at<T>(a.gq, a.gs, a, hd, i)) + d, x, a.D - d);
 }
 
-// delta alone, where the queries' gradient is not wanted: one wavefront to a row
+// delta alone, where the queries' gradient is not wanted: one wavefront to a row (and to the rows a launch's wavefronts further on, so that its threads can be
+// counted in 32 bits)
+constexpr long kDeltaBlocks = 1L << 20;
 template <typename T> __global__ void __launch_bounds__(256) attn_delta_kernel(Args a)
 {
-    const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6), nh = at / a.rows;
-    if (at >= (long)a.N * a.Hkv * a.rows) return;
-    const int n = (int)(nh / a.Hkv), lane = threadIdx.x & 63;
-    const Head hd{n, (int)(nh - (long)n * a.Hkv), nh};
-    const T *g = row_at<T>(a.g, a.gs, a, hd, (int)(at - nh * a.rows)), *o = row_at<T>(a.o, a.gs, a, hd, (int)(at - nh * a.rows));
-    const T *low = a.o_low ? row_at<T>(a.o_low, a.gs, a, hd, (int)(at - nh * a.rows)) : nullptr;
-    float x = 0.f;
-    for (int d = lane; d < a.D; d += 64) x = fmaf(elem_to_f32<T>(g[d]), elem_to_f32<T>(o[d]) + (low ? elem_to_f32<T>(low[d]) : 0.f), x);
+    const long total = (long)a.N * a.Hkv * a.rows;
+    const int lane = threadIdx.x & 63;
+    for (long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6); at < total; at += 4L * gridDim.x) {
+        const long nh = at / a.rows;
+        const int n = (int)(nh / a.Hkv);
+        const Head hd{n, (int)(nh - (long)n * a.Hkv), nh};
+        const T *g = row_at<T>(a.g, a.gs, a, hd, (int)(at - nh * a.rows)), *o = row_at<T>(a.o, a.gs, a, hd, (int)(at - nh * a.rows));
+        const T *low = a.o_low ? row_at<T>(a.o_low, a.gs, a, hd, (int)(at - nh * a.rows)) : nullptr;
+        float x = 0.f;
+        for (int d = lane; d < a.D; d += 64) x = fmaf(elem_to_f32<T>(g[d]), elem_to_f32<T>(o[d]) + (low ? elem_to_f32<T>(low[d]) : 0.f), x);
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
-    if (lane == 0) a.delta[at] = x;
+        for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+        if (lane == 0) a.delta[at] = x;
+    }
 }
 
 struct BwdPlan { Walks q, kv; size_t delta_bytes, bytes; };
@@ -410,7 +415,7 @@ template <typename T> BwdPlan bwd_plan(const d2c_attention_desc &q)
 template <typename T, int DP, int NP, bool WHOLE> int launch_bwd(Args a, const BwdPlan &p, hipStream_t st)
 {
     if (a.Lq > 0 && !a.gq && (a.gk || a.gv)) {
-        hipLaunchKernelGGL(attn_delta_kernel<T>, dim3((unsigned)(((long)a.N * a.Hkv * a.rows + 3) / 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(attn_delta_kernel<T>, dim3((unsigned)std::min(((long)a.N * a.Hkv * a.rows + 3) / 4, kDeltaBlocks)), dim3(256), 0, st, a);
         if (int rc = d2c_check_launch("attn_delta_kernel")) return rc;
     } else if (a.Lq > 0 && a.gq) {
         constexpr int lds = QShape<T, DP, WHOLE>::LDS;
