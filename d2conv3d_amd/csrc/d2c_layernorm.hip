@@ -174,9 +174,17 @@ template <typename T, typename TP, int LANES, int NV> __global__ void __launch_b
         if (row - sub + step < a.rows) request(row + step);
         float h[NV][VEC], t[NV][VEC], A = 0.f, B = 0.f;
 #pragma unroll
+        for (int i = 0; i < NV; i++) x.floats(i, h[i]);
+        if (!(fabsf(st.x * st.y) < INFINITY)) {      // (zeros behind a row's end would become infinities, and meet zeros)
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++)
+                    if ((i * LANES + lane) * VEC + j >= a.C) h[i][j] = st.x;
+        }
+#pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (i * LANES + lane) * VEC;
-            x.floats(i, h[i]);
             g.floats(i, t[i]);
             if constexpr (!KEEP) load_params<TP, VEC>(a.w, c, a.C, 1.f, w[0]);
 #pragma unroll
