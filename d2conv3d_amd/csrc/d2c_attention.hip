@@ -278,7 +278,8 @@ template <typename T, int LANES, int R> struct TokenShape {
 // every group of lanes keeps its own maximum, sum and output of each of the R rows until the end.  No LDS and no barrier on the way, the next keys requested
 // while these are worked on.  Bound: memory, latency where the memory is short.  Measured with the join: one token of 16 heads that share 4, 12960
 // positions of 64 channels, bfloat16, 12.4 us (13 MB: 2.6 at a copy's rate; two launches are 8 of them); two samples' 30000 positions of 128 channels 22.4 us,
-// float32 23 (attn_fwd_kernel 28.8 and 58).
+// float32 23 (attn_fwd_kernel 28.8 and 58).  Weights stay in float32: bfloat16 pairs on the dot instruction took 48.0, 48.1 us (one row), 21.0, 21.6 (four), 68.5, 71.6
+// (eight rows of 16 heads on 30000 positions of 128 channels) and lost 2^-9 of each.
 template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bounds__(256) attn_token_kernel(Args a)
 {
     using Shape = TokenShape<T, LANES, R>;
@@ -360,36 +361,17 @@ template <typename T, int LANES, int R, bool WHOLE> __global__ void __launch_bou
                 l[r] += s[u][r];
             }
         }
-        if constexpr (sizeof(T) == 2 && WHOLE) {      // two keys to an instruction, weights as bfloat16 (as the matrix kernels take them)
 #pragma unroll
-            for (int u = 0; u < LOADS; u += 2) {
-                const uint32_t x[4] = {vw[u].x, vw[u].y, vw[u].z, vw[u].w}, y[4] = {vw[u + 1].x, vw[u + 1].y, vw[u + 1].z, vw[u + 1].w};
-                uint32_t pair[8];
+        for (int u = 0; u < LOADS; u++) {
+            alignas(16) T e[VEC];
+            float vf[VEC];
+            *reinterpret_cast<uint4 *>(e) = vw[u];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    pair[2 * i] = __builtin_amdgcn_perm(y[i], x[i], 0x05040100u);
-                    pair[2 * i + 1] = __builtin_amdgcn_perm(y[i], x[i], 0x07060302u);
-                }
+            for (int i = 0; i < VEC; i++) vf[i] = elem_to_f32<T>(e[i]);
 #pragma unroll
-                for (int r = 0; r < R; r++) {
-                    const uint32_t p = pack_bf16x2(s[u][r], s[u + 1][r]);
+            for (int r = 0; r < R; r++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) o[r][i] = dot_pair(p, pair[i], o[r][i]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < LOADS; u++) {
-                alignas(16) T e[VEC];
-                float vf[VEC];
-                *reinterpret_cast<uint4 *>(e) = vw[u];
-#pragma unroll
-                for (int i = 0; i < VEC; i++) vf[i] = elem_to_f32<T>(e[i]);
-#pragma unroll
-                for (int r = 0; r < R; r++)
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) o[r][i] = fmaf(s[u][r], vf[i], o[r][i]);
-            }
+                for (int i = 0; i < VEC; i++) o[r][i] = fmaf(s[u][r], vf[i], o[r][i]);
         }
     }
     // the groups of a wavefront, two values to a step where half the wavefront can go on with either (32 sums of 8 lanes: 56 instructions for 256), then the
