@@ -47,11 +47,11 @@ template <typename T, int DP, int WK, bool WHOLE> struct FwdShape {
 //
 // One pass over the keys with the running maximum and sum of a softmax; the weights p go from one product's accumulator into the next one's operand without
 // leaving their registers, so that LDS holds K and V alone, which come through it once for 128 rows.  Registers are kept to what three workgroups of a compute
-// unit have room for at 64 channels (two take 1.18 times as long, one 1.95).  Bound: the matrix instructions (busy 0.4 to 0.5 of the time) and the exponentials,
-// maxima, sums and roundings between them (0.4 to 0.57), which do not overlap further at the clock that the card keeps under them (1.9 to 2.0 GHz): without the
+// unit have room for at 64 channels (two take 1.18 times as long, one 1.95).  Bound: the matrix instructions (busy 0.41 of the time at 64 channels, 0.43 at 128)
+// and the exponentials, maxima, sums and roundings between them (0.66, 0.35), which do not overlap further at the clock that the card keeps under them (1.95 GHz): without the
 // exponentials 0.80 of the time, without the second product 0.80, without either's loads 0.95 each.
 // Measured, bfloat16: 12960 positions reading 25920, 8 heads of 64, 0.82 ms (0.84 PFLOP/s; a library product of 8192 cubed 1.27); 1620 reading 64800, 8 heads of
-// 128 that share 2 key heads, 0.46 ms with the join (0.94 PFLOP/s).  float32: 1417 reading 3001, 6 heads of 40, 44 us.
+// 128 that share 2 key heads, 0.46 ms with the join (0.94 PFLOP/s).  float32: 1417 reading 3001, 6 heads of 40, 43 us.
 template <typename T, int DP, int NP, int WK, bool WHOLE> __global__ void __launch_bounds__(256, (FwdShape<T, DP, WK, WHOLE>::WAVES)) attn_fwd_kernel(Args a)
 {
     using Shape = FwdShape<T, DP, WK, WHOLE>;

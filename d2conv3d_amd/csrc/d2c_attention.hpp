@@ -38,10 +38,13 @@ struct Args {
 };
 
 template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 1 : 3;
-// Terms of the weights p and of ds, which are rounded to the matrix instruction's operands: bfloat16 problems take one, whose errors are as large as the
-// rounding of the result and average out over many keys.  Where there are 64 keys or fewer, they do not (two keys: weights just above 1/2, where the
-// spacing is widest), nor in the gradients of a small problem, and a second term costs nothing there that counts.  (Heads of an odd size run on the same
-// kernels and have it, too.)
+// Terms of the weights p and of ds, which are rounded to the matrix instruction's operands: bfloat16 problems take one, whose errors (2^-9 of each; the row's sum is
+// that of the weights before) are as large as the rounding of the result and average out over many keys: 2.4e-3 of a result in all, 1.7e-3 of them by its own
+// rounding.  A second term everywhere would take 1.34 to 1.45 times as long (1620 rows on 64800 keys of 8 heads of 128, 470, 628 us; 12960 on 25920 of 64,
+// forward and backward, 3260, 4717).  Where a call has 64 keys or fewer, errors do not average out (two keys: weights just above 1/2, where the spacing is
+// widest), nor in the gradients of a small problem: these have the second term, at 1.11 to 1.16 times the backward kernels' time where the line is (512 rows on
+// 1024 keys of 8 heads of 64, 38.1, 42.9 us; of 128, 54.6, 63.0; whole passes are the host's 55 to 85 us either way).  Calls count, not samples: two keys that a mask leaves
+// of 1000 have weights of one term in a large call.  (Heads of an odd size, and rows that lie further apart than 32-bit offsets reach, run on the same kernels and have it, too.)
 template <typename T, bool FAST> constexpr int kWeightTerms = sizeof(T) == 4 ? 3 : FAST ? 1 : 2;
 constexpr int kExactKeys = 64;
 constexpr long kExactScores = 1L << 22;

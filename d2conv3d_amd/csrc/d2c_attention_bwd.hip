@@ -22,7 +22,7 @@ template <typename T, int DP, bool WHOLE> struct QShape {
 // s and dp of a tile of keys, then dq += ds k.  As attn_fwd_kernel: rows along the lanes, ds into the last product's operand in registers, K and V through LDS
 // (K read twice, by rows and by columns).  Bound: as there, matrix instructions first (3 products to one exponential).
 // Measured, bfloat16: 12960 rows, 25920 keys, 8 heads of 64, 1.04 ms (0.99 PFLOP/s); 1620 rows, 12960 keys (3/4 of them read), 2 samples, 0.13 ms.
-// float32: 1417 rows, 3001 keys, 6 heads of 40, 62 us.
+// float32: 1417 rows, 3001 keys, 6 heads of 40, 60 us.
 template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, (QShape<T, DP, WHOLE>::WAVES)) attn_bwd_q_kernel(Args a)
 {
     using KV = typename QShape<T, DP, WHOLE>::KV;
@@ -169,9 +169,10 @@ template <typename T, int DP, bool WHOLE> struct KvShape {
 
 // Keys along the lanes, their K and V in registers from first to last; queries and grad_out of a tile of rows through LDS, each read by rows (s, dp) and by
 // columns (dk, dv).  dp starts from -delta, one subtraction less to a score.  K and V in LDS, too, would make room for a third workgroup to a compute unit, and takes
-// 1.5 times as long at 64 channels: the LDS is read six times a tile then.  Bound: matrix instructions (4 products to one exponential), behind them LDS.
+// 1.5 times as long at 64 channels: the LDS is read six times a tile then.  A mask costs nothing and saves nothing here: rows of tiles whose keys are all not to be read are walked
+// over, too (behind a sample's length they are not).  Bound: matrix instructions (4 products to one exponential), behind them LDS.
 // Measured, bfloat16: 12960 rows, 25920 keys, 8 heads of 64, 1.38 ms (1.0 PFLOP/s); 1620 rows, 12960 keys (3/4 of them read), 2 samples, 0.21 ms.
-// float32: 1417 rows, 3001 keys, 6 heads of 40, 75 us.
+// float32: 1417 rows, 3001 keys, 6 heads of 40, 72 us.
 template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, (KvShape<T, DP, WHOLE>::WAVES)) attn_bwd_kv_kernel(Args a)
 {
     using QG = typename KvShape<T, DP, WHOLE>::QG;

@@ -525,8 +525,11 @@ int d2c_rotary3d(const d2c_rotary3d_desc *desc, const void *x, const float *posi
  * rounding took off it, which the gradients of queries and keys would miss) are for the backward call (NULL: not kept, and
  * the backward call takes out_low as 0).
  * Results do not depend on the order in which workgroups run.  Sums are made in an order that sizes, strides, GPU and part_limit
- * determine.  Workgroups that share a row's keys (or a key's rows) leave partial sums in the workspace, of `part_limit` bytes at most: 0 is
- * D2C_ATTENTION_PART_BYTES, a negative number none, with which a call runs in the least memory and takes longer where rows, or keys, are few. */
+ * determine.  Workgroups that share a row's keys (or a key's rows) leave partial sums in the workspace, of `part_limit` bytes at
+ * most: 0 is D2C_ATTENTION_PART_BYTES, a negative number none, with which a call runs in the least memory and takes longer where
+ * rows, or keys, are few.
+ * Infinities that are read: a key whose score is -infinity has weight 0; an infinite value or grad_out makes its channel of out
+ * or of the values' gradient infinite, and no other. */
 #define D2C_ATTENTION_PART_BYTES (256L << 20)
 typedef struct d2c_attention_desc {
     int32_t N, Lq, Lk, Hq, Hkv, D, dtype;
