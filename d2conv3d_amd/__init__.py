@@ -16,6 +16,7 @@ from .grid import offsets_from_size_map
 from .util import add_deformable_conv
 from .depthwise_conv import DepthwiseConv3d, depthwise_separable_conv3d, install_as_fast_depthwise_conv3d
 from .attention import CrossAttention3d, LayerNorm, cross_attention, layer_norm, rotary3d
+from .memory import PagedMemory, memory_append, memory_attention, memory_evict
 
 __all__ = [
     "deform_conv1d", "deform_conv3d", "deform_conv3d_sized", "DeformConv1d", "DeformConv3d", "DeformConvNd",
@@ -27,6 +28,7 @@ __all__ = [
     "offsets_from_size_map", "add_deformable_conv", "install_as_dconv_native",
     "DepthwiseConv3d", "depthwise_separable_conv3d", "install_as_fast_depthwise_conv3d",
     "CrossAttention3d", "LayerNorm", "cross_attention", "layer_norm", "rotary3d",
+    "PagedMemory", "memory_append", "memory_attention", "memory_evict",
 ]
 
 

@@ -40,6 +40,8 @@ EXPORTS = (
     "d2c_layer_norm_forward", "d2c_layer_norm_backward_workspace_bytes", "d2c_layer_norm_backward", "d2c_rotary3d",
     "d2c_attention_forward_workspace_bytes", "d2c_attention_forward",
     "d2c_attention_backward_workspace_bytes", "d2c_attention_backward",
+    "d2c_memory_append", "d2c_memory_attention_workspace_bytes", "d2c_memory_attention",
+    "d2c_memory_evict_workspace_bytes", "d2c_memory_evict",
 )
 
 
@@ -103,6 +105,15 @@ class Rotary3dDesc(ctypes.Structure):
 class AttentionDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("N", "Lq", "Lk", "Hq", "Hkv", "D", "dtype")] + [("scale", ctypes.c_float)] + [
         (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")] + [("part_limit", ctypes.c_int64)]
+
+
+class MemoryDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("streams", "heads", "D", "dtype", "pages", "page", "per_stream")] + [
+        ("table_stride", ctypes.c_int64), ("key_stride", ctypes.c_int64 * 3), ("value_stride", ctypes.c_int64 * 3)]
+
+
+class MemoryQueryDesc(ctypes.Structure):
+    _fields_ = [("query_heads", ctypes.c_int32), ("scale", ctypes.c_float), ("query_stride", ctypes.c_int64 * 2)]
 
 
 class Conv1dDesc(ctypes.Structure):
@@ -216,6 +227,13 @@ def load():
         f.argtypes, f.restype = [pat], sz
     lib.d2c_attention_forward.argtypes, lib.d2c_attention_forward.restype = [pat] + [vp] * 9 + [sz, vp], ctypes.c_int
     lib.d2c_attention_backward.argtypes, lib.d2c_attention_backward.restype = [pat] + [vp] * 13 + [sz, vp], ctypes.c_int
+    pme, pmq, i64 = ctypes.POINTER(MemoryDesc), ctypes.POINTER(MemoryQueryDesc), ctypes.c_int64
+    lib.d2c_memory_append.argtypes = [pme] + [vp] * 9 + [ctypes.POINTER(i64)] * 2 + [vp, i64, vp]
+    lib.d2c_memory_append.restype = ctypes.c_int
+    lib.d2c_memory_attention_workspace_bytes.argtypes, lib.d2c_memory_attention_workspace_bytes.restype = [pme, pmq, i32], sz
+    lib.d2c_memory_attention.argtypes, lib.d2c_memory_attention.restype = [pme, pmq] + [vp] * 8 + [sz, vp], ctypes.c_int
+    lib.d2c_memory_evict_workspace_bytes.argtypes, lib.d2c_memory_evict_workspace_bytes.restype = [pme, i32], sz
+    lib.d2c_memory_evict.argtypes, lib.d2c_memory_evict.restype = [pme] + [vp] * 7 + [i32, i32, vp, sz, vp], ctypes.c_int
     lib.d2c_profile_enable.argtypes, lib.d2c_profile_enable.restype = [ctypes.c_int], None
     lib.d2c_profile_reset.argtypes, lib.d2c_profile_reset.restype = [], None
     lib.d2c_profile_read.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int)]

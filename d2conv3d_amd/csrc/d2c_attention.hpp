@@ -401,6 +401,37 @@ D2C_DEV void other_half(float v, float &x, float &y)
 D2C_DEV float half_max(float v) { float x, y; other_half(v, x, y); return fmaxf(x, y); }
 D2C_DEV float half_sum(float v) { float x, y; other_half(v, x, y); return x + y; }
 
+// ---- one to eight rows, by lanes
+template <int LANES, typename Op> D2C_DEV float over_groups(float v, Op op)      // over the lanes that lie a multiple of LANES apart
+{
+    if constexpr (LANES <= 4) v = op(v, dpp_f32<0x124>(v));    // lanes of sixteen, turned by 4
+    if constexpr (LANES <= 8) v = op(v, dpp_f32<0x128>(v));    // ... by 8
+    if constexpr (LANES <= 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    float x, y;
+    other_half(v, x, y);
+    return op(x, y);
+}
+
+// x + the products of two pairs
+D2C_DEV float dot_pair(uint32_t a, uint32_t b, float x)
+{
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, a), __builtin_bit_cast(bf16x2_t, b), x, false);
+}
+// 16 bytes against 16 bytes
+template <typename T> D2C_DEV float dot_words(const uint4 &a, const uint4 &b)
+{
+    if constexpr (sizeof(T) == 2) return dot_pair(a.w, b.w, dot_pair(a.z, b.z, dot_pair(a.y, b.y, dot_pair(a.x, b.x, 0.f))));
+    else return fmaf(__uint_as_float(a.w), __uint_as_float(b.w), fmaf(__uint_as_float(a.z), __uint_as_float(b.z),
+                fmaf(__uint_as_float(a.y), __uint_as_float(b.y), __uint_as_float(a.x) * __uint_as_float(b.x))));
+}
+
+template <typename T, int LANES, int R> struct TokenShape {
+    static constexpr int VEC = 16 / (int)sizeof(T), DP = LANES * VEC, LOADS = R <= 4 ? 4 : 2, KEYS = 64 / LANES, STEP = 4 * LOADS * KEYS;
+};
+
 // The rows of a tile of keys to request: a key that is not to be read is replaced by one of the tile's that is (any_key, of `words`), so that
 // what it holds is nowhere read: its score is put to -infinity, and its weight 0 meets zeros that are put in the place of that other key's value (which
 // may be infinite).

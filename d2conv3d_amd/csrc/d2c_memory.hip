@@ -1,0 +1,838 @@
+// A memory of keys and values in pages: tokens appended, read by one new token of each stream, evicted by accumulated weight.
+//
+//   attention  s_j = scale <q, k_j>,  p_j = exp(s_j - max s) / sum exp(s - max s),  o = sum_j p_j v_j,  usage_j += sum over rows of p_j
+//   eviction   a slot stays if its token is one of the newest, or if its usage is among the largest of the others
+#include <type_traits>
+#include "d2c_attention.hpp"
+
+using namespace d2c_attn;
+
+namespace {
+
+struct MemArgs {
+    const void *q;
+    void *key, *value, *out;
+    const int32_t *table, *lengths;
+    float *usage;                 // or NULL
+    float *part, *part_ml;        // [units + places][R][part_width(D)], and (maximum, sum) of each row
+    int32_t *covered;             // [units][2]: the first and the last workgroup that has a piece of the unit
+    int32_t *begins;              // [places][4]: unit and step that a workgroup begins with, its steps
+    float *scores;                // [streams * heads * group][slots], of base 2
+    long qs[2], ks[3], vs[3], table_stride, slots_padded;
+    FastDiv page;
+    int N, heads, group, D, pages, slots, row_groups, units, places, least;
+    float scale2;
+};
+
+D2C_DEV int slots_of(const MemArgs &a, int n) { return min(max(a.lengths[n], 0), a.slots); }
+// Steps of a stream's walk: one at least, so that a stream without slots has a unit that writes its zeros
+template <int STEP> D2C_DEV int steps_of(const MemArgs &a, int n) { return max(1, (slots_of(a, n) + STEP - 1) / STEP); }
+
+template <typename Op> D2C_DEV int wave_scan(int v, Op op)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(v, d, 64);
+        if (lane >= d) v = op(v, x);
+    }
+    return v;
+}
+
+// Where this workgroup begins.  The steps of all units (stream, key head, rows of up to eight; in this order) are one line, of which every workgroup takes as
+// many as the others: streams of any lengths load all compute units alike, and no length is known on the host.  False: nothing left for this one.
+template <int STEP> D2C_DEV bool find_begin(const MemArgs &a, int &unit, int &t, int &budget)
+{
+    __shared__ int s_wave[4], s_found[2];
+    const int tid = threadIdx.x, wave = tid >> 6, per_stream = a.heads * a.row_groups;
+    auto add = [](int x, int y) INLINE { return x + y; };
+    int c = 0;
+    for (int n = tid; n < a.N; n += 256) c += steps_of<STEP>(a, n);
+    int scan = wave_scan(c, add);
+    if ((tid & 63) == 63) s_wave[wave] = scan;
+    __syncthreads();
+    const long total = (long)(s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3]) * per_stream;
+    budget = max((int)((total + a.places - 1) / a.places), a.least);
+    const long start = (long)blockIdx.x * budget;
+    if (start >= total) return false;
+    long base = 0;
+    for (int n0 = 0; n0 < a.N; n0 += 256) {
+        const int n = n0 + tid;
+        if (a.N > 256) {
+            c = n < a.N ? steps_of<STEP>(a, n) : 0;
+            scan = wave_scan(c, add);
+            __syncthreads();
+            if ((tid & 63) == 63) s_wave[wave] = scan;
+            __syncthreads();
+        }
+        long before = base + scan - c;
+        for (int w = 0; w < wave; w++) before += s_wave[w];
+        if (n < a.N && before * per_stream <= start && start < (before + c) * per_stream) { s_found[0] = n; s_found[1] = (int)before; }
+        base += s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+    }
+    __syncthreads();
+    const int n = s_found[0], steps = steps_of<STEP>(a, n), off = (int)(start - (long)s_found[1] * per_stream);
+    unit = n * per_stream + off / steps;
+    t = off % steps;
+    return true;
+}
+
+// The weights of a unit's slots from s0 to s1, added up over all rows of its key head.  s_ml: maximum and 1 / sum of the rows
+D2C_DEV void add_usage(const MemArgs &a, int n, int h, int s0, int s1, const float2 *s_ml)
+{
+    const float *scores = a.scores + (long)(n * a.heads + h) * a.group * a.slots_padded;
+    for (int s = s0 + (int)threadIdx.x; s < s1; s += 256) {
+        const int p = fdiv(s, a.page), id = a.table[n * a.table_stride + p];
+        if ((unsigned)id >= (unsigned)a.pages) continue;
+        float x = 0.f;
+        for (int r = 0; r < a.group; r++) x += __builtin_amdgcn_exp2f(scores[r * a.slots_padded + s] - s_ml[r].x) * s_ml[r].y;
+        a.usage[((long)id * a.heads + h) * a.page.d + (s - p * a.page.d)] += x;
+    }
+}
+// (a row whose sum is 0 has no slot, or none whose score is above -infinity: no weights)
+D2C_DEV float2 usage_ml(float top, float sum) { return make_float2(top == -INFINITY ? 0.f : top, sum == 0.f ? 0.f : 1.f / sum); }
+
+// One new token of each stream.  As attn_token_kernel, by lanes and without matrix instructions: LANES lanes hold a slot's key and value, 16 bytes each, a wavefront
+// 64 / LANES slots; every group of lanes keeps its own maximum, sum and output of each of the R rows until the end of the unit's piece.  The page of a slot is
+// asked for two steps ahead, its key and value one.  ONE: a workgroup to a unit (short memories), which needs no second launch.
+// Bound: memory.
+template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __launch_bounds__(256) mem_attn_kernel(MemArgs a)
+{
+    using Shape = TokenShape<T, LANES, R>;
+    constexpr int VEC = Shape::VEC, DP = Shape::DP, LOADS = Shape::LOADS, KEYS = Shape::KEYS, STEP = Shape::STEP;
+    __shared__ __align__(16) float s_o[4][R][DP];
+    __shared__ float2 s_ml[4][R];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = lane % LANES * VEC;
+    int unit = blockIdx.x, t = 0, budget = 1 << 30;
+    if constexpr (!ONE) {
+        const bool some = find_begin<STEP>(a, unit, t, budget);
+        if (threadIdx.x < 4) a.begins[blockIdx.x * 4 + threadIdx.x] = threadIdx.x == 0 ? (some ? unit : -1) : threadIdx.x == 1 ? t : budget;
+        if (!some) return;
+    }
+    auto load = [&](const T *row) INLINE {      // this lane's 16 bytes; zeros behind the row's end
+        if constexpr (WHOLE) {
+            const AnyVec<T> v = load_any(row + min(d0, a.D - VEC));
+            return make_uint4(v[0], v[1], v[2], v[3]);
+        } else return d0 < a.D ? load_run<T>(row + d0, a.D - d0) : make_uint4(0, 0, 0, 0);
+    };
+    for (; budget > 0 && unit < a.units; unit++, t = 0) {
+        const int nh = unit / a.row_groups, row0 = (unit - nh * a.row_groups) * R, n = nh / a.heads, h = nh - n * a.heads;
+        const int rows = min(R, a.group - row0), slots = slots_of(a, n), steps = max(1, (slots + STEP - 1) / STEP);
+        const int t0 = t, t1 = ONE ? steps : min(steps, t + budget);
+        budget -= t1 - t0;
+        const T *kb = reinterpret_cast<const T *>(a.key) + h * a.ks[1], *vb = reinterpret_cast<const T *>(a.value) + h * a.vs[1];
+        const int32_t *table = a.table + n * a.table_stride;
+        float *scores = a.usage ? a.scores + ((long)nh * a.group + row0) * a.slots_padded : nullptr;
+
+        uint4 k[LOADS], v[LOADS];
+        bool there[LOADS];
+        int id[LOADS], in_page[LOADS];
+        auto slot_of = [&](int step, int u) INLINE { return step * STEP + (u * 4 + wave) * KEYS + lane / LANES; };
+        auto look = [&](int step) INLINE {
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                const int s = min(slot_of(step, u), slots - 1), p = fdiv(s, a.page);
+                id[u] = table[p];
+                in_page[u] = s - p * a.page.d;
+            }
+        };
+        auto request = [&](int step) INLINE {
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                const bool valid = (unsigned)id[u] < (unsigned)a.pages;
+                there[u] = valid && slot_of(step, u) < slots;
+                const long page = valid ? id[u] : 0;
+                k[u] = load(kb + page * a.ks[0] + in_page[u] * a.ks[2]);
+                v[u] = load(vb + page * a.vs[0] + in_page[u] * a.vs[2]);
+            }
+        };
+        if (slots > 0) {
+            look(t);
+            request(t);
+            if (t + 1 < t1) look(t + 1);
+        }
+        uint4 q[R];
+        float o[R][VEC], m[R], l[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const uint4 w = load(reinterpret_cast<const T *>(a.q) + n * a.qs[0] + (long)(h * a.group + row0 + min(r, rows - 1)) * a.qs[1]);
+            q[r] = r < rows ? w : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) o[r][i] = 0.f;
+            m[r] = -INFINITY;
+            l[r] = 0.f;
+        }
+        for (; t < t1 && slots > 0; t++) {
+            uint4 vw[LOADS];
+            float s[LOADS][R];
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                vw[u] = there[u] ? v[u] : make_uint4(0, 0, 0, 0);
+                // (a lane behind a row's end has its last piece again, which is no part of the score)
+                uint4 kw = k[u];
+                if (WHOLE && a.D < DP && d0 >= a.D) kw = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float x = lanes_sum<LANES>(dot_words<T>(q[r], kw)) * a.scale2;
+                    s[u][r] = there[u] ? x : -INFINITY;
+                }
+            }
+            if (scores) {
+#pragma unroll
+                for (int u = 0; u < LOADS; u++) {
+                    const int slot = slot_of(t, u);
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+                        if (lane % LANES == r % LANES && r < rows && slot < slots) scores[r * a.slots_padded + slot] = s[u][r];
+                }
+            }
+            if (t + 1 < t1) {
+                request(t + 1);
+                if (t + 2 < t1) look(t + 2);
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float top = s[0][r];
+#pragma unroll
+                for (int u = 1; u < LOADS; u++) top = fmaxf(top, s[u][r]);
+                // (the maximum follows where it has grown by more than a factor of 2^8 of the weights)
+                if (__any(top > m[r] + 8.f)) {
+                    const float grown = fmaxf(top, m[r]), f = grown == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[r] - grown);
+                    m[r] = grown;
+                    l[r] *= f;
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) o[r][i] *= f;
+                }
+                const float base = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+                for (int u = 0; u < LOADS; u++) {
+                    s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - base);
+                    l[r] += s[u][r];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < LOADS; u++) {
+                alignas(16) T e[VEC];
+                float vf[VEC];
+                *reinterpret_cast<uint4 *>(e) = vw[u];
+#pragma unroll
+                for (int i = 0; i < VEC; i++) vf[i] = elem_to_f32<T>(e[i]);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) o[r][i] = fmaf(s[u][r], vf[i], o[r][i]);
+            }
+        }
+        t = t1;
+        // the groups of lanes, two values to a step where half the wavefront can go on with either, then the wavefronts
+        float x[R * VEC];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float top = over_groups<LANES>(m[r], [](float x, float y) INLINE { return fmaxf(x, y); });
+            const float f = m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[r] - top);
+            l[r] = over_groups<LANES>(l[r] * f, [](float x, float y) INLINE { return x + y; });
+#pragma unroll
+            for (int i = 0; i < VEC; i++) x[r * VEC + i] = o[r][i] * f;
+            if (lane == 0) s_ml[wave][r] = make_float2(top, l[r]);
+        }
+        constexpr int HALVINGS = LANES <= 16 ? 2 : 1;
+#pragma unroll
+        for (int i = 0; i < R * VEC / 2; i++) {
+            const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1]), false, false);
+            x[i] = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+        }
+        if constexpr (HALVINGS == 2) {
+#pragma unroll
+            for (int i = 0; i < R * VEC / 4; i++) {
+                const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1]), false, false);
+                x[i] = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < (R * VEC >> HALVINGS); i++) {
+            if constexpr (LANES <= 4) x[i] += dpp_f32<0x124>(x[i]);
+            if constexpr (LANES <= 8) x[i] += dpp_f32<0x128>(x[i]);
+            const int at = HALVINGS == 2 ? 4 * i + (lane >> 4 & 1) * 2 + (lane >> 5) : 2 * i + (lane >> 5);
+            if (LANES >= 16 || (lane & 15) < LANES) s_o[wave][at / VEC][d0 + at % VEC] = x[i];
+        }
+        __syncthreads();
+        const bool direct = ONE || (t0 == 0 && t1 == steps);
+        const long piece = ONE ? unit : (long)unit + blockIdx.x;
+        for (int i = threadIdx.x; i < rows * DP; i += 256) {
+            const int r = i / DP, d = i - r * DP;
+            if (d >= a.D) continue;
+            float top = s_ml[0][r].x, sum = 0.f, x = 0.f;
+#pragma unroll
+            for (int w = 1; w < 4; w++) top = fmaxf(top, s_ml[w][r].x);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float f = __builtin_amdgcn_exp2f(s_ml[w][r].x - base);
+                sum = fmaf(s_ml[w][r].y, f, sum);
+                x = fmaf(s_o[w][r][d], f, x);
+            }
+            if (!ONE && d == 0) *reinterpret_cast<float2 *>(a.part_ml + (piece * R + r) * 2) = make_float2(top, sum);
+            if (direct) reinterpret_cast<T *>(a.out)[((long)n * a.heads * a.group + h * a.group + row0 + r) * a.D + d] = f32_to_elem<T>(sum == 0.f ? 0.f : x / sum);
+            else a.part[(piece * R + r) * part_width(a.D) + d] = x;
+        }
+        if (!ONE && threadIdx.x == 0) {
+            if (t0 == 0) a.covered[unit * 2] = blockIdx.x;
+            if (t1 == steps) a.covered[unit * 2 + 1] = blockIdx.x;
+        }
+        if constexpr (ONE) {
+            if (a.usage) {      // (one group of rows)
+                __shared__ float2 s_row[R];
+                if ((int)threadIdx.x < rows) {
+                    const int r = threadIdx.x;
+                    float top = s_ml[0][r].x, sum = 0.f;
+#pragma unroll
+                    for (int w = 1; w < 4; w++) top = fmaxf(top, s_ml[w][r].x);
+                    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) sum = fmaf(s_ml[w][r].y, __builtin_amdgcn_exp2f(s_ml[w][r].x - base), sum);
+                    s_row[r] = usage_ml(top, sum);
+                }
+                __syncthreads();
+                add_usage(a, n, h, 0, slots, s_row);
+            }
+            return;
+        }
+        __syncthreads();      // (s_o and s_ml are written again by the next unit's piece)
+    }
+}
+
+// Units that several workgroups have shared: blocks from 0, one to a row, put their pieces together.  Where weights are added up: blocks from `rows` on, one to each
+// workgroup of the walk, go over the same slots once more, by their scores.
+template <typename T, int LANES, int R> __global__ void __launch_bounds__(256) mem_join_kernel(MemArgs a, int rows, int step)
+{
+    constexpr int GROUPS = 256 / LANES;
+    __shared__ float4 s_x[256];
+    __shared__ float2 s_ml[256];
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x < rows) {
+        const int nh = blockIdx.x / a.group, row = blockIdx.x - nh * a.group, unit = nh * a.row_groups + row / R, r = row % R;
+        const int w0 = a.covered[unit * 2], w1 = a.covered[unit * 2 + 1];
+        if (w0 == w1) return;
+        const int lane = tid % LANES, group = tid / LANES, d = lane * 4, width = part_width(a.D);
+        float all = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int w = w0 + group; w <= w1; w += 4 * GROUPS) {
+            float2 ml[4];
+            float4 y[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const long from = (long)(unit + min(w + u * GROUPS, w1)) * R + r;
+                ml[u] = *reinterpret_cast<const float2 *>(a.part_ml + from * 2);
+                y[u] = *reinterpret_cast<const float4 *>(a.part + from * width + min(d, width - 4));
+            }
+            float top = all;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (w + u * GROUPS > w1) ml[u] = make_float2(-INFINITY, 0.f);
+                top = fmaxf(top, ml[u].x);
+            }
+            const float base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(all - base);
+            all = top;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] *= f;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (w + u * GROUPS > w1) continue;
+                const float g = __builtin_amdgcn_exp2f(ml[u].x - base);
+                l = fmaf(ml[u].y, g, l);
+                x[0] = fmaf(y[u].x, g, x[0]); x[1] = fmaf(y[u].y, g, x[1]); x[2] = fmaf(y[u].z, g, x[2]); x[3] = fmaf(y[u].w, g, x[3]);
+            }
+        }
+        s_x[tid] = make_float4(x[0], x[1], x[2], x[3]);
+        s_ml[tid] = make_float2(all, l);
+        __syncthreads();
+        if (group != 0) return;
+        const int some = min(GROUPS, w1 - w0 + 1);
+        for (int g = 1; g < some; g++) all = fmaxf(all, s_ml[g * LANES].x);
+        const float base = all == -INFINITY ? 0.f : all;
+        l = x[0] = x[1] = x[2] = x[3] = 0.f;
+        for (int g = 0; g < some; g++) {
+            const float2 ml = s_ml[g * LANES];
+            const float4 y = s_x[tid + g * LANES];
+            const float f = __builtin_amdgcn_exp2f(ml.x - base);
+            l = fmaf(ml.y, f, l);
+            x[0] = fmaf(y.x, f, x[0]); x[1] = fmaf(y.y, f, x[1]); x[2] = fmaf(y.z, f, x[2]); x[3] = fmaf(y.w, f, x[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = l == 0.f ? 0.f : x[i] / l;
+        if (d < a.D) store4<T>(reinterpret_cast<T *>(a.out) + ((long)nh * a.group + row) * a.D + d, x, a.D - d);
+        return;
+    }
+    const int32_t *begin = a.begins + ((int)blockIdx.x - rows) * 4;
+    int unit = begin[0], t = begin[1], budget = begin[2];
+    if (unit < 0) return;
+    for (; budget > 0 && unit < a.units; unit++, t = 0) {
+        const int nh = unit / a.row_groups, n = nh / a.heads, h = nh - n * a.heads, slots = slots_of(a, n), steps = max(1, (slots + step - 1) / step);
+        const int t1 = min(steps, t + budget);
+        budget -= t1 - t;
+        if (unit != nh * a.row_groups || slots == 0) continue;      // (the first group of rows goes for all of them)
+        __syncthreads();
+        for (int row = tid >> 6; row < a.group; row += 4) {
+            const int u = unit + row / R, w0 = a.covered[u * 2], w1 = a.covered[u * 2 + 1];
+            float top = -INFINITY, sum = 0.f;
+            for (int w = w0 + (tid & 63); w <= w1; w += 64) {
+                const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + ((long)(u + w) * R + row % R) * 2);
+                const float grown = fmaxf(top, ml.x), base = grown == -INFINITY ? 0.f : grown;
+                sum = sum * __builtin_amdgcn_exp2f(top - base) + ml.y * __builtin_amdgcn_exp2f(ml.x - base);
+                top = grown;
+            }
+            float all = top;
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) all = fmaxf(all, __shfl_xor(all, d, 64));
+            sum *= __builtin_amdgcn_exp2f(top - (all == -INFINITY ? 0.f : all));
+            sum = lanes_sum<64>(sum);
+            if ((tid & 63) == 0) s_ml[row] = usage_ml(all, sum);
+        }
+        __syncthreads();
+        add_usage(a, n, h, t * step, min(slots, t1 * step), s_ml);
+    }
+}
+
+// ---------------------------------------------------------------- append
+struct AppendArgs {
+    const void *nk, *nv;
+    void *key, *value;
+    const int32_t *table, *starts;      // starts: or NULL
+    int32_t *lengths, *seen, *positions;
+    float *usage;
+    long nks[2], nvs[2], ks[3], vs[3], table_stride, tokens;
+    FastDiv page;
+    int N, heads, D, pages, slots;
+};
+D2C_DEV long start_of(const AppendArgs &a, int n) { return min(max((long)a.starts[n], 0L), a.tokens); }
+
+// One new token of one stream's head: its key and value by pieces of 16 bytes, its usage and position
+template <typename T> D2C_DEV void put_piece(const AppendArgs &a, long token, int n, long slot, int position, int h, int piece, int pieces)
+{
+    if (slot >= a.slots) return;
+    const int p = fdiv((int)slot, a.page), id = a.table[n * a.table_stride + p], at = (int)slot - p * a.page.d;
+    if ((unsigned)id >= (unsigned)a.pages) return;
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const bool second = piece >= pieces;
+    const int d = (second ? piece - pieces : piece) * VEC;
+    const T *from = second ? reinterpret_cast<const T *>(a.nv) + token * a.nvs[0] + h * a.nvs[1] : reinterpret_cast<const T *>(a.nk) + token * a.nks[0] + h * a.nks[1];
+    T *to = second ? reinterpret_cast<T *>(a.value) + id * a.vs[0] + h * a.vs[1] + at * a.vs[2] : reinterpret_cast<T *>(a.key) + id * a.ks[0] + h * a.ks[1] + at * a.ks[2];
+    store_run<T>(to + d, load_run<T>(from + d, a.D - d), a.D - d);
+    if (piece == 0) {
+        const long i = ((long)id * a.heads + h) * a.page.d + at;
+        a.usage[i] = 0.f;
+        a.positions[i] = position;
+    }
+}
+// A token of each stream: a workgroup to a stream, which then lets its counts grow
+template <typename T> __global__ void __launch_bounds__(256) mem_append_one_kernel(AppendArgs a)
+{
+    const int n = blockIdx.x, pieces = (a.D * (int)sizeof(T) + 15) / 16, all = a.heads * pieces * 2;
+    const int length = min(max(a.lengths[n], 0), a.slots), seen = a.seen[n];
+    for (int i = threadIdx.x; i < all; i += 256) put_piece<T>(a, n, n, length, seen, i / (pieces * 2), i % (pieces * 2), pieces);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a.lengths[n] = min(length + 1, a.slots);
+        a.seen[n] = seen + 1;
+    }
+}
+// Packed tokens: a thread has one piece of a row (a token's head) and goes from row to row
+template <typename T> __global__ void __launch_bounds__(256) mem_append_kernel(AppendArgs a, FastDiv heads)
+{
+    const int pieces = (a.D * (int)sizeof(T) + 15) / 16, two = 2 * pieces, per = 256 / two, sub = threadIdx.x / two;
+    if (sub >= per) return;
+    const int rows = (int)a.tokens * a.heads;
+    for (long i = (long)blockIdx.x * per + sub; i < rows; i += (long)gridDim.x * per) {
+        const int token = fdiv((int)i, heads), h = (int)i - token * a.heads;
+        int lo = 0, hi = a.N;      // the last stream that begins at or before the token
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start_of(a, mid) <= token) lo = mid; else hi = mid;
+        }
+        const long first = start_of(a, lo);
+        if (token < first || token >= start_of(a, lo + 1)) continue;
+        const long later = token - first;
+        put_piece<T>(a, token, lo, min(max(a.lengths[lo], 0), a.slots) + later, (int)(a.seen[lo] + later), h, threadIdx.x - sub * two, pieces);
+    }
+}
+__global__ void __launch_bounds__(256) mem_count_kernel(AppendArgs a)
+{
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= a.N) return;
+    const long some = max(start_of(a, n + 1) - start_of(a, n), 0L);
+    a.lengths[n] = (int)min((long)min(max(a.lengths[n], 0), a.slots) + some, (long)a.slots);
+    a.seen[n] = (int)(a.seen[n] + some);
+}
+
+// ---------------------------------------------------------------- evict
+struct EvictArgs {
+    void *key, *value;
+    const int32_t *table, *seen;
+    int32_t *lengths, *positions;
+    float *usage;
+    uint32_t *ranks;             // [units][slots_padded]
+    int32_t *holes, *fillers;    // [units][pairs]
+    int32_t *counts;             // [units]
+    long ks[3], vs[3], table_stride, slots_padded;
+    FastDiv page;
+    int N, heads, D, pages, slots, keep, recent, pairs;
+};
+
+// What a slot is ranked by: usage as a number that sorts like it (NaN above all), above it what is to stay whatever its usage, below it what is not there
+D2C_DEV uint32_t rank_of(float usage, bool stays)
+{
+    if (stays) return 0xffffffffu;
+    if (usage != usage) return 0xfffffffeu;
+    const uint32_t u = __float_as_uint(usage + 0.f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// A workgroup to a stream's head.  The keep-th largest rank by its digits (11, 11 and 10 bits, a histogram of each in LDS), then the slots that go before `keep`
+// and those that stay behind it, each in rising order.
+constexpr int kEvictThreads = 1024;
+__global__ void __launch_bounds__(kEvictThreads) mem_rank_kernel(EvictArgs a)
+{
+    constexpr int BINS = 2048, WAVES = kEvictThreads / 64;
+    __shared__ int s_hist[BINS], s_wave[3][WAVES], s_digit[2];
+    const int unit = blockIdx.x, n = unit / a.heads, h = unit - n * a.heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int slots = min(max(a.lengths[n], 0), a.slots);
+    if (slots <= a.keep) {
+        if (tid == 0) a.counts[unit] = 0;
+        return;
+    }
+    uint32_t *ranks = a.ranks + unit * a.slots_padded;
+    const long newest = (long)a.seen[n] - a.recent;
+    uint32_t prefix = 0;
+    int wanted = a.keep;
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        for (int i = tid; i < BINS; i += kEvictThreads) s_hist[i] = 0;
+        __syncthreads();
+        if (pass == 0) {
+            for (int s = tid; s < slots; s += kEvictThreads) {
+                const int p = fdiv(s, a.page), id = a.table[n * a.table_stride + p];
+                uint32_t rank = 0;
+                if ((unsigned)id < (unsigned)a.pages) {
+                    const long i = ((long)id * a.heads + h) * a.page.d + (s - p * a.page.d);
+                    rank = rank_of(a.usage[i], a.positions[i] >= newest);
+                }
+                ranks[s] = rank;
+                atomicAdd(&s_hist[rank >> 21], 1);
+            }
+        } else {
+            const uint32_t mask = pass == 1 ? 0xffe00000u : 0xfffffc00u;
+            for (int s = tid; s < slots; s += kEvictThreads) {
+                const uint32_t rank = ranks[s];
+                if ((rank & mask) == prefix) atomicAdd(&s_hist[(rank >> shift) & (pass == 1 ? 2047 : 1023)], 1);
+            }
+        }
+        __syncthreads();
+        // bins from the top: thread i has bins 2047 - 2i and 2046 - 2i
+        const int high = s_hist[BINS - 1 - 2 * tid], low = s_hist[BINS - 2 - 2 * tid];
+        const int scan = wave_scan(high + low, [](int x, int y) INLINE { return x + y; });
+        if (lane == 63) s_wave[0][wave] = scan;
+        __syncthreads();
+        int above = scan - high - low;
+        for (int w = 0; w < wave; w++) above += s_wave[0][w];
+        if (above < wanted && wanted <= above + high) { s_digit[0] = BINS - 1 - 2 * tid; s_digit[1] = wanted - above; }
+        else if (above + high < wanted && wanted <= above + high + low) { s_digit[0] = BINS - 2 - 2 * tid; s_digit[1] = wanted - above - high; }
+        __syncthreads();
+        prefix |= (uint32_t)s_digit[0] << shift;
+        wanted = s_digit[1];      // how many of this digit stay, in the end: of the rank itself, lowest slots first
+        __syncthreads();
+    }
+    // a wavefront has neighbouring slots: 64 at a time, places by the lanes before
+    const int per = ((slots + WAVES * 64 - 1) / (WAVES * 64)) * 64, s0 = min(wave * per, slots), s1 = min(s0 + per, slots);
+    int equal = 0;
+    for (int s = s0; s < s1; s += 64) equal += __popcll(__ballot(s + lane < s1 && ranks[min(s + lane, s1 - 1)] == prefix));
+    if (lane == 0) s_wave[0][wave] = equal;
+    __syncthreads();
+    int ties = 0;
+    for (int w = 0; w < wave; w++) ties += s_wave[0][w];
+    const uint64_t before = (1ull << lane) - 1;
+    for (int write = 0; write < 2; write++) {
+        int seen = ties, holes = 0, fillers = 0;
+        if (write)
+            for (int w = 0; w < wave; w++) { holes += s_wave[1][w]; fillers += s_wave[2][w]; }
+        for (int s = s0; s < s1; s += 64) {
+            const bool live = s + lane < s1;
+            const uint32_t rank = ranks[min(s + lane, s1 - 1)];
+            const uint64_t same = __ballot(live && rank == prefix);
+            const bool stays = rank > prefix || (rank == prefix && seen + __popcll(same & before) < wanted);
+            seen += __popcll(same);
+            const uint64_t hole = __ballot(live && !stays && s + lane < a.keep), filler = __ballot(live && stays && s + lane >= a.keep);
+            if (write) {
+                if ((hole >> lane) & 1) a.holes[(long)unit * a.pairs + holes + __popcll(hole & before)] = s + lane;
+                if ((filler >> lane) & 1) a.fillers[(long)unit * a.pairs + fillers + __popcll(filler & before)] = s + lane;
+            }
+            holes += __popcll(hole);
+            fillers += __popcll(filler);
+        }
+        if (!write) {
+            if (lane == 0) { s_wave[1][wave] = holes; s_wave[2][wave] = fillers; }
+            __syncthreads();
+        } else if (wave == WAVES - 1 && lane == 0) a.counts[unit] = holes;
+    }
+}
+
+// What stays behind `keep` into the places of what goes before it: reads and writes meet nowhere.  A thread has one piece of 16 bytes of a key or value and goes
+// from pair to pair, four requested at a time.
+template <typename T> __global__ void __launch_bounds__(256) mem_move_kernel(EvictArgs a, int blocks)
+{
+    constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
+    const int unit = blockIdx.x / blocks, block = blockIdx.x - unit * blocks, n = unit / a.heads, h = unit - n * a.heads, count = a.counts[unit];
+    if (block == 0 && h == 0 && threadIdx.x == 0) a.lengths[n] = min(min(max(a.lengths[n], 0), a.slots), a.keep);
+    const int pieces = (a.D + VEC - 1) / VEC, two = 2 * pieces, per = 256 / two, sub = threadIdx.x / two, part = threadIdx.x - sub * two;
+    if (sub >= per) return;
+    const bool second = part >= pieces;
+    const int d = (second ? part - pieces : part) * VEC;
+    T *base = reinterpret_cast<T *>(second ? a.value : a.key) + h * (second ? a.vs[1] : a.ks[1]) + d;
+    const long ps = second ? a.vs[0] : a.ks[0], ss = second ? a.vs[2] : a.ks[2];
+    const int32_t *table = a.table + n * a.table_stride, *holes = a.holes + (long)unit * a.pairs, *fillers = a.fillers + (long)unit * a.pairs;
+    for (int i = block * per + sub; i < count; i += blocks * per * AT_ONCE) {
+        T *to[AT_ONCE];
+        uint4 x[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            to[u] = nullptr;
+            if (i + u * blocks * per >= count) continue;
+            const int hole = holes[i + u * blocks * per], filler = fillers[i + u * blocks * per], tp = fdiv(hole, a.page), fp = fdiv(filler, a.page);
+            const int td = table[tp], fd = table[fp], ti = hole - tp * a.page.d, fi = filler - fp * a.page.d;
+            if ((unsigned)td >= (unsigned)a.pages || (unsigned)fd >= (unsigned)a.pages) continue;
+            to[u] = base + td * ps + ti * ss;
+            x[u] = load_run<T>(base + fd * ps + fi * ss, a.D - d);
+            if (part == 0) {
+                const long into = ((long)td * a.heads + h) * a.page.d + ti, of = ((long)fd * a.heads + h) * a.page.d + fi;
+                a.usage[into] = a.usage[of];
+                a.positions[into] = a.positions[of];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++)
+            if (to[u]) store_run<T>(to[u], x[u], a.D - d);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+int check(const d2c_memory_desc *q)
+{
+    if (!q) { d2c_set_error("memory: null description"); return D2C_ERR_SHAPE; }
+    if (q->dtype != D2C_F32 && q->dtype != D2C_BF16) { d2c_set_error("memory: float32 or bfloat16 only"); return D2C_ERR_DTYPE; }
+    if (q->streams < 0 || q->pages < 0 || q->per_stream < 0 || q->heads <= 0 || q->D <= 0 || q->page <= 0) {
+        d2c_set_error("memory: sizes must not be negative, heads, their size and the page's positive");
+        return D2C_ERR_SHAPE;
+    }
+    if (q->D > 128) { d2c_set_error("memory: heads of up to 128 channels, got %d", q->D); return D2C_ERR_UNSUPPORTED; }
+    // (slots of a stream, steps of all and a launch's threads are counted in 32 bits)
+    if ((long)q->per_stream * q->page >= (1L << 30) || (long)q->streams * q->heads >= (1L << 21) || q->streams >= (1 << 20)) {
+        d2c_set_error("memory: too many streams, heads or slots");
+        return D2C_ERR_SHAPE;
+    }
+    return D2C_OK;
+}
+int check(const d2c_memory_desc *q, const d2c_memory_query_desc *x)
+{
+    if (int rc = check(q)) return rc;
+    if (!x) { d2c_set_error("memory_attention: null description"); return D2C_ERR_SHAPE; }
+    if (x->query_heads <= 0 || x->query_heads % q->heads != 0) {
+        d2c_set_error("memory_attention: %d query heads are no positive multiple of %d key heads", x->query_heads, q->heads);
+        return D2C_ERR_SHAPE;
+    }
+    if (x->query_heads / q->heads > 256) { d2c_set_error("memory_attention: up to 256 query heads to a key head"); return D2C_ERR_UNSUPPORTED; }
+    if (!(x->scale > 0.f) || !(x->scale < INFINITY)) { d2c_set_error("memory_attention: scale must be positive and finite"); return D2C_ERR_SHAPE; }
+    const long slots = (long)q->per_stream * q->page;
+    if ((long)q->streams * x->query_heads >= (1L << 23) || (long)q->streams * x->query_heads * (slots / 32 + 1) >= (1L << 30)) { d2c_set_error("memory_attention: too many streams, heads or slots"); return D2C_ERR_SHAPE; }
+    return D2C_OK;
+}
+int need(const void *ws, size_t have, size_t bytes)
+{
+    if (!bytes || (ws && have >= bytes && !((uintptr_t)ws & 255u))) return D2C_OK;
+    d2c_set_error("workspace of %zu bytes (256-byte aligned) required, got %zu at %p", bytes, have, ws);
+    return D2C_ERR_WORKSPACE;
+}
+
+// f(T, LANES, R) as constants
+template <typename F> auto for_rows(const d2c_memory_desc &q, int group, F f)
+{
+    auto with_type = [&](auto zero) {
+        using T = decltype(zero);
+        constexpr int L32 = 32 * (int)sizeof(T) / 16;
+        auto with_lanes = [&](auto lanes) {
+            if (group <= 1) return f(zero, lanes, std::integral_constant<int, 1>{});
+            if (group <= 2) return f(zero, lanes, std::integral_constant<int, 2>{});
+            if (group <= 4) return f(zero, lanes, std::integral_constant<int, 4>{});
+            return f(zero, lanes, std::integral_constant<int, 8>{});
+        };
+        if (q.D <= 32) return with_lanes(std::integral_constant<int, L32>{});
+        if (q.D <= 64) return with_lanes(std::integral_constant<int, 2 * L32>{});
+        return with_lanes(std::integral_constant<int, 4 * L32>{});
+    };
+    return q.dtype == D2C_BF16 ? with_type(bf16_t{}) : with_type(float{});
+}
+
+// Memories of up to so many steps (of 32 to 256 slots) are read by a workgroup to each unit
+constexpr int kOneSteps = 4;
+struct MemPlan { int rows, step, row_groups, units, places, least; bool one; size_t part_bytes, ml_bytes, covered_bytes, begins_bytes, scores_bytes, bytes; long slots_padded; };
+MemPlan mem_plan(const d2c_memory_desc &q, const d2c_memory_query_desc &x, bool track)
+{
+    MemPlan p{};
+    const int group = x.query_heads / q.heads;
+    for_rows(q, group, [&](auto zero, auto lanes, auto r) {
+        p.rows = decltype(r)::value;
+        p.step = TokenShape<decltype(zero), decltype(lanes)::value, decltype(r)::value>::STEP;
+        return 0;
+    });
+    const long slots = (long)q.per_stream * q.page;
+    p.row_groups = (group + p.rows - 1) / p.rows;
+    p.units = q.streams * q.heads * p.row_groups;
+    p.one = slots <= (long)kOneSteps * p.step && !(track && p.row_groups > 1);
+    p.places = 2 * std::max(d2c_num_cus(), 1);
+    p.least = 2;
+    p.slots_padded = (slots + 63) / 64 * 64;
+    if (track) p.scores_bytes = d2c_align_up((size_t)q.streams * x.query_heads * p.slots_padded * 4);
+    if (!p.one) {
+        const size_t lines = ((size_t)p.units + p.places) * p.rows;
+        p.part_bytes = d2c_align_up(lines * part_width(q.D) * 4);
+        p.ml_bytes = d2c_align_up(lines * 8);
+        p.covered_bytes = d2c_align_up((size_t)p.units * 8);
+        p.begins_bytes = d2c_align_up((size_t)p.places * 16);
+    }
+    p.bytes = p.part_bytes + p.ml_bytes + p.covered_bytes + p.begins_bytes + p.scores_bytes;
+    return p;
+}
+
+struct EvictPlan { int pairs; long slots_padded; size_t ranks_bytes, list_bytes, bytes; };
+EvictPlan evict_plan(const d2c_memory_desc &q, int keep)
+{
+    EvictPlan p{};
+    const long slots = (long)q.per_stream * q.page;
+    const size_t units = (size_t)q.streams * q.heads;
+    if (slots <= keep || units == 0) return p;
+    p.pairs = (int)std::min((long)keep, slots - keep);
+    p.slots_padded = (slots + 63) / 64 * 64;
+    p.ranks_bytes = d2c_align_up(units * p.slots_padded * 4);
+    p.list_bytes = d2c_align_up(units * p.pairs * 4);
+    p.bytes = p.ranks_bytes + 2 * p.list_bytes + d2c_align_up(units * 4);
+    return p;
+}
+
+}  // namespace
+
+extern "C" int d2c_memory_append(const d2c_memory_desc *q, void *key, void *value, const int32_t *table, int32_t *lengths, int32_t *seen,
+                                 float *usage, int32_t *positions, const void *new_key, const void *new_value, const int64_t new_key_stride[2],
+                                 const int64_t new_value_stride[2], const int32_t *starts, int64_t tokens, void *stream)
+{
+    if (int rc = check(q)) return rc;
+    if (tokens < 0 || tokens * q->heads >= (1L << 31) || (!starts && tokens != q->streams)) { d2c_set_error("memory_append: %ld tokens for %d streams", (long)tokens, q->streams); return D2C_ERR_SHAPE; }
+    if (q->streams == 0) return D2C_OK;
+    if (!lengths || !seen || (q->per_stream > 0 && !table) || (q->pages > 0 && (!key || !value || !usage || !positions)) || (tokens > 0 && (!new_key || !new_value))) {
+        d2c_set_error("null tensor pointer");
+        return D2C_ERR_SHAPE;
+    }
+    AppendArgs a{};
+    a.nk = new_key; a.nv = new_value; a.key = key; a.value = value; a.table = table; a.starts = starts; a.lengths = lengths; a.seen = seen;
+    a.positions = positions; a.usage = usage;
+    for (int i = 0; i < 2; i++) { a.nks[i] = new_key_stride[i]; a.nvs[i] = new_value_stride[i]; }
+    for (int i = 0; i < 3; i++) { a.ks[i] = q->key_stride[i]; a.vs[i] = q->value_stride[i]; }
+    a.table_stride = q->table_stride; a.tokens = tokens; a.page = make_fastdiv(q->page);
+    a.N = q->streams; a.heads = q->heads; a.D = q->D; a.pages = q->pages; a.slots = q->per_stream * q->page;
+    hipStream_t st = (hipStream_t)stream;
+    const bool half = q->dtype == D2C_BF16;
+    if (!starts) {
+        if (half) hipLaunchKernelGGL(mem_append_one_kernel<bf16_t>, dim3(a.N), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL(mem_append_one_kernel<float>, dim3(a.N), dim3(256), 0, st, a);
+        return d2c_check_launch("mem_append_one_kernel");
+    }
+    if (tokens > 0) {
+        const long per = 256 / (2 * ((a.D * (half ? 2 : 4) + 15) / 16));
+        const unsigned blocks = (unsigned)std::min((tokens * a.heads + per - 1) / per, 1L << 20);
+        if (half) hipLaunchKernelGGL(mem_append_kernel<bf16_t>, dim3(blocks), dim3(256), 0, st, a, make_fastdiv(a.heads));
+        else hipLaunchKernelGGL(mem_append_kernel<float>, dim3(blocks), dim3(256), 0, st, a, make_fastdiv(a.heads));
+        if (int rc = d2c_check_launch("mem_append_kernel")) return rc;
+    }
+    hipLaunchKernelGGL(mem_count_kernel, dim3((a.N + 255) / 256), dim3(256), 0, st, a);
+    return d2c_check_launch("mem_count_kernel");
+}
+
+extern "C" size_t d2c_memory_attention_workspace_bytes(const d2c_memory_desc *q, const d2c_memory_query_desc *x, int32_t track)
+{
+    if (check(q, x) != D2C_OK || q->streams == 0) return 0;
+    return mem_plan(*q, *x, track != 0).bytes;
+}
+
+extern "C" int d2c_memory_attention(const d2c_memory_desc *q, const d2c_memory_query_desc *x, const void *query, const void *key,
+                                    const void *value, const int32_t *table, const int32_t *lengths, float *usage, void *out, void *ws,
+                                    size_t ws_bytes, void *stream)
+{
+    if (int rc = check(q, x)) return rc;
+    if (q->streams == 0) return D2C_OK;
+    const long slots = (long)q->per_stream * q->page;
+    if (!query || !out || !lengths || (slots > 0 && !table) || (q->pages > 0 && (!key || !value))) { d2c_set_error("null tensor pointer"); return D2C_ERR_SHAPE; }
+    const MemPlan p = mem_plan(*q, *x, usage != nullptr);
+    if (int rc = need(ws, ws_bytes, p.bytes)) return rc;
+    MemArgs a{};
+    a.q = query; a.key = const_cast<void *>(key); a.value = const_cast<void *>(value); a.out = out; a.table = table; a.lengths = lengths; a.usage = usage;
+    char *w = (char *)ws;
+    a.part = (float *)w; a.part_ml = (float *)(w + p.part_bytes); a.covered = (int32_t *)(w + p.part_bytes + p.ml_bytes);
+    a.begins = (int32_t *)(w + p.part_bytes + p.ml_bytes + p.covered_bytes);
+    a.scores = (float *)(w + p.part_bytes + p.ml_bytes + p.covered_bytes + p.begins_bytes);
+    for (int i = 0; i < 2; i++) a.qs[i] = x->query_stride[i];
+    for (int i = 0; i < 3; i++) { a.ks[i] = q->key_stride[i]; a.vs[i] = q->value_stride[i]; }
+    a.table_stride = q->table_stride; a.slots_padded = p.slots_padded; a.page = make_fastdiv(q->page);
+    a.N = q->streams; a.heads = q->heads; a.group = x->query_heads / q->heads; a.D = q->D; a.pages = q->pages;
+    a.slots = q->pages > 0 ? (int)slots : 0;      // (without pages no slot is there)
+    a.row_groups = p.row_groups; a.units = p.units; a.places = p.places; a.least = p.least;
+    a.scale2 = x->scale * 1.44269504088896340736f;
+    hipStream_t st = (hipStream_t)stream;
+    return for_rows(*q, a.group, [&](auto zero, auto lanes, auto r) {
+        using T = decltype(zero);
+        constexpr int LANES = decltype(lanes)::value, R = decltype(r)::value;
+        const bool whole = q->D * sizeof(T) % 16 == 0;
+        const dim3 grid(p.one ? p.units : p.places);
+        auto launch = [&](auto whole, auto one) {
+            hipLaunchKernelGGL((mem_attn_kernel<T, LANES, R, decltype(whole)::value, decltype(one)::value>), grid, dim3(256), 0, st, a);
+            return d2c_check_launch("mem_attn_kernel");
+        };
+        int rc;
+        if (whole) rc = p.one ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
+        else rc = p.one ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
+        if (rc || p.one) return rc;
+        constexpr int JOIN = LANES * 16 / (int)sizeof(T) / 4;      // lanes of four columns
+        const int rows = q->streams * x->query_heads;
+        hipLaunchKernelGGL((mem_join_kernel<T, JOIN, R>), dim3(rows + (usage ? p.places : 0)), dim3(256), 0, st, a, rows, p.step);
+        return d2c_check_launch("mem_join_kernel");
+    });
+}
+
+extern "C" size_t d2c_memory_evict_workspace_bytes(const d2c_memory_desc *q, int32_t keep)
+{
+    if (check(q) != D2C_OK || keep <= 0) return 0;
+    return evict_plan(*q, keep).bytes;
+}
+
+extern "C" int d2c_memory_evict(const d2c_memory_desc *q, void *key, void *value, const int32_t *table, int32_t *lengths, const int32_t *seen,
+                                float *usage, int32_t *positions, int32_t keep, int32_t recent, void *ws, size_t ws_bytes, void *stream)
+{
+    if (int rc = check(q)) return rc;
+    if (keep <= 0 || recent < 0 || recent > keep) { d2c_set_error("memory_evict: keep %d must be positive, recent %d in 0 .. keep", keep, recent); return D2C_ERR_SHAPE; }
+    const EvictPlan p = evict_plan(*q, keep);
+    if (p.pairs == 0) return D2C_OK;
+    if (!table || !lengths || !seen || (q->pages > 0 && (!key || !value || !usage || !positions))) { d2c_set_error("null tensor pointer"); return D2C_ERR_SHAPE; }
+    if (int rc = need(ws, ws_bytes, p.bytes)) return rc;
+    EvictArgs a{};
+    a.key = key; a.value = value; a.table = table; a.seen = seen; a.lengths = lengths; a.positions = positions; a.usage = usage;
+    a.ranks = (uint32_t *)ws; a.holes = (int32_t *)((char *)ws + p.ranks_bytes); a.fillers = (int32_t *)((char *)ws + p.ranks_bytes + p.list_bytes);
+    a.counts = (int32_t *)((char *)ws + p.ranks_bytes + 2 * p.list_bytes);
+    for (int i = 0; i < 3; i++) { a.ks[i] = q->key_stride[i]; a.vs[i] = q->value_stride[i]; }
+    a.table_stride = q->table_stride; a.slots_padded = p.slots_padded; a.page = make_fastdiv(q->page);
+    a.N = q->streams; a.heads = q->heads; a.D = q->D; a.pages = q->pages; a.slots = q->per_stream * q->page; a.keep = keep; a.recent = recent; a.pairs = p.pairs;
+    hipStream_t st = (hipStream_t)stream;
+    const int units = a.N * a.heads, vec = q->dtype == D2C_BF16 ? 8 : 4;
+    hipLaunchKernelGGL(mem_rank_kernel, dim3(units), dim3(kEvictThreads), 0, st, a);
+    if (int rc = d2c_check_launch("mem_rank_kernel")) return rc;
+    const int per = 256 / (2 * ((a.D + vec - 1) / vec));
+    const int blocks = (int)std::max(std::min((a.pairs + per * 4L - 1) / (per * 4L), (1L << 22) / units), 1L);
+    if (q->dtype == D2C_BF16) hipLaunchKernelGGL(mem_move_kernel<bf16_t>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks);
+    else hipLaunchKernelGGL(mem_move_kernel<float>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks);
+    return d2c_check_launch("mem_move_kernel");
+}

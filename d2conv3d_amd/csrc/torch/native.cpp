@@ -867,6 +867,97 @@ py::object cross_attention(const Tensor &query, const Tensor &key, const Tensor 
     return py::cast(recorded);
 }
 
+// ---------------------------------------------------------------- a memory in pages
+// The description of a memory whose tensors the kernels can take as they are; false: one that the Python code has something to say about
+bool memory_desc(d2c_memory_desc &q, const Tensor &key, const Tensor &value, const Tensor &table, const Tensor &lengths, const Tensor &usage, const Tensor &positions)
+{
+    for (const Tensor *t : {&key, &value})
+        if (!plain_strided(*t) || t->dim() != 4 || t->numel() == 0 || t->device() != key.device() || !inner_contiguous(*t) || t->scalar_type() != key.scalar_type()) return false;
+    const int dt = dtype_code(key);
+    if ((dt != D2C_F32 && dt != D2C_BF16) || key.sizes() != value.sizes() || key.size(3) > 128) return false;
+    for (int i = 0; i < 3; i++)
+        if (key.size(i) >= (1ll << 31)) return false;
+    if (!plain_strided(table) || table.dim() != 2 || table.numel() == 0 || table.device() != key.device() || table.scalar_type() != at::kInt || !inner_contiguous(table) ||
+        table.size(0) >= (1ll << 31) || table.size(1) >= (1ll << 31))
+        return false;
+    if (!plain(lengths) || lengths.device() != key.device() || lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != table.size(0)) return false;
+    for (const Tensor *t : {&usage, &positions})
+        if (!plain(*t) || t->device() != key.device() || t->dim() != 3 || t->size(0) != key.size(0) || t->size(1) != key.size(1) || t->size(2) != key.size(2)) return false;
+    if (usage.scalar_type() != at::kFloat || positions.scalar_type() != at::kInt) return false;
+    std::memset(&q, 0, sizeof q);
+    q.streams = (int)table.size(0); q.heads = (int)key.size(1); q.D = (int)key.size(3); q.dtype = dt;
+    q.pages = (int)key.size(0); q.page = (int)key.size(2); q.per_stream = (int)table.size(1);
+    q.table_stride = table.stride(0);
+    for (int i = 0; i < 3; i++) { q.key_stride[i] = key.stride(i); q.value_stride[i] = value.stride(i); }
+    return true;
+}
+bool is_counts(const Tensor &t, const Tensor &like) { return plain(t) && t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == like.size(0); }
+// (a change that autograd is to notice where it has saved the tensor)
+void changed(std::initializer_list<const Tensor *> tensors)
+{
+    for (const Tensor *t : tensors) t->unsafeGetTensorImpl()->bump_version();
+}
+
+py::object memory_append(const Tensor &key, const Tensor &value, const Tensor &table, const Tensor &lengths, const Tensor &seen, const Tensor &usage,
+                         const Tensor &positions, const Tensor &new_key, const Tensor &new_value, const opt_tensor &starts)
+{
+    d2c_memory_desc q;
+    const Tensor first = starts.value_or(Tensor());
+    if (!memory_desc(q, key, value, table, lengths, usage, positions) || !is_counts(seen, lengths) || wants_grad(new_key, new_value)) return py::none();
+    for (const Tensor *t : {&new_key, &new_value})
+        if (!plain_strided(*t) || t->dim() != 3 || t->numel() == 0 || t->device() != key.device() || !inner_contiguous(*t) || t->scalar_type() != key.scalar_type() ||
+            t->size(0) != new_key.size(0) || t->size(1) != q.heads || t->size(2) != q.D)
+            return py::none();
+    if (first.defined()) {
+        if (!plain(first) || first.device() != key.device() || first.scalar_type() != at::kInt || first.dim() != 1 || first.size(0) != (int64_t)q.streams + 1) return py::none();
+    } else if (new_key.size(0) != q.streams) return py::none();
+    c10::DeviceGuard guard(key.device());
+    const int64_t ks[2] = {new_key.stride(0), new_key.stride(1)}, vs[2] = {new_value.stride(0), new_value.stride(1)};
+    changed({&key, &value, &lengths, &seen, &usage, &positions});
+    check(d2c_memory_append(&q, ptr(key), ptr(value), (const int32_t *)ptr(table), (int32_t *)ptr(lengths), (int32_t *)ptr(seen), (float *)ptr(usage),
+                            (int32_t *)ptr(positions), ptr(new_key), ptr(new_value), ks, vs, (const int32_t *)ptr(first), new_key.size(0), stream_of(key)),
+          "memory_append");
+    return py::bool_(true);
+}
+
+py::object memory_attention(const Tensor &query, const Tensor &key, const Tensor &value, const Tensor &table, const Tensor &lengths, const Tensor &usage,
+                            const Tensor &positions, const std::optional<double> &scale, bool track)
+{
+    d2c_memory_desc q;
+    if (!memory_desc(q, key, value, table, lengths, usage, positions) || wants_grad(query, key, value)) return py::none();
+    if (!plain_strided(query) || query.dim() != 3 || query.numel() == 0 || query.device() != key.device() || !inner_contiguous(query) || query.scalar_type() != key.scalar_type() ||
+        query.size(0) != q.streams || query.size(2) != q.D || query.size(1) % q.heads != 0 || query.size(1) / q.heads > 256)
+        return py::none();
+    const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.D);
+    if (!(s > 0.0) || !((float)s > 0.f) || !((float)s < INFINITY)) return py::none();
+    const d2c_memory_query_desc x{(int)query.size(1), (float)s, {query.stride(0), query.stride(1)}};
+    c10::DeviceGuard guard(key.device());
+    const Tensor out = at::empty(query.sizes(), query.options().requires_grad(false));
+    const size_t nb = d2c_memory_attention_workspace_bytes(&q, &x, track);
+    const Tensor ws = small_workspace(nb, key);
+    if (track) changed({&usage});
+    check(d2c_memory_attention(&q, &x, ptr(query), ptr(key), ptr(value), (const int32_t *)ptr(table), (const int32_t *)ptr(lengths), track ? (float *)ptr(usage) : nullptr,
+                               ptr(out), ptr(ws), nb, stream_of(key)),
+          "memory_attention");
+    return py::cast(out);
+}
+
+py::object memory_evict(const Tensor &key, const Tensor &value, const Tensor &table, const Tensor &lengths, const Tensor &seen, const Tensor &usage, const Tensor &positions,
+                        int64_t keep, int64_t recent)
+{
+    d2c_memory_desc q;
+    if (!memory_desc(q, key, value, table, lengths, usage, positions) || !is_counts(seen, lengths)) return py::none();
+    if (keep <= 0 || keep >= (1ll << 31) || recent < 0 || recent > keep) return py::none();
+    c10::DeviceGuard guard(key.device());
+    const size_t nb = d2c_memory_evict_workspace_bytes(&q, (int)keep);
+    const Tensor ws = small_workspace(nb, key);
+    changed({&key, &value, &lengths, &usage, &positions});
+    check(d2c_memory_evict(&q, ptr(key), ptr(value), (const int32_t *)ptr(table), (int32_t *)ptr(lengths), (const int32_t *)ptr(seen), (float *)ptr(usage),
+                           (int32_t *)ptr(positions), (int)keep, (int)recent, ptr(ws), nb, stream_of(key)),
+          "memory_evict");
+    return py::bool_(true);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m)
@@ -883,4 +974,7 @@ PYBIND11_MODULE(_native, m)
     m.def("layer_norm", &layer_norm);
     m.def("rotary3d", &rotary3d);
     m.def("cross_attention", &cross_attention);
+    m.def("memory_append", &memory_append);
+    m.def("memory_attention", &memory_attention);
+    m.def("memory_evict", &memory_evict);
 }

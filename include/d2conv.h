@@ -547,6 +547,47 @@ int d2c_attention_backward(const d2c_attention_desc *desc, const void *grad_out,
                            const void *out_low, const float *lse, void *grad_query, void *grad_key, void *grad_value, void *workspace,
                            size_t workspace_bytes, void *stream);
 
+/* A memory of keys and values in pages, for streams that are read token by token.  key and value [pages][heads][page][D] with strides
+ * (page, head, slot; channels adjacent), usage (float32) and positions (int32) [pages][heads][page] contiguous.  Slot s of stream n
+ * lies at slot s % page of page table[n][s / page] (table: int32 [streams][per_stream], rows table_stride elements apart); slots of
+ * a page whose number is not in 0 .. pages - 1 are not there.  lengths [streams]: slots that a stream has (taken into 0 .. per_stream *
+ * page); seen [streams]: tokens that it has had.  Which slot holds which token may differ from head to head.
+ *
+ * d2c_memory_append: token i of stream n's new ones goes to slot lengths[n] + i with usage 0 and position seen[n] + i, and lengths[n] and
+ * seen[n] grow by their number.  new_key, new_value [tokens][heads][D] with strides (token, head); stream n's are the tokens starts[n]
+ * .. starts[n + 1] - 1 (int32 [streams + 1], rising; taken into 0 .. tokens), or, starts NULL, token n (tokens == streams).  What has no slot
+ * is dropped, lengths stay within the slots.  Streams of one memory share no page that they write to.
+ *
+ * d2c_memory_attention: one token of each stream, query [streams][query_heads][D] with strides (stream, head), query_heads a multiple of
+ * heads, 256 to a head at most, D up to 128; out [streams][query_heads][D] contiguous:
+ *     out[n,h] = sum_s softmax_s(scale * <query[n,h], key[n,s,h']>) value[n,s,h']
+ * over the slots that are there (none: 0).  usage not NULL: softmax_s of the query heads that share a key head is added to the slot's usage.
+ * Results do not depend on the order in which workgroups run.
+ *
+ * d2c_memory_evict: of every stream with more than `keep` (> 0) slots, and for each head alone, these stay: slots whose position is at least
+ * seen[n] - recent, and of the others those of the largest usage (ties: the lower slot; NaN above all numbers), `keep` in all.  What stays
+ * behind slot keep - 1 moves into the places of what goes before it, the i-th into the i-th, with its usage and position; nothing else
+ * moves.  lengths[n] becomes keep.  (Slots that are not there are the first to go.) */
+typedef struct d2c_memory_desc {
+    int32_t streams, heads, D, dtype, pages, page, per_stream;
+    int64_t table_stride, key_stride[3], value_stride[3];
+} d2c_memory_desc;
+typedef struct d2c_memory_query_desc {
+    int32_t query_heads;
+    float scale;
+    int64_t query_stride[2];
+} d2c_memory_query_desc;
+int d2c_memory_append(const d2c_memory_desc *desc, void *key, void *value, const int32_t *table, int32_t *lengths, int32_t *seen,
+                      float *usage, int32_t *positions, const void *new_key, const void *new_value, const int64_t new_key_stride[2],
+                      const int64_t new_value_stride[2], const int32_t *starts, int64_t tokens, void *stream);
+size_t d2c_memory_attention_workspace_bytes(const d2c_memory_desc *desc, const d2c_memory_query_desc *query_desc, int32_t track);
+int d2c_memory_attention(const d2c_memory_desc *desc, const d2c_memory_query_desc *query_desc, const void *query, const void *key,
+                         const void *value, const int32_t *table, const int32_t *lengths, float *usage, void *out, void *workspace,
+                         size_t workspace_bytes, void *stream);
+size_t d2c_memory_evict_workspace_bytes(const d2c_memory_desc *desc, int32_t keep);
+int d2c_memory_evict(const d2c_memory_desc *desc, void *key, void *value, const int32_t *table, int32_t *lengths, const int32_t *seen,
+                     float *usage, int32_t *positions, int32_t keep, int32_t recent, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Test hook for the matrix-core backward pass: 1 (default) builds grad_input from
  * per-voxel sample lists, every element written once; 0 scatters with fp32 atomics
  * like the reference (dconv3d_gpu.cu:637).  A value n >= 2 is mode 1 with lists
