@@ -15,7 +15,7 @@ from .modules import (
 from .grid import offsets_from_size_map
 from .util import add_deformable_conv
 from .depthwise_conv import DepthwiseConv3d, depthwise_separable_conv3d, install_as_fast_depthwise_conv3d
-from .attention import CrossAttention3d, LayerNorm, cross_attention, layer_norm, rotary3d
+from .attention import CrossAttention3d, LayerNorm, cross_attention, layer_norm, packed_attention, rotary3d
 from .memory import PagedMemory, memory_append, memory_attention, memory_evict
 
 __all__ = [
@@ -28,7 +28,7 @@ __all__ = [
     "offsets_from_size_map", "add_deformable_conv", "install_as_dconv_native",
     "DepthwiseConv3d", "depthwise_separable_conv3d", "install_as_fast_depthwise_conv3d",
     "CrossAttention3d", "LayerNorm", "cross_attention", "layer_norm", "rotary3d",
-    "PagedMemory", "memory_append", "memory_attention", "memory_evict",
+    "packed_attention", "PagedMemory", "memory_append", "memory_attention", "memory_evict",
 ]
 
 

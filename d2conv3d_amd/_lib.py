@@ -40,6 +40,8 @@ EXPORTS = (
     "d2c_layer_norm_forward", "d2c_layer_norm_backward_workspace_bytes", "d2c_layer_norm_backward", "d2c_rotary3d",
     "d2c_attention_forward_workspace_bytes", "d2c_attention_forward",
     "d2c_attention_backward_workspace_bytes", "d2c_attention_backward",
+    "d2c_packed_attention_forward_workspace_bytes", "d2c_packed_attention_forward",
+    "d2c_packed_attention_backward_workspace_bytes", "d2c_packed_attention_backward",
     "d2c_memory_append", "d2c_memory_attention_workspace_bytes", "d2c_memory_attention",
     "d2c_memory_evict_workspace_bytes", "d2c_memory_evict",
 )
@@ -105,6 +107,11 @@ class Rotary3dDesc(ctypes.Structure):
 class AttentionDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("N", "Lq", "Lk", "Hq", "Hkv", "D", "dtype")] + [("scale", ctypes.c_float)] + [
         (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")] + [("part_limit", ctypes.c_int64)]
+
+
+class PackedAttentionDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("sequences", "Hq", "Hkv", "D", "dtype", "causal", "frame")] + [("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int64) for n in ("queries", "keys")] + [(n, ctypes.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride")]
 
 
 class MemoryDesc(ctypes.Structure):
@@ -227,6 +234,12 @@ def load():
         f.argtypes, f.restype = [pat], sz
     lib.d2c_attention_forward.argtypes, lib.d2c_attention_forward.restype = [pat] + [vp] * 9 + [sz, vp], ctypes.c_int
     lib.d2c_attention_backward.argtypes, lib.d2c_attention_backward.restype = [pat] + [vp] * 13 + [sz, vp], ctypes.c_int
+    ppa = ctypes.POINTER(PackedAttentionDesc)
+    for d in ("forward", "backward"):
+        f = getattr(lib, f"d2c_packed_attention_{d}_workspace_bytes")
+        f.argtypes, f.restype = [ppa], sz
+    lib.d2c_packed_attention_forward.argtypes, lib.d2c_packed_attention_forward.restype = [ppa] + [vp] * 9 + [sz, vp], ctypes.c_int
+    lib.d2c_packed_attention_backward.argtypes, lib.d2c_packed_attention_backward.restype = [ppa] + [vp] * 13 + [sz, vp], ctypes.c_int
     pme, pmq, i64 = ctypes.POINTER(MemoryDesc), ctypes.POINTER(MemoryQueryDesc), ctypes.c_int64
     lib.d2c_memory_append.argtypes = [pme] + [vp] * 9 + [ctypes.POINTER(i64)] * 2 + [vp, i64, vp]
     lib.d2c_memory_append.restype = ctypes.c_int

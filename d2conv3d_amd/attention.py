@@ -5,6 +5,7 @@ the reference, whose decoder joins the features of different frames by convoluti
     layer_norm        torch.nn.functional.layer_norm over the last dimension
     rotary3d          rotary position embedding with three axes
     cross_attention   softmax(scale q k^T) v over the keys that are there, query heads sharing key heads
+    packed_attention  the same inside each of several sequences that lie behind each other, up to a token's own place or frame
     CrossAttention3d  the block: a clip's feature map reads the feature map of remembered frames
 
 float32 and bfloat16 run as they are (sums and statistics in float32); float16 is computed in float32 and returned as
@@ -285,6 +286,103 @@ def cross_attention(query, key, value, key_lengths=None, key_mask=None, scale=No
         return cross_attention(query.float(), key.float(), value.float(), key_lengths, key_mask, scale).half()
     _check(query.dtype in _TYPES, f"cross_attention: unsupported dtype {query.dtype}")
     return _CrossAttentionFunction.apply(query, key, value, key_lengths, key_mask, scale)
+
+
+# ---------------------------------------------------------------- attention inside packed sequences
+def _long2(*v):
+    return (ctypes.c_int64 * 2)(*v)
+
+
+def _heads_contiguous(t):
+    return t if t.stride(2) == 1 or t.size(2) == 1 else t.contiguous()
+
+
+class _PackedAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, value, starts, key_starts, causal, frame, scale):
+        lib, dev = _lib.load(), query.device
+        q, k, v = (_heads_contiguous(t) for t in (query, key, value))
+        T, Hq, D = q.shape
+        Tk, Hkv = k.shape[:2]
+        desc = _lib.PackedAttentionDesc(starts.numel() - 1, Hq, Hkv, D, _DT[q.dtype], int(causal), frame, scale, T, Tk, _long2(*q.stride()[:2]),
+                                        _long2(*k.stride()[:2]), _long2(*v.stride()[:2]))
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+        grad = any(ctx.needs_input_grad)
+        lse = torch.empty((Hkv, T * (Hq // Hkv)), dtype=torch.float32, device=dev) if grad else None
+        low = torch.empty_like(out) if grad and out.dtype == torch.bfloat16 else None
+        with torch.cuda.device(dev):
+            nb = lib.d2c_packed_attention_forward_workspace_bytes(ctypes.byref(desc))
+            ws = _workspace(nb, dev)
+            rc = lib.d2c_packed_attention_forward(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(starts), _ptr(key_starts), _ptr(out),
+                                                  _ptr(low), _ptr(lse), _ptr(ws), nb, _stream(dev))
+        _lib.check(rc, "packed_attention forward")
+        ctx.save_for_backward(q, k, v, starts, key_starts, out, low, lse)
+        ctx.desc = desc
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        lib = _lib.load()
+        q, k, v, starts, key_starts, out, low, lse = ctx.saved_tensors
+        desc, dev, need = ctx.desc, q.device, ctx.needs_input_grad
+        q, k, v = (_heads_contiguous(t) for t in (q, k, v))
+        desc.q_stride, desc.k_stride, desc.v_stride = (_long2(*t.stride()[:2]) for t in (q, k, v))
+        g = grad_out.to(q.dtype).contiguous()
+        gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((q, k, v), need))
+        with torch.cuda.device(dev):
+            nb = lib.d2c_packed_attention_backward_workspace_bytes(ctypes.byref(desc))
+            ws = _workspace(nb, dev)
+            rc = lib.d2c_packed_attention_backward(ctypes.byref(desc), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(starts), _ptr(key_starts),
+                                                   _ptr(out), _ptr(low), _ptr(lse), _ptr(gq), _ptr(gk), _ptr(gv), _ptr(ws), nb, _stream(dev))
+        _lib.check(rc, "packed_attention backward")
+        return (gq, gk, gv) + (None,) * 5
+
+
+def packed_attention(query, key, value, starts, key_starts=None, causal=True, frame=1, scale=None):
+    """Attention inside each of several sequences that lie behind each other: `query` [tokens, Hq, D], `key` and `value` [tokens, Hkv, D]
+    with Hq a multiple of Hkv (query heads h * Hq / Hkv .. share key head h) and heads of up to 128 channels; `scale` 1 / sqrt(D)
+    by default.
+
+    `starts` [sequences + 1] (whole numbers, rising): sequence s has tokens starts[s] .. starts[s + 1] - 1, none, one or many; `key_starts`
+    the same for its keys where these are others (default: starts), whose last tokens then are the queries.  `causal`: query i of Lq
+    is token p = Lk - Lq + i and reads the keys up to its own, or, with `frame` tokens to a frame, up to the end of its frame; what it
+    does not read has no influence on it whatever it holds.  Otherwise all keys of its sequence.  A query without keys, or of no sequence, is 0 and has gradients of
+    0.  Any strides with the channels adjacent are read in place.  Sums in an order that sizes, strides, starts and GPU determine.
+    (Starts that do not rise have results of no meaning, and touch nothing else.)"""
+    out = _try_native("packed_attention", query, key, value, starts, key_starts, causal, frame, scale)
+    if out is not None:
+        return out
+    _check_tensors("packed_attention", query=query, key=key, value=value, starts=starts, key_starts=key_starts)
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        _check(t.dim() == 3, f"packed_attention: {name} must be [tokens, H, D], got {t.dim()} dimensions")
+    T, Hq, D = query.shape
+    _check(key.shape == value.shape, f"packed_attention: key {tuple(key.shape)} and value {tuple(value.shape)} differ in shape")
+    Tk, Hkv = key.shape[:2]
+    _check(key.size(2) == D, f"packed_attention: key {tuple(key.shape)} does not fit query {tuple(query.shape)}")
+    _check(D > 0 and Hq > 0 and Hkv > 0 and Hq % Hkv == 0,
+           f"packed_attention: {Hq} query heads must be a positive multiple of {Hkv} key heads, of {D} > 0 channels")
+    _check(D <= 128, f"packed_attention: heads of up to 128 channels, got {D}")
+    _check(query.dtype == key.dtype == value.dtype, "packed_attention: query, key and value must have one dtype")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    _check(0.0 < scale < math.inf, f"packed_attention: scale must be positive and finite, got {scale}")
+    frame = int(frame)
+    _check(0 < frame <= 1 << 30, f"packed_attention: a frame has 1 to 2^30 tokens, got {frame}")
+
+    def whole(name, t, tokens):
+        _check(t.dim() == 1 and t.numel() > 0 and not t.is_floating_point() and not t.is_complex() and t.dtype != torch.bool,
+               f"packed_attention: {name} must be whole numbers [sequences + 1]")
+        return (t.clamp(0, tokens) if t.dtype == torch.int64 else t).to(torch.int32).contiguous()
+    starts = whole("starts", starts, T)
+    if key_starts is not None:
+        key_starts = whole("key_starts", key_starts, Tk)
+        _check(key_starts.numel() == starts.numel(), f"packed_attention: {starts.numel()} starts and {key_starts.numel()} key_starts")
+    else:
+        _check(T == Tk, f"packed_attention: without key_starts as many keys as queries, got {Tk} and {T}")
+    if query.dtype == torch.float16:
+        return packed_attention(query.float(), key.float(), value.float(), starts, key_starts, causal, frame, scale).half()
+    _check(query.dtype in _TYPES, f"packed_attention: unsupported dtype {query.dtype}")
+    return _PackedAttentionFunction.apply(query, key, value, starts, key_starts, bool(causal), frame, scale)
 
 
 class LayerNorm(nn.LayerNorm):

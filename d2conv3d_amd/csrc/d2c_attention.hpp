@@ -287,12 +287,12 @@ inline bool fast_kernels(const d2c_attention_desc &q, bool gradients)
     const int64_t g[3] = {0, (int64_t)q.Hq * q.D, q.D};
     return q.D % 8 == 0 && keys_near(q.k_stride[1]) && keys_near(q.v_stride[1]) && rows_near(q.q_stride) && rows_near(g);
 }
-template <typename T, bool GRADIENTS, typename F> auto for_width(const d2c_attention_desc &q, F f)      // f(Width, fast_kernels)
+template <typename F> auto pick_width(int D, bool fast, F f)      // f(Width, fast)
 {
-    const int pieces = (q.D + 7) / 8;
+    const int pieces = (D + 7) / 8;
     auto pick = [&](auto width) {      // (of the four widths with as many channels)
         constexpr int DP = decltype(width)::DP, NP = DP / 8;
-        if (!fast_kernels(q, GRADIENTS)) return f(Width<DP, NP>{}, std::false_type{});
+        if (!fast) return f(Width<DP, NP>{}, std::false_type{});
         if (pieces == NP - 3) return f(Width<DP, NP - 3>{}, std::true_type{});
         if (pieces == NP - 2) return f(Width<DP, NP - 2>{}, std::true_type{});
         if (pieces == NP - 1) return f(Width<DP, NP - 1>{}, std::true_type{});
@@ -303,6 +303,7 @@ template <typename T, bool GRADIENTS, typename F> auto for_width(const d2c_atten
     if (pieces <= 12) return pick(Width<96, 12>{});
     return pick(Width<128, 16>{});
 }
+template <typename T, bool GRADIENTS, typename F> auto for_width(const d2c_attention_desc &q, F f) { return pick_width(q.D, fast_kernels(q, GRADIENTS), f); }      // f(Width, fast_kernels)
 
 // Floats to a row of partial sums: whole pieces of 16 bytes (what is behind a row's end is read and dropped)
 inline __host__ __device__ int part_width(int D) { return (D + 3) & ~3; }

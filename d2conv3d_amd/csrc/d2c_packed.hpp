@@ -1,0 +1,230 @@
+// Attention inside sequences that lie behind each other: what the forward and the backward kernels share.  Formulas and operand
+// orders: d2c_attention.hpp.
+//
+// Where a sequence begins is known on the GPU only.  Tiles never span sequences; region i (0: what lies before the first sequence, 1 .. S: the sequences, S + 1: what
+// lies behind the last) begins with tile  B_i = floor(first row / rows of a tile) + i  of one line: it has at most B_{i+1} - B_i tiles, so that a workgroup
+// finds its own by the starts alone, and the line is longer than the tiles that there are by at most one tile to a region.
+#pragma once
+#include "d2c_attention.hpp"
+
+namespace d2c_packed {
+using namespace d2c_attn;
+
+struct PackedArgs {
+    const void *q, *k, *v, *g, *o, *o_low;
+    const int32_t *starts, *key_starts;
+    void *out, *out_low, *gq, *gk, *gv;
+    float *lse, *delta;                     // [Hkv][T * group]
+    float *part, *part_ml;                  // [splits][tiles][Hkv][128][part_width(D)] (keys' kernel: twice), and (forward) [..][2]
+    long qs[2], ks[2], vs[2], gs[2];        // strides of token, head
+    int T, Tk, S, Hq, Hkv, group, D, tiles, splits, causal;
+    FastDiv by_group, frame;
+    float scale, scale2;
+};
+
+constexpr int kRows = 128;      // of a tile: rows, or keys
+
+D2C_DEV int bound_of(const int32_t *starts, int S, int T, int i) { return i == 0 ? 0 : i > S + 1 ? T : min(max(starts[i - 1], 0), T); }
+// First token of region i, and how many tokens it has
+D2C_DEV void region_of(const int32_t *starts, int S, int T, int i, int &first, int &count)
+{
+    first = bound_of(starts, S, T, i);
+    count = max((i > S ? T : bound_of(starts, S, T, i + 1)) - first, 0);
+}
+// The region of tile `at` of the line, and which of its tiles that is.  `group`: rows to a token
+D2C_DEV void find_tile(const int32_t *starts, int S, int T, int group, int at, int &region, int &tile)
+{
+    const int lane = threadIdx.x & 63;
+    auto begin = [&](int i) INLINE { return (int)((long)bound_of(starts, S, T, i) * group / kRows) + i; };
+    region = 0;
+    for (int i0 = 0; i0 <= S + 1; i0 += 64) {
+        const int i = i0 + lane;
+        const uint64_t before = __ballot(i <= S + 1 && begin(min(i, S + 1)) <= at);
+        if (before == 0) break;
+        region = i0 + (before == ~0ull ? 63 : __builtin_ctzll(~before) - 1);
+        if (before != ~0ull) break;
+    }
+    region = __builtin_amdgcn_readfirstlane(region);
+    tile = at - begin(region);
+}
+
+// A workgroup's sequence and tile
+struct PackedUnit { int q0, lq, k0, lk, rows, tile, h, at, split; };
+// (neighbouring workgroups have neighbouring heads, so that a head's meet in an XCD's L2 where the heads are a multiple of 8.  BY_KEYS: tiles of keys, from the first on; else tiles
+// of rows, from the last on: the longest walks of a sequence come first)
+template <bool BY_KEYS> D2C_DEV PackedUnit unit_of(const PackedArgs &a, int index)
+{
+    PackedUnit u;
+    const int rest = index / a.Hkv, line = rest % a.tiles;
+    u.h = index - rest * a.Hkv;
+    u.split = rest / a.tiles;
+    u.at = BY_KEYS ? line : a.tiles - 1 - line;
+    int region;
+    find_tile(BY_KEYS ? a.key_starts : a.starts, a.S, BY_KEYS ? a.Tk : a.T, BY_KEYS ? 1 : a.group, u.at, region, u.tile);
+    u.q0 = u.lq = u.k0 = u.lk = 0;
+    if (!BY_KEYS || (region >= 1 && region <= a.S)) region_of(a.starts, a.S, a.T, region, u.q0, u.lq);
+    if (BY_KEYS || (region >= 1 && region <= a.S)) region_of(a.key_starts, a.S, a.Tk, region, u.k0, u.lk);
+    u.rows = u.lq * a.group;
+    return u;
+}
+// Keys that position `pos` of a sequence reads
+D2C_DEV int limit_of(const PackedArgs &a, const PackedUnit &u, int pos)
+{
+    if (!a.causal) return u.lk;
+    const int p = u.lk - u.lq + pos;
+    return p < 0 ? 0 : min(u.lk, (fdiv(p, a.frame) + 1) * a.frame.d);
+}
+D2C_DEV int limit_of_row(const PackedArgs &a, const PackedUnit &u, int row) { return limit_of(a, u, fdiv(row, a.by_group)); }
+
+// Row `row` of a tensor [tokens][Hq][D] with strides s
+template <typename T> D2C_DEV const T *row_at(const void *base, const long *s, const PackedArgs &a, const PackedUnit &u, int row)
+{
+    const int pos = fdiv(row, a.by_group);
+    return reinterpret_cast<const T *>(base) + (long)(u.q0 + pos) * s[0] + (long)(u.h * a.group + row - pos * a.group) * s[1];
+}
+
+// The keys and values of a sequence's key head, a tile of KT keys at a time
+template <typename T, typename KV, int KT, bool WHOLE> struct PackedKeyTiles {
+    const T *kb, *vb;
+    long ks, vs;
+    unsigned koff[WHOLE ? KV::PER : 1], voff[WHOLE ? KV::PER : 1];
+    D2C_DEV PackedKeyTiles(const PackedArgs &a, const PackedUnit &u)
+    {
+        kb = reinterpret_cast<const T *>(a.k) + (long)u.k0 * a.ks[0] + u.h * a.ks[1];
+        vb = reinterpret_cast<const T *>(a.v) + (long)u.k0 * a.vs[0] + u.h * a.vs[1];
+        ks = a.ks[0]; vs = a.vs[0];
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int i = 0; i < KV::PER; i++) {
+                const unsigned row = KV::row_of(i), d = KV::column_of(i, a.D);
+                koff[i] = (row * (unsigned)ks + d) * (unsigned)sizeof(T);
+                voff[i] = (row * (unsigned)vs + d) * (unsigned)sizeof(T);
+            }
+        }
+    }
+    // left: keys of the sequence from the tile's first on (one at least); those behind repeat the last
+    D2C_DEV void request(const PackedArgs &a, KV &k, KV &v, int tile, int left) const
+    {
+        const T *kt = kb + (long)tile * KT * ks, *vt = vb + (long)tile * KT * vs;
+        if constexpr (WHOLE) {
+            unsigned ko[KV::PER], vo[KV::PER];
+#pragma unroll
+            for (int i = 0; i < KV::PER; i++) { ko[i] = koff[i]; vo[i] = voff[i]; }
+            if (left < KT) {
+#pragma unroll
+                for (int i = 0; i < KV::PER; i++) {
+                    const unsigned step = KV::row_of(i) < left ? 0u : (unsigned)(left - 1 - KV::row_of(i)) * (unsigned)sizeof(T);
+                    ko[i] += step * (unsigned)ks;
+                    vo[i] += step * (unsigned)vs;
+                }
+            }
+            k.load_at(kt, ko);
+            v.load_at(vt, vo);
+        } else {
+            k.load(a.D, [&](int i) INLINE { return kt + min(i, left - 1) * ks; });
+            v.load(a.D, [&](int i) INLINE { return vt + min(i, left - 1) * vs; });
+        }
+    }
+};
+
+// Whether a thread's pieces of a tile hold an infinity or NaN
+template <typename T, typename Pieces> D2C_DEV bool not_finite(const Pieces &x)
+{
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < Pieces::PER; i++)
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; j++) {
+            const uint32_t w[4] = {x.r[i].v[j].x, x.r[i].v[j].y, x.r[i].v[j].z, x.r[i].v[j].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // (float32: what rounds to an infinite bfloat16 term counts as one)
+                if (sizeof(T) == 4) bad = bad || (w[e] & 0x7fffffffu) > 0x7f7f7fffu;
+                else bad = bad || (w[e] & 0x7f800000u) == 0x7f800000u || (w[e] & 0x7f80u) == 0x7f80u;
+            }
+        }
+    return bad;
+}
+
+// Infinities and NaN of 16 bytes of elements (of bfloat16 terms, which an operand in LDS is made of) as zeros
+D2C_DEV uint4 finite_pairs(const uint4 &x)
+{
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0xffffu;
+        if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// ... and of a thread's pieces of a tile
+template <typename T, typename Pieces> D2C_DEV void clean(Pieces &x)
+{
+#pragma unroll
+    for (int i = 0; i < Pieces::PER; i++)
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; j++) {
+            if constexpr (sizeof(T) == 2) x.r[i].v[j] = finite_pairs(x.r[i].v[j]);
+            else {
+                uint4 &v = x.r[i].v[j];
+                for (uint32_t *w : {&v.x, &v.y, &v.z, &v.w})
+                    if ((*w & 0x7fffffffu) > 0x7f7f7fffu) *w = 0;
+            }
+        }
+}
+// An operand of a product whose weights are 0 where a pair is not to be read: in a tile of which some pairs are not, its infinities and NaN are left out of the product,
+// whose zeros they would turn into NaN: rows r0 .. r0 + 31 of a tile in LDS, by all 256 threads between two barriers of the workgroup's ...
+template <typename Pieces> D2C_DEV void clean_rows(unsigned char *lds, int r0)
+{
+    constexpr int ROW = Pieces::PIECES * 16;
+#pragma unroll 1
+    for (int i = threadIdx.x * 16; i < 32 * ROW; i += 256 * 16)
+#pragma unroll 1
+        for (int t = 0; t < Pieces::P; t++) {
+            uint4 *p = reinterpret_cast<uint4 *>(lds + t * Pieces::TERM + r0 * ROW + i);
+            *p = finite_pairs(*p);
+        }
+}
+// ... and added once at the end, to the sums of those that read them: what a sum has once taken in stays.  x: row(j) of D, j from first to end, read(j): whether this lane's
+// column reads it.  AS_NAN: what it makes whatever its weight (a key's, or query's, own infinity: its weight is NaN, or the 0 of a score of -infinity)
+template <typename T, bool AS_NAN, int ND, typename Row, typename Read> D2C_DEV void take_in(f32x16 (&acc)[ND], int D, int first, int end, Row row, Read read)
+{
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll 1
+    for (int j = first; j < end; j++) {
+        const T *p = row(j);
+        const bool yes = read(j);
+#pragma unroll
+        for (int i = 0; i < ND; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int d = i * 32 + 8 * (r / 4) + 4 * half + r % 4;
+                const float y = elem_to_f32<T>(p[min(d, D - 1)]);
+                const bool finite = sizeof(T) == 4 ? fabsf(y) <= 0x1.fefffep127f : fabsf(y) < INFINITY;
+                if (yes && !finite) acc[i][r] += AS_NAN ? NAN : y * 2.f;
+                asm volatile("" : "+v"(acc[i][r]) : : "memory");      // (one value at a time)
+            }
+    }
+}
+
+PackedArgs make_args(const d2c_packed_attention_desc &q, const int32_t *starts, const int32_t *key_starts);
+// Whether a problem runs on the kernels that load whole pieces by offsets of 32 bits inside a tile
+inline bool fast_kernels(const d2c_packed_attention_desc &q)
+{
+    const long size = (long)d2c_elem_size(q.dtype), limit = 1L << 31;
+    auto near = [&](const int64_t *s) { return s[0] >= 0 && s[1] >= 0 && 129 * s[0] * size + (q.Hq / q.Hkv) * s[1] * size < limit; };
+    return q.D % 8 == 0 && near(q.q_stride) && near(q.k_stride) && near(q.v_stride) && 130L * q.Hq * q.D * size < limit;
+}
+inline int tiles_of(long rows, int sequences) { return (int)(rows / kRows) + sequences + 2; }
+
+// How many workgroups share the walk of a tile: as many as fill the GPU's places where tiles are few, of `steps` steps each or more on the average
+inline int splits_of(long units, long places, long walk, long step, long steps, double unit_bytes)
+{
+    long s = std::max(std::min({places / std::max(units, 1L), walk / (step * steps), 16L}), 1L);
+    while (s > 1 && (double)s * (double)units * unit_bytes > (double)D2C_ATTENTION_PART_BYTES) s--;
+    return (int)s;
+}
+
+}  // namespace d2c_packed
+
+int d2c_packed_attention_check(const d2c_packed_attention_desc *q);

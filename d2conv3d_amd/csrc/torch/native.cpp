@@ -867,6 +867,104 @@ py::object cross_attention(const Tensor &query, const Tensor &key, const Tensor 
     return py::cast(recorded);
 }
 
+// ---------------------------------------------------------------- packed_attention
+void strides(d2c_packed_attention_desc &q, const Tensor &query, const Tensor &key, const Tensor &value)
+{
+    for (int i = 0; i < 2; i++) { q.q_stride[i] = query.stride(i); q.k_stride[i] = key.stride(i); q.v_stride[i] = value.stride(i); }
+}
+struct PackedAttentionBackward : public Node {
+    d2c_packed_attention_desc q;
+    SavedVariable query, key, value, starts, key_starts, out, low, lse;
+    bool has_key_starts = false, has_low = false;
+    std::string name() const override { return "PackedAttentionBackward"; }
+    void release_variables() override
+    {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *v : {&query, &key, &value, &starts, &key_starts, &out, &low, &lse}) v->reset_data();
+    }
+    variable_list apply(variable_list &&grads) override
+    {
+        variable_list r(3);
+        const std::lock_guard<std::mutex> lock(mutex_);
+        if (!grads[0].defined()) grads[0] = input_metadata(0).zeros_like();
+        {
+            at::NoGradGuard no_grad;
+            const Tensor vq = with_inner_contiguous(query.unpack()), vk = with_inner_contiguous(key.unpack()), vv = with_inner_contiguous(value.unpack());
+            const Tensor vo = out.unpack(shared_from_this()).contiguous(), vl = lse.unpack().contiguous(), vs = starts.unpack().contiguous();
+            Tensor vks, vlow;
+            if (has_low) vlow = low.unpack().contiguous();
+            if (has_key_starts) vks = key_starts.unpack().contiguous();
+            strides(q, vq, vk, vv);
+            c10::DeviceGuard guard(vq.device());
+            const hipStream_t st = stream_of(vq);
+            const Tensor g = grads[0].contiguous();
+            if (should_compute_output(0)) r[0] = no_grad_empty_like(vq);
+            if (should_compute_output(1)) r[1] = no_grad_empty_like(vk);
+            if (should_compute_output(2)) r[2] = no_grad_empty_like(vv);
+            const size_t nb = d2c_packed_attention_backward_workspace_bytes(&q);
+            const Tensor ws = small_workspace(nb, vq);
+            check(d2c_packed_attention_backward(&q, ptr(g), ptr(vq), ptr(vk), ptr(vv), (const int32_t *)ptr(vs), (const int32_t *)ptr(vks), ptr(vo), ptr(vlow),
+                                                (const float *)ptr(vl), ptr(r[0]), ptr(r[1]), ptr(r[2]), ptr(ws), nb, st),
+                  "packed_attention backward");
+        }
+        once_differentiable(r, grads[0]);
+        return r;
+    }
+};
+
+py::object packed_attention(const Tensor &query, const Tensor &key, const Tensor &value, const Tensor &starts, const opt_tensor &key_starts, bool causal,
+                            int64_t frame, const std::optional<double> &scale)
+{
+    const Tensor other = key_starts.value_or(Tensor());
+    for (const Tensor *t : {&query, &key, &value}) {
+        if (!plain_strided(*t) || t->dim() != 3 || t->device() != query.device() || !inner_contiguous(*t) || t->scalar_type() != query.scalar_type()) return py::none();
+        for (int i = 0; i < 3; i++)
+            if (t->size(i) == 0 || t->size(i) >= (1ll << 31)) return py::none();
+    }
+    const int dt = dtype_code(query);
+    if ((dt != D2C_F32 && dt != D2C_BF16) || key.sizes() != value.sizes() || key.size(2) != query.size(2) || query.size(1) % key.size(1) != 0 || query.size(2) > 128 ||
+        frame <= 0 || frame > (1ll << 30))
+        return py::none();
+    auto is_starts = [&](const Tensor &t) {
+        return plain(t) && t.device() == query.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) > 0 && t.size(0) <= (1ll << 30);
+    };
+    if (!is_starts(starts) || (other.defined() ? !is_starts(other) || other.size(0) != starts.size(0) : key.size(0) != query.size(0))) return py::none();
+    d2c_packed_attention_desc q;
+    std::memset(&q, 0, sizeof q);
+    q.sequences = (int)starts.size(0) - 1; q.Hq = (int)query.size(1); q.Hkv = (int)key.size(1); q.D = (int)query.size(2); q.dtype = dt;
+    q.causal = causal; q.frame = (int)frame; q.queries = query.size(0); q.keys = key.size(0);
+    const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.D);
+    if (!(s > 0.0) || !((float)s > 0.f) || !((float)s < INFINITY)) return py::none();
+    q.scale = (float)s;
+    strides(q, query, key, value);
+    const bool grad = wants_grad(query, key, value);
+    std::shared_ptr<PackedAttentionBackward> node;
+    if (grad) {
+        node = std::shared_ptr<PackedAttentionBackward>(new PackedAttentionBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(query, key, value));
+    }
+    c10::DeviceGuard guard(query.device());
+    const auto opt = query.options().requires_grad(false);
+    Tensor out = at::empty(query.sizes(), opt), low, lse;
+    if (grad && dt == D2C_BF16) low = at::empty(query.sizes(), opt);
+    if (grad) lse = at::empty({q.Hkv, q.queries * (q.Hq / q.Hkv)}, opt.dtype(at::kFloat));
+    const size_t nb = d2c_packed_attention_forward_workspace_bytes(&q);
+    const Tensor ws = small_workspace(nb, query);
+    check(d2c_packed_attention_forward(&q, ptr(query), ptr(key), ptr(value), (const int32_t *)ptr(starts), (const int32_t *)ptr(other), ptr(out), ptr(low), (float *)ptr(lse),
+                                       ptr(ws), nb, stream_of(query)),
+          "packed_attention forward");
+    if (!grad) return py::cast(out);
+    node->q = q;
+    node->query = SavedVariable(query, false); node->key = SavedVariable(key, false); node->value = SavedVariable(value, false);
+    node->lse = SavedVariable(lse, false); node->starts = SavedVariable(starts, false);
+    node->has_low = low.defined(); node->has_key_starts = other.defined();
+    if (low.defined()) node->low = SavedVariable(low, false);
+    if (other.defined()) node->key_starts = SavedVariable(other, false);
+    Tensor recorded = record(out, node);
+    node->out = SavedVariable(recorded, true);
+    return py::cast(recorded);
+}
+
 // ---------------------------------------------------------------- a memory in pages
 // The description of a memory whose tensors the kernels can take as they are; false: one that the Python code has something to say about
 bool memory_desc(d2c_memory_desc &q, const Tensor &key, const Tensor &value, const Tensor &table, const Tensor &lengths, const Tensor &usage, const Tensor &positions)
@@ -974,6 +1072,7 @@ PYBIND11_MODULE(_native, m)
     m.def("layer_norm", &layer_norm);
     m.def("rotary3d", &rotary3d);
     m.def("cross_attention", &cross_attention);
+    m.def("packed_attention", &packed_attention);
     m.def("memory_append", &memory_append);
     m.def("memory_attention", &memory_attention);
     m.def("memory_evict", &memory_evict);

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._ops import _DT, _ptr, _stream, _try_native, _workspace
-from .attention import _check, _check_tensors
+from .attention import _check, _check_tensors, _heads_contiguous
 
 _TYPES = (torch.float32, torch.bfloat16)
 
@@ -92,10 +92,6 @@ def _memory_desc(what, m, also=()):
 
 def _no_gradient(what, *tensors):
     _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)), f"{what} takes no gradient: call it under torch.no_grad()")
-
-
-def _heads_contiguous(t):
-    return t if t.stride(2) == 1 or t.size(2) == 1 else t.contiguous()
 
 
 def memory_append(memory, key, value, starts=None):

@@ -547,6 +547,33 @@ int d2c_attention_backward(const d2c_attention_desc *desc, const void *grad_out,
                            const void *out_low, const float *lse, void *grad_query, void *grad_key, void *grad_value, void *workspace,
                            size_t workspace_bytes, void *stream);
 
+/* Attention inside each of several sequences that lie behind each other.  query [queries, Hq, D], key and value [keys, Hkv, D] with strides
+ * (token, head; channels adjacent), Hq a multiple of Hkv, D up to 128.  Sequence s has the queries starts[s] .. starts[s + 1] - 1 and the keys
+ * key_starts[s] .. key_starts[s + 1] - 1 (int32 [sequences + 1], rising, taken into 0 .. queries or keys; key_starts NULL: starts).  Its
+ * queries are the last of its Lk tokens: query i of Lq is token p = Lk - Lq + i, and reads, `causal`, the first
+ *     min(Lk, (floor(p / frame) + 1) * frame)        (p < 0: none)
+ * keys -- frame 1: up to its own token; otherwise up to the end of its frame of so many tokens -- and all Lk if not.  Keys and values that
+ * a query does not read have no influence on it whatever they hold.  A query without keys is 0, as are queries of no sequence; so are their
+ * gradients and those of keys that nobody reads.  out, grad_out and the gradients are contiguous.  `lse` [Hkv, queries * Hq / Hkv] and, bfloat16,
+ * `out_low` (as out) are for the backward call (see d2c_attention_forward).
+ * Sums are made in an order that sizes, strides, starts and GPU determine.  Starts that do not rise: results of no meaning, but nothing outside
+ * the tensors is read or written. */
+typedef struct d2c_packed_attention_desc {
+    int32_t sequences, Hq, Hkv, D, dtype, causal, frame;
+    float scale;
+    int64_t queries, keys;
+    int64_t q_stride[2], k_stride[2], v_stride[2];
+} d2c_packed_attention_desc;
+size_t d2c_packed_attention_forward_workspace_bytes(const d2c_packed_attention_desc *desc);
+int d2c_packed_attention_forward(const d2c_packed_attention_desc *desc, const void *query, const void *key, const void *value,
+                                 const int32_t *starts, const int32_t *key_starts, void *out, void *out_low, float *lse,
+                                 void *workspace, size_t workspace_bytes, void *stream);
+size_t d2c_packed_attention_backward_workspace_bytes(const d2c_packed_attention_desc *desc);
+int d2c_packed_attention_backward(const d2c_packed_attention_desc *desc, const void *grad_out, const void *query, const void *key,
+                                  const void *value, const int32_t *starts, const int32_t *key_starts, const void *out,
+                                  const void *out_low, const float *lse, void *grad_query, void *grad_key, void *grad_value,
+                                  void *workspace, size_t workspace_bytes, void *stream);
+
 /* A memory of keys and values in pages, for streams that are read token by token.  key and value [pages][heads][page][D] with strides
  * (page, head, slot; channels adjacent), usage (float32) and positions (int32) [pages][heads][page] contiguous.  Slot s of stream n
  * lies at slot s % page of page table[n][s / page] (table: int32 [streams][per_stream], rows table_stride elements apart); slots of
