@@ -17,7 +17,7 @@ struct MemArgs {
     float *part, *part_ml;        // [units + places][R][part_width(D)], and (maximum, sum) of each row
     int32_t *covered;             // [units][2]: the first and the last workgroup that has a piece of the unit
     int32_t *begins;              // [places][4]: unit and step that a workgroup begins with, its steps
-    float *scores;                // [streams * heads * group][slots], of base 2
+    float *scores;                // [units][slots][R], of base 2
     long qs[2], ks[3], vs[3], table_stride, slots_padded;
     FastDiv page;
     int N, heads, group, D, pages, slots, row_groups, units, places, least;
@@ -28,15 +28,25 @@ D2C_DEV int slots_of(const MemArgs &a, int n) { return min(max(a.lengths[n], 0),
 // Steps of a stream's walk: one at least, so that a stream without slots has a unit that writes its zeros
 template <int STEP> D2C_DEV int steps_of(const MemArgs &a, int n) { return max(1, (slots_of(a, n) + STEP - 1) / STEP); }
 
-template <typename Op> D2C_DEV int wave_scan(int v, Op op)
+// Sum over the lanes up to this one, without LDS
+template <int CTRL, int ROWS> D2C_DEV int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+D2C_DEV int wave_scan(int v)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int x = __shfl_up(v, d, 64);
-        if (lane >= d) v = op(v, x);
-    }
+    v = dpp_add<0x111, 0xf>(v);      // inside rows of sixteen lanes: from 1, 2, 4, 8 lanes before
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);      // the second and fourth row: the last lane of the row before
+    v = dpp_add<0x143, 0xc>(v);      // the upper half: the last lane of the lower
     return v;
+}
+// ... of a wavefront's sums, those before `wave`: all requested at once
+template <int WAVES> D2C_DEV int before_wave(const int *sums, int wave)
+{
+    int x = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) x += w < wave ? sums[w] : 0;
+    return x;
 }
 
 // Where this workgroup begins.  The steps of all units (stream, key head, rows of up to eight; in this order) are one line, of which every workgroup takes as
@@ -45,10 +55,9 @@ template <int STEP> D2C_DEV bool find_begin(const MemArgs &a, int &unit, int &t,
 {
     __shared__ int s_wave[4], s_found[2];
     const int tid = threadIdx.x, wave = tid >> 6, per_stream = a.heads * a.row_groups;
-    auto add = [](int x, int y) INLINE { return x + y; };
     int c = 0;
     for (int n = tid; n < a.N; n += 256) c += steps_of<STEP>(a, n);
-    int scan = wave_scan(c, add);
+    int scan = wave_scan(c);
     if ((tid & 63) == 63) s_wave[wave] = scan;
     __syncthreads();
     const long total = (long)(s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3]) * per_stream;
@@ -60,13 +69,12 @@ template <int STEP> D2C_DEV bool find_begin(const MemArgs &a, int &unit, int &t,
         const int n = n0 + tid;
         if (a.N > 256) {
             c = n < a.N ? steps_of<STEP>(a, n) : 0;
-            scan = wave_scan(c, add);
+            scan = wave_scan(c);
             __syncthreads();
             if ((tid & 63) == 63) s_wave[wave] = scan;
             __syncthreads();
         }
-        long before = base + scan - c;
-        for (int w = 0; w < wave; w++) before += s_wave[w];
+        const long before = base + scan - c + before_wave<4>(s_wave, wave);
         if (n < a.N && before * per_stream <= start && start < (before + c) * per_stream) { s_found[0] = n; s_found[1] = (int)before; }
         base += s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
     }
@@ -77,16 +85,30 @@ template <int STEP> D2C_DEV bool find_begin(const MemArgs &a, int &unit, int &t,
     return true;
 }
 
-// The weights of a unit's slots from s0 to s1, added up over all rows of its key head.  s_ml: maximum and 1 / sum of the rows
-D2C_DEV void add_usage(const MemArgs &a, int n, int h, int s0, int s1, const float2 *s_ml)
+// The weights of a key head's slots from s0 to s1, added up over all its rows, R to a unit.  s_ml: maximum and 1 / sum of the rows
+template <int R> D2C_DEV void add_usage(const MemArgs &a, int unit, int n, int h, int s0, int s1, const float2 *s_ml)
 {
-    const float *scores = a.scores + (long)(n * a.heads + h) * a.group * a.slots_padded;
     for (int s = s0 + (int)threadIdx.x; s < s1; s += 256) {
         const int p = fdiv(s, a.page), id = a.table[n * a.table_stride + p];
         if ((unsigned)id >= (unsigned)a.pages) continue;
+        float *to = a.usage + ((long)id * a.heads + h) * a.page.d + (s - p * a.page.d);
+        const float old = *to;
         float x = 0.f;
-        for (int r = 0; r < a.group; r++) x += __builtin_amdgcn_exp2f(scores[r * a.slots_padded + s] - s_ml[r].x) * s_ml[r].y;
-        a.usage[((long)id * a.heads + h) * a.page.d + (s - p * a.page.d)] += x;
+        for (int g = 0; g < a.row_groups; g++) {
+            float score[R];
+            const float *from = a.scores + ((long)(unit + g) * a.slots_padded + s) * R;
+            if constexpr (R % 4 == 0) {
+#pragma unroll
+                for (int r = 0; r < R; r += 4) *reinterpret_cast<float4 *>(score + r) = *reinterpret_cast<const float4 *>(from + r);
+            } else {
+#pragma unroll
+                for (int r = 0; r < R; r++) score[r] = from[r];
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++)
+                if (g * R + r < a.group) x += __builtin_amdgcn_exp2f(score[r] - s_ml[g * R + r].x) * s_ml[g * R + r].y;
+        }
+        *to = old + x;
     }
 }
 // (a row whose sum is 0 has no slot, or none whose score is above -infinity: no weights)
@@ -122,7 +144,7 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
         budget -= t1 - t0;
         const T *kb = reinterpret_cast<const T *>(a.key) + h * a.ks[1], *vb = reinterpret_cast<const T *>(a.value) + h * a.vs[1];
         const int32_t *table = a.table + n * a.table_stride;
-        float *scores = a.usage ? a.scores + ((long)nh * a.group + row0) * a.slots_padded : nullptr;
+        float *scores = a.usage ? a.scores + (long)unit * a.slots_padded * R : nullptr;
 
         uint4 k[LOADS], v[LOADS];
         bool there[LOADS];
@@ -178,12 +200,19 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
                 }
             }
             if (scores) {
+                // (all lanes of a slot have its scores: lane u of them writes those of load u, all rows together)
+                static_assert(LOADS <= LANES, "");
+                float mine[R];
 #pragma unroll
-                for (int u = 0; u < LOADS; u++) {
-                    const int slot = slot_of(t, u);
+                for (int r = 0; r < R; r++) {
+                    mine[r] = s[0][r];
 #pragma unroll
-                    for (int r = 0; r < R; r++)
-                        if (lane % LANES == r % LANES && r < rows && slot < slots) scores[r * a.slots_padded + slot] = s[u][r];
+                    for (int u = 1; u < LOADS; u++) mine[r] = lane % LANES == u ? s[u][r] : mine[r];
+                }
+                const int slot = slot_of(t, lane % LANES);
+                if (lane % LANES < LOADS && slot < slots) {
+#pragma unroll
+                    for (int r = 0; r < R; r++) scores[(long)slot * R + r] = mine[r];
                 }
             }
             if (t + 1 < t1) {
@@ -293,7 +322,7 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
                     s_row[r] = usage_ml(top, sum);
                 }
                 __syncthreads();
-                add_usage(a, n, h, 0, slots, s_row);
+                add_usage<R>(a, unit, n, h, 0, slots, s_row);
             }
             return;
         }
@@ -301,8 +330,9 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
     }
 }
 
-// Units that several workgroups have shared: blocks from 0, one to a row, put their pieces together.  Where weights are added up: blocks from `rows` on, one to each
+// Units that several workgroups have shared: blocks from 0, one to a row, put their pieces together.  Where weights are added up: blocks from `rows` on, kUsageBlocks to each
 // workgroup of the walk, go over the same slots once more, by their scores.
+constexpr int kUsageBlocks = 4;
 template <typename T, int LANES, int R> __global__ void __launch_bounds__(256) mem_join_kernel(MemArgs a, int rows, int step)
 {
     constexpr int GROUPS = 256 / LANES;
@@ -363,14 +393,17 @@ template <typename T, int LANES, int R> __global__ void __launch_bounds__(256) m
         if (d < a.D) store4<T>(reinterpret_cast<T *>(a.out) + ((long)nh * a.group + row) * a.D + d, x, a.D - d);
         return;
     }
-    const int32_t *begin = a.begins + ((int)blockIdx.x - rows) * 4;
+    const int32_t *begin = a.begins + ((int)blockIdx.x - rows) / kUsageBlocks * 4;
     int unit = begin[0], t = begin[1], budget = begin[2];
     if (unit < 0) return;
+    const int part = ((int)blockIdx.x - rows) % kUsageBlocks;
     for (; budget > 0 && unit < a.units; unit++, t = 0) {
         const int nh = unit / a.row_groups, n = nh / a.heads, h = nh - n * a.heads, slots = slots_of(a, n), steps = max(1, (slots + step - 1) / step);
         const int t1 = min(steps, t + budget);
         budget -= t1 - t;
         if (unit != nh * a.row_groups || slots == 0) continue;      // (the first group of rows goes for all of them)
+        const int s0 = t * step, some = min(slots, t1 * step) - s0, from = s0 + (int)((long)some * part / kUsageBlocks), to = s0 + (int)((long)some * (part + 1) / kUsageBlocks);
+        if (from == to) continue;
         __syncthreads();
         for (int row = tid >> 6; row < a.group; row += 4) {
             const int u = unit + row / R, w0 = a.covered[u * 2], w1 = a.covered[u * 2 + 1];
@@ -389,7 +422,7 @@ template <typename T, int LANES, int R> __global__ void __launch_bounds__(256) m
             if ((tid & 63) == 0) s_ml[row] = usage_ml(all, sum);
         }
         __syncthreads();
-        add_usage(a, n, h, t * step, min(slots, t1 * step), s_ml);
+        add_usage<R>(a, unit, n, h, from, to, s_ml);
     }
 }
 
@@ -436,23 +469,65 @@ template <typename T> __global__ void __launch_bounds__(256) mem_append_one_kern
         a.seen[n] = seen + 1;
     }
 }
-// Packed tokens: a thread has one piece of a row (a token's head) and goes from row to row
-template <typename T> __global__ void __launch_bounds__(256) mem_append_kernel(AppendArgs a, FastDiv heads)
+// Packed tokens, kAppendTokens to a workgroup: a thread to a token finds its place, then all of them move pieces of 16 bytes, four requested at a time
+constexpr int kAppendTokens = 8;
+template <typename T> __global__ void __launch_bounds__(256) mem_append_kernel(AppendArgs a, FastDiv by_pieces)
 {
-    const int pieces = (a.D * (int)sizeof(T) + 15) / 16, two = 2 * pieces, per = 256 / two, sub = threadIdx.x / two;
-    if (sub >= per) return;
-    const int rows = (int)a.tokens * a.heads;
-    for (long i = (long)blockIdx.x * per + sub; i < rows; i += (long)gridDim.x * per) {
-        const int token = fdiv((int)i, heads), h = (int)i - token * a.heads;
-        int lo = 0, hi = a.N;      // the last stream that begins at or before the token
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (start_of(a, mid) <= token) lo = mid; else hi = mid;
+    constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
+    __shared__ int s_page[kAppendTokens], s_slot[kAppendTokens];      // (page -1: nowhere)
+    const long token0 = (long)blockIdx.x * kAppendTokens;
+    const int tid = threadIdx.x;
+    if (tid < kAppendTokens) {
+        int id = -1, at = 0;
+        const long token = token0 + tid;
+        if (token < a.tokens) {
+            int lo = 0, hi = a.N;      // the last stream that begins at or before the token
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (start_of(a, mid) <= token) lo = mid; else hi = mid;
+            }
+            const long first = start_of(a, lo), slot = min(max(a.lengths[lo], 0), a.slots) + token - first;
+            if (token >= first && token < start_of(a, lo + 1) && slot < a.slots) {
+                const int p = fdiv((int)slot, a.page);
+                id = a.table[lo * a.table_stride + p];
+                at = (int)slot - p * a.page.d;
+                if ((unsigned)id >= (unsigned)a.pages) id = -1;
+                else
+                    for (int h = 0; h < a.heads; h++) {
+                        const long i = ((long)id * a.heads + h) * a.page.d + at;
+                        a.usage[i] = 0.f;
+                        a.positions[i] = (int)(a.seen[lo] + token - first);
+                    }
+            }
         }
-        const long first = start_of(a, lo);
-        if (token < first || token >= start_of(a, lo + 1)) continue;
-        const long later = token - first;
-        put_piece<T>(a, token, lo, min(max(a.lengths[lo], 0), a.slots) + later, (int)(a.seen[lo] + later), h, threadIdx.x - sub * two, pieces);
+        s_page[tid] = id;
+        s_slot[tid] = at;
+    }
+    __syncthreads();
+    const int pieces = by_pieces.d, all = kAppendTokens * a.heads * pieces;      // (of keys; the same again of values)
+    for (int i0 = tid; i0 < 2 * all; i0 += 256 * AT_ONCE) {
+        T *to[AT_ONCE];
+        uint4 x[AT_ONCE];
+        int left[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            to[u] = nullptr;
+            int i = i0 + u * 256;
+            if (i >= 2 * all) continue;
+            const bool second = i >= all;
+            if (second) i -= all;
+            const int row = fdiv(i, by_pieces), d = (i - row * pieces) * VEC, which = row / a.heads, h = row - which * a.heads, id = s_page[which];
+            if (id < 0) continue;
+            left[u] = a.D - d;
+            const T *from = second ? reinterpret_cast<const T *>(a.nv) + (token0 + which) * a.nvs[0] + h * a.nvs[1]
+                                   : reinterpret_cast<const T *>(a.nk) + (token0 + which) * a.nks[0] + h * a.nks[1];
+            to[u] = d + (second ? reinterpret_cast<T *>(a.value) + id * a.vs[0] + h * a.vs[1] + s_slot[which] * a.vs[2]
+                                : reinterpret_cast<T *>(a.key) + id * a.ks[0] + h * a.ks[1] + s_slot[which] * a.ks[2]);
+            x[u] = load_run<T>(from + d, left[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++)
+            if (to[u]) store_run<T>(to[u], x[u], left[u]);
     }
 }
 __global__ void __launch_bounds__(256) mem_count_kernel(AppendArgs a)
@@ -487,129 +562,264 @@ D2C_DEV uint32_t rank_of(float usage, bool stays)
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// A workgroup to a stream's head.  The keep-th largest rank by its digits (11, 11 and 10 bits, a histogram of each in LDS), then the slots that go before `keep`
-// and those that stay behind it, each in rising order.
-constexpr int kEvictThreads = 1024;
-__global__ void __launch_bounds__(kEvictThreads) mem_rank_kernel(EvictArgs a)
+// A workgroup to a stream's head.  The keep-th largest rank by its digits (11, 11 and 10 bits, a histogram of each in LDS, the first in several copies, whose few bins many
+// lanes meet in), then the slots that go before `keep` and those that stay behind it, each in rising order.  A wavefront has neighbouring slots, 64 at a time, whose
+// truth values are one word each: counted by a lane to a word.
+// LDS: their ranks stay there; else in memory.  PAGED: pages are multiples of 64 slots, so that a wavefront's 64 lie in one.  Loops are short rather than unrolled: every
+// instruction is fetched anew by every launch (ranks in registers, 32 to a thread and all loops unrolled: 45 us where this takes 2x).
+constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kEvictLds = 26 << 10;      // (slots)
+template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads) mem_rank_kernel(EvictArgs a)
 {
-    constexpr int BINS = 2048, WAVES = kEvictThreads / 64;
-    __shared__ int s_hist[BINS], s_wave[3][WAVES], s_digit[2];
-    const int unit = blockIdx.x, n = unit / a.heads, h = unit - n * a.heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int BINS = 2048, COPIES = 4, AT_ONCE = 4, WORDS = 64;
+    constexpr int LIST = (COPIES - 1) * BINS, REQUESTS = PAGED ? 16 : 8;
+    extern __shared__ __align__(16) uint32_t s_ranks[];
+    __shared__ __align__(16) int s_hist[COPIES][BINS];
+    __shared__ __align__(16) uint4 s_words[kEvictWaves][WORDS];      // of 64 slots: which ranks are above the border, which are at it
+    __shared__ int s_wave[3][kEvictWaves], s_digit[2], s_met;
+    const int unit = blockIdx.x, n = unit / a.heads, h = unit - n * a.heads, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int slots = min(max(a.lengths[n], 0), a.slots);
     if (slots <= a.keep) {
         if (tid == 0) a.counts[unit] = 0;
         return;
     }
-    uint32_t *ranks = a.ranks + unit * a.slots_padded;
-    const long newest = (long)a.seen[n] - a.recent;
-    uint32_t prefix = 0;
-    int wanted = a.keep;
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        for (int i = tid; i < BINS; i += kEvictThreads) s_hist[i] = 0;
-        __syncthreads();
-        if (pass == 0) {
-            for (int s = tid; s < slots; s += kEvictThreads) {
-                const int p = fdiv(s, a.page), id = a.table[n * a.table_stride + p];
-                uint32_t rank = 0;
-                if ((unsigned)id < (unsigned)a.pages) {
-                    const long i = ((long)id * a.heads + h) * a.page.d + (s - p * a.page.d);
-                    rank = rank_of(a.usage[i], a.positions[i] >= newest);
-                }
-                ranks[s] = rank;
-                atomicAdd(&s_hist[rank >> 21], 1);
-            }
+    const int per = (slots + kEvictThreads - 1) / kEvictThreads * 64, s0 = min(wave * per, slots), s1 = min(s0 + per, slots), numbers = (s1 - s0 + 63) / 64;
+    const int newest = (int)max((long)a.seen[n] - a.recent, -(1L << 31));
+    const int32_t *table = a.table + n * a.table_stride;
+    // the ranks of 64 slots from s on; 0 behind the last, which then are the first to go
+    auto rank_at = [&](int s) INLINE {
+        int id, in_page;
+        if constexpr (PAGED) {
+            const int p = fdiv(min(s, slots - 1), a.page);
+            id = table[p];
+            in_page = s - p * a.page.d + lane;
+            if (s >= slots) in_page = lane;
         } else {
-            const uint32_t mask = pass == 1 ? 0xffe00000u : 0xfffffc00u;
-            for (int s = tid; s < slots; s += kEvictThreads) {
-                const uint32_t rank = ranks[s];
-                if ((rank & mask) == prefix) atomicAdd(&s_hist[(rank >> shift) & (pass == 1 ? 2047 : 1023)], 1);
+            const int at = min(s + lane, slots - 1), p = fdiv(at, a.page);
+            id = table[p];
+            in_page = at - p * a.page.d;
+        }
+        const bool valid = (unsigned)id < (unsigned)a.pages;
+        const long page = (long)((valid ? id : 0) * a.heads + h) * a.page.d;
+        const uint32_t rank = rank_of(a.usage[page + (unsigned)in_page], a.positions[page + (unsigned)in_page] >= newest);
+        return valid && s + lane < s1 ? rank : 0u;
+    };
+    uint32_t *ranks = LDS ? nullptr : a.ranks + unit * a.slots_padded;
+    uint32_t *s_list = reinterpret_cast<uint32_t *>(s_hist[1]);      // ranks of the second pass's digit, in the place of the first pass's copies
+    // f(number, rank) for the wavefront's slots s0 + 64 number + lane from number `first` on, 4 at a time and WORDS at most
+    auto for_slots = [&](int first, auto f) INLINE {
+#pragma unroll 1
+        for (int i = first; i < min(numbers, first + WORDS); i += AT_ONCE) {
+            uint32_t r[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int s = s0 + (i + u) * 64 + lane;
+                r[u] = 0;
+                if constexpr (LDS) r[u] = s_ranks[min(s, s1 - 1)];
+                else r[u] = ranks[min(s, s1 - 1)];
+                if (s >= s1) r[u] = 0;
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) f(i + u, r[u]);
+        }
+    };
+    if (tid == 0) s_met = 0;
+    for (int i = tid; i < COPIES * BINS / 4; i += kEvictThreads) reinterpret_cast<int4 *>(&s_hist[0][0])[i] = make_int4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int i = 0; i < numbers; i += REQUESTS) {
+        uint32_t r[REQUESTS];
+#pragma unroll
+        for (int u = 0; u < REQUESTS; u++) r[u] = rank_at(s0 + (i + u) * 64);
+#pragma unroll
+        for (int u = 0; u < REQUESTS; u++) {
+            const int s = s0 + (i + u) * 64 + lane;
+            if (s < s1) {
+                if constexpr (LDS) s_ranks[s] = r[u];
+                else ranks[s] = r[u];
             }
         }
+    }
+    uint32_t prefix = 0;
+    int wanted = a.keep;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        if (pass > 0)
+            for (int i = tid; i < BINS / 4; i += kEvictThreads) reinterpret_cast<int4 *>(s_hist[0])[i] = make_int4(0, 0, 0, 0);
+        __syncthreads();
+        if (pass == 0)
+            for (int first = 0; first < numbers; first += WORDS)
+                for_slots(first, [&](int, uint32_t rank) INLINE {
+                    if (rank != 0) atomicAdd(&s_hist[lane % COPIES][rank >> 21], 1);
+                });
+        else if (pass == 1)
+            for (int first = 0; first < numbers; first += WORDS)
+                for_slots(first, [&](int, uint32_t rank) INLINE {
+                    if ((rank >> 21) != (prefix >> 21)) return;
+                    atomicAdd(&s_hist[0][(rank >> 10) & 2047], 1);
+                    const int at = atomicAdd(&s_met, 1);      // (in any order: they are only counted)
+                    if (at < LIST) s_list[at] = rank;
+                });
+        else if (s_met <= LIST)
+            for (int i = tid; i < s_met; i += kEvictThreads) {
+                if ((s_list[i] >> 10) == (prefix >> 10)) atomicAdd(&s_hist[0][s_list[i] & 1023], 1);
+            }
+        else
+            for (int first = 0; first < numbers; first += WORDS)
+                for_slots(first, [&](int, uint32_t rank) INLINE {
+                    if ((rank >> 10) == (prefix >> 10)) atomicAdd(&s_hist[0][rank & 1023], 1);
+                });
         __syncthreads();
         // bins from the top: thread i has bins 2047 - 2i and 2046 - 2i
-        const int high = s_hist[BINS - 1 - 2 * tid], low = s_hist[BINS - 2 - 2 * tid];
-        const int scan = wave_scan(high + low, [](int x, int y) INLINE { return x + y; });
+        int high = 0, low = 0;
+#pragma unroll 1
+        for (int c = 0; c < (pass == 0 ? COPIES : 1); c++) {
+            const int2 two = *reinterpret_cast<const int2 *>(&s_hist[c][BINS - 2 - 2 * tid]);
+            high += two.y; low += two.x;
+        }
+        // (slots of rank 0 are counted nowhere: where others do not make up `keep`, the last bin has what is wanted)
+        if (tid == kEvictThreads - 1) low = a.slots;
+        const int scan = wave_scan(high + low);
         if (lane == 63) s_wave[0][wave] = scan;
         __syncthreads();
-        int above = scan - high - low;
-        for (int w = 0; w < wave; w++) above += s_wave[0][w];
+        const int above = scan - high - low + before_wave<kEvictWaves>(s_wave[0], wave);
         if (above < wanted && wanted <= above + high) { s_digit[0] = BINS - 1 - 2 * tid; s_digit[1] = wanted - above; }
         else if (above + high < wanted && wanted <= above + high + low) { s_digit[0] = BINS - 2 - 2 * tid; s_digit[1] = wanted - above - high; }
         __syncthreads();
         prefix |= (uint32_t)s_digit[0] << shift;
         wanted = s_digit[1];      // how many of this digit stay, in the end: of the rank itself, lowest slots first
-        __syncthreads();
     }
-    // a wavefront has neighbouring slots: 64 at a time, places by the lanes before
-    const int per = ((slots + WAVES * 64 - 1) / (WAVES * 64)) * 64, s0 = min(wave * per, slots), s1 = min(s0 + per, slots);
+    // lane i has the words of number first + i
+    uint64_t above = 0, same = 0;
+    auto find_words = [&](int first) INLINE {
+        for_slots(first, [&](int i, uint32_t rank) INLINE {
+            const uint64_t x = __ballot(rank > prefix), y = __ballot(rank == prefix);
+            s_words[wave][i - first] = make_uint4((uint32_t)x, (uint32_t)(x >> 32), (uint32_t)y, (uint32_t)(y >> 32));      // (all lanes the same)
+        });
+        __builtin_amdgcn_wave_barrier();
+        const uint4 w = s_words[wave][min(lane, WORDS - 1)];
+        // (slots behind the last have a rank of 0, which may be the border)
+        const int s = s0 + (first + lane) * 64;
+        const uint64_t live = s >= s1 || lane >= WORDS ? 0 : s1 - s >= 64 ? ~0ull : (1ull << (s1 - s)) - 1;
+        above = live & ((uint64_t)w.x | (uint64_t)w.y << 32);
+        same = live & ((uint64_t)w.z | (uint64_t)w.w << 32);
+        return live;
+    };
     int equal = 0;
-    for (int s = s0; s < s1; s += 64) equal += __popcll(__ballot(s + lane < s1 && ranks[min(s + lane, s1 - 1)] == prefix));
+    for (int first = 0; first < numbers; first += WORDS) {
+        find_words(first);
+        equal += __builtin_amdgcn_readlane(wave_scan(__popcll(same)), 63);
+    }
     if (lane == 0) s_wave[0][wave] = equal;
     __syncthreads();
-    int ties = 0;
-    for (int w = 0; w < wave; w++) ties += s_wave[0][w];
-    const uint64_t before = (1ull << lane) - 1;
-    for (int write = 0; write < 2; write++) {
-        int seen = ties, holes = 0, fillers = 0;
-        if (write)
-            for (int w = 0; w < wave; w++) { holes += s_wave[1][w]; fillers += s_wave[2][w]; }
-        for (int s = s0; s < s1; s += 64) {
-            const bool live = s + lane < s1;
-            const uint32_t rank = ranks[min(s + lane, s1 - 1)];
-            const uint64_t same = __ballot(live && rank == prefix);
-            const bool stays = rank > prefix || (rank == prefix && seen + __popcll(same & before) < wanted);
-            seen += __popcll(same);
-            const uint64_t hole = __ballot(live && !stays && s + lane < a.keep), filler = __ballot(live && stays && s + lane >= a.keep);
-            if (write) {
-                if ((hole >> lane) & 1) a.holes[(long)unit * a.pairs + holes + __popcll(hole & before)] = s + lane;
-                if ((filler >> lane) & 1) a.fillers[(long)unit * a.pairs + fillers + __popcll(filler & before)] = s + lane;
-            }
-            holes += __popcll(hole);
-            fillers += __popcll(filler);
-        }
-        if (!write) {
-            if (lane == 0) { s_wave[1][wave] = holes; s_wave[2][wave] = fillers; }
-            __syncthreads();
-        } else if (wave == WAVES - 1 && lane == 0) a.counts[unit] = holes;
+    const int ties = before_wave<kEvictWaves>(s_wave[0], wave);
+    // of this lane's words: slots that go before `keep`, slots that stay behind it
+    int seen = ties;
+    uint64_t hole = 0, filler = 0;
+    auto sort_out = [&](int first) INLINE {
+        const uint64_t live = find_words(first);
+        const int count = __popcll(same), scan = wave_scan(count);
+        int left = min(max(wanted - (seen + scan - count), 0), count);      // of the ties: the first so many stay
+        seen += __builtin_amdgcn_readlane(scan, 63);
+        uint64_t stays = above, rest = same;
+        if (left == count) stays |= same;
+        else
+            for (; left > 0; left--) { stays |= rest & -rest; rest &= rest - 1; }
+        const int s = s0 + (first + lane) * 64;
+        const uint64_t low = s >= a.keep ? 0 : a.keep - s >= 64 ? ~0ull : (1ull << (a.keep - s)) - 1;
+        hole = live & ~stays & low;
+        filler = stays & ~low;
+    };
+    int holes = 0, fillers = 0;
+    for (int first = 0; first < numbers; first += WORDS) {
+        sort_out(first);
+        holes += __builtin_amdgcn_readlane(wave_scan(__popcll(hole)), 63);
+        fillers += __builtin_amdgcn_readlane(wave_scan(__popcll(filler)), 63);
     }
+    if (lane == 0) { s_wave[1][wave] = holes; s_wave[2][wave] = fillers; }
+    __syncthreads();
+    holes = before_wave<kEvictWaves>(s_wave[1], wave);
+    fillers = before_wave<kEvictWaves>(s_wave[2], wave);
+    seen = ties;
+    int32_t *to = a.holes + (long)unit * a.pairs, *of = a.fillers + (long)unit * a.pairs;
+    for (int first = 0; first < numbers; first += WORDS) {
+        if (numbers > WORDS) sort_out(first);
+        const int h1 = wave_scan(__popcll(hole)), f1 = wave_scan(__popcll(filler)), h0 = holes + h1 - __popcll(hole), f0 = fillers + f1 - __popcll(filler);
+        auto put = [&](int32_t *list, uint64_t mine, int base, int i, int slot) INLINE {
+            const uint32_t lo = __builtin_amdgcn_readlane((int)mine, i), hi = __builtin_amdgcn_readlane((int)(mine >> 32), i);
+            const unsigned at = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, __builtin_amdgcn_readlane(base, i)));
+            if (__builtin_amdgcn_inverse_ballot_w64((uint64_t)lo | (uint64_t)hi << 32)) list[at] = slot;
+        };
+        for (int i = 0; i < min(numbers - first, WORDS); i++) {
+            const int s = s0 + (first + i) * 64;
+            if (s < a.keep) put(to, hole, h0, i, s + lane);
+            if (s + 64 > a.keep) put(of, filler, f0, i, s + lane);
+        }
+        holes += __builtin_amdgcn_readlane(h1, 63);
+        fillers += __builtin_amdgcn_readlane(f1, 63);
+    }
+    if (wave == kEvictWaves - 1 && lane == 0) a.counts[unit] = holes;
+}
+template <bool PAGED> int launch_rank(const EvictArgs &a, int units, hipStream_t st)
+{
+    const dim3 grid(units), block(kEvictThreads);
+    if (a.slots <= kEvictLds) {
+        constexpr int most = kEvictLds * 4;
+        if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&mem_rank_kernel<true, PAGED>), most, "mem_rank_kernel")) return rc;
+        hipLaunchKernelGGL((mem_rank_kernel<true, PAGED>), grid, block, (unsigned)a.slots * 4, st, a);
+    } else hipLaunchKernelGGL((mem_rank_kernel<false, PAGED>), grid, block, 0, st, a);
+    return d2c_check_launch("mem_rank_kernel");
 }
 
-// What stays behind `keep` into the places of what goes before it: reads and writes meet nowhere.  A thread has one piece of 16 bytes of a key or value and goes
-// from pair to pair, four requested at a time.
-template <typename T> __global__ void __launch_bounds__(256) mem_move_kernel(EvictArgs a, int blocks)
+// What stays behind `keep` into the places of what goes before it: reads and writes meet nowhere.  kMovePairs to a workgroup: a thread to a pair finds both places and
+// moves usage and position, then all of them move pieces of 16 bytes, four requested at a time.
+constexpr int kMovePairs = 64;
+template <typename T> __global__ void __launch_bounds__(256) mem_move_kernel(EvictArgs a, int blocks, FastDiv by_pieces)
 {
     constexpr int VEC = 16 / (int)sizeof(T), AT_ONCE = 4;
-    const int unit = blockIdx.x / blocks, block = blockIdx.x - unit * blocks, n = unit / a.heads, h = unit - n * a.heads, count = a.counts[unit];
-    if (block == 0 && h == 0 && threadIdx.x == 0) a.lengths[n] = min(min(max(a.lengths[n], 0), a.slots), a.keep);
-    const int pieces = (a.D + VEC - 1) / VEC, two = 2 * pieces, per = 256 / two, sub = threadIdx.x / two, part = threadIdx.x - sub * two;
-    if (sub >= per) return;
-    const bool second = part >= pieces;
-    const int d = (second ? part - pieces : part) * VEC;
-    T *base = reinterpret_cast<T *>(second ? a.value : a.key) + h * (second ? a.vs[1] : a.ks[1]) + d;
-    const long ps = second ? a.vs[0] : a.ks[0], ss = second ? a.vs[2] : a.ks[2];
-    const int32_t *table = a.table + n * a.table_stride, *holes = a.holes + (long)unit * a.pairs, *fillers = a.fillers + (long)unit * a.pairs;
-    for (int i = block * per + sub; i < count; i += blocks * per * AT_ONCE) {
-        T *to[AT_ONCE];
-        uint4 x[AT_ONCE];
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; u++) {
-            to[u] = nullptr;
-            if (i + u * blocks * per >= count) continue;
-            const int hole = holes[i + u * blocks * per], filler = fillers[i + u * blocks * per], tp = fdiv(hole, a.page), fp = fdiv(filler, a.page);
-            const int td = table[tp], fd = table[fp], ti = hole - tp * a.page.d, fi = filler - fp * a.page.d;
-            if ((unsigned)td >= (unsigned)a.pages || (unsigned)fd >= (unsigned)a.pages) continue;
-            to[u] = base + td * ps + ti * ss;
-            x[u] = load_run<T>(base + fd * ps + fi * ss, a.D - d);
-            if (part == 0) {
-                const long into = ((long)td * a.heads + h) * a.page.d + ti, of = ((long)fd * a.heads + h) * a.page.d + fi;
-                a.usage[into] = a.usage[of];
-                a.positions[into] = a.positions[of];
+    __shared__ int s_to[kMovePairs][2], s_of[kMovePairs][2];      // page (-1: nowhere) and place
+    const int unit = blockIdx.x / blocks, block = blockIdx.x - unit * blocks, n = unit / a.heads, h = unit - n * a.heads, count = a.counts[unit], tid = threadIdx.x;
+    if (block == 0 && h == 0 && tid == 0) a.lengths[n] = min(min(max(a.lengths[n], 0), a.slots), a.keep);
+    const int32_t *table = a.table + n * a.table_stride;
+    for (int first = block * kMovePairs; first < count; first += blocks * kMovePairs) {
+        const int some = min(kMovePairs, count - first);
+        if (tid < some) {
+            const int hole = a.holes[(long)unit * a.pairs + first + tid], filler = a.fillers[(long)unit * a.pairs + first + tid];
+            const int tp = fdiv(hole, a.page), fp = fdiv(filler, a.page), td = table[tp], fd = table[fp], ti = hole - tp * a.page.d, fi = filler - fp * a.page.d;
+            const bool valid = (unsigned)td < (unsigned)a.pages && (unsigned)fd < (unsigned)a.pages;
+            s_to[tid][0] = valid ? td : -1; s_to[tid][1] = ti;
+            s_of[tid][0] = fd; s_of[tid][1] = fi;
+            if (valid) {
+                const long to = ((long)td * a.heads + h) * a.page.d + ti, of = ((long)fd * a.heads + h) * a.page.d + fi;
+                a.usage[to] = a.usage[of];
+                a.positions[to] = a.positions[of];
             }
         }
+        __syncthreads();
+        const int pieces = by_pieces.d, all = some * pieces;      // (of keys; the same again of values)
+        for (int i0 = tid; i0 < 2 * all; i0 += 256 * AT_ONCE) {
+            T *to[AT_ONCE];
+            uint4 x[AT_ONCE];
+            int left[AT_ONCE];
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; u++)
-            if (to[u]) store_run<T>(to[u], x[u], a.D - d);
+            for (int u = 0; u < AT_ONCE; u++) {
+                to[u] = nullptr;
+                int i = i0 + u * 256;
+                if (i >= 2 * all) continue;
+                const bool second = i >= all;
+                if (second) i -= all;
+                const int pair = fdiv(i, by_pieces), d = (i - pair * pieces) * VEC, page = s_to[pair][0];
+                if (page < 0) continue;
+                T *base = reinterpret_cast<T *>(second ? a.value : a.key) + h * (second ? a.vs[1] : a.ks[1]) + d;
+                const long ps = second ? a.vs[0] : a.ks[0], ss = second ? a.vs[2] : a.ks[2];
+                left[u] = a.D - d;
+                to[u] = base + page * ps + s_to[pair][1] * ss;
+                x[u] = load_run<T>(base + s_of[pair][0] * ps + s_of[pair][1] * ss, left[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++)
+                if (to[u]) store_run<T>(to[u], x[u], left[u]);
+        }
+        __syncthreads();
     }
 }
 
@@ -689,7 +899,7 @@ MemPlan mem_plan(const d2c_memory_desc &q, const d2c_memory_query_desc &x, bool 
     p.places = 2 * std::max(d2c_num_cus(), 1);
     p.least = 2;
     p.slots_padded = (slots + 63) / 64 * 64;
-    if (track) p.scores_bytes = d2c_align_up((size_t)q.streams * x.query_heads * p.slots_padded * 4);
+    if (track) p.scores_bytes = d2c_align_up((size_t)p.units * p.rows * p.slots_padded * 4);
     if (!p.one) {
         const size_t lines = ((size_t)p.units + p.places) * p.rows;
         p.part_bytes = d2c_align_up(lines * part_width(q.D) * 4);
@@ -710,7 +920,7 @@ EvictPlan evict_plan(const d2c_memory_desc &q, int keep)
     if (slots <= keep || units == 0) return p;
     p.pairs = (int)std::min((long)keep, slots - keep);
     p.slots_padded = (slots + 63) / 64 * 64;
-    p.ranks_bytes = d2c_align_up(units * p.slots_padded * 4);
+    p.ranks_bytes = slots <= kEvictLds ? 0 : d2c_align_up(units * p.slots_padded * 4);
     p.list_bytes = d2c_align_up(units * p.pairs * 4);
     p.bytes = p.ranks_bytes + 2 * p.list_bytes + d2c_align_up(units * 4);
     return p;
@@ -723,7 +933,7 @@ extern "C" int d2c_memory_append(const d2c_memory_desc *q, void *key, void *valu
                                  const int64_t new_value_stride[2], const int32_t *starts, int64_t tokens, void *stream)
 {
     if (int rc = check(q)) return rc;
-    if (tokens < 0 || tokens * q->heads >= (1L << 31) || (!starts && tokens != q->streams)) { d2c_set_error("memory_append: %ld tokens for %d streams", (long)tokens, q->streams); return D2C_ERR_SHAPE; }
+    if (tokens < 0 || tokens >= (1L << 26) || (!starts && tokens != q->streams)) { d2c_set_error("memory_append: %ld tokens for %d streams", (long)tokens, q->streams); return D2C_ERR_SHAPE; }
     if (q->streams == 0) return D2C_OK;
     if (!lengths || !seen || (q->per_stream > 0 && !table) || (q->pages > 0 && (!key || !value || !usage || !positions)) || (tokens > 0 && (!new_key || !new_value))) {
         d2c_set_error("null tensor pointer");
@@ -744,10 +954,10 @@ extern "C" int d2c_memory_append(const d2c_memory_desc *q, void *key, void *valu
         return d2c_check_launch("mem_append_one_kernel");
     }
     if (tokens > 0) {
-        const long per = 256 / (2 * ((a.D * (half ? 2 : 4) + 15) / 16));
-        const unsigned blocks = (unsigned)std::min((tokens * a.heads + per - 1) / per, 1L << 20);
-        if (half) hipLaunchKernelGGL(mem_append_kernel<bf16_t>, dim3(blocks), dim3(256), 0, st, a, make_fastdiv(a.heads));
-        else hipLaunchKernelGGL(mem_append_kernel<float>, dim3(blocks), dim3(256), 0, st, a, make_fastdiv(a.heads));
+        const dim3 blocks((unsigned)((tokens + kAppendTokens - 1) / kAppendTokens));
+        const FastDiv pieces = make_fastdiv((a.D * (half ? 2 : 4) + 15) / 16);
+        if (half) hipLaunchKernelGGL(mem_append_kernel<bf16_t>, blocks, dim3(256), 0, st, a, pieces);
+        else hipLaunchKernelGGL(mem_append_kernel<float>, blocks, dim3(256), 0, st, a, pieces);
         if (int rc = d2c_check_launch("mem_append_kernel")) return rc;
     }
     hipLaunchKernelGGL(mem_count_kernel, dim3((a.N + 255) / 256), dim3(256), 0, st, a);
@@ -799,7 +1009,7 @@ extern "C" int d2c_memory_attention(const d2c_memory_desc *q, const d2c_memory_q
         if (rc || p.one) return rc;
         constexpr int JOIN = LANES * 16 / (int)sizeof(T) / 4;      // lanes of four columns
         const int rows = q->streams * x->query_heads;
-        hipLaunchKernelGGL((mem_join_kernel<T, JOIN, R>), dim3(rows + (usage ? p.places : 0)), dim3(256), 0, st, a, rows, p.step);
+        hipLaunchKernelGGL((mem_join_kernel<T, JOIN, R>), dim3(rows + (usage ? p.places * kUsageBlocks : 0)), dim3(256), 0, st, a, rows, p.step);
         return d2c_check_launch("mem_join_kernel");
     });
 }
@@ -828,11 +1038,10 @@ extern "C" int d2c_memory_evict(const d2c_memory_desc *q, void *key, void *value
     a.N = q->streams; a.heads = q->heads; a.D = q->D; a.pages = q->pages; a.slots = q->per_stream * q->page; a.keep = keep; a.recent = recent; a.pairs = p.pairs;
     hipStream_t st = (hipStream_t)stream;
     const int units = a.N * a.heads, vec = q->dtype == D2C_BF16 ? 8 : 4;
-    hipLaunchKernelGGL(mem_rank_kernel, dim3(units), dim3(kEvictThreads), 0, st, a);
-    if (int rc = d2c_check_launch("mem_rank_kernel")) return rc;
-    const int per = 256 / (2 * ((a.D + vec - 1) / vec));
-    const int blocks = (int)std::max(std::min((a.pairs + per * 4L - 1) / (per * 4L), (1L << 22) / units), 1L);
-    if (q->dtype == D2C_BF16) hipLaunchKernelGGL(mem_move_kernel<bf16_t>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks);
-    else hipLaunchKernelGGL(mem_move_kernel<float>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks);
+    if (int rc = q->page % 64 == 0 ? launch_rank<true>(a, units, st) : launch_rank<false>(a, units, st)) return rc;
+    const int blocks = (int)std::max(std::min((a.pairs + kMovePairs - 1L) / kMovePairs, (1L << 22) / units), 1L);
+    const FastDiv pieces = make_fastdiv((a.D + vec - 1) / vec);
+    if (q->dtype == D2C_BF16) hipLaunchKernelGGL(mem_move_kernel<bf16_t>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks, pieces);
+    else hipLaunchKernelGGL(mem_move_kernel<float>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks, pieces);
     return d2c_check_launch("mem_move_kernel");
 }

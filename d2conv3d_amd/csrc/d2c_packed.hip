@@ -35,9 +35,10 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
     const int lim = live ? limit_of_row(a, u, row) : 0, least = limit_of_row(a, u, row0);
     const int wave_row = row0 + wave * 32, wave_least = wave_row < u.rows ? limit_of_row(a, u, wave_row) : 0;
     const int wave_most = wave_row < u.rows ? limit_of_row(a, u, min(wave_row + 31, u.rows - 1)) : 0;
-    const int tiles = (limit_of_row(a, u, min(row0 + kRows, u.rows) - 1) + KT - 1) / KT;
-    const int t1 = (int)((long)tiles * (u.split + 1) / a.splits);
-    const int t0 = (int)((long)tiles * u.split / a.splits);
+    const Walk walk = row_walk(a, u);
+    if (u.split >= walk.splits) return;
+    const int t1 = (int)((long)walk.steps * (u.split + 1) / walk.splits);
+    const int t0 = (int)((long)walk.steps * u.split / walk.splits);
     int t = t0;
 
     KV k, v;
@@ -145,7 +146,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
     l = half_sum(l);
     const float mc = m == -INFINITY ? -INFINITY : m * c;
     if (!live) return;
-    if (a.splits > 1) {
+    if (walk.splits > 1) {
         const long at = (((long)u.split * a.tiles + u.at) * a.Hkv + u.h) * kRows + tile_row;
         float *po = a.part + at * part_width(a.D);
 #pragma unroll
@@ -179,25 +180,26 @@ template <typename T> __global__ void __launch_bounds__(256) packed_join_kernel(
 {
     const PackedUnit u = unit_of<false>(a, blockIdx.x / 8);
     const int tile_row = blockIdx.x % 8 * 16 + threadIdx.x / 16, row = u.tile * kRows + tile_row;
-    if (row >= u.rows) return;
+    const int splits = row_walk(a, u).splits;
+    if (row >= u.rows || splits == 1) return;
     const long step = (long)a.tiles * a.Hkv * kRows, first = ((long)u.at * a.Hkv + u.h) * kRows + tile_row;
     const int width = part_width(a.D);
     T *orow = const_cast<T *>(row_at<T>(a.out, a.gs, a, u, row));
     for (int d = threadIdx.x % 16 * 4; d < a.D; d += 64) {
         float all = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < a.splits; s0 += 4) {
+        for (int s0 = 0; s0 < splits; s0 += 4) {
             float2 ml[4];
             float4 y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const long at = first + min(s0 + i, a.splits - 1) * step;
+                const long at = first + min(s0 + i, splits - 1) * step;
                 ml[i] = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
                 y[i] = *reinterpret_cast<const float4 *>(a.part + at * width + d);
             }
             float top = all;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (s0 + i >= a.splits) ml[i] = make_float2(-INFINITY, 0.f);
+                if (s0 + i >= splits) ml[i] = make_float2(-INFINITY, 0.f);
                 top = fmaxf(top, ml[i].x);
             }
             const float base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(all - base);
@@ -207,7 +209,7 @@ template <typename T> __global__ void __launch_bounds__(256) packed_join_kernel(
             for (int i = 0; i < 4; i++) x[i] *= f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (s0 + i >= a.splits) continue;
+                if (s0 + i >= splits) continue;
                 const float g = __builtin_amdgcn_exp2f(ml[i].x - base);
                 l = fmaf(ml[i].y, g, l);
                 x[0] = fmaf(y[i].x, g, x[0]); x[1] = fmaf(y[i].y, g, x[1]); x[2] = fmaf(y[i].z, g, x[2]); x[3] = fmaf(y[i].w, g, x[3]);
@@ -222,7 +224,7 @@ template <typename T> __global__ void __launch_bounds__(256) packed_join_kernel(
     }
 }
 
-struct FwdPlan { int tiles, splits; size_t part_bytes, bytes; };
+struct FwdPlan { int tiles; Split split; size_t part_bytes, bytes; };
 template <typename T> FwdPlan fwd_plan(const d2c_packed_attention_desc &q)
 {
     FwdPlan p{};
@@ -232,12 +234,12 @@ template <typename T> FwdPlan fwd_plan(const d2c_packed_attention_desc &q)
         constexpr int DP = decltype(width)::DP, NP = decltype(width)::NP;
         constexpr bool WHOLE = decltype(whole)::value;
         using Shape = FwdShape<T, DP, WHOLE>;
-        p.splits = splits_of((long)p.tiles * q.Hkv, cus * resident(reinterpret_cast<const void *>(&packed_fwd_kernel<T, DP, NP, WHOLE>), Shape::LDS),
-                             q.sequences > 0 ? q.keys / q.sequences : 0, Shape::KT, 8, kRows * (part_width(q.D) * 4.0 + 8));
+        p.split = split_walks(q, (long)p.tiles * q.Hkv, cus * resident(reinterpret_cast<const void *>(&packed_fwd_kernel<T, DP, NP, WHOLE>), Shape::LDS), q.keys, Shape::KT,
+                              kRows * (part_width(q.D) * 4.0 + 8));
         return 0;
     });
-    if (p.splits > 1) {
-        const size_t lines = (size_t)p.splits * p.tiles * q.Hkv * kRows;
+    if (p.split.splits > 1) {
+        const size_t lines = (size_t)p.split.splits * p.tiles * q.Hkv * kRows;
         p.part_bytes = d2c_align_up(lines * part_width(q.D) * 4);
         p.bytes = p.part_bytes + d2c_align_up(lines * 8);
     }
@@ -250,17 +252,17 @@ template <typename T> int forward(PackedArgs a, const d2c_packed_attention_desc 
         d2c_set_error("workspace of %zu bytes (256-byte aligned) required, got %zu at %p", p.bytes, ws_bytes, ws);
         return D2C_ERR_WORKSPACE;
     }
-    a.tiles = p.tiles; a.splits = p.splits;
+    a.tiles = p.tiles; a.splits = p.split.splits; a.chunk = p.split.chunk; a.step = sizeof(T) == 2 ? 64 : 32;
     a.part = (float *)ws; a.part_ml = (float *)((char *)ws + p.part_bytes);
     const int rc = pick_width(q.D, fast_kernels(q), [&](auto width, auto whole) {
         constexpr int DP = decltype(width)::DP, NP = decltype(width)::NP;
         constexpr bool WHOLE = decltype(whole)::value;
         constexpr int lds = FwdShape<T, DP, WHOLE>::LDS;
         if (int e = d2c_allow_lds(reinterpret_cast<const void *>(&packed_fwd_kernel<T, DP, NP, WHOLE>), lds, "packed_fwd_kernel")) return e;
-        hipLaunchKernelGGL((packed_fwd_kernel<T, DP, NP, WHOLE>), dim3((unsigned)(p.tiles * q.Hkv * p.splits)), dim3(256), lds, st, a);
+        hipLaunchKernelGGL((packed_fwd_kernel<T, DP, NP, WHOLE>), dim3((unsigned)(p.tiles * q.Hkv * p.split.splits)), dim3(256), lds, st, a);
         return d2c_check_launch("packed_fwd_kernel");
     });
-    if (rc || p.splits == 1) return rc;
+    if (rc || p.split.splits == 1) return rc;
     hipLaunchKernelGGL(packed_join_kernel<T>, dim3((unsigned)(p.tiles * q.Hkv * 8)), dim3(256), 0, st, a);
     return d2c_check_launch("packed_join_kernel");
 }

@@ -17,7 +17,8 @@ struct PackedArgs {
     float *lse, *delta;                     // [Hkv][T * group]
     float *part, *part_ml;                  // [splits][tiles][Hkv][128][part_width(D)] (keys' kernel: twice), and (forward) [..][2]
     long qs[2], ks[2], vs[2], gs[2];        // strides of token, head
-    int T, Tk, S, Hq, Hkv, group, D, tiles, splits, causal;
+    int T, Tk, S, Hq, Hkv, group, D, tiles, causal;
+    int splits, chunk, step;                // see Walk; step: keys (rows) of a step
     FastDiv by_group, frame;
     float scale, scale2;
 };
@@ -217,12 +218,34 @@ inline bool fast_kernels(const d2c_packed_attention_desc &q)
 }
 inline int tiles_of(long rows, int sequences) { return (int)(rows / kRows) + sequences + 2; }
 
-// How many workgroups share the walk of a tile: as many as fill the GPU's places where tiles are few, of `steps` steps each or more on the average
-inline int splits_of(long units, long places, long walk, long step, long steps, double unit_bytes)
+// The steps of a unit's walk, and how many workgroups share it: as many as make pieces of `chunk` steps, `splits` at most.  Long walks beside short ones (a sequence's last
+// rows beside its first, its first keys beside its last) would be what the GPU waits for in the end.
+struct Walk { int first, steps, splits; };
+D2C_DEV Walk walk_of(const PackedArgs &a, int first, int steps) { return {first, steps, min(max((steps + a.chunk - 1) / a.chunk, 1), a.splits)}; }
+// ... of rows: keys up to the last that the last of them reads
+D2C_DEV Walk row_walk(const PackedArgs &a, const PackedUnit &u)
 {
-    long s = std::max(std::min({places / std::max(units, 1L), walk / (step * steps), 16L}), 1L);
+    const int row0 = u.tile * kRows;
+    return walk_of(a, 0, row0 < u.rows ? (limit_of_row(a, u, min(row0 + kRows, u.rows) - 1) + a.step - 1) / a.step : 0);
+}
+// ... of keys: rows from the first that reads the first of them
+D2C_DEV Walk key_walk(const PackedArgs &a, const PackedUnit &u)
+{
+    const int key0 = u.tile * kRows, first = a.causal ? max(fdiv(key0, a.frame) * a.frame.d - (u.lk - u.lq), 0) * a.group / a.step : 0;
+    return walk_of(a, first, max((u.rows + a.step - 1) / a.step - first, 0));
+}
+// On the host, where only the average length is known: the longest walk is taken to be twice that of a sequence of the average length, or that of the only sequence
+struct Split { int splits, chunk; };
+inline Split split_walks(const d2c_packed_attention_desc &q, long units, long places, long along, long step, double unit_bytes)
+{
+    const long sequences = std::max(q.sequences, 1), average = along / sequences / step + 1, longest = sequences == 1 ? average : 2 * average;
+    const double each = (double)units * (double)average * (q.causal ? 0.5 : 1.0) / (double)places;      // steps that every place gets
+    if ((double)longest <= 1.25 * each) return {1, 1 << 30};
+    // (pieces of 4 steps where all of them have a place at once, else of 8)
+    const long chunk = std::max((long)(each * 0.3), units * (longest / 4 + 1) * (q.causal ? 1 : 2) <= 2 * places ? 4L : 8L);
+    long s = std::min((longest + chunk - 1) / chunk, 16L);
     while (s > 1 && (double)s * (double)units * unit_bytes > (double)D2C_ATTENTION_PART_BYTES) s--;
-    return (int)s;
+    return {(int)s, s > 1 ? (int)chunk : 1 << 30};
 }
 
 }  // namespace d2c_packed

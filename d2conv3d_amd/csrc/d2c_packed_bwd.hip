@@ -36,9 +36,10 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
     const int lim = live ? limit_of_row(a, u, row) : 0, least = limit_of_row(a, u, row0);
     const int wave_row = row0 + wave * 32, wave_least = wave_row < u.rows ? limit_of_row(a, u, wave_row) : 0;
     const int wave_most = wave_row < u.rows ? limit_of_row(a, u, min(wave_row + 31, u.rows - 1)) : 0;
-    const int tiles = (limit_of_row(a, u, min(row0 + kRows, u.rows) - 1) + KT - 1) / KT;
-    const int t1 = (int)((long)tiles * (u.split + 1) / a.splits);
-    const int t0 = (int)((long)tiles * u.split / a.splits);
+    const Walk walk = row_walk(a, u);
+    if (u.split >= walk.splits) return;
+    const int t1 = (int)((long)walk.steps * (u.split + 1) / walk.splits);
+    const int t0 = (int)((long)walk.steps * u.split / walk.splits);
     int t = t0;
 
     KV k, v;
@@ -135,7 +136,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
         take_in<T, true>(dq, a.D, max(least / KT, t0) * KT, min(t1 * KT, wave_most), [&](int j) INLINE { return source.kb + (long)j * source.ks; },
                          [&](int j) INLINE { return j < lim; });
     if (!live) return;
-    if (a.splits > 1) {
+    if (walk.splits > 1) {
         float *p = a.part + ((((long)u.split * a.tiles + u.at) * a.Hkv + u.h) * kRows + tile_row) * part_width(a.D);
 #pragma unroll
         for (int i = 0; i < ND; i++)
@@ -185,11 +186,10 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
     if (key0 >= u.lk) return;
     const int tile_key = wave * 32 + (lane & 31), key = key0 + tile_key, keys_end = min(key0 + kRows, u.lk);
     const bool live = key < u.lk;
-    // the first row that reads the tile's first key, and the tiles of rows from its own on
-    const int first = a.causal ? max(fdiv(key0, a.frame) * a.frame.d - (u.lk - u.lq), 0) * a.group : 0;
-    const int tile0 = first / RT, tiles = max((u.rows + RT - 1) / RT - tile0, 0);
-    const int t1 = tile0 + (int)((long)tiles * (u.split + 1) / a.splits);
-    const int t0 = tile0 + (int)((long)tiles * u.split / a.splits);
+    const Walk walk = key_walk(a, u);
+    if (u.split >= walk.splits) return;
+    const int t1 = walk.first + (int)((long)walk.steps * (u.split + 1) / walk.splits);
+    const int t0 = walk.first + (int)((long)walk.steps * u.split / walk.splits);
     int t = t0;
 
     QG q, g;
@@ -358,7 +358,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
         take_in<T, true>(dk, a.D, first_row, end, [&](int j) INLINE { return row_at<T>(a.q, a.qs, a, u, j); }, read);
     }
     if (!live) return;
-    const float fk = a.splits > 1 ? 1.f : a.scale;
+    const float fk = walk.splits > 1 ? 1.f : a.scale;
 #pragma unroll
     for (int i = 0; i < ND; i++)
 #pragma unroll
@@ -366,7 +366,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
             const int d = i * 32 + j * 8 + half * 4;
             const float x[4] = {dk[i][j * 4] * fk, dk[i][j * 4 + 1] * fk, dk[i][j * 4 + 2] * fk, dk[i][j * 4 + 3] * fk};
             const float y[4] = {dv[i][j * 4], dv[i][j * 4 + 1], dv[i][j * 4 + 2], dv[i][j * 4 + 3]};
-            if (a.splits > 1) {
+            if (walk.splits > 1) {
                 const long step = (long)a.tiles * a.Hkv * kRows, line = ((long)u.at * a.Hkv + u.h) * kRows + tile_key;
                 store4<float>(a.part + (2L * u.split * step + line) * part_width(a.D) + d, x, a.D - d);
                 store4<float>(a.part + ((2L * u.split + 1) * step + line) * part_width(a.D) + d, y, a.D - d);
@@ -383,7 +383,8 @@ template <typename T, bool KV> __global__ void __launch_bounds__(256) packed_bwd
 {
     const PackedUnit u = unit_of<KV>(a, blockIdx.x / 8);
     const int line = blockIdx.x % 8 * 16 + threadIdx.x / 16, at = u.tile * kRows + line, which = KV ? blockIdx.y : 0;
-    if (at >= (KV ? u.lk : u.rows) || (KV && !(which ? a.gv : a.gk))) return;
+    const int splits = (KV ? key_walk(a, u) : row_walk(a, u)).splits;
+    if (splits == 1 || at >= (KV ? u.lk : u.rows) || (KV && !(which ? a.gv : a.gk))) return;
     const long step = (long)a.tiles * a.Hkv * kRows, first = ((long)u.at * a.Hkv + u.h) * kRows + line;
     const int width = part_width(a.D);
     T *to;
@@ -392,14 +393,14 @@ template <typename T, bool KV> __global__ void __launch_bounds__(256) packed_bwd
     const float f = which == 0 ? a.scale : 1.f;
     for (int d = threadIdx.x % 16 * 4; d < a.D; d += 64) {
         float x[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < a.splits; s0 += 4) {
+        for (int s0 = 0; s0 < splits; s0 += 4) {
             float4 y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                y[i] = *reinterpret_cast<const float4 *>(a.part + (((long)min(s0 + i, a.splits - 1) * (KV ? 2 : 1) + which) * step + first) * width + d);
+                y[i] = *reinterpret_cast<const float4 *>(a.part + (((long)min(s0 + i, splits - 1) * (KV ? 2 : 1) + which) * step + first) * width + d);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (s0 + i >= a.splits) continue;
+                if (s0 + i >= splits) continue;
                 x[0] += y[i].x; x[1] += y[i].y; x[2] += y[i].z; x[3] += y[i].w;
             }
         }
@@ -427,11 +428,11 @@ template <typename T> __global__ void __launch_bounds__(256) packed_delta_kernel
     }
 }
 
-struct BwdPlan { int q_tiles, q_splits, kv_tiles, kv_splits; size_t delta_bytes, bytes; };
+struct BwdPlan { int q_tiles, kv_tiles; Split q, kv; size_t delta_bytes, bytes; };
 template <typename T> BwdPlan bwd_plan(const d2c_packed_attention_desc &q)
 {
     BwdPlan p{};
-    const long group = q.Hq / q.Hkv, rows = q.queries * group, cus = std::max(d2c_num_cus(), 1), sequences = std::max(q.sequences, 1);
+    const long group = q.Hq / q.Hkv, rows = q.queries * group, cus = std::max(d2c_num_cus(), 1);
     p.q_tiles = tiles_of(rows, q.sequences);
     p.kv_tiles = tiles_of(q.keys, q.sequences);
     const double unit = kRows * (part_width(q.D) * 4.0);
@@ -440,13 +441,12 @@ template <typename T> BwdPlan bwd_plan(const d2c_packed_attention_desc &q)
         constexpr bool WHOLE = decltype(whole)::value;
         using Q = QShape<T, DP, WHOLE>;
         using KV = KvShape<T, DP, WHOLE>;
-        p.q_splits = splits_of((long)p.q_tiles * q.Hkv, cus * resident(reinterpret_cast<const void *>(&packed_bwd_q_kernel<T, DP, NP, WHOLE>), Q::LDS), q.keys / sequences, Q::KT, 8, unit);
-        p.kv_splits = splits_of((long)p.kv_tiles * q.Hkv, cus * resident(reinterpret_cast<const void *>(&packed_bwd_kv_kernel<T, DP, NP, WHOLE>), KV::LDS), rows / sequences, KV::RT, 8,
-                                2 * unit);
+        p.q = split_walks(q, (long)p.q_tiles * q.Hkv, cus * resident(reinterpret_cast<const void *>(&packed_bwd_q_kernel<T, DP, NP, WHOLE>), Q::LDS), q.keys, Q::KT, unit);
+        p.kv = split_walks(q, (long)p.kv_tiles * q.Hkv, cus * resident(reinterpret_cast<const void *>(&packed_bwd_kv_kernel<T, DP, NP, WHOLE>), KV::LDS), rows, KV::RT, 2 * unit);
         return 0;
     });
     p.delta_bytes = d2c_align_up((size_t)rows * q.Hkv * 4);
-    const size_t q_part = p.q_splits > 1 ? (size_t)p.q_splits * p.q_tiles * q.Hkv * (size_t)unit : 0, kv_part = p.kv_splits > 1 ? 2 * (size_t)p.kv_splits * p.kv_tiles * q.Hkv * (size_t)unit : 0;
+    const size_t q_part = p.q.splits > 1 ? (size_t)p.q.splits * p.q_tiles * q.Hkv * (size_t)unit : 0, kv_part = p.kv.splits > 1 ? 2 * (size_t)p.kv.splits * p.kv_tiles * q.Hkv * (size_t)unit : 0;
     p.bytes = p.delta_bytes + d2c_align_up(std::max(q_part, kv_part));
     return p;
 }
@@ -459,7 +459,7 @@ template <typename T, int DP, int NP, bool WHOLE> int launch_bwd(PackedArgs a, c
     } else if (a.T > 0 && a.gq) {
         constexpr int lds = QShape<T, DP, WHOLE>::LDS;
         if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&packed_bwd_q_kernel<T, DP, NP, WHOLE>), lds, "packed_bwd_q_kernel")) return rc;
-        a.tiles = p.q_tiles; a.splits = p.q_splits;
+        a.tiles = p.q_tiles; a.splits = p.q.splits; a.chunk = p.q.chunk; a.step = QShape<T, DP, WHOLE>::KT;
         hipLaunchKernelGGL((packed_bwd_q_kernel<T, DP, NP, WHOLE>), dim3((unsigned)(a.tiles * a.Hkv * a.splits)), dim3(256), lds, st, a);
         if (int rc = d2c_check_launch("packed_bwd_q_kernel")) return rc;
         if (a.splits > 1) {
@@ -470,7 +470,7 @@ template <typename T, int DP, int NP, bool WHOLE> int launch_bwd(PackedArgs a, c
     if (a.Tk == 0 || !(a.gk || a.gv)) return D2C_OK;
     constexpr int lds = KvShape<T, DP, WHOLE>::LDS;
     if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&packed_bwd_kv_kernel<T, DP, NP, WHOLE>), lds, "packed_bwd_kv_kernel")) return rc;
-    a.tiles = p.kv_tiles; a.splits = p.kv_splits;
+    a.tiles = p.kv_tiles; a.splits = p.kv.splits; a.chunk = p.kv.chunk; a.step = KvShape<T, DP, WHOLE>::RT;
     hipLaunchKernelGGL((packed_bwd_kv_kernel<T, DP, NP, WHOLE>), dim3((unsigned)(a.tiles * a.Hkv * a.splits)), dim3(256), lds, st, a);
     if (int rc = d2c_check_launch("packed_bwd_kv_kernel")) return rc;
     if (a.splits == 1) return D2C_OK;

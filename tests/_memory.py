@@ -22,12 +22,10 @@ def make(lengths, page, heads, D, dtype, seed=0, per=None, garbage=math.nan):
     there = torch.zeros(pages, heads, page, dtype=torch.bool)
     for i, length in enumerate(lengths):
         length = min(max(length, 0), per * page)
-        for h in range(heads):
-            order = (torch.randperm(length, generator=gen) + 5).int()
-            for s in range(length):
-                m["positions"][m["table"][i, s // page], h, s % page] = order[s]
-        for s in range(length):
-            there[m["table"][i, s // page], :, s % page] = True
+        slot = torch.arange(length)
+        at = m["table"][i].long()[slot // page], slice(None), slot % page
+        m["positions"][at] = torch.stack([(torch.randperm(length, generator=gen) + 5).int() for _ in range(heads)], 1)
+        there[at] = True
     m["key"][~there], m["value"][~there] = garbage, garbage
     m["usage"][~there], m["positions"][~there] = 1e30, 2 ** 31 - 1
     return m
@@ -100,14 +98,15 @@ def evict(m, keep, recent):
             continue
         m["lengths"][n] = keep
         for h in range(m["key"].shape[1]):
+            page, place = (torch.tensor([0 if x is None else x[i] for x in at]) for i in (0, 1))
+            usage, newest = old["usage"][page, h, place].tolist(), (old["positions"][page, h, place] >= int(old["seen"][n]) - recent).tolist()
+
             def rank(s):      # sorts as what stays first does
                 if at[s] is None:
                     return (3, 0.0, s)
-                page, place = at[s]
-                use = float(old["usage"][page, h, place])
-                if int(old["positions"][page, h, place]) >= int(old["seen"][n]) - recent:
+                if newest[s]:
                     return (0, 0.0, s)
-                return (1, 0.0, s) if math.isnan(use) else (2, -use, s)
+                return (1, 0.0, s) if math.isnan(usage[s]) else (2, -usage[s], s)
             stays = set(sorted(range(len(at)), key=rank)[:keep])
             holes = [s for s in range(keep) if s not in stays]
             fillers = [s for s in range(keep, len(at)) if s in stays]

@@ -173,7 +173,8 @@ def test_starts_that_do_not_rise(dev):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lengths,page,heads,D,keep,recent", [
     ([40], 16, 1, 64, 39, 0), ([40], 16, 1, 64, 1, 1), ([40], 16, 2, 64, 20, 20), ([100, 20, 0, 64, 33], 16, 3, 40, 33, 5), ([200, 300], 50, 2, 24, 150, 149),
-    ([2500, 64], 64, 2, 32, 1300, 200), ([4100], 128, 1, 128, 64, 0), ([1025, 1024, 1026], 8, 1, 7, 1024, 100)])
+    ([2500, 64], 64, 2, 32, 1300, 200), ([4100], 128, 1, 128, 64, 0), ([1025, 1024, 1026], 8, 1, 7, 1024, 100),
+    ([9000, 8192, 100], 64, 1, 8, 4000, 4000), ([20000], 50, 1, 8, 15000, 1), ([33000, 32769], 64, 1, 8, 20000, 3000), ([70001], 16, 1, 8, 66000, 100)])
 def test_evict(lengths, page, heads, D, keep, recent, dtype, dev):
     m = make(lengths, page, heads, D, dtype, seed=keep)
     memory = on(dev, m)
