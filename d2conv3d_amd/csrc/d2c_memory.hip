@@ -17,10 +17,10 @@ struct MemArgs {
     float *part, *part_ml;        // [units + places][R][part_width(D)], and (maximum, sum) of each row
     int32_t *covered;             // [units][2]: the first and the last workgroup that has a piece of the unit
     int32_t *begins;              // [places][4]: unit and step that a workgroup begins with, its steps
-    float *scores;                // [units][slots][R], of base 2
+    float *scores;                // [units][slots][score_rows], of base 2
     long qs[2], ks[3], vs[3], table_stride, slots_padded;
     FastDiv page;
-    int N, heads, group, D, pages, slots, row_groups, units, places, least;
+    int N, heads, group, D, pages, slots, row_groups, units, places, least, score_rows;
     float scale2;
 };
 
@@ -96,10 +96,11 @@ template <int R> D2C_DEV void add_usage(const MemArgs &a, int unit, int n, int h
         float x = 0.f;
         for (int g = 0; g < a.row_groups; g++) {
             float score[R];
-            const float *from = a.scores + ((long)(unit + g) * a.slots_padded + s) * R;
+            const float *from = a.scores + ((long)(unit + g) * a.slots_padded + s) * a.score_rows;
             if constexpr (R % 4 == 0) {
 #pragma unroll
-                for (int r = 0; r < R; r += 4) *reinterpret_cast<float4 *>(score + r) = *reinterpret_cast<const float4 *>(from + r);
+                for (int r = 0; r < R; r += 4)
+                    if (r < a.score_rows && g * R + r < a.group) *reinterpret_cast<float4 *>(score + r) = *reinterpret_cast<const float4 *>(from + r);
             } else {
 #pragma unroll
                 for (int r = 0; r < R; r++) score[r] = from[r];
@@ -125,8 +126,11 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
     __shared__ __align__(16) float s_o[4][R][DP];
     __shared__ float2 s_ml[4][R];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = lane % LANES * VEC;
-    int unit = blockIdx.x, t = 0, budget = 1 << 30;
-    if constexpr (!ONE) {
+    // (ONE: with weights to add up, all groups of a key head's rows one after the other)
+    __shared__ float2 s_row[ONE ? 256 : 1];
+    int unit = ONE && a.usage ? blockIdx.x * a.row_groups : blockIdx.x, t = 0, budget = 1 << 30, units = a.units;
+    if constexpr (ONE) units = min(units, unit + (a.usage ? a.row_groups : 1));
+    else {
         const bool some = find_begin<STEP>(a, unit, t, budget);
         if (threadIdx.x < 4) a.begins[blockIdx.x * 4 + threadIdx.x] = threadIdx.x == 0 ? (some ? unit : -1) : threadIdx.x == 1 ? t : budget;
         if (!some) return;
@@ -137,7 +141,7 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
             return make_uint4(v[0], v[1], v[2], v[3]);
         } else return d0 < a.D ? load_run<T>(row + d0, a.D - d0) : make_uint4(0, 0, 0, 0);
     };
-    for (; budget > 0 && unit < a.units; unit++, t = 0) {
+    for (; budget > 0 && unit < units; unit++, t = 0) {
         const int nh = unit / a.row_groups, row0 = (unit - nh * a.row_groups) * R, n = nh / a.heads, h = nh - n * a.heads;
         const int rows = min(R, a.group - row0), slots = slots_of(a, n), steps = max(1, (slots + STEP - 1) / STEP);
         const int t0 = t, t1 = ONE ? steps : min(steps, t + budget);
@@ -309,8 +313,7 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
             if (t1 == steps) a.covered[unit * 2 + 1] = blockIdx.x;
         }
         if constexpr (ONE) {
-            if (a.usage) {      // (one group of rows)
-                __shared__ float2 s_row[R];
+            if (a.usage) {
                 if ((int)threadIdx.x < rows) {
                     const int r = threadIdx.x;
                     float top = s_ml[0][r].x, sum = 0.f;
@@ -319,14 +322,188 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
                     const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
                     for (int w = 0; w < 4; w++) sum = fmaf(s_ml[w][r].y, __builtin_amdgcn_exp2f(s_ml[w][r].x - base), sum);
-                    s_row[r] = usage_ml(top, sum);
+                    s_row[row0 + r] = usage_ml(top, sum);
                 }
                 __syncthreads();
-                add_usage<R>(a, unit, n, h, 0, slots, s_row);
+                if (unit + 1 == units) add_usage<R>(a, unit + 1 - a.row_groups, n, h, 0, slots, s_row);
             }
-            return;
         }
         __syncthreads();      // (s_o and s_ml are written again by the next unit's piece)
+    }
+}
+
+// More than four rows of a key head, bfloat16: their products on the matrix instruction, whose columns are the rows (R of them, up to 32).  A wavefront has 32 slots of a step to
+// itself: a lane asks for a slot's key and value (its half of every 16 channels), keys are the instruction's operand as they come, values go through a tile of the wavefront's own in LDS
+// and are read back by columns.  No barrier until the end of a unit's piece, where the four wavefronts' sums meet.  Weights are two terms, which cost little here.
+// Bound: memory.
+constexpr int kWideStep = 128;
+template <int DP, bool WHOLE, int R, bool ONE> __global__ void __launch_bounds__(256, 2) mem_attn_wide_kernel(MemArgs a)
+{
+    typedef bf16_t T;
+    using V = Tile<T, DP, 32, 64, WHOLE>;
+    constexpr int ND = DP / 32, NK = DP / 16, LINE = DP + 1, SUMS = 4 * R * LINE * 4, TILES = 4 * V::BYTES;
+    __shared__ __align__(16) unsigned char s_mem[SUMS > TILES ? SUMS : TILES];
+    __shared__ float2 s_ml[4][R], s_row[ONE ? 256 : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, row = lane & 31;
+    unsigned char *s_v = s_mem + wave * V::BYTES;
+    float *s_o = reinterpret_cast<float *>(s_mem);
+    int unit = ONE && a.usage ? blockIdx.x * a.row_groups : blockIdx.x, t = 0, budget = 1 << 30, units = a.units;
+    if constexpr (ONE) units = min(units, unit + (a.usage ? a.row_groups : 1));
+    else {
+        const bool some = find_begin<kWideStep>(a, unit, t, budget);
+        if (threadIdx.x < 4) a.begins[blockIdx.x * 4 + threadIdx.x] = threadIdx.x == 0 ? (some ? unit : -1) : threadIdx.x == 1 ? t : budget;
+        if (!some) return;
+    }
+    for (; budget > 0 && unit < units; unit++, t = 0) {
+        const int nh = unit / a.row_groups, row0 = (unit - nh * a.row_groups) * R, n = nh / a.heads, h = nh - n * a.heads;
+        const int rows = min(R, a.group - row0), slots = slots_of(a, n), steps = max(1, (slots + kWideStep - 1) / kWideStep);
+        const int t0 = t, t1 = ONE ? steps : min(steps, t + budget);
+        budget -= t1 - t0;
+        const T *kb = reinterpret_cast<const T *>(a.key) + h * a.ks[1], *vb = reinterpret_cast<const T *>(a.value) + h * a.vs[1];
+        const int32_t *table = a.table + n * a.table_stride;
+        float *scores = a.usage ? a.scores + (long)unit * a.slots_padded * a.score_rows : nullptr;
+
+        Raw8<T> k[NK], v[NK];
+        bool there = false;
+        int id = -1, in_page = 0;
+        auto look = [&](int step) INLINE {
+            const int s = min(step * kWideStep + wave * 32 + row, slots - 1), p = fdiv(s, a.page);
+            id = table[p];
+            in_page = s - p * a.page.d;
+        };
+        auto request = [&](int step) INLINE {
+            const bool valid = (unsigned)id < (unsigned)a.pages;
+            there = valid && step * kWideStep + wave * 32 + row < slots;
+            const long page = valid ? id : 0;
+            const T *kr = kb + page * a.ks[0] + in_page * a.ks[2], *vr = vb + page * a.vs[0] + in_page * a.vs[2];
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                k[i] = load8_of<WHOLE, T>(kr, i * 16 + half * 8, a.D, true);
+                v[i] = load8_of<WHOLE, T>(vr, i * 16 + half * 8, a.D, there);
+            }
+        };
+        if (slots > 0) {
+            look(t);
+            request(t);
+            if (t + 1 < t1) look(t + 1);
+        }
+        Frag<1> q[NK];
+        {
+            const T *qr = reinterpret_cast<const T *>(a.q) + n * a.qs[0] + (long)(h * a.group + row0 + min(row, rows - 1)) * a.qs[1];
+#pragma unroll
+            for (int i = 0; i < NK; i++) q[i] = terms_of<T>(load8_of<WHOLE, T>(qr, i * 16 + half * 8, a.D, row < rows));
+        }
+        f32x16 o[ND];
+#pragma unroll
+        for (int i = 0; i < ND; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[i][r] = 0.f;
+        float m = -INFINITY, lift = -INFINITY, l = 0.f;
+        const float c = a.scale2;
+
+        for (; t < t1 && slots > 0; t++) {
+            const uint32_t some = (uint32_t)__ballot(there);
+            f32x16 s;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                *reinterpret_cast<uint4 *>(s_v + piece_at<DP>(row, i * 2 + half)) = v[i].v[0];
+                mma(s, terms_of<T>(k[i]), q[i]);
+            }
+            if (t + 1 < t1) {
+                request(t + 1);
+                if (t + 2 < t1) look(t + 2);
+            }
+            if (some != 0xffffffffu) {
+                const uint32_t b = some >> (half * 4);
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (!((b >> (8 * (r / 4) + r % 4)) & 1)) s[r] = -INFINITY;
+            }
+            if (scores) {
+                float *tile = scores + (long)t * kWideStep * a.score_rows;
+                const unsigned at = (wave * 32 + half * 4) * a.score_rows + row;
+                const int left = row < rows ? slots - (t * kWideStep + wave * 32 + half * 4) : 0;
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (8 * (r / 4) + r % 4 < left) (tile + (8 * (r / 4) + r % 4) * a.score_rows)[at] = s[r] * c;
+            }
+            if (some == 0) continue;
+            float top = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+            // (the maximum follows where it has grown by more than a factor of 2^8 of the weights)
+            if (__any(top > lift)) {
+                const float grown = half_max(top);
+                if (grown > lift) {
+                    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - grown) * c);
+                    m = grown;
+                    lift = m + 8.f / c;
+                    l *= f;
+#pragma unroll
+                    for (int i = 0; i < ND; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) o[i][r] *= f;
+                }
+            }
+            const float mc = m == -INFINITY ? 0.f : m * c;
+            float p[16];
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -mc));
+                l += p[r];
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+                const Frag<2> pf = make_frag<2, WEIGHTS>(p + kk * 8);
+#pragma unroll
+                for (int d = 0; d < ND; d++) mma(o[d], V::columns(s_v, kk * 16, d * 32, lane), pf);
+            }
+        }
+        t = t1;
+        l = half_sum(l);
+        // the wavefronts' sums, in the place of their tiles
+        if (half == 0 && row < R) s_ml[wave][row] = make_float2(m == -INFINITY ? -INFINITY : m * c, l);
+        __syncthreads();
+        if (row < rows) {
+            float *to = s_o + (wave * R + row) * LINE;
+#pragma unroll
+            for (int i = 0; i < ND; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) to[i * 32 + 8 * (r / 4) + 4 * half + r % 4] = o[i][r];
+        }
+        __syncthreads();
+        const bool direct = ONE || (t0 == 0 && t1 == steps);
+        const long piece = ONE ? unit : (long)unit + blockIdx.x;
+        for (int i = threadIdx.x; i < rows * DP; i += 256) {
+            const int r = i / DP, d = i - r * DP;
+            if (d >= a.D) continue;
+            float top = s_ml[0][r].x, sum = 0.f, x = 0.f;
+#pragma unroll
+            for (int w = 1; w < 4; w++) top = fmaxf(top, s_ml[w][r].x);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float f = __builtin_amdgcn_exp2f(s_ml[w][r].x - base);
+                sum = fmaf(s_ml[w][r].y, f, sum);
+                x = fmaf(s_o[(w * R + r) * LINE + d], f, x);
+            }
+            if (d == 0) {
+                if constexpr (ONE) s_row[row0 + r] = usage_ml(top, sum);
+                else *reinterpret_cast<float2 *>(a.part_ml + (piece * R + r) * 2) = make_float2(top, sum);
+            }
+            if (direct) reinterpret_cast<T *>(a.out)[((long)n * a.heads * a.group + h * a.group + row0 + r) * a.D + d] = f32_to_elem<T>(sum == 0.f ? 0.f : x / sum);
+            else a.part[(piece * R + r) * part_width(a.D) + d] = x;
+        }
+        if (!ONE && threadIdx.x == 0) {
+            if (t0 == 0) a.covered[unit * 2] = blockIdx.x;
+            if (t1 == steps) a.covered[unit * 2 + 1] = blockIdx.x;
+        }
+        __syncthreads();      // (tiles and sums are written again by the next unit's piece)
+        if constexpr (ONE) {
+            if (a.usage && unit + 1 == units) add_usage<R>(a, unit + 1 - a.row_groups, n, h, 0, slots, s_row);
+        }
     }
 }
 
@@ -880,26 +1057,31 @@ template <typename F> auto for_rows(const d2c_memory_desc &q, int group, F f)
     return q.dtype == D2C_BF16 ? with_type(bf16_t{}) : with_type(float{});
 }
 
-// Memories of up to so many steps (of 32 to 256 slots) are read by a workgroup to each unit
-constexpr int kOneSteps = 4;
-struct MemPlan { int rows, step, row_groups, units, places, least; bool one; size_t part_bytes, ml_bytes, covered_bytes, begins_bytes, scores_bytes, bytes; long slots_padded; };
+// Memories of up to so many steps (of 32 to 256 slots) are read by a workgroup to each unit, in one launch: 8 heads of 64, bfloat16, 512 slots of 1 stream 6.9 us (else 9.3), 1024
+// 10.5 (8.9); of 64 streams, whose units fill the GPU, 1024 21.7 (24.3)
+constexpr int kOneSteps = 4, kOneStepsMany = 8;
+// bfloat16 calls of more rows to a key head run on the matrix instruction
+constexpr int kTokenRows = 4;
+struct MemPlan { int rows, score_rows, step, row_groups, units, places, least; bool wide, one; size_t part_bytes, ml_bytes, covered_bytes, begins_bytes, scores_bytes, bytes; long slots_padded; };
 MemPlan mem_plan(const d2c_memory_desc &q, const d2c_memory_query_desc &x, bool track)
 {
     MemPlan p{};
     const int group = x.query_heads / q.heads;
-    for_rows(q, group, [&](auto zero, auto lanes, auto r) {
-        p.rows = decltype(r)::value;
+    p.wide = q.dtype == D2C_BF16 && group > kTokenRows;
+    if (p.wide) { p.rows = group <= 16 ? 16 : 32; p.step = kWideStep; p.score_rows = (std::min(group, p.rows) + 3) / 4 * 4; }
+    else for_rows(q, group, [&](auto zero, auto lanes, auto r) {
+        p.rows = p.score_rows = decltype(r)::value;
         p.step = TokenShape<decltype(zero), decltype(lanes)::value, decltype(r)::value>::STEP;
         return 0;
     });
     const long slots = (long)q.per_stream * q.page;
     p.row_groups = (group + p.rows - 1) / p.rows;
     p.units = q.streams * q.heads * p.row_groups;
-    p.one = slots <= (long)kOneSteps * p.step && !(track && p.row_groups > 1);
     p.places = 2 * std::max(d2c_num_cus(), 1);
     p.least = 2;
+    p.one = slots <= (long)(p.units >= p.places ? kOneStepsMany : kOneSteps) * p.step;
     p.slots_padded = (slots + 63) / 64 * 64;
-    if (track) p.scores_bytes = d2c_align_up((size_t)p.units * p.rows * p.slots_padded * 4);
+    if (track) p.scores_bytes = d2c_align_up((size_t)p.units * p.score_rows * p.slots_padded * 4);
     if (!p.one) {
         const size_t lines = ((size_t)p.units + p.places) * p.rows;
         p.part_bytes = d2c_align_up(lines * part_width(q.D) * 4);
@@ -991,26 +1173,45 @@ extern "C" int d2c_memory_attention(const d2c_memory_desc *q, const d2c_memory_q
     a.table_stride = q->table_stride; a.slots_padded = p.slots_padded; a.page = make_fastdiv(q->page);
     a.N = q->streams; a.heads = q->heads; a.group = x->query_heads / q->heads; a.D = q->D; a.pages = q->pages;
     a.slots = q->pages > 0 ? (int)slots : 0;      // (without pages no slot is there)
-    a.row_groups = p.row_groups; a.units = p.units; a.places = p.places; a.least = p.least;
+    a.score_rows = p.score_rows; a.row_groups = p.row_groups; a.units = p.units; a.places = p.places; a.least = p.least;
     a.scale2 = x->scale * 1.44269504088896340736f;
     hipStream_t st = (hipStream_t)stream;
+    const bool whole = q->D * d2c_elem_size(q->dtype) % 16 == 0;
+    const dim3 grid(p.one ? (usage ? p.units / p.row_groups : p.units) : p.places), joins((unsigned)(q->streams * x->query_heads + (usage ? p.places * kUsageBlocks : 0)));
+    auto join = [&](auto zero, auto lanes, auto r) {
+        hipLaunchKernelGGL((mem_join_kernel<decltype(zero), decltype(lanes)::value, decltype(r)::value>), joins, dim3(256), 0, st, a, q->streams * x->query_heads, p.step);
+        return d2c_check_launch("mem_join_kernel");
+    };
+    auto for_two = [&](bool yes, auto f) { return yes ? f(std::true_type{}) : f(std::false_type{}); };
+    if (p.wide) {
+        auto launch = [&](auto dp, auto r) {
+            constexpr int DP = decltype(dp)::value, R = decltype(r)::value;
+            const int rc = for_two(whole, [&](auto w) {
+                return for_two(p.one, [&](auto one) {
+                    hipLaunchKernelGGL((mem_attn_wide_kernel<DP, decltype(w)::value, R, decltype(one)::value>), grid, dim3(256), 0, st, a);
+                    return d2c_check_launch("mem_attn_wide_kernel");
+                });
+            });
+            if (rc || p.one) return rc;
+            return join(bf16_t{}, std::integral_constant<int, DP <= 32 ? 8 : DP <= 64 ? 16 : 32>{}, r);
+        };
+        auto with_rows = [&](auto dp) { return p.rows == 16 ? launch(dp, std::integral_constant<int, 16>{}) : launch(dp, std::integral_constant<int, 32>{}); };
+        if (q->D <= 32) return with_rows(std::integral_constant<int, 32>{});
+        if (q->D <= 64) return with_rows(std::integral_constant<int, 64>{});
+        if (q->D <= 96) return with_rows(std::integral_constant<int, 96>{});
+        return with_rows(std::integral_constant<int, 128>{});
+    }
     return for_rows(*q, a.group, [&](auto zero, auto lanes, auto r) {
         using T = decltype(zero);
         constexpr int LANES = decltype(lanes)::value, R = decltype(r)::value;
-        const bool whole = q->D * sizeof(T) % 16 == 0;
-        const dim3 grid(p.one ? p.units : p.places);
-        auto launch = [&](auto whole, auto one) {
-            hipLaunchKernelGGL((mem_attn_kernel<T, LANES, R, decltype(whole)::value, decltype(one)::value>), grid, dim3(256), 0, st, a);
-            return d2c_check_launch("mem_attn_kernel");
-        };
-        int rc;
-        if (whole) rc = p.one ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
-        else rc = p.one ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
+        const int rc = for_two(whole, [&](auto w) {
+            return for_two(p.one, [&](auto one) {
+                hipLaunchKernelGGL((mem_attn_kernel<T, LANES, R, decltype(w)::value, decltype(one)::value>), grid, dim3(256), 0, st, a);
+                return d2c_check_launch("mem_attn_kernel");
+            });
+        });
         if (rc || p.one) return rc;
-        constexpr int JOIN = LANES * 16 / (int)sizeof(T) / 4;      // lanes of four columns
-        const int rows = q->streams * x->query_heads;
-        hipLaunchKernelGGL((mem_join_kernel<T, JOIN, R>), dim3(rows + (usage ? p.places * kUsageBlocks : 0)), dim3(256), 0, st, a, rows, p.step);
-        return d2c_check_launch("mem_join_kernel");
+        return join(zero, std::integral_constant<int, LANES * 16 / (int)sizeof(T) / 4>{}, r);      // (lanes of four columns)
     });
 }
 

@@ -30,6 +30,14 @@ CASES = [
     ([40], 16, 9, 1, 64),
     ([4000, 1], 64, 2, 1, 104),
     ([5000], 64, 5, 1, 127),
+    ([3, 20], 8, 18, 1, 80),           # rows in groups, memories that one workgroup reads
+    ([700, 0, 129], 64, 16, 2, 128),
+    ([400, 1], 16, 16, 1, 32),
+    ([256, 1000], 64, 34, 2, 64),
+    ([31, 33], 16, 32, 1, 128),
+    ([2000], 16, 33, 1, 40),
+    ([5000, 40], 64, 70, 1, 88),
+    ([100, 9000], 64, 6, 1, 20),
 ]
 
 
