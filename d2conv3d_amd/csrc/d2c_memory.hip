@@ -17,7 +17,7 @@ struct MemArgs {
     float *part, *part_ml;        // [units + places][R][part_width(D)], and (maximum, sum) of each row
     int32_t *covered;             // [units][2]: the first and the last workgroup that has a piece of the unit
     int32_t *begins;              // [places][4]: unit and step that a workgroup begins with, its steps
-    float *scores;                // [units][slots][score_rows], of base 2
+    float *scores;                // [units][slots][score_rows], or [units][score_rows][slots], of base 2
     long qs[2], ks[3], vs[3], table_stride, slots_padded;
     FastDiv page;
     int N, heads, group, D, pages, slots, row_groups, units, places, least, score_rows;
@@ -85,8 +85,9 @@ template <int STEP> D2C_DEV bool find_begin(const MemArgs &a, int &unit, int &t,
     return true;
 }
 
-// The weights of a key head's slots from s0 to s1, added up over all its rows, R to a unit.  s_ml: maximum and 1 / sum of the rows
-template <int R> D2C_DEV void add_usage(const MemArgs &a, int unit, int n, int h, int s0, int s1, const float2 *s_ml)
+// The weights of a key head's slots from s0 to s1, added up over all its rows, R to a unit.  s_ml: maximum and 1 / sum of the rows.  Scores lie slot by slot, a unit's rows
+// together, or (PLANES) row by row
+template <int R, bool PLANES> D2C_DEV void add_usage(const MemArgs &a, int unit, int n, int h, int s0, int s1, const float2 *s_ml)
 {
     for (int s = s0 + (int)threadIdx.x; s < s1; s += 256) {
         const int p = fdiv(s, a.page), id = a.table[n * a.table_stride + p];
@@ -95,19 +96,25 @@ template <int R> D2C_DEV void add_usage(const MemArgs &a, int unit, int n, int h
         const float old = *to;
         float x = 0.f;
         for (int g = 0; g < a.row_groups; g++) {
-            float score[R];
-            const float *from = a.scores + ((long)(unit + g) * a.slots_padded + s) * a.score_rows;
-            if constexpr (R % 4 == 0) {
-#pragma unroll
-                for (int r = 0; r < R; r += 4)
-                    if (r < a.score_rows && g * R + r < a.group) *reinterpret_cast<float4 *>(score + r) = *reinterpret_cast<const float4 *>(from + r);
+            const float *from = a.scores + (long)(unit + g) * a.slots_padded * a.score_rows;
+            if constexpr (PLANES) {
+                const int rows = min(R, a.group - g * R);
+#pragma unroll 4
+                for (int r = 0; r < rows; r++) x += __builtin_amdgcn_exp2f(from[r * a.slots_padded + s] - s_ml[g * R + r].x) * s_ml[g * R + r].y;
             } else {
+                float score[R];
+                from += (long)s * R;
+                if constexpr (R % 4 == 0) {
 #pragma unroll
-                for (int r = 0; r < R; r++) score[r] = from[r];
+                    for (int r = 0; r < R; r += 4) *reinterpret_cast<float4 *>(score + r) = *reinterpret_cast<const float4 *>(from + r);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < R; r++) score[r] = from[r];
+                }
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    if (g * R + r < a.group) x += __builtin_amdgcn_exp2f(score[r] - s_ml[g * R + r].x) * s_ml[g * R + r].y;
             }
-#pragma unroll
-            for (int r = 0; r < R; r++)
-                if (g * R + r < a.group) x += __builtin_amdgcn_exp2f(score[r] - s_ml[g * R + r].x) * s_ml[g * R + r].y;
         }
         *to = old + x;
     }
@@ -325,7 +332,7 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
                     s_row[row0 + r] = usage_ml(top, sum);
                 }
                 __syncthreads();
-                if (unit + 1 == units) add_usage<R>(a, unit + 1 - a.row_groups, n, h, 0, slots, s_row);
+                if (unit + 1 == units) add_usage<R, false>(a, unit + 1 - a.row_groups, n, h, 0, slots, s_row);
             }
         }
         __syncthreads();      // (s_o and s_ml are written again by the next unit's piece)
@@ -333,19 +340,19 @@ template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __
 }
 
 // More than four rows of a key head, bfloat16: their products on the matrix instruction, whose columns are the rows (R of them, up to 32).  A wavefront has 32 slots of a step to
-// itself: a lane asks for a slot's key and value (its half of every 16 channels), keys are the instruction's operand as they come, values go through a tile of the wavefront's own in LDS
-// and are read back by columns.  No barrier until the end of a unit's piece, where the four wavefronts' sums meet.  Weights are two terms, which cost little here.
+// itself, whose keys and values go through tiles of its own in LDS: neighbouring lanes ask for a whole slot's (pieces of 16 channels straight into the operand's place took 1.2 times as
+// long where pages are scattered).  No barrier until the end of a unit's piece, where the four wavefronts' sums meet.  Weights are two terms, which cost little here.
 // Bound: memory.
 constexpr int kWideStep = 128;
 template <int DP, bool WHOLE, int R, bool ONE> __global__ void __launch_bounds__(256, 2) mem_attn_wide_kernel(MemArgs a)
 {
     typedef bf16_t T;
     using V = Tile<T, DP, 32, 64, WHOLE>;
-    constexpr int ND = DP / 32, NK = DP / 16, LINE = DP + 1, SUMS = 4 * R * LINE * 4, TILES = 4 * V::BYTES;
+    constexpr int ND = DP / 32, NK = DP / 16, LINE = DP + 1, SUMS = 4 * R * LINE * 4, TILES = 8 * V::BYTES, PER = V::PIECES / 2;
     __shared__ __align__(16) unsigned char s_mem[SUMS > TILES ? SUMS : TILES];
     __shared__ float2 s_ml[4][R], s_row[ONE ? 256 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, row = lane & 31;
-    unsigned char *s_v = s_mem + wave * V::BYTES;
+    unsigned char *s_k = s_mem + wave * 2 * V::BYTES, *s_v = s_k + V::BYTES;
     float *s_o = reinterpret_cast<float *>(s_mem);
     int unit = ONE && a.usage ? blockIdx.x * a.row_groups : blockIdx.x, t = 0, budget = 1 << 30, units = a.units;
     if constexpr (ONE) units = min(units, unit + (a.usage ? a.row_groups : 1));
@@ -363,23 +370,23 @@ template <int DP, bool WHOLE, int R, bool ONE> __global__ void __launch_bounds__
         const int32_t *table = a.table + n * a.table_stride;
         float *scores = a.usage ? a.scores + (long)unit * a.slots_padded * a.score_rows : nullptr;
 
-        Raw8<T> k[NK], v[NK];
+        Raw8<T> k[PER], v[PER];
         bool there = false;
         int id = -1, in_page = 0;
+        // lane % 32 knows the place of its slot of a step
         auto look = [&](int step) INLINE {
             const int s = min(step * kWideStep + wave * 32 + row, slots - 1), p = fdiv(s, a.page);
             id = table[p];
             in_page = s - p * a.page.d;
         };
         auto request = [&](int step) INLINE {
-            const bool valid = (unsigned)id < (unsigned)a.pages;
-            there = valid && step * kWideStep + wave * 32 + row < slots;
-            const long page = valid ? id : 0;
-            const T *kr = kb + page * a.ks[0] + in_page * a.ks[2], *vr = vb + page * a.vs[0] + in_page * a.vs[2];
+            there = (unsigned)id < (unsigned)a.pages && step * kWideStep + wave * 32 + row < slots;
+            const int known = there ? id : -1;
 #pragma unroll
-            for (int i = 0; i < NK; i++) {
-                k[i] = load8_of<WHOLE, T>(kr, i * 16 + half * 8, a.D, true);
-                v[i] = load8_of<WHOLE, T>(vr, i * 16 + half * 8, a.D, there);
+            for (int i = 0; i < PER; i++) {
+                const int from = (i * 64 + lane) / V::PIECES, d = (i * 64 + lane) % V::PIECES * 8, page = __shfl(known, from, 64), at = __shfl(in_page, from, 64);
+                k[i] = load8_of<WHOLE, T>(kb + max(page, 0) * a.ks[0] + at * a.ks[2], d, a.D, page >= 0);
+                v[i] = load8_of<WHOLE, T>(vb + max(page, 0) * a.vs[0] + at * a.vs[2], d, a.D, page >= 0);
             }
         };
         if (slots > 0) {
@@ -407,10 +414,13 @@ template <int DP, bool WHOLE, int R, bool ONE> __global__ void __launch_bounds__
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = 0.f;
 #pragma unroll
-            for (int i = 0; i < NK; i++) {
-                *reinterpret_cast<uint4 *>(s_v + piece_at<DP>(row, i * 2 + half)) = v[i].v[0];
-                mma(s, terms_of<T>(k[i]), q[i]);
+            for (int i = 0; i < PER; i++) {
+                const int at = piece_at<DP>((i * 64 + lane) / V::PIECES, (i * 64 + lane) % V::PIECES);
+                *reinterpret_cast<uint4 *>(s_k + at) = k[i].v[0];
+                *reinterpret_cast<uint4 *>(s_v + at) = v[i].v[0];
             }
+#pragma unroll
+            for (int i = 0; i < NK; i++) mma(s, V::rows(s_k, row, i, half), q[i]);
             if (t + 1 < t1) {
                 request(t + 1);
                 if (t + 2 < t1) look(t + 2);
@@ -422,12 +432,14 @@ template <int DP, bool WHOLE, int R, bool ONE> __global__ void __launch_bounds__
                     if (!((b >> (8 * (r / 4) + r % 4)) & 1)) s[r] = -INFINITY;
             }
             if (scores) {
-                float *tile = scores + (long)t * kWideStep * a.score_rows;
-                const unsigned at = (wave * 32 + half * 4) * a.score_rows + row;
-                const int left = row < rows ? slots - (t * kWideStep + wave * 32 + half * 4) : 0;
+                // (four neighbouring slots of a row at a time; what is behind the last of them is not read)
+                if (row < rows && t * kWideStep + wave * 32 < slots) {
+                    float *to = scores + row * a.slots_padded + t * kWideStep + wave * 32 + half * 4;
 #pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (8 * (r / 4) + r % 4 < left) (tile + (8 * (r / 4) + r % 4) * a.score_rows)[at] = s[r] * c;
+                    for (int j = 0; j < 4; j++)
+                        if (t * kWideStep + wave * 32 + j * 8 < a.slots_padded)
+                            *reinterpret_cast<float4 *>(to + j * 8) = make_float4(s[j * 4] * c, s[j * 4 + 1] * c, s[j * 4 + 2] * c, s[j * 4 + 3] * c);
+                }
             }
             if (some == 0) continue;
             float top = s[0];
@@ -502,7 +514,7 @@ template <int DP, bool WHOLE, int R, bool ONE> __global__ void __launch_bounds__
         }
         __syncthreads();      // (tiles and sums are written again by the next unit's piece)
         if constexpr (ONE) {
-            if (a.usage && unit + 1 == units) add_usage<R>(a, unit + 1 - a.row_groups, n, h, 0, slots, s_row);
+            if (a.usage && unit + 1 == units) add_usage<R, true>(a, unit + 1 - a.row_groups, n, h, 0, slots, s_row);
         }
     }
 }
@@ -510,7 +522,7 @@ template <int DP, bool WHOLE, int R, bool ONE> __global__ void __launch_bounds__
 // Units that several workgroups have shared: blocks from 0, one to a row, put their pieces together.  Where weights are added up: blocks from `rows` on, kUsageBlocks to each
 // workgroup of the walk, go over the same slots once more, by their scores.
 constexpr int kUsageBlocks = 4;
-template <typename T, int LANES, int R> __global__ void __launch_bounds__(256) mem_join_kernel(MemArgs a, int rows, int step)
+template <typename T, int LANES, int R, bool WIDE> __global__ void __launch_bounds__(256) mem_join_kernel(MemArgs a, int rows, int step)
 {
     constexpr int GROUPS = 256 / LANES;
     __shared__ float4 s_x[256];
@@ -599,7 +611,7 @@ template <typename T, int LANES, int R> __global__ void __launch_bounds__(256) m
             if ((tid & 63) == 0) s_ml[row] = usage_ml(all, sum);
         }
         __syncthreads();
-        add_usage<R>(a, unit, n, h, from, to, s_ml);
+        add_usage<R, WIDE>(a, unit, n, h, from, to, s_ml);
     }
 }
 
@@ -1060,7 +1072,8 @@ template <typename F> auto for_rows(const d2c_memory_desc &q, int group, F f)
 // Memories of up to so many steps (of 32 to 256 slots) are read by a workgroup to each unit, in one launch: 8 heads of 64, bfloat16, 512 slots of 1 stream 6.9 us (else 9.3), 1024
 // 10.5 (8.9); of 64 streams, whose units fill the GPU, 1024 21.7 (24.3)
 constexpr int kOneSteps = 4, kOneStepsMany = 8;
-// bfloat16 calls of more rows to a key head run on the matrix instruction
+// bfloat16 calls of more rows to a key head run on the matrix instruction (four rows, 64 channels, 32 streams of up to 12960 slots with weights added up: 77 us by lanes, 80 there; five
+// rows, 64 streams of 4096: 19 there; 12 rows, 46 streams of 4096, 96 channels: 424 by lanes, 118 there)
 constexpr int kTokenRows = 4;
 struct MemPlan { int rows, score_rows, step, row_groups, units, places, least; bool wide, one; size_t part_bytes, ml_bytes, covered_bytes, begins_bytes, scores_bytes, bytes; long slots_padded; };
 MemPlan mem_plan(const d2c_memory_desc &q, const d2c_memory_query_desc &x, bool track)
@@ -1068,7 +1081,7 @@ MemPlan mem_plan(const d2c_memory_desc &q, const d2c_memory_query_desc &x, bool 
     MemPlan p{};
     const int group = x.query_heads / q.heads;
     p.wide = q.dtype == D2C_BF16 && group > kTokenRows;
-    if (p.wide) { p.rows = group <= 16 ? 16 : 32; p.step = kWideStep; p.score_rows = (std::min(group, p.rows) + 3) / 4 * 4; }
+    if (p.wide) { p.rows = group <= 16 ? 16 : 32; p.step = kWideStep; p.score_rows = std::min(group, p.rows); }
     else for_rows(q, group, [&](auto zero, auto lanes, auto r) {
         p.rows = p.score_rows = decltype(r)::value;
         p.step = TokenShape<decltype(zero), decltype(lanes)::value, decltype(r)::value>::STEP;
@@ -1179,7 +1192,7 @@ extern "C" int d2c_memory_attention(const d2c_memory_desc *q, const d2c_memory_q
     const bool whole = q->D * d2c_elem_size(q->dtype) % 16 == 0;
     const dim3 grid(p.one ? (usage ? p.units / p.row_groups : p.units) : p.places), joins((unsigned)(q->streams * x->query_heads + (usage ? p.places * kUsageBlocks : 0)));
     auto join = [&](auto zero, auto lanes, auto r) {
-        hipLaunchKernelGGL((mem_join_kernel<decltype(zero), decltype(lanes)::value, decltype(r)::value>), joins, dim3(256), 0, st, a, q->streams * x->query_heads, p.step);
+        hipLaunchKernelGGL((mem_join_kernel<decltype(zero), decltype(lanes)::value, decltype(r)::value, (decltype(r)::value > 8)>), joins, dim3(256), 0, st, a, q->streams * x->query_heads, p.step);
         return d2c_check_launch("mem_join_kernel");
     };
     auto for_two = [&](bool yes, auto f) { return yes ? f(std::true_type{}) : f(std::false_type{}); };
