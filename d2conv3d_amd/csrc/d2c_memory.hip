@@ -754,8 +754,9 @@ D2C_DEV uint32_t rank_of(float usage, bool stays)
 // A workgroup to a stream's head.  The keep-th largest rank by its digits (11, 11 and 10 bits, a histogram of each in LDS, the first in several copies, whose few bins many
 // lanes meet in), then the slots that go before `keep` and those that stay behind it, each in rising order.  A wavefront has neighbouring slots, 64 at a time, whose
 // truth values are one word each: counted by a lane to a word.
-// LDS: their ranks stay there; else in memory.  PAGED: pages are multiples of 64 slots, so that a wavefront's 64 lie in one.  Loops are short rather than unrolled: every
-// instruction is fetched anew by every launch (ranks in registers, 32 to a thread and all loops unrolled: 45 us where this takes 2x).
+// LDS: their ranks stay there; else in memory.  PAGED: pages are multiples of 64 slots, so that a wavefront's 64 lie in one.
+// Bound: a compute unit's instructions and the latency of its chain (counts, pages, usage, three histograms).  64 units of up to 25920 slots 32 us (44 with a request for each
+// number's page on its own; 51 with ranks in registers and loops unrolled, whose instructions every launch fetches anew); 4 units of 3240 slots in pages of 16, 11 us.
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kEvictLds = 26 << 10;      // (slots)
 template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads) mem_rank_kernel(EvictArgs a)
 {
@@ -774,24 +775,6 @@ template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads)
     const int per = (slots + kEvictThreads - 1) / kEvictThreads * 64, s0 = min(wave * per, slots), s1 = min(s0 + per, slots), numbers = (s1 - s0 + 63) / 64;
     const int newest = (int)max((long)a.seen[n] - a.recent, -(1L << 31));
     const int32_t *table = a.table + n * a.table_stride;
-    // the ranks of 64 slots from s on; 0 behind the last, which then are the first to go
-    auto rank_at = [&](int s) INLINE {
-        int id, in_page;
-        if constexpr (PAGED) {
-            const int p = fdiv(min(s, slots - 1), a.page);
-            id = table[p];
-            in_page = s - p * a.page.d + lane;
-            if (s >= slots) in_page = lane;
-        } else {
-            const int at = min(s + lane, slots - 1), p = fdiv(at, a.page);
-            id = table[p];
-            in_page = at - p * a.page.d;
-        }
-        const bool valid = (unsigned)id < (unsigned)a.pages;
-        const long page = (long)((valid ? id : 0) * a.heads + h) * a.page.d;
-        const uint32_t rank = rank_of(a.usage[page + (unsigned)in_page], a.positions[page + (unsigned)in_page] >= newest);
-        return valid && s + lane < s1 ? rank : 0u;
-    };
     uint32_t *ranks = LDS ? nullptr : a.ranks + unit * a.slots_padded;
     uint32_t *s_list = reinterpret_cast<uint32_t *>(s_hist[1]);      // ranks of the second pass's digit, in the place of the first pass's copies
     // f(number, rank) for the wavefront's slots s0 + 64 number + lane from number `first` on, 4 at a time and WORDS at most
@@ -813,17 +796,33 @@ template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads)
     };
     if (tid == 0) s_met = 0;
     for (int i = tid; i < COPIES * BINS / 4; i += kEvictThreads) reinterpret_cast<int4 *>(&s_hist[0][0])[i] = make_int4(0, 0, 0, 0);
+    // ranks, REQUESTS numbers at a time; 0 for what is not there.  (PAGED: lane l asks for the page of number l of 64, so that no number waits for its own)
+    int pages_of = 0;
 #pragma unroll 1
     for (int i = 0; i < numbers; i += REQUESTS) {
-        uint32_t r[REQUESTS];
+        int id[REQUESTS], in_page[REQUESTS], positions[REQUESTS];
+        float usage[REQUESTS];
+        if (PAGED && i % 64 == 0) pages_of = table[fdiv(min(s0 + (i + lane) * 64, slots - 1), a.page)];
 #pragma unroll
-        for (int u = 0; u < REQUESTS; u++) r[u] = rank_at(s0 + (i + u) * 64);
+        for (int u = 0; u < REQUESTS; u++) {
+            const int s = min(s0 + (i + u) * 64 + lane, slots - 1), p = fdiv(s, a.page);
+            if constexpr (PAGED) id[u] = __builtin_amdgcn_readlane(pages_of, i % 64 + u);
+            else id[u] = table[p];
+            in_page[u] = s - p * a.page.d;
+        }
+#pragma unroll
+        for (int u = 0; u < REQUESTS; u++) {
+            const long at = (long)(((unsigned)id[u] < (unsigned)a.pages ? id[u] : 0) * a.heads + h) * a.page.d + in_page[u];
+            usage[u] = a.usage[at];
+            positions[u] = a.positions[at];
+        }
 #pragma unroll
         for (int u = 0; u < REQUESTS; u++) {
             const int s = s0 + (i + u) * 64 + lane;
+            const uint32_t rank = (unsigned)id[u] < (unsigned)a.pages ? rank_of(usage[u], positions[u] >= newest) : 0u;
             if (s < s1) {
-                if constexpr (LDS) s_ranks[s] = r[u];
-                else ranks[s] = r[u];
+                if constexpr (LDS) s_ranks[s] = rank;
+                else ranks[s] = rank;
             }
         }
     }
