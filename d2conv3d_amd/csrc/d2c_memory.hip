@@ -125,7 +125,8 @@ D2C_DEV float2 usage_ml(float top, float sum) { return make_float2(top == -INFIN
 // One new token of each stream.  As attn_token_kernel, by lanes and without matrix instructions: LANES lanes hold a slot's key and value, 16 bytes each, a wavefront
 // 64 / LANES slots; every group of lanes keeps its own maximum, sum and output of each of the R rows until the end of the unit's piece.  The page of a slot is
 // asked for two steps ahead, its key and value one.  ONE: a workgroup to a unit (short memories), which needs no second launch.
-// Bound: memory.
+// Bound: memory.  Measured, bfloat16, four rows: two streams of 129600 slots, 2 heads of 128, pages of 64 in any order, 54.8 us (265 MB, 4.8 TB/s; a copy 5.1) and the join 5.6; 32 streams of up
+// to 12960, 4 heads of 64, with scores written for the weights, 55 us (222 MB).  Three workgroups to a compute unit instead of two are 3 us longer on the first and no shorter on the second.
 template <typename T, int LANES, int R, bool WHOLE, bool ONE> __global__ void __launch_bounds__(256) mem_attn_kernel(MemArgs a)
 {
     using Shape = TokenShape<T, LANES, R>;
@@ -520,7 +521,8 @@ template <int DP, bool WHOLE, int R, bool ONE> __global__ void __launch_bounds__
 }
 
 // Units that several workgroups have shared: blocks from 0, one to a row, put their pieces together.  Where weights are added up: blocks from `rows` on, kUsageBlocks to each
-// workgroup of the walk, go over the same slots once more, by their scores.
+// workgroup of the walk, go over the same slots once more, by their scores.  Bound: the latency of its chain; 12.8 us where 32 streams' weights are added up (20 MB; 2 or 8 blocks to a
+// workgroup, and requests before the rows' sums are known, are no shorter).
 constexpr int kUsageBlocks = 4;
 template <typename T, int LANES, int R, bool WIDE> __global__ void __launch_bounds__(256) mem_join_kernel(MemArgs a, int rows, int step)
 {
@@ -646,7 +648,7 @@ template <typename T> D2C_DEV void put_piece(const AppendArgs &a, long token, in
         a.positions[i] = position;
     }
 }
-// A token of each stream: a workgroup to a stream, which then lets its counts grow
+// A token of each stream: a workgroup to a stream, which then lets its counts grow.  One launch; latency: 64 streams of 4 heads of 64, 3.0 us.
 template <typename T> __global__ void __launch_bounds__(256) mem_append_one_kernel(AppendArgs a)
 {
     const int n = blockIdx.x, pieces = (a.D * (int)sizeof(T) + 15) / 16, all = a.heads * pieces * 2;
@@ -658,7 +660,8 @@ template <typename T> __global__ void __launch_bounds__(256) mem_append_one_kern
         a.seen[n] = seen + 1;
     }
 }
-// Packed tokens, kAppendTokens to a workgroup: a thread to a token finds its place, then all of them move pieces of 16 bytes, four requested at a time
+// Packed tokens, kAppendTokens to a workgroup: a thread to a token finds its place, then all of them move pieces of 16 bytes, four requested at a time.  Bound: memory; four clips of up to 12960
+// tokens, 8 heads of 64, bfloat16, 21 us (93 MB, 4.4 TB/s).
 constexpr int kAppendTokens = 8;
 template <typename T> __global__ void __launch_bounds__(256) mem_append_kernel(AppendArgs a, FastDiv by_pieces)
 {
@@ -754,15 +757,13 @@ D2C_DEV uint32_t rank_of(float usage, bool stays)
 // A workgroup to a stream's head.  The keep-th largest rank by its digits (11, 11 and 10 bits, a histogram of each in LDS, the first in several copies, whose few bins many
 // lanes meet in), then the slots that go before `keep` and those that stay behind it, each in rising order.  A wavefront has neighbouring slots, 64 at a time, whose
 // truth values are one word each: counted by a lane to a word.
-// LDS: their ranks stay there; else in memory.  PAGED: pages are multiples of 64 slots, so that a wavefront's 64 lie in one.
-// Bound: a compute unit's instructions and the latency of its chain (counts, pages, usage, three histograms).  64 units of up to 25920 slots 32 us (44 with a request for each
-// number's page on its own; 51 with ranks in registers and loops unrolled, whose instructions every launch fetches anew); 4 units of 3240 slots in pages of 16, 11 us.
-constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kEvictLds = 26 << 10;      // (slots)
-template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads) mem_rank_kernel(EvictArgs a)
+// Bound: a compute unit's instructions and the latency of its chain (counts, pages, usage, three histograms).  64 units of up to 25920 slots 35 us (33 with the ranks in LDS, as far as they have
+// room there; 44 with a request for each page after the other; 51 with ranks in registers and loops unrolled, whose instructions every launch fetches anew), 4 units of 3240 slots 10.5.
+constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+__global__ void __launch_bounds__(kEvictThreads) mem_rank_kernel(EvictArgs a)
 {
     constexpr int BINS = 2048, COPIES = 4, AT_ONCE = 4, WORDS = 64;
-    constexpr int LIST = (COPIES - 1) * BINS, REQUESTS = PAGED ? 16 : 8;
-    extern __shared__ __align__(16) uint32_t s_ranks[];
+    constexpr int LIST = (COPIES - 1) * BINS, REQUESTS = 8;
     __shared__ __align__(16) int s_hist[COPIES][BINS];
     __shared__ __align__(16) uint4 s_words[kEvictWaves][WORDS];      // of 64 slots: which ranks are above the border, which are at it
     __shared__ int s_wave[3][kEvictWaves], s_digit[2], s_met;
@@ -775,7 +776,7 @@ template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads)
     const int per = (slots + kEvictThreads - 1) / kEvictThreads * 64, s0 = min(wave * per, slots), s1 = min(s0 + per, slots), numbers = (s1 - s0 + 63) / 64;
     const int newest = (int)max((long)a.seen[n] - a.recent, -(1L << 31));
     const int32_t *table = a.table + n * a.table_stride;
-    uint32_t *ranks = LDS ? nullptr : a.ranks + unit * a.slots_padded;
+    uint32_t *ranks = a.ranks + unit * a.slots_padded;
     uint32_t *s_list = reinterpret_cast<uint32_t *>(s_hist[1]);      // ranks of the second pass's digit, in the place of the first pass's copies
     // f(number, rank) for the wavefront's slots s0 + 64 number + lane from number `first` on, 4 at a time and WORDS at most
     auto for_slots = [&](int first, auto f) INLINE {
@@ -785,9 +786,7 @@ template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads)
 #pragma unroll
             for (int u = 0; u < AT_ONCE; u++) {
                 const int s = s0 + (i + u) * 64 + lane;
-                r[u] = 0;
-                if constexpr (LDS) r[u] = s_ranks[min(s, s1 - 1)];
-                else r[u] = ranks[min(s, s1 - 1)];
+                r[u] = ranks[min(s, s1 - 1)];
                 if (s >= s1) r[u] = 0;
             }
 #pragma unroll
@@ -796,18 +795,15 @@ template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads)
     };
     if (tid == 0) s_met = 0;
     for (int i = tid; i < COPIES * BINS / 4; i += kEvictThreads) reinterpret_cast<int4 *>(&s_hist[0][0])[i] = make_int4(0, 0, 0, 0);
-    // ranks, REQUESTS numbers at a time; 0 for what is not there.  (PAGED: lane l asks for the page of number l of 64, so that no number waits for its own)
-    int pages_of = 0;
+    // ranks, REQUESTS numbers at a time; 0 for what is not there
 #pragma unroll 1
     for (int i = 0; i < numbers; i += REQUESTS) {
         int id[REQUESTS], in_page[REQUESTS], positions[REQUESTS];
         float usage[REQUESTS];
-        if (PAGED && i % 64 == 0) pages_of = table[fdiv(min(s0 + (i + lane) * 64, slots - 1), a.page)];
 #pragma unroll
         for (int u = 0; u < REQUESTS; u++) {
             const int s = min(s0 + (i + u) * 64 + lane, slots - 1), p = fdiv(s, a.page);
-            if constexpr (PAGED) id[u] = __builtin_amdgcn_readlane(pages_of, i % 64 + u);
-            else id[u] = table[p];
+            id[u] = table[p];
             in_page[u] = s - p * a.page.d;
         }
 #pragma unroll
@@ -820,10 +816,7 @@ template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads)
         for (int u = 0; u < REQUESTS; u++) {
             const int s = s0 + (i + u) * 64 + lane;
             const uint32_t rank = (unsigned)id[u] < (unsigned)a.pages ? rank_of(usage[u], positions[u] >= newest) : 0u;
-            if (s < s1) {
-                if constexpr (LDS) s_ranks[s] = rank;
-                else ranks[s] = rank;
-            }
+            if (s < s1) ranks[s] = rank;
         }
     }
     uint32_t prefix = 0;
@@ -947,19 +940,9 @@ template <bool LDS, bool PAGED> __global__ void __launch_bounds__(kEvictThreads)
     }
     if (wave == kEvictWaves - 1 && lane == 0) a.counts[unit] = holes;
 }
-template <bool PAGED> int launch_rank(const EvictArgs &a, int units, hipStream_t st)
-{
-    const dim3 grid(units), block(kEvictThreads);
-    if (a.slots <= kEvictLds) {
-        constexpr int most = kEvictLds * 4;
-        if (int rc = d2c_allow_lds(reinterpret_cast<const void *>(&mem_rank_kernel<true, PAGED>), most, "mem_rank_kernel")) return rc;
-        hipLaunchKernelGGL((mem_rank_kernel<true, PAGED>), grid, block, (unsigned)a.slots * 4, st, a);
-    } else hipLaunchKernelGGL((mem_rank_kernel<false, PAGED>), grid, block, 0, st, a);
-    return d2c_check_launch("mem_rank_kernel");
-}
-
 // What stays behind `keep` into the places of what goes before it: reads and writes meet nowhere.  kMovePairs to a workgroup: a thread to a pair finds both places and
-// moves usage and position, then all of them move pieces of 16 bytes, four requested at a time.
+// moves usage and position, then all of them move pieces of 16 bytes, four requested at a time.  Bound: memory, rows of 128 bytes here and there; eight streams of 8 heads of 64, bfloat16, 36 us
+// (145 MB, 4.0 TB/s; 44 with both places looked up for every piece).
 constexpr int kMovePairs = 64;
 template <typename T> __global__ void __launch_bounds__(256) mem_move_kernel(EvictArgs a, int blocks, FastDiv by_pieces)
 {
@@ -1114,7 +1097,7 @@ EvictPlan evict_plan(const d2c_memory_desc &q, int keep)
     if (slots <= keep || units == 0) return p;
     p.pairs = (int)std::min((long)keep, slots - keep);
     p.slots_padded = (slots + 63) / 64 * 64;
-    p.ranks_bytes = slots <= kEvictLds ? 0 : d2c_align_up(units * p.slots_padded * 4);
+    p.ranks_bytes = d2c_align_up(units * p.slots_padded * 4);
     p.list_bytes = d2c_align_up(units * p.pairs * 4);
     p.bytes = p.ranks_bytes + 2 * p.list_bytes + d2c_align_up(units * 4);
     return p;
@@ -1251,7 +1234,8 @@ extern "C" int d2c_memory_evict(const d2c_memory_desc *q, void *key, void *value
     a.N = q->streams; a.heads = q->heads; a.D = q->D; a.pages = q->pages; a.slots = q->per_stream * q->page; a.keep = keep; a.recent = recent; a.pairs = p.pairs;
     hipStream_t st = (hipStream_t)stream;
     const int units = a.N * a.heads, vec = q->dtype == D2C_BF16 ? 8 : 4;
-    if (int rc = q->page % 64 == 0 ? launch_rank<true>(a, units, st) : launch_rank<false>(a, units, st)) return rc;
+    hipLaunchKernelGGL(mem_rank_kernel, dim3(units), dim3(kEvictThreads), 0, st, a);
+    if (int rc = d2c_check_launch("mem_rank_kernel")) return rc;
     const int blocks = (int)std::max(std::min((a.pairs + kMovePairs - 1L) / kMovePairs, (1L << 22) / units), 1L);
     const FastDiv pieces = make_fastdiv((a.D + vec - 1) / vec);
     if (q->dtype == D2C_BF16) hipLaunchKernelGGL(mem_move_kernel<bf16_t>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks, pieces);

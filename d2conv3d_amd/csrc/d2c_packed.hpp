@@ -234,14 +234,17 @@ D2C_DEV Walk key_walk(const PackedArgs &a, const PackedUnit &u)
     const int key0 = u.tile * kRows, first = a.causal ? max(fdiv(key0, a.frame) * a.frame.d - (u.lk - u.lq), 0) * a.group / a.step : 0;
     return walk_of(a, first, max((u.rows + a.step - 1) / a.step - first, 0));
 }
-// On the host, where only the average length is known: the longest walk is taken to be twice that of a sequence of the average length, or that of the only sequence
+// On the host, where only the average length is known: the longest walk is taken to be twice that of a sequence of the average length, or that of the only sequence.  Pieces cost a second
+// launch and their sums' way through memory, so walks are cut where one is longer than what every place gets anyway, into pieces of a third of that: one sequence of 25920, forward and backward,
+// 3.44 ms (4.99 whole, 3.95 in pieces of three quarters, 3.67 of a fifth); six of up to 12960 2.98 whole, 3.07 to 3.16 in pieces.
 struct Split { int splits, chunk; };
 inline Split split_walks(const d2c_packed_attention_desc &q, long units, long places, long along, long step, double unit_bytes)
 {
     const long sequences = std::max(q.sequences, 1), average = along / sequences / step + 1, longest = sequences == 1 ? average : 2 * average;
     const double each = (double)units * (double)average * (q.causal ? 0.5 : 1.0) / (double)places;      // steps that every place gets
     if ((double)longest <= 1.25 * each) return {1, 1 << 30};
-    // (pieces of 4 steps where all of them have a place at once, else of 8)
+    // (of 4 steps at least where all of them have a place at once, else of 8: four sequences of up to 350, float32, 14.3 us in pieces of 4, 18.7 of 8; three of up to 1417, forward and backward, 134 in
+    // pieces of 4, 121 of 6 or 8, 145 of 12)
     const long chunk = std::max((long)(each * 0.3), units * (longest / 4 + 1) * (q.causal ? 1 : 2) <= 2 * places ? 4L : 8L);
     long s = std::min((longest + chunk - 1) / chunk, 16L);
     while (s > 1 && (double)s * (double)units * unit_bytes > (double)D2C_ATTENTION_PART_BYTES) s--;
