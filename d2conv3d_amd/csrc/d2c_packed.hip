@@ -24,7 +24,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
 {
     using Shape = FwdShape<T, DP, WHOLE>;
     using KV = typename Shape::KV;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, true>, ND = DP / 32, NK = kSteps<NP>, KT = Shape::KT, NS = KT / 32, BUFFERS = Shape::BUFFERS;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, KT = Shape::KT, NS = KT / 32, BUFFERS = Shape::BUFFERS;
     constexpr bool END = WHOLE && NP % 2 == 1;
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ int s_bad;      // whether a tile's values were cleaned
@@ -234,7 +234,7 @@ template <typename T> FwdPlan fwd_plan(const d2c_packed_attention_desc &q)
     FwdPlan p{};
     p.tiles = tiles_of(q.queries * (q.Hq / q.Hkv), q.sequences);
     const long cus = std::max(d2c_num_cus(), 1);
-    pick_width(q.D, fast_kernels(q), [&](auto width, auto whole) {
+    pick_width(q.D, fast_kernels(q, false), [&](auto width, auto whole) {
         constexpr int DP = decltype(width)::DP, NP = decltype(width)::NP;
         constexpr bool WHOLE = decltype(whole)::value;
         using Shape = FwdShape<T, DP, WHOLE>;
@@ -258,7 +258,7 @@ template <typename T> int forward(PackedArgs a, const d2c_packed_attention_desc 
     }
     a.tiles = p.tiles; a.splits = p.split.splits; a.chunk = p.split.chunk; a.step = sizeof(T) == 2 ? 64 : 32;
     a.part = (float *)ws; a.part_ml = (float *)((char *)ws + p.part_bytes);
-    const int rc = pick_width(q.D, fast_kernels(q), [&](auto width, auto whole) {
+    const int rc = pick_width(q.D, fast_kernels(q, false), [&](auto width, auto whole) {
         constexpr int DP = decltype(width)::DP, NP = decltype(width)::NP;
         constexpr bool WHOLE = decltype(whole)::value;
         constexpr int lds = FwdShape<T, DP, WHOLE>::LDS;

@@ -209,9 +209,12 @@ template <typename T, bool AS_NAN, int ND, typename Row, typename Read> D2C_DEV 
 }
 
 PackedArgs make_args(const d2c_packed_attention_desc &q, const int32_t *starts, const int32_t *key_starts);
-// Whether a problem runs on the kernels that load whole pieces by offsets of 32 bits inside a tile
-inline bool fast_kernels(const d2c_packed_attention_desc &q)
+// Whether a problem runs on the kernels that load whole pieces by offsets of 32 bits inside a tile and, bfloat16, take one term of the weights: not where sequences have 64 keys or fewer on
+// the average, nor the backward pass where scores are few, whose errors do not average out (see kWeightTerms)
+inline bool fast_kernels(const d2c_packed_attention_desc &q, bool gradients)
 {
+    const long average = q.keys / std::max(q.sequences, 1);
+    if (q.dtype == D2C_BF16 && (average <= kExactKeys || (gradients && q.queries * q.Hq <= kExactScores / average))) return false;
     const long size = (long)d2c_elem_size(q.dtype), limit = 1L << 31;
     auto near = [&](const int64_t *s) { return s[0] >= 0 && s[1] >= 0 && 129 * s[0] * size + (q.Hq / q.Hkv) * s[1] * size < limit; };
     return q.D % 8 == 0 && near(q.q_stride) && near(q.k_stride) && near(q.v_stride) && 130L * q.Hq * q.D * size < limit;

@@ -25,7 +25,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
 {
     using Shape = QShape<T, DP, WHOLE>;
     using KV = typename Shape::KV;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, true>, ND = DP / 32, NK = kSteps<NP>, KT = Shape::KT, BUFFERS = Shape::BUFFERS;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, KT = Shape::KT, BUFFERS = Shape::BUFFERS;
     constexpr bool END = WHOLE && NP % 2 == 1;
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ int s_bad[2][4];
@@ -181,7 +181,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
 {
     using Shape = KvShape<T, DP, WHOLE>;
     using QG = typename Shape::QG;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, true>, ND = DP / 32, NK = kSteps<NP>, RT = Shape::RT, BUFFERS = Shape::BUFFERS;
+    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, RT = Shape::RT, BUFFERS = Shape::BUFFERS;
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ int s_bad[2][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -440,7 +440,7 @@ template <typename T> BwdPlan bwd_plan(const d2c_packed_attention_desc &q)
     p.q_tiles = tiles_of(rows, q.sequences);
     p.kv_tiles = tiles_of(q.keys, q.sequences);
     const double unit = kRows * (part_width(q.D) * 4.0);
-    pick_width(q.D, fast_kernels(q), [&](auto width, auto whole) {
+    pick_width(q.D, fast_kernels(q, true), [&](auto width, auto whole) {
         constexpr int DP = decltype(width)::DP, NP = decltype(width)::NP;
         constexpr bool WHOLE = decltype(whole)::value;
         using Q = QShape<T, DP, WHOLE>;
@@ -489,7 +489,7 @@ template <typename T> int backward(PackedArgs a, const d2c_packed_attention_desc
         return D2C_ERR_WORKSPACE;
     }
     a.delta = (float *)ws; a.part = (float *)((char *)ws + p.delta_bytes);
-    return pick_width(q.D, fast_kernels(q), [&](auto width, auto whole) { return launch_bwd<T, decltype(width)::DP, decltype(width)::NP, decltype(whole)::value>(a, p, st); });
+    return pick_width(q.D, fast_kernels(q, true), [&](auto width, auto whole) { return launch_bwd<T, decltype(width)::DP, decltype(width)::NP, decltype(whole)::value>(a, p, st); });
 }
 
 }  // namespace

@@ -211,7 +211,7 @@ def test_far_apart(dtype, dev):
     """Tokens whose elements lie beyond offsets of 32 bits inside a tile, and sequences that do from the first."""
     D, tokens = 64, 40
     q, k, v, g, starts, _ = make([25, 15], [25, 15], 2, 1, D, dtype, 22)
-    want = run(dev, q, k, v, g, starts)
+    exact = reference(q, k, v, g, starts, starts)
     step = 2 ** 26 if dtype == torch.bfloat16 else 2 ** 25
     pool = torch.empty(step * tokens + 1024, dtype=dtype, device=dev)
     far = [pool[at:].as_strided(t.shape, (step, D, 1)) for t, at in ((q, 0), (k, 256), (v, 512))]
@@ -219,7 +219,7 @@ def test_far_apart(dtype, dev):
         for a, b in zip(far, (q, k, v)):
             a.copy_(b)
     with torch.no_grad():
-        check([d2c.packed_attention(*far, starts.to(dev))], *(x[:1] for x in reference(q, k, v, g, starts, starts)))
+        check([d2c.packed_attention(*far, starts.to(dev))], *(x[:1] for x in exact))
     step = 2 ** 16
     tokens = 2 ** 31 // step + 2 ** 13
     del pool, far
@@ -233,8 +233,8 @@ def test_far_apart(dtype, dev):
     far = [t.detach().requires_grad_() for t in far]
     out = d2c.packed_attention(*far, (starts + tokens - 40).to(dev))
     got = torch.autograd.grad(out, far, grad)
-    for a, b in zip((out, *got), want):
-        assert torch.equal(a[-40:], b) and not bool(a[:-40].any())
+    check([t[-40:] for t in (out, *got)], *exact)
+    assert not any(bool(t[:-40].any()) for t in (out, *got))
 
 
 def test_differences(dev):
@@ -302,7 +302,7 @@ def test_captured_and_replayed(dtype, dev):
 
 
 def test_starts_that_do_not_rise(dev):
-    """Nothing outside the tensors is touched: guards on all sides of what is read and written."""
+    """Results of no meaning, from inside the tensors: starts of any numbers run, and calls behind them are what they are."""
     q, k, v, g, starts, _ = make([100, 100], [100, 100], 2, 1, 64, torch.float32, 30)
     for bad in ([0, 150, 100], [200, 100, 0], [-50, 1000, 20], [2 ** 31 - 1, -2 ** 31, 5]):
         for a, b in ((bad, bad), ([0, 100, 200], bad), (bad, [0, 100, 200])):
