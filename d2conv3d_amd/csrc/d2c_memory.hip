@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(kEvictThreads) mem_rank_kernel(EvictArgs a)
     __shared__ int s_wave[3][kEvictWaves], s_digit[2], s_met;
     const int unit = blockIdx.x, n = unit / a.heads, h = unit - n * a.heads, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int slots = min(max(a.lengths[n], 0), a.slots);
-    if (slots <= a.keep) {
+    if (slots <= a.keep || a.pages == 0) {      // (without pages there is nothing to rank, nor to read)
         if (tid == 0) a.counts[unit] = 0;
         return;
     }
@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(kEvictThreads) mem_rank_kernel(EvictArgs a)
         }
 #pragma unroll
         for (int u = 0; u < REQUESTS; u++) {
-            const long at = (long)(((unsigned)id[u] < (unsigned)a.pages ? id[u] : 0) * a.heads + h) * a.page.d + in_page[u];
+            const long at = ((long)((unsigned)id[u] < (unsigned)a.pages ? id[u] : 0) * a.heads + h) * a.page.d + in_page[u];
             usage[u] = a.usage[at];
             positions[u] = a.positions[at];
         }

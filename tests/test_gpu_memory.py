@@ -327,6 +327,45 @@ def test_no_streams_and_no_pages(dev):
     bare.evict(3)
 
 
+def test_streams_of_a_pool_without_pages(dev):
+    """Tables whose every number is outside the pool, which has no page: nothing is read, streams lose what is not there."""
+    m = make([20, 3, 0], 8, 2, 16, torch.float32, 61)
+    memory = on(dev, {f: t[:0] if f in ("key", "value", "usage", "positions") else t for f, t in m.items()})
+    t = torch.ones(3, 2, 16, device=dev)
+    assert not bool(memory.attend(t, track=True).any())
+    memory.evict(5, 2)
+    assert memory.lengths.tolist() == [5, 3, 0] and memory.seen.tolist() == m["seen"].tolist()
+    memory.append(t, t)
+    assert memory.lengths.tolist() == [6, 4, 1] and memory.seen.tolist() == (m["seen"] + 1).tolist()
+    assert not bool(memory.attend(t, track=True).any())
+
+
+def test_more_pages_and_heads_than_32_bits_count(dev):
+    """Usage and positions behind the 2^31st: a page's number times the heads."""
+    heads, pages = 1 << 20, 2060
+    gen = torch.Generator(device=dev).manual_seed(62)
+    usage = torch.rand((4, heads, 1), generator=gen, device=dev)
+    positions = torch.arange(4, dtype=torch.int32, device=dev).view(4, 1, 1).expand(4, heads, 1).contiguous()
+    key = torch.randn((4, heads, 1, 1), generator=gen, device=dev).to(torch.bfloat16)
+    count = torch.full((1,), 4, dtype=torch.int32, device=dev)
+    at = torch.tensor([[pages - 1, 1, pages - 2, 0]], dtype=torch.int32, device=dev)
+
+    def spread(t):
+        out = torch.zeros((pages, *t.shape[1:]), dtype=t.dtype, device=dev)
+        out[at[0].long()] = t
+        return out
+    far = d2c.PagedMemory(spread(key), spread(-key), at, count.clone(), count.clone(), spread(usage), spread(positions))
+    near = d2c.PagedMemory(key, -key, torch.arange(4, dtype=torch.int32, device=dev).view(1, 4), count.clone(), count.clone(), usage.clone(), positions.clone())
+    for memory in (near, far):
+        memory.evict(2, 1)
+    assert far.lengths.tolist() == [2]
+    a, b, c = usage[:3, :, 0]
+    best = torch.where((a >= b) & (a >= c), 0, torch.where(b >= c, 1, 2))      # (beside the newest, 3)
+    assert torch.equal(near.positions[:2, :, 0].sort(dim=0).values.long(), torch.stack([best, torch.full_like(best, 3)]))
+    for f in ("key", "value", "usage", "positions"):
+        assert torch.equal(getattr(near, f), getattr(far, f)[at[0].long()]), f
+
+
 def test_refused_on_the_gpu(dev):
     memory = d2c.PagedMemory.empty(2, 40, 2, 16, page=8, dtype=torch.float32, device=dev)
     q = torch.zeros(2, 4, 16, device=dev)
