@@ -366,8 +366,8 @@ def packed_attention(query, key, value, starts, key_starts=None, causal=True, fr
     _check(query.dtype == key.dtype == value.dtype, "packed_attention: query, key and value must have one dtype")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     _check(0.0 < scale < math.inf, f"packed_attention: scale must be positive and finite, got {scale}")
+    _check(int(frame) == frame and 0 < frame <= 1 << 30, f"packed_attention: a frame has 1 to 2^30 tokens, got {frame}")
     frame = int(frame)
-    _check(0 < frame <= 1 << 30, f"packed_attention: a frame has 1 to 2^30 tokens, got {frame}")
 
     def whole(name, t, tokens):
         _check(t.dim() == 1 and t.numel() > 0 and not t.is_floating_point() and not t.is_complex() and t.dtype != torch.bool,

@@ -1112,7 +1112,8 @@ extern "C" int d2c_memory_append(const d2c_memory_desc *q, void *key, void *valu
     if (int rc = check(q)) return rc;
     if (tokens < 0 || tokens >= (1L << 26) || (!starts && tokens != q->streams)) { d2c_set_error("memory_append: %ld tokens for %d streams", (long)tokens, q->streams); return D2C_ERR_SHAPE; }
     if (q->streams == 0) return D2C_OK;
-    if (!lengths || !seen || (q->per_stream > 0 && !table) || (q->pages > 0 && (!key || !value || !usage || !positions)) || (tokens > 0 && (!new_key || !new_value))) {
+    if (!lengths || !seen || (q->per_stream > 0 && !table) || (q->pages > 0 && (!key || !value || !usage || !positions)) || (tokens > 0 && (!new_key || !new_value)) ||
+        !new_key_stride || !new_value_stride) {
         d2c_set_error("null tensor pointer");
         return D2C_ERR_SHAPE;
     }

@@ -990,6 +990,14 @@ bool memory_desc(d2c_memory_desc &q, const Tensor &key, const Tensor &value, con
     return true;
 }
 bool is_counts(const Tensor &t, const Tensor &like) { return plain(t) && t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == like.size(0); }
+// Whether a call may write to these keys and values: no two of their elements are the same (expanded tensors), and no gradient of them is wanted
+bool writable(const Tensor &key, const Tensor &value)
+{
+    for (const Tensor *t : {&key, &value})
+        for (int i = 0; i < 3; i++)
+            if (t->size(i) > 1 && t->stride(i) <= 0) return false;
+    return !wants_grad(key, value);
+}
 // (a change that autograd is to notice where it has saved the tensor)
 void changed(std::initializer_list<const Tensor *> tensors)
 {
@@ -1001,7 +1009,7 @@ py::object memory_append(const Tensor &key, const Tensor &value, const Tensor &t
 {
     d2c_memory_desc q;
     const Tensor first = starts.value_or(Tensor());
-    if (!memory_desc(q, key, value, table, lengths, usage, positions) || !is_counts(seen, lengths) || wants_grad(new_key, new_value)) return py::none();
+    if (!memory_desc(q, key, value, table, lengths, usage, positions) || !is_counts(seen, lengths) || !writable(key, value) || wants_grad(new_key, new_value)) return py::none();
     for (const Tensor *t : {&new_key, &new_value})
         if (!plain_strided(*t) || t->dim() != 3 || t->numel() == 0 || t->device() != key.device() || !inner_contiguous(*t) || t->scalar_type() != key.scalar_type() ||
             t->size(0) != new_key.size(0) || t->size(1) != q.heads || t->size(2) != q.D)
@@ -1044,7 +1052,7 @@ py::object memory_evict(const Tensor &key, const Tensor &value, const Tensor &ta
                         int64_t keep, int64_t recent)
 {
     d2c_memory_desc q;
-    if (!memory_desc(q, key, value, table, lengths, usage, positions) || !is_counts(seen, lengths)) return py::none();
+    if (!memory_desc(q, key, value, table, lengths, usage, positions) || !is_counts(seen, lengths) || !writable(key, value)) return py::none();
     if (keep <= 0 || keep >= (1ll << 31) || recent < 0 || recent > keep) return py::none();
     c10::DeviceGuard guard(key.device());
     const size_t nb = d2c_memory_evict_workspace_bytes(&q, (int)keep);

@@ -27,7 +27,8 @@ class PagedMemory:
     int32: slot s of stream n is slot s % page of page table[n, s // page] (a number outside the pool: those slots are not there);
     `lengths` [streams] int32: slots that a stream has; `seen` [streams] int32: tokens it has had; `usage` [pages, heads, page]
     float32: the weights that a slot's token has got; `positions` [pages, heads, page] int32: which of the stream's tokens it is.
-    The tensors are the caller's, and all that a call changes.  Streams that are written to share no page."""
+    The tensors are the caller's, and all that a call changes.  Streams that are written to (reading with `track` writes usage) share no
+    page, and none has a page twice."""
 
     __slots__ = ("key", "value", "table", "lengths", "seen", "usage", "positions")
 
@@ -65,8 +66,8 @@ class PagedMemory:
         return self
 
 
-def _memory_desc(what, m, also=()):
-    """The description of a memory, its tensors checked."""
+def _memory_desc(what, m, written=False):
+    """The description of a memory, its tensors checked; `written`: the call changes keys and values."""
     _check(isinstance(m, PagedMemory), f"{what}: memory must be a PagedMemory")
     _check_tensors(what, **{name: getattr(m, name) for name in PagedMemory.__slots__})
     k = m.key
@@ -77,6 +78,9 @@ def _memory_desc(what, m, also=()):
     _check(heads > 0 and page > 0 and channels > 0, f"{what}: heads, slots of a page and channels must be positive, got {tuple(k.shape)}")
     _check(channels <= 128, f"{what}: heads of up to 128 channels, got {channels}")
     _check(all(t.stride(3) == 1 or channels == 1 for t in (k, m.value)), f"{what}: the channels of key and value must be adjacent")
+    if written:
+        _check(all(t.size(i) <= 1 or t.stride(i) > 0 for t in (k, m.value) for i in range(3)), f"{what}: key and value must not overlap themselves (expanded tensors)")
+        _no_gradient(what, k, m.value)
     _check(m.table.dim() == 2 and m.table.dtype == torch.int32 and (m.table.stride(1) == 1 or m.table.size(1) <= 1),
            f"{what}: table must be int32 [streams, pages of a stream], rows without gaps")
     streams = m.table.size(0)
@@ -103,7 +107,7 @@ def memory_append(memory, key, value, starts=None):
         m = memory
         if _try_native("memory_append", m.key, m.value, m.table, m.lengths, m.seen, m.usage, m.positions, key, value, starts):
             return
-    desc = _memory_desc("memory_append", memory)
+    desc = _memory_desc("memory_append", memory, True)
     _check_tensors("memory_append", memory=memory.key, key=key, value=value, starts=starts)
     for name, t in (("key", key), ("value", value)):
         _check(t.dim() == 3 and tuple(t.shape[1:]) == (desc.heads, desc.D) and t.dtype == memory.key.dtype,
@@ -172,12 +176,14 @@ def memory_evict(memory, keep, recent=0):
     largest usage (the lower slot of two with the same; a usage that is no number counts as the largest), `keep` in all.  Tokens that stay behind slot keep - 1
     move into the places of those that go, in order, with their usage and position; no other token moves.  lengths becomes
     keep there."""
+    for name, v in (("keep", keep), ("recent", recent)):
+        _check(int(v) == v, f"memory_evict: {name} must be a whole number, got {v}")
     keep, recent = int(keep), int(recent)
     if isinstance(memory, PagedMemory):
         m = memory
         if _try_native("memory_evict", m.key, m.value, m.table, m.lengths, m.seen, m.usage, m.positions, keep, recent):
             return
-    desc = _memory_desc("memory_evict", memory)
+    desc = _memory_desc("memory_evict", memory, True)
     _check(0 < keep < 1 << 31, f"memory_evict: keep must be positive, got {keep}")
     _check(0 <= recent <= keep, f"memory_evict: recent must be in 0 .. keep ({keep}), got {recent}")
     changed = (memory.key, memory.value, memory.lengths, memory.usage, memory.positions)

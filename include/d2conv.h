@@ -583,7 +583,7 @@ int d2c_packed_attention_backward(const d2c_packed_attention_desc *desc, const v
  * d2c_memory_append: token i of stream n's new ones goes to slot lengths[n] + i with usage 0 and position seen[n] + i, and lengths[n] and
  * seen[n] grow by their number.  new_key, new_value [tokens][heads][D] with strides (token, head); stream n's are the tokens starts[n]
  * .. starts[n + 1] - 1 (int32 [streams + 1], rising; taken into 0 .. tokens), or, starts NULL, token n (tokens == streams).  What has no slot
- * is dropped, lengths stay within the slots.  Streams of one memory share no page that they write to.
+ * is dropped, lengths stay within the slots.  Streams share no page that a call writes to, and none has such a page twice.
  *
  * d2c_memory_attention: one token of each stream, query [streams][query_heads][D] with strides (stream, head), query_heads a multiple of
  * heads, 256 to a head at most, D up to 128; out [streams][query_heads][D] contiguous:

@@ -376,7 +376,18 @@ def test_refused_on_the_gpu(dev):
                           (lambda: memory.append(k[:1], k[:1]), "one token of each"), (lambda: memory.append(k, k[:1]), "values"),
                           (lambda: memory.append(k, k, torch.zeros(2, device=dev, dtype=torch.int32)), "whole numbers"),
                           (lambda: memory.append(k, k, torch.zeros(3, device=dev)), "whole numbers"), (lambda: memory.evict(0), "positive"),
-                          (lambda: memory.evict(3, 4), "recent"), (lambda: memory.evict(3, -1), "recent")):
+                          (lambda: memory.evict(2.5), "whole number"), (lambda: memory.evict(3, 0.5), "whole number"), (lambda: memory.evict(3, 4), "recent"), (lambda: memory.evict(3, -1), "recent")):
         with pytest.raises(RuntimeError, match=message):
             call()
+    assert not bool(memory.lengths.any())
+    # keys that lie in one place, and keys whose gradient is wanted, are read, but not written to
+    for change in (lambda t: t[:1].expand(t.shape), lambda t: t.clone().requires_grad_()):
+        for which in ("key", "value"):
+            other = d2c.PagedMemory(*(getattr(memory, f) for f in _memory.FIELDS))
+            setattr(other, which, change(getattr(memory, which)))
+            for call in (lambda: other.append(k, k), lambda: other.evict(3)):
+                with pytest.raises(RuntimeError, match="overlap themselves|no gradient"):
+                    call()
+            with torch.no_grad():
+                other.attend(q)
     assert not bool(memory.lengths.any())

@@ -55,10 +55,12 @@ def test_calls_that_are_refused():
     assert lib.d2c_memory_append(ctypes.byref(desc()), *(None,) * 9, strides, strides, None, 2, None) != 0 and "null" in _lib.last_error()
     for tokens in (-1, 3, 1 << 40):
         assert lib.d2c_memory_append(ctypes.byref(desc()), *(None,) * 9, strides, strides, None, tokens, None) != 0 and "tokens" in _lib.last_error()
+    some = ctypes.c_void_p(4096)
+    assert lib.d2c_memory_append(ctypes.byref(desc()), *(some,) * 9, None, strides, None, 2, None) != 0 and "null" in _lib.last_error()
+    assert lib.d2c_memory_append(ctypes.byref(desc()), *(some,) * 9, strides, None, None, 2, None) != 0 and "null" in _lib.last_error()
     for keep, recent in ((0, 0), (-1, 0), (5, 6), (5, -1)):
         assert lib.d2c_memory_evict(ctypes.byref(desc()), *(None,) * 7, keep, recent, None, 0, None) != 0 and "keep" in _lib.last_error()
     # a workspace that is not there, too small, or not aligned
-    some = ctypes.c_void_p(4096)
     nb = lib.d2c_memory_evict_workspace_bytes(ctypes.byref(desc()), 3)
     assert nb > 0
     for ws, have in ((None, 0), (ctypes.c_void_p(1 << 20), nb - 1), (ctypes.c_void_p((1 << 20) + 16), nb)):

@@ -66,6 +66,7 @@ STARTS = torch.tensor([0, 4, 6]).as_subclass(OnTheGpu)
     ((gpu(6, 2, 16), gpu(6, 1, 16), gpu(6, 1, 16), gpu(0, dtype=torch.int32)), {}, "whole numbers"),
     ((gpu(6, 2, 16), gpu(6, 1, 16), gpu(6, 1, 16), STARTS, STARTS[:2]), {}, "key_starts"),
     ((gpu(6, 2, 16), gpu(6, 1, 16), gpu(6, 1, 16), STARTS), dict(frame=0), "frame"),
+    ((gpu(6, 2, 16), gpu(6, 1, 16), gpu(6, 1, 16), STARTS), dict(frame=1.5), "frame"),
     ((gpu(6, 2, 16), gpu(6, 1, 16), gpu(6, 1, 16), STARTS), dict(scale=-1.0), "scale"),
     ((gpu(6, 2, 16).double(), gpu(6, 1, 16).double(), gpu(6, 1, 16).double(), STARTS), {}, "unsupported dtype"),
 ])
