@@ -32,18 +32,19 @@ D2C_DEV void region_of(const int32_t *starts, int S, int T, int i, int &first, i
     first = bound_of(starts, S, T, i);
     count = max((i > S ? T : bound_of(starts, S, T, i + 1)) - first, 0);
 }
-// The region of tile `at` of the line, and which of its tiles that is.  `group`: rows to a token
+// The region of tile `at` of the line, and which of its tiles that is.  `group`: rows to a token.  64 regions to a vote, three votes to 2^18: 6480 sequences of 8 tokens, 8 heads
+// of 64, bfloat16, 448 us (1466 with regions taken 64 after 64)
 D2C_DEV void find_tile(const int32_t *starts, int S, int T, int group, int at, int &region, int &tile)
 {
     const int lane = threadIdx.x & 63;
     auto begin = [&](int i) INLINE { return (int)((long)bound_of(starts, S, T, i) * group / kRows) + i; };
     region = 0;
-    for (int i0 = 0; i0 <= S + 1; i0 += 64) {
-        const int i = i0 + lane;
-        const uint64_t before = __ballot(i <= S + 1 && begin(min(i, S + 1)) <= at);
-        if (before == 0) break;
-        region = i0 + (before == ~0ull ? 63 : __builtin_ctzll(~before) - 1);
-        if (before != ~0ull) break;
+    for (int n = S + 2; n > 1;) {      // (it is one of the n regions from `region` on; each lane asks for one of 64, the first of which is known to begin in time)
+        const int step = (n + 63) / 64, i = lane * step;
+        const uint64_t before = __ballot(i < n && begin(region + min(i, n - 1)) <= at);
+        const int last = before == ~0ull ? 63 : __builtin_ctzll(~before) - 1;
+        region += last * step;
+        n = min(step, n - last * step);
     }
     region = __builtin_amdgcn_readfirstlane(region);
     tile = at - begin(region);

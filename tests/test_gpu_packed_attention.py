@@ -51,6 +51,7 @@ CASES = [
     ([1] * 70 + [3, 0, 130], None, 2, 1, 48, True, 1, 1, 1),
     ([2, 3, 1, 0] * 60, None, 1, 1, 8, True, 2, 0, 0),
     ([526], [984], 8, 8, 120, True, 1, 0, 0),
+    ([1, 2, 0, 3] * 1100, None, 1, 1, 8, True, 1, 2, 1),     # more sequences than two steps of the search tell apart
 ]
 
 
