@@ -32,22 +32,25 @@ D2C_DEV void region_of(const int32_t *starts, int S, int T, int i, int &first, i
     first = bound_of(starts, S, T, i);
     count = max((i > S ? T : bound_of(starts, S, T, i + 1)) - first, 0);
 }
-// The region of tile `at` of the line, and which of its tiles that is.  `group`: rows to a token.  64 regions to a vote, three votes to 2^18: 6480 sequences of 8 tokens, 8 heads
-// of 64, bfloat16, 448 us (1466 with regions taken 64 after 64)
-D2C_DEV void find_tile(const int32_t *starts, int S, int T, int group, int at, int &region, int &tile)
+// The region of tile `at` of the line, which of its tiles that is, its first token and how many it has.  `group`: rows to a token.  63 regions to a vote, three votes to 250000; the last has the
+// region's bounds as well.  6480 sequences of 8 tokens, 8 heads of 64, bfloat16: 440 us (448 with the bounds asked for afterwards, 1466 with regions taken 64 after 64)
+D2C_DEV void find_tile(const int32_t *starts, int S, int T, int group, int at, int &region, int &tile, int &first, int &count)
 {
     const int lane = threadIdx.x & 63;
-    auto begin = [&](int i) INLINE { return (int)((long)bound_of(starts, S, T, i) * group / kRows) + i; };
+    auto begin = [&](int bound, int i) INLINE { return (int)((long)bound * group / kRows) + i; };
     region = 0;
-    for (int n = S + 2; n > 1;) {      // (it is one of the n regions from `region` on; each lane asks for one of 64, the first of which is known to begin in time)
-        const int step = (n + 63) / 64, i = lane * step;
-        const uint64_t before = __ballot(i < n && begin(region + min(i, n - 1)) <= at);
-        const int last = before == ~0ull ? 63 : __builtin_ctzll(~before) - 1;
+    for (int n = S + 2;;) {      // (it is one of the n regions from `region` on, whose first is known to begin in time)
+        const int step = (n + 62) / 63, i = lane * step, bound = bound_of(starts, S, T, region + i);
+        const int last = __builtin_ctzll(~__ballot(i < n && begin(bound, region + i) <= at)) - 1;      // (lane 63 is behind all of them)
         region += last * step;
+        if (step == 1) {
+            first = __builtin_amdgcn_readlane(bound, last);
+            count = max(__builtin_amdgcn_readlane(bound, last + 1) - first, 0);
+            break;
+        }
         n = min(step, n - last * step);
     }
-    region = __builtin_amdgcn_readfirstlane(region);
-    tile = at - begin(region);
+    tile = at - begin(first, region);
 }
 
 // A workgroup's sequence and tile
@@ -61,11 +64,16 @@ template <bool BY_KEYS> D2C_DEV PackedUnit unit_of(const PackedArgs &a, int inde
     u.h = index - rest * a.Hkv;
     u.split = rest / a.tiles;
     u.at = BY_KEYS ? line : a.tiles - 1 - line;
-    int region;
-    find_tile(BY_KEYS ? a.key_starts : a.starts, a.S, BY_KEYS ? a.Tk : a.T, BY_KEYS ? 1 : a.group, u.at, region, u.tile);
+    int region, first, count;
+    find_tile(BY_KEYS ? a.key_starts : a.starts, a.S, BY_KEYS ? a.Tk : a.T, BY_KEYS ? 1 : a.group, u.at, region, u.tile, first, count);
     u.q0 = u.lq = u.k0 = u.lk = 0;
-    if (!BY_KEYS || (region >= 1 && region <= a.S)) region_of(a.starts, a.S, a.T, region, u.q0, u.lq);
-    if (BY_KEYS || (region >= 1 && region <= a.S)) region_of(a.key_starts, a.S, a.Tk, region, u.k0, u.lk);
+    (BY_KEYS ? u.k0 : u.q0) = first;
+    (BY_KEYS ? u.lk : u.lq) = count;
+    if (region >= 1 && region <= a.S) {
+        int &other = BY_KEYS ? u.q0 : u.k0, &others = BY_KEYS ? u.lq : u.lk;
+        if (a.starts == a.key_starts && a.T == a.Tk) { other = first; others = count; }
+        else region_of(BY_KEYS ? a.starts : a.key_starts, a.S, BY_KEYS ? a.T : a.Tk, region, other, others);
+    }
     u.rows = u.lq * a.group;
     return u;
 }
