@@ -119,6 +119,32 @@ def test_pages_that_are_not_there(short, dtype, dev):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length,hq", [(60, 1), (60, 4), (60, 8), (60, 20), (4000, 1), (4000, 4), (4000, 7), (4000, 16), (4000, 40)])
+def test_infinities_that_are_read(length, hq, dtype, dev):
+    """An infinite value, or one that is no number, in a slot that is there is all of its channel; a score of -infinity has no weight, one of
+    +infinity leaves no number."""
+    D, slot = 40, 37
+    m = make([length, length], 16, 1, D, dtype, 71)
+    q = torch.randn(2, hq, D, generator=torch.Generator().manual_seed(72)).to(dtype)
+    q[:, :, 5] = torch.where(torch.arange(hq) % 2 == 0, -1.0, 1.0).to(dtype)
+    at = (int(m["table"][1, slot // 16]), 0, slot % 16)
+    as_it_is = on(dev, m).attend(q.to(dev)).cpu()
+    for i, x in enumerate((math.inf, -math.inf, math.nan)):
+        m["value"][at][i] = x
+    here = on(dev, m).attend(q.to(dev)).cpu()
+    assert torch.equal(here[0], as_it_is[0]) and torch.equal(here[1, :, 3:], as_it_is[1, :, 3:])
+    assert bool((here[1, :, 0] == math.inf).all()) and bool((here[1, :, 1] == -math.inf).all()) and bool(here[1, :, 2].isnan().all())
+    m["value"][at] = 1.0
+    m["key"][at][5] = math.inf
+    here = on(dev, m).attend(q.to(dev)).cpu()
+    assert torch.equal(here[0], as_it_is[0]) and bool(here[1, 1::2].isnan().all())
+    m["key"][at] = 0.0
+    m["key"][at][5] = torch.finfo(dtype).max / 4      # (a finite score so low that its weight is 0 as well)
+    low = on(dev, m).attend(q.to(dev)).cpu()
+    assert torch.equal(here[1, 0::2], low[1, 0::2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_strides(dtype, dev):
     """Pages with the heads inside, a query that is part of a projection, rows of a table that lie apart, heads at an odd place."""
     m = make([200, 77], 16, 2, 40, dtype, seed=10, garbage=0.0)
