@@ -44,7 +44,7 @@ template <typename T> constexpr int kTerms = sizeof(T) == 2 ? 1 : 3;
 // forward and backward, 3260, 4717).  Where a call has 64 keys or fewer, errors do not average out (two keys: weights just above 1/2, where the spacing is
 // widest), nor in the gradients of a small problem: these have the second term, at 1.11 to 1.16 times the backward kernels' time where the line is (512 rows on
 // 1024 keys of 8 heads of 64, 38.1, 42.9 us; of 128, 54.6, 63.0; whole passes are the host's 55 to 85 us either way).  Calls count, not samples: two keys that a mask leaves
-// of 1000 have weights of one term in a large call.  (Heads of an odd size, and rows that lie further apart than 32-bit offsets reach, run on the same kernels and have it, too.)
+// of 1000 have weights of one term in a large call (attention inside packed sequences tells tile by tile: d2c_packed.hpp).  (Heads of an odd size, and rows that lie further apart than 32-bit offsets reach, run on the same kernels and have it, too.)
 template <typename T, bool FAST> constexpr int kWeightTerms = sizeof(T) == 4 ? 3 : FAST ? 1 : 2;
 constexpr int kExactKeys = 64;
 constexpr long kExactScores = 1L << 22;

@@ -20,19 +20,16 @@ template <typename T, int DP, bool WHOLE> struct FwdShape {
 // workgroups of a compute unit have room for at 64 channels.  Bound: matrix instructions and the exponentials, maxima, sums and roundings between them.
 // Measured, bfloat16: 16 pieces of up to 4096 queries on up to 12288 keys, 16 heads of 128 that share 4, 1.94 ms (0.96 PFLOP/s; a library product of 8192 cubed 1.22); one sequence of 25920, 8
 // heads of 64 that share 2, 0.79 ms (0.87); six of up to 12960 in frames of 1620, 8 heads of 64, 0.73 ms (0.79).  float32: three of up to 1417, 6 heads of 40, 32 us and the join 5.8.
-template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, 2) packed_fwd_kernel(PackedArgs a)
+template <typename T, int DP, int NP, bool WHOLE, int PW> D2C_DEV void fwd_rows(const PackedArgs &a, const PackedUnit &u)
 {
     using Shape = FwdShape<T, DP, WHOLE>;
     using KV = typename Shape::KV;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, KT = Shape::KT, NS = KT / 32, BUFFERS = Shape::BUFFERS;
+    constexpr int P = kTerms<T>, ND = DP / 32, NK = kSteps<NP>, KT = Shape::KT, NS = KT / 32, BUFFERS = Shape::BUFFERS;
     constexpr bool END = WHOLE && NP % 2 == 1;
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ int s_bad;      // whether a tile's values were cleaned
     if (threadIdx.x == 0) s_bad = 0;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const PackedUnit u = unit_of<false>(a, blockIdx.x);
-    const int row0 = u.tile * kRows;
-    if (row0 >= u.rows) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, row0 = u.tile * kRows;
     const int tile_row = wave * 32 + (lane & 31), row = row0 + tile_row;
     const bool live = row < u.rows;
     // limits rise with the rows: this lane's, the smallest of the workgroup's, the largest and the smallest of the wavefront's
@@ -176,6 +173,14 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
             if (a.out_low) store4_low<T>(reinterpret_cast<T *>(a.out_low) + (orow - reinterpret_cast<T *>(a.out)) + d, x, a.D - d);
         }
     if (a.lse && half == 0) a.lse[(long)u.h * a.T * a.group + (long)u.q0 * a.group + row] = l == 0.f ? INFINITY : mc + log2f(l);
+}
+
+template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, 2) packed_fwd_kernel(PackedArgs a)
+{
+    const PackedUnit u = unit_of<false>(a, blockIdx.x);
+    if (u.tile * kRows >= u.rows) return;
+    constexpr int TERMS = kWeightTerms<T, WHOLE>;
+    with_terms<TERMS>(a, u, TERMS == 1 && few_keys(a, u), [](const PackedArgs &b, const PackedUnit &w, auto terms) INLINE { fwd_rows<T, DP, NP, WHOLE, decltype(terms)::value>(b, w); });
 }
 
 // The partial results of the workgroups that shared a walk: a workgroup to 16 rows of a tile, a thread to four columns and those 64 further on, four splits

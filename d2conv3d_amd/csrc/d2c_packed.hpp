@@ -85,6 +85,34 @@ D2C_DEV int limit_of(const PackedArgs &a, const PackedUnit &u, int pos)
     return p < 0 ? 0 : min(u.lk, (fdiv(p, a.frame) + 1) * a.frame.d);
 }
 D2C_DEV int limit_of_row(const PackedArgs &a, const PackedUnit &u, int row) { return limit_of(a, u, fdiv(row, a.by_group)); }
+// The first row that reads key `key`
+D2C_DEV int first_row(const PackedArgs &a, const PackedUnit &u, int key) { return a.causal ? max(fdiv(key, a.frame) * a.frame.d - (u.lk - u.lq), 0) * a.group : 0; }
+
+// Kernels of one term of the weights (bfloat16, see kWeightTerms) take two for tiles that have sums of 64 terms or fewer, which do not average out: a tile of rows whose first reads no more
+// keys, a tile of keys whose last is read by no more rows.  So results whose sums are as short, a short sequence's and those of a long one's first and last tokens, have two whatever they are
+// packed with.  Such tiles' walks are short, as limits go by token or frame: forward and backward, 8 heads of 64, 500 sequences of 100 take 366 us (350 with one term everywhere), 200 of 200 279 (271);
+// the longer the sequences, the fewer such tiles.  Rows of 2 to 4 keys are off by up to 0.0068 of sum p |v| with one term, by 0.0039, the result's own rounding, with two.
+D2C_DEV bool few_keys(const PackedArgs &a, const PackedUnit &u) { return limit_of_row(a, u, u.tile * kRows) <= kExactKeys; }
+D2C_DEV bool few_rows(const PackedArgs &a, const PackedUnit &u) { return u.rows - first_row(a, u, min(u.tile * kRows + kRows, u.lk) - 1) <= kExactKeys; }
+// f(arguments, unit, terms): two bodies of a kernel, of which a workgroup takes one.  The second reads the kernel's arguments anew and has a copy of the unit that the compiler knows nothing of: it
+// would take what both bodies have in common in front of the branch, and the first was 2 to 10% slower for it (products of the second term behind a branch inside the loop made kernels take 30
+// to 45 registers more, or spill up to 340).
+template <int TERMS, typename F> D2C_DEV void with_terms(const PackedArgs &a, const PackedUnit &u, bool few, F f)
+{
+    if constexpr (TERMS == 1)
+        if (few) {
+            auto *args = (const __attribute__((address_space(4))) PackedArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+            asm volatile("" : "+s"(args));
+            const PackedArgs b = *(const PackedArgs *)args;
+            PackedUnit w = u;
+            for (int *x : {&w.q0, &w.lq, &w.k0, &w.lk, &w.rows, &w.tile, &w.h, &w.at, &w.split}) {
+                *x = __builtin_amdgcn_readfirstlane(*x);
+                asm volatile("" : "+s"(*x));
+            }
+            return f(b, w, std::integral_constant<int, 2>{});
+        }
+    f(a, u, std::integral_constant<int, TERMS>{});
+}
 
 // Row `row` of a tensor [tokens][Hq][D] with strides s
 template <typename T> D2C_DEV const T *row_at(const void *base, const long *s, const PackedArgs &a, const PackedUnit &u, int row)
@@ -218,8 +246,8 @@ template <typename T, bool AS_NAN, int ND, typename Row, typename Read> D2C_DEV 
 }
 
 PackedArgs make_args(const d2c_packed_attention_desc &q, const int32_t *starts, const int32_t *key_starts);
-// Whether a problem runs on the kernels that load whole pieces by offsets of 32 bits inside a tile and, bfloat16, take one term of the weights: not where sequences have 64 keys or fewer on
-// the average, nor the backward pass where scores are few, whose errors do not average out (see kWeightTerms)
+// Whether a problem runs on the kernels that load whole pieces by offsets of 32 bits inside a tile and, bfloat16, take one term of the weights but in few tiles (with_terms): not where sequences
+// have 64 keys or fewer on the average, nor the backward pass where scores are few, whose errors do not average out (see kWeightTerms)
 inline bool fast_kernels(const d2c_packed_attention_desc &q, bool gradients)
 {
     const long average = q.keys / std::max(q.sequences, 1);
@@ -243,7 +271,7 @@ D2C_DEV Walk row_walk(const PackedArgs &a, const PackedUnit &u)
 // ... of keys: rows from the first that reads the first of them
 D2C_DEV Walk key_walk(const PackedArgs &a, const PackedUnit &u)
 {
-    const int key0 = u.tile * kRows, first = a.causal ? max(fdiv(key0, a.frame) * a.frame.d - (u.lk - u.lq), 0) * a.group / a.step : 0;
+    const int first = first_row(a, u, u.tile * kRows) / a.step;
     return walk_of(a, first, max((u.rows + a.step - 1) / a.step - first, 0));
 }
 // On the host, where only the average length is known: the longest walk is taken to be twice that of a sequence of the average length, or that of the only sequence.  Pieces cost a second

@@ -21,18 +21,15 @@ template <typename T, int DP, bool WHOLE> struct QShape {
 // twice, by rows and by columns; where it holds infinities or NaN and some rows do not read all of the tile, it is cleaned in LDS between the two).  Bound: matrix instructions (3 products to
 // one exponential).  Measured, bfloat16: one sequence of 25920, 8 heads of 64 that share 2, 1.06 ms (0.98 PFLOP/s); six of up to 12960 in frames, 8 heads of 64, 0.97 ms (0.90).  float32: three of up to
 // 1417, 6 heads of 40, 35 us and the join 4.9.
-template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, (QShape<T, DP, WHOLE>::WAVES)) packed_bwd_q_kernel(PackedArgs a)
+template <typename T, int DP, int NP, bool WHOLE, int PW> D2C_DEV void bwd_rows(const PackedArgs &a, const PackedUnit &u)
 {
     using Shape = QShape<T, DP, WHOLE>;
     using KV = typename Shape::KV;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, KT = Shape::KT, BUFFERS = Shape::BUFFERS;
+    constexpr int P = kTerms<T>, ND = DP / 32, NK = kSteps<NP>, KT = Shape::KT, BUFFERS = Shape::BUFFERS;
     constexpr bool END = WHOLE && NP % 2 == 1;
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ int s_bad[2][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const PackedUnit u = unit_of<false>(a, blockIdx.x);
-    const int row0 = u.tile * kRows;
-    if (row0 >= u.rows) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, row0 = u.tile * kRows;
     const int tile_row = wave * 32 + (lane & 31), row = row0 + tile_row;
     const bool live = row < u.rows;
     const int lim = live ? limit_of_row(a, u, row) : 0, least = limit_of_row(a, u, row0);
@@ -161,6 +158,14 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
         }
 }
 
+template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, (QShape<T, DP, WHOLE>::WAVES)) packed_bwd_q_kernel(PackedArgs a)
+{
+    const PackedUnit u = unit_of<false>(a, blockIdx.x);
+    if (u.tile * kRows >= u.rows) return;
+    constexpr int TERMS = kWeightTerms<T, WHOLE>;
+    with_terms<TERMS>(a, u, TERMS == 1 && few_keys(a, u), [](const PackedArgs &b, const PackedUnit &w, auto terms) INLINE { bwd_rows<T, DP, NP, WHOLE, decltype(terms)::value>(b, w); });
+}
+
 template <typename T, int DP, bool WHOLE> struct KvShape {
     // V of the workgroup's keys in LDS where registers do not hold it beside the sums
     static constexpr bool V_LDS = sizeof(T) == 2 && DP == 128;
@@ -177,17 +182,14 @@ template <typename T, int DP, bool WHOLE> struct KvShape {
 // (dk, dv).  dp starts from -delta.  As attn_bwd_kv_kernel; the walk begins with the first row that reads a key of the tile.  Bound: matrix instructions (4 products to one exponential), behind
 // them LDS.  Measured, bfloat16: one sequence of 25920, 8 heads of 64 that share 2, 1.54 ms and the join 24 us (0.90 PFLOP/s; 3.1 ms before walks were cut in pieces, the first keys' being as long
 // as the whole sequence); six of up to 12960 in frames, 8 heads of 64, 1.25 ms (0.93).  float32: three of up to 1417, 6 heads of 40, 45 us and the join 5.7.
-template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, (KvShape<T, DP, WHOLE>::WAVES)) packed_bwd_kv_kernel(PackedArgs a)
+template <typename T, int DP, int NP, bool WHOLE, int PW> D2C_DEV void bwd_keys(const PackedArgs &a, const PackedUnit &u)
 {
     using Shape = KvShape<T, DP, WHOLE>;
     using QG = typename Shape::QG;
-    constexpr int P = kTerms<T>, PW = kWeightTerms<T, WHOLE>, ND = DP / 32, NK = kSteps<NP>, RT = Shape::RT, BUFFERS = Shape::BUFFERS;
+    constexpr int P = kTerms<T>, ND = DP / 32, NK = kSteps<NP>, RT = Shape::RT, BUFFERS = Shape::BUFFERS;
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ int s_bad[2][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const PackedUnit u = unit_of<true>(a, blockIdx.x);
-    const int key0 = u.tile * kRows;
-    if (key0 >= u.lk) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, key0 = u.tile * kRows;
     const int tile_key = wave * 32 + (lane & 31), key = key0 + tile_key, keys_end = min(key0 + kRows, u.lk);
     const bool live = key < u.lk;
     const Walk walk = key_walk(a, u);
@@ -380,6 +382,14 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
                 if (a.gv) store4<T>(reinterpret_cast<T *>(a.gv) + at, y, a.D - d);
             }
         }
+}
+
+template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bounds__(256, (KvShape<T, DP, WHOLE>::WAVES)) packed_bwd_kv_kernel(PackedArgs a)
+{
+    const PackedUnit u = unit_of<true>(a, blockIdx.x);
+    if (u.tile * kRows >= u.lk) return;
+    constexpr int TERMS = kWeightTerms<T, WHOLE>;
+    with_terms<TERMS>(a, u, TERMS == 1 && few_rows(a, u), [](const PackedArgs &b, const PackedUnit &w, auto terms) INLINE { bwd_keys<T, DP, NP, WHOLE, decltype(terms)::value>(b, w); });
 }
 
 // Sums of the workgroups that shared a walk: a workgroup to 16 rows (or keys) of a tile, a thread to four columns and those 64 further on, four splits requested at a time.
