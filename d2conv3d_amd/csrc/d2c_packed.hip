@@ -324,7 +324,7 @@ extern "C" int d2c_packed_attention_forward(const d2c_packed_attention_desc *q, 
 {
     if (int rc = d2c_packed_attention_check(q)) return rc;
     if (q->queries == 0) return D2C_OK;
-    if (!query || !out || (q->keys > 0 && (!key || !value)) || (q->sequences > 0 && !starts)) { d2c_set_error("null tensor pointer"); return D2C_ERR_SHAPE; }
+    if (!query || !out || (q->keys > 0 && (!key || !value)) || !starts) { d2c_set_error("null tensor pointer"); return D2C_ERR_SHAPE; }
     PackedArgs a = make_args(*q, starts, key_starts);
     a.q = query; a.k = key; a.v = value; a.out = out; a.lse = lse;
     a.out_low = q->dtype == D2C_BF16 ? out_low : nullptr;

@@ -517,7 +517,7 @@ extern "C" int d2c_packed_attention_backward(const d2c_packed_attention_desc *q,
 {
     if (int rc = d2c_packed_attention_check(q)) return rc;
     if (q->queries == 0 && q->keys == 0) return D2C_OK;
-    if ((q->queries > 0 && (!grad_out || !query || !out || !lse)) || (q->keys > 0 && (!key || !value)) || (q->sequences > 0 && !starts)) {
+    if ((q->queries > 0 && (!grad_out || !query || !out || !lse)) || (q->keys > 0 && (!key || !value)) || !starts) {
         d2c_set_error("null tensor pointer");
         return D2C_ERR_SHAPE;
     }

@@ -549,7 +549,7 @@ int d2c_attention_backward(const d2c_attention_desc *desc, const void *grad_out,
 
 /* Attention inside each of several sequences that lie behind each other.  query [queries, Hq, D], key and value [keys, Hkv, D] with strides
  * (token, head; channels adjacent), Hq a multiple of Hkv, D up to 128.  Sequence s has the queries starts[s] .. starts[s + 1] - 1 and the keys
- * key_starts[s] .. key_starts[s + 1] - 1 (int32 [sequences + 1], rising, taken into 0 .. queries or keys; key_starts NULL: starts).  Its
+ * key_starts[s] .. key_starts[s + 1] - 1 (int32 [sequences + 1], one even where there are no sequences; rising, taken into 0 .. queries or keys; key_starts NULL: starts).  Its
  * queries are the last of its Lk tokens: query i of Lq is token p = Lk - Lq + i, and reads, `causal`, the first
  *     min(Lk, (floor(p / frame) + 1) * frame)        (p < 0: none)
  * keys -- frame 1: up to its own token; otherwise up to the end of its frame of so many tokens -- and all Lk if not.  Keys and values that
