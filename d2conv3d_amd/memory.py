@@ -6,12 +6,14 @@ computes clip after clip.)
     memory_attention   one new token of each stream reads what its stream has
     memory_evict       streams that are too long lose the tokens that were read least
 
-For inference: nothing here is differentiated.  float32 and bfloat16; weights, sums and usage are held in float32.
+For inference: nothing here is differentiated or recorded (a call whose gradient or tangent is wanted, or that torch.jit.trace would
+record, is refused).  float32 and bfloat16; weights, sums and usage are held in float32.
 """
 import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._ops import _DT, _ptr, _stream, _try_native, _workspace
@@ -94,6 +96,15 @@ def _memory_desc(what, m, written=False):
     return _lib.MemoryDesc(streams, heads, channels, _DT[k.dtype], pages, page, m.table.size(1), m.table.stride(0), *strides)
 
 
+def _not_recorded(what, memory, *tensors):
+    """No trace, of which the library's call would be no part, and no tangent, which the result would lack."""
+    _check(not torch.jit.is_tracing(), f"{what} is not recorded by torch.jit.trace: call it outside of what is traced")
+    if isinstance(memory, PagedMemory):
+        tensors += (memory.key, memory.value, memory.usage)
+    _check(all(forward_ad.unpack_dual(t).tangent is None for t in tensors if isinstance(t, torch.Tensor)),
+           f"{what} takes no forward-mode tangent")
+
+
 def _no_gradient(what, *tensors):
     _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)), f"{what} takes no gradient: call it under torch.no_grad()")
 
@@ -107,6 +118,7 @@ def memory_append(memory, key, value, starts=None):
         m = memory
         if _try_native("memory_append", m.key, m.value, m.table, m.lengths, m.seen, m.usage, m.positions, key, value, starts):
             return
+    _not_recorded("memory_append", memory, key, value)
     desc = _memory_desc("memory_append", memory, True)
     _check_tensors("memory_append", memory=memory.key, key=key, value=value, starts=starts)
     for name, t in (("key", key), ("value", value)):
@@ -145,6 +157,7 @@ def memory_attention(query, memory, scale=None, track=False):
         out = _try_native("memory_attention", query, m.key, m.value, m.table, m.lengths, m.usage, m.positions, scale, bool(track))
         if out is not None:
             return out
+    _not_recorded("memory_attention", memory, query)
     desc = _memory_desc("memory_attention", memory)
     _check_tensors("memory_attention", memory=memory.key, query=query)
     _check(query.dim() == 3 and query.size(0) == desc.streams and query.size(2) == desc.D and query.dtype == memory.key.dtype,
@@ -183,6 +196,7 @@ def memory_evict(memory, keep, recent=0):
         m = memory
         if _try_native("memory_evict", m.key, m.value, m.table, m.lengths, m.seen, m.usage, m.positions, keep, recent):
             return
+    _not_recorded("memory_evict", memory)
     desc = _memory_desc("memory_evict", memory, True)
     _check(0 < keep < 1 << 31, f"memory_evict: keep must be positive, got {keep}")
     _check(0 <= recent <= keep, f"memory_evict: recent must be in 0 .. keep ({keep}), got {recent}")
