@@ -186,9 +186,10 @@ def memory_attention(query, memory, scale=None, track=False):
 
 def memory_evict(memory, keep, recent=0):
     """Streams of more than `keep` tokens lose some, each head its own: the newest `recent` stay, and of the others those of the
-    largest usage (the lower slot of two with the same; a usage that is no number counts as the largest), `keep` in all.  Tokens that stay behind slot keep - 1
-    move into the places of those that go, in order, with their usage and position; no other token moves.  lengths becomes
-    keep there."""
+    largest usage (the lower slot of two with the same; a usage that is no number counts as the largest), `keep` in all.  Tokens that
+    stay behind slot keep - 1 move into the places of those that go, in order, with their usage and position; no other token moves.
+    lengths becomes keep there.  Slots that are not there (of pages outside the pool) count and are the first to go; where one lies
+    before `keep`, the token that would move into it is lost, even a newest one: let the pages of a stream's first `keep` slots be there."""
     for name, v in (("keep", keep), ("recent", recent)):
         _check(int(v) == v, f"memory_evict: {name} must be a whole number, got {v}")
     keep, recent = int(keep), int(recent)

@@ -594,7 +594,8 @@ int d2c_packed_attention_backward(const d2c_packed_attention_desc *desc, const v
  * d2c_memory_evict: of every stream with more than `keep` (> 0) slots, and for each head alone, these stay: slots whose position is at least
  * seen[n] - recent, and of the others those of the largest usage (ties: the lower slot; NaN above all numbers), `keep` in all.  What stays
  * behind slot keep - 1 moves into the places of what goes before it, the i-th into the i-th, with its usage and position; nothing else
- * moves.  lengths[n] becomes keep.  (Slots that are not there are the first to go.) */
+ * moves.  lengths[n] becomes keep.  Slots that are not there count among the slots and are the first to go: where such a slot lies before `keep`, the
+ * token that would move into it is lost, one of the newest like any other.  (So a stream whose first `keep` slots are all there loses what it is said to, and no more.) */
 typedef struct d2c_memory_desc {
     int32_t streams, heads, D, dtype, pages, page, per_stream;
     int64_t table_stride, key_stride[3], value_stride[3];
