@@ -1088,6 +1088,27 @@ MemPlan mem_plan(const d2c_memory_desc &q, const d2c_memory_query_desc &x, bool 
     return p;
 }
 
+// A call's streams, as many at a time as the limit has room for what goes by their slots, `bytes` of each: tables may have room for many times what streams hold, and lengths are not known here.
+// All parts but the last have the same number.
+inline int streams_at_once(int streams, size_t bytes, size_t limit)
+{
+    const long most = std::max((long)(limit / std::max(bytes, (size_t)1)), 1L), parts = (streams + most - 1) / most;
+    return parts <= 1 ? streams : (int)((streams + parts - 1) / parts);
+}
+inline d2c_memory_desc with_streams(d2c_memory_desc q, int streams) { q.streams = streams; return q; }
+// f(first stream, description of a part): the first result that is not D2C_OK
+template <typename F> int for_streams(const d2c_memory_desc &q, int at_once, F f)
+{
+    for (int n = 0; n < q.streams; n += at_once)
+        if (int rc = f(n, with_streams(q, std::min(at_once, q.streams - n)))) return rc;
+    return D2C_OK;
+}
+// Scores of a tracked call: as the partial sums of attention, 256 MB at most (64 streams with room for 129600 tokens, 48 query heads: 1.6 GB otherwise)
+int attention_streams(const d2c_memory_desc &q, const d2c_memory_query_desc &x, bool track)
+{
+    return track ? streams_at_once(q.streams, mem_plan(with_streams(q, 1), x, true).scores_bytes, D2C_ATTENTION_PART_BYTES) : q.streams;
+}
+
 struct EvictPlan { int pairs; long slots_padded; size_t ranks_bytes, list_bytes, bytes; };
 EvictPlan evict_plan(const d2c_memory_desc &q, int keep)
 {
@@ -1101,6 +1122,91 @@ EvictPlan evict_plan(const d2c_memory_desc &q, int keep)
     p.list_bytes = d2c_align_up(units * p.pairs * 4);
     p.bytes = p.ranks_bytes + 2 * p.list_bytes + d2c_align_up(units * 4);
     return p;
+}
+// Ranks and places: 1 GB at most.  (They are ranked by a workgroup to a stream's head, so that a limit which leaves compute units empty would cost time: two workgroups to each, of streams of
+// 129600 slots, take 0.5 GB)
+constexpr size_t kEvictBytes = (size_t)1 << 30;
+int evict_streams(const d2c_memory_desc &q, int keep) { return streams_at_once(q.streams, evict_plan(with_streams(q, 1), keep).bytes, kEvictBytes); }
+
+// Streams whose scores have room at once
+int attend(const d2c_memory_desc *q, const d2c_memory_query_desc *x, const void *query, const void *key, const void *value, const int32_t *table, const int32_t *lengths, float *usage, void *out,
+           void *ws, size_t ws_bytes, hipStream_t st)
+{
+    const long slots = (long)q->per_stream * q->page;
+    const MemPlan p = mem_plan(*q, *x, usage != nullptr);
+    if (int rc = need(ws, ws_bytes, p.bytes)) return rc;
+    MemArgs a{};
+    a.q = query; a.key = const_cast<void *>(key); a.value = const_cast<void *>(value); a.out = out; a.table = table; a.lengths = lengths; a.usage = usage;
+    char *w = (char *)ws;
+    a.part = (float *)w; a.part_ml = (float *)(w + p.part_bytes); a.covered = (int32_t *)(w + p.part_bytes + p.ml_bytes);
+    a.begins = (int32_t *)(w + p.part_bytes + p.ml_bytes + p.covered_bytes);
+    a.scores = (float *)(w + p.part_bytes + p.ml_bytes + p.covered_bytes + p.begins_bytes);
+    for (int i = 0; i < 2; i++) a.qs[i] = x->query_stride[i];
+    for (int i = 0; i < 3; i++) { a.ks[i] = q->key_stride[i]; a.vs[i] = q->value_stride[i]; }
+    a.table_stride = q->table_stride; a.slots_padded = p.slots_padded; a.page = make_fastdiv(q->page);
+    a.N = q->streams; a.heads = q->heads; a.group = x->query_heads / q->heads; a.D = q->D; a.pages = q->pages;
+    a.slots = q->pages > 0 ? (int)slots : 0;      // (without pages no slot is there)
+    a.score_rows = p.score_rows; a.row_groups = p.row_groups; a.units = p.units; a.places = p.places; a.least = p.least;
+    a.scale2 = x->scale * 1.44269504088896340736f;
+    const bool whole = q->D * d2c_elem_size(q->dtype) % 16 == 0;
+    const dim3 grid(p.one ? (usage ? p.units / p.row_groups : p.units) : p.places), joins((unsigned)(q->streams * x->query_heads + (usage ? p.places * kUsageBlocks : 0)));
+    auto join = [&](auto zero, auto lanes, auto r) {
+        hipLaunchKernelGGL((mem_join_kernel<decltype(zero), decltype(lanes)::value, decltype(r)::value, (decltype(r)::value > 8)>), joins, dim3(256), 0, st, a, q->streams * x->query_heads, p.step);
+        return d2c_check_launch("mem_join_kernel");
+    };
+    auto for_two = [&](bool yes, auto f) { return yes ? f(std::true_type{}) : f(std::false_type{}); };
+    if (p.wide) {
+        auto launch = [&](auto dp, auto r) {
+            constexpr int DP = decltype(dp)::value, R = decltype(r)::value;
+            const int rc = for_two(whole, [&](auto w) {
+                return for_two(p.one, [&](auto one) {
+                    hipLaunchKernelGGL((mem_attn_wide_kernel<DP, decltype(w)::value, R, decltype(one)::value>), grid, dim3(256), 0, st, a);
+                    return d2c_check_launch("mem_attn_wide_kernel");
+                });
+            });
+            if (rc || p.one) return rc;
+            return join(bf16_t{}, std::integral_constant<int, DP <= 32 ? 8 : DP <= 64 ? 16 : 32>{}, r);
+        };
+        auto with_rows = [&](auto dp) { return p.rows == 16 ? launch(dp, std::integral_constant<int, 16>{}) : launch(dp, std::integral_constant<int, 32>{}); };
+        if (q->D <= 32) return with_rows(std::integral_constant<int, 32>{});
+        if (q->D <= 64) return with_rows(std::integral_constant<int, 64>{});
+        if (q->D <= 96) return with_rows(std::integral_constant<int, 96>{});
+        return with_rows(std::integral_constant<int, 128>{});
+    }
+    return for_rows(*q, a.group, [&](auto zero, auto lanes, auto r) {
+        using T = decltype(zero);
+        constexpr int LANES = decltype(lanes)::value, R = decltype(r)::value;
+        const int rc = for_two(whole, [&](auto w) {
+            return for_two(p.one, [&](auto one) {
+                hipLaunchKernelGGL((mem_attn_kernel<T, LANES, R, decltype(w)::value, decltype(one)::value>), grid, dim3(256), 0, st, a);
+                return d2c_check_launch("mem_attn_kernel");
+            });
+        });
+        if (rc || p.one) return rc;
+        return join(zero, std::integral_constant<int, LANES * 16 / (int)sizeof(T) / 4>{}, r);      // (lanes of four columns)
+    });
+}
+
+// Streams whose ranks have room at once
+int evict(const d2c_memory_desc *q, void *key, void *value, const int32_t *table, int32_t *lengths, const int32_t *seen, float *usage, int32_t *positions, int keep, int recent, void *ws,
+          hipStream_t st)
+{
+    const EvictPlan p = evict_plan(*q, keep);
+    EvictArgs a{};
+    a.key = key; a.value = value; a.table = table; a.seen = seen; a.lengths = lengths; a.positions = positions; a.usage = usage;
+    a.ranks = (uint32_t *)ws; a.holes = (int32_t *)((char *)ws + p.ranks_bytes); a.fillers = (int32_t *)((char *)ws + p.ranks_bytes + p.list_bytes);
+    a.counts = (int32_t *)((char *)ws + p.ranks_bytes + 2 * p.list_bytes);
+    for (int i = 0; i < 3; i++) { a.ks[i] = q->key_stride[i]; a.vs[i] = q->value_stride[i]; }
+    a.table_stride = q->table_stride; a.slots_padded = p.slots_padded; a.page = make_fastdiv(q->page);
+    a.N = q->streams; a.heads = q->heads; a.D = q->D; a.pages = q->pages; a.slots = q->per_stream * q->page; a.keep = keep; a.recent = recent; a.pairs = p.pairs;
+    const int units = a.N * a.heads, vec = q->dtype == D2C_BF16 ? 8 : 4;
+    hipLaunchKernelGGL(mem_rank_kernel, dim3(units), dim3(kEvictThreads), 0, st, a);
+    if (int rc = d2c_check_launch("mem_rank_kernel")) return rc;
+    const int blocks = (int)std::max(std::min((a.pairs + kMovePairs - 1L) / kMovePairs, (1L << 22) / units), 1L);
+    const FastDiv pieces = make_fastdiv((a.D + vec - 1) / vec);
+    if (q->dtype == D2C_BF16) hipLaunchKernelGGL(mem_move_kernel<bf16_t>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks, pieces);
+    else hipLaunchKernelGGL(mem_move_kernel<float>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks, pieces);
+    return d2c_check_launch("mem_move_kernel");
 }
 
 }  // namespace
@@ -1145,7 +1251,10 @@ extern "C" int d2c_memory_append(const d2c_memory_desc *q, void *key, void *valu
 extern "C" size_t d2c_memory_attention_workspace_bytes(const d2c_memory_desc *q, const d2c_memory_query_desc *x, int32_t track)
 {
     if (check(q, x) != D2C_OK || q->streams == 0) return 0;
-    return mem_plan(*q, *x, track != 0).bytes;
+    const int at_once = attention_streams(*q, *x, track != 0), last = (q->streams - 1) % at_once + 1;
+    const size_t bytes = mem_plan(with_streams(*q, at_once), *x, track != 0).bytes;
+    // (a smaller last part may take two launches where the others take one)
+    return last == at_once ? bytes : std::max(bytes, mem_plan(with_streams(*q, last), *x, track != 0).bytes);
 }
 
 extern "C" int d2c_memory_attention(const d2c_memory_desc *q, const d2c_memory_query_desc *x, const void *query, const void *key,
@@ -1156,65 +1265,20 @@ extern "C" int d2c_memory_attention(const d2c_memory_desc *q, const d2c_memory_q
     if (q->streams == 0) return D2C_OK;
     const long slots = (long)q->per_stream * q->page;
     if (!query || !out || !lengths || (slots > 0 && !table) || (q->pages > 0 && (!key || !value))) { d2c_set_error("null tensor pointer"); return D2C_ERR_SHAPE; }
-    const MemPlan p = mem_plan(*q, *x, usage != nullptr);
-    if (int rc = need(ws, ws_bytes, p.bytes)) return rc;
-    MemArgs a{};
-    a.q = query; a.key = const_cast<void *>(key); a.value = const_cast<void *>(value); a.out = out; a.table = table; a.lengths = lengths; a.usage = usage;
-    char *w = (char *)ws;
-    a.part = (float *)w; a.part_ml = (float *)(w + p.part_bytes); a.covered = (int32_t *)(w + p.part_bytes + p.ml_bytes);
-    a.begins = (int32_t *)(w + p.part_bytes + p.ml_bytes + p.covered_bytes);
-    a.scores = (float *)(w + p.part_bytes + p.ml_bytes + p.covered_bytes + p.begins_bytes);
-    for (int i = 0; i < 2; i++) a.qs[i] = x->query_stride[i];
-    for (int i = 0; i < 3; i++) { a.ks[i] = q->key_stride[i]; a.vs[i] = q->value_stride[i]; }
-    a.table_stride = q->table_stride; a.slots_padded = p.slots_padded; a.page = make_fastdiv(q->page);
-    a.N = q->streams; a.heads = q->heads; a.group = x->query_heads / q->heads; a.D = q->D; a.pages = q->pages;
-    a.slots = q->pages > 0 ? (int)slots : 0;      // (without pages no slot is there)
-    a.score_rows = p.score_rows; a.row_groups = p.row_groups; a.units = p.units; a.places = p.places; a.least = p.least;
-    a.scale2 = x->scale * 1.44269504088896340736f;
-    hipStream_t st = (hipStream_t)stream;
-    const bool whole = q->D * d2c_elem_size(q->dtype) % 16 == 0;
-    const dim3 grid(p.one ? (usage ? p.units / p.row_groups : p.units) : p.places), joins((unsigned)(q->streams * x->query_heads + (usage ? p.places * kUsageBlocks : 0)));
-    auto join = [&](auto zero, auto lanes, auto r) {
-        hipLaunchKernelGGL((mem_join_kernel<decltype(zero), decltype(lanes)::value, decltype(r)::value, (decltype(r)::value > 8)>), joins, dim3(256), 0, st, a, q->streams * x->query_heads, p.step);
-        return d2c_check_launch("mem_join_kernel");
-    };
-    auto for_two = [&](bool yes, auto f) { return yes ? f(std::true_type{}) : f(std::false_type{}); };
-    if (p.wide) {
-        auto launch = [&](auto dp, auto r) {
-            constexpr int DP = decltype(dp)::value, R = decltype(r)::value;
-            const int rc = for_two(whole, [&](auto w) {
-                return for_two(p.one, [&](auto one) {
-                    hipLaunchKernelGGL((mem_attn_wide_kernel<DP, decltype(w)::value, R, decltype(one)::value>), grid, dim3(256), 0, st, a);
-                    return d2c_check_launch("mem_attn_wide_kernel");
-                });
-            });
-            if (rc || p.one) return rc;
-            return join(bf16_t{}, std::integral_constant<int, DP <= 32 ? 8 : DP <= 64 ? 16 : 32>{}, r);
-        };
-        auto with_rows = [&](auto dp) { return p.rows == 16 ? launch(dp, std::integral_constant<int, 16>{}) : launch(dp, std::integral_constant<int, 32>{}); };
-        if (q->D <= 32) return with_rows(std::integral_constant<int, 32>{});
-        if (q->D <= 64) return with_rows(std::integral_constant<int, 64>{});
-        if (q->D <= 96) return with_rows(std::integral_constant<int, 96>{});
-        return with_rows(std::integral_constant<int, 128>{});
-    }
-    return for_rows(*q, a.group, [&](auto zero, auto lanes, auto r) {
-        using T = decltype(zero);
-        constexpr int LANES = decltype(lanes)::value, R = decltype(r)::value;
-        const int rc = for_two(whole, [&](auto w) {
-            return for_two(p.one, [&](auto one) {
-                hipLaunchKernelGGL((mem_attn_kernel<T, LANES, R, decltype(w)::value, decltype(one)::value>), grid, dim3(256), 0, st, a);
-                return d2c_check_launch("mem_attn_kernel");
-            });
-        });
-        if (rc || p.one) return rc;
-        return join(zero, std::integral_constant<int, LANES * 16 / (int)sizeof(T) / 4>{}, r);      // (lanes of four columns)
+    const int at_once = attention_streams(*q, *x, usage != nullptr);
+    if (at_once < q->streams)      // (before the first part runs)
+        if (int rc = need(ws, ws_bytes, d2c_memory_attention_workspace_bytes(q, x, usage != nullptr))) return rc;
+    const size_t size = d2c_elem_size(q->dtype);
+    return for_streams(*q, at_once, [&](int n, const d2c_memory_desc &part) {
+        return attend(&part, x, (const char *)query + n * x->query_stride[0] * size, key, value, table + n * q->table_stride, lengths + n, usage,
+                      (char *)out + (size_t)n * x->query_heads * q->D * size, ws, ws_bytes, (hipStream_t)stream);
     });
 }
 
 extern "C" size_t d2c_memory_evict_workspace_bytes(const d2c_memory_desc *q, int32_t keep)
 {
     if (check(q) != D2C_OK || keep <= 0) return 0;
-    return evict_plan(*q, keep).bytes;
+    return evict_plan(with_streams(*q, evict_streams(*q, keep)), keep).bytes;
 }
 
 extern "C" int d2c_memory_evict(const d2c_memory_desc *q, void *key, void *value, const int32_t *table, int32_t *lengths, const int32_t *seen,
@@ -1222,24 +1286,10 @@ extern "C" int d2c_memory_evict(const d2c_memory_desc *q, void *key, void *value
 {
     if (int rc = check(q)) return rc;
     if (keep <= 0 || recent < 0 || recent > keep) { d2c_set_error("memory_evict: keep %d must be positive, recent %d in 0 .. keep", keep, recent); return D2C_ERR_SHAPE; }
-    const EvictPlan p = evict_plan(*q, keep);
-    if (p.pairs == 0) return D2C_OK;
+    if (evict_plan(*q, keep).pairs == 0) return D2C_OK;
     if (!table || !lengths || !seen || (q->pages > 0 && (!key || !value || !usage || !positions))) { d2c_set_error("null tensor pointer"); return D2C_ERR_SHAPE; }
-    if (int rc = need(ws, ws_bytes, p.bytes)) return rc;
-    EvictArgs a{};
-    a.key = key; a.value = value; a.table = table; a.seen = seen; a.lengths = lengths; a.positions = positions; a.usage = usage;
-    a.ranks = (uint32_t *)ws; a.holes = (int32_t *)((char *)ws + p.ranks_bytes); a.fillers = (int32_t *)((char *)ws + p.ranks_bytes + p.list_bytes);
-    a.counts = (int32_t *)((char *)ws + p.ranks_bytes + 2 * p.list_bytes);
-    for (int i = 0; i < 3; i++) { a.ks[i] = q->key_stride[i]; a.vs[i] = q->value_stride[i]; }
-    a.table_stride = q->table_stride; a.slots_padded = p.slots_padded; a.page = make_fastdiv(q->page);
-    a.N = q->streams; a.heads = q->heads; a.D = q->D; a.pages = q->pages; a.slots = q->per_stream * q->page; a.keep = keep; a.recent = recent; a.pairs = p.pairs;
-    hipStream_t st = (hipStream_t)stream;
-    const int units = a.N * a.heads, vec = q->dtype == D2C_BF16 ? 8 : 4;
-    hipLaunchKernelGGL(mem_rank_kernel, dim3(units), dim3(kEvictThreads), 0, st, a);
-    if (int rc = d2c_check_launch("mem_rank_kernel")) return rc;
-    const int blocks = (int)std::max(std::min((a.pairs + kMovePairs - 1L) / kMovePairs, (1L << 22) / units), 1L);
-    const FastDiv pieces = make_fastdiv((a.D + vec - 1) / vec);
-    if (q->dtype == D2C_BF16) hipLaunchKernelGGL(mem_move_kernel<bf16_t>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks, pieces);
-    else hipLaunchKernelGGL(mem_move_kernel<float>, dim3((unsigned)blocks * units), dim3(256), 0, st, a, blocks, pieces);
-    return d2c_check_launch("mem_move_kernel");
+    if (int rc = need(ws, ws_bytes, d2c_memory_evict_workspace_bytes(q, keep))) return rc;
+    return for_streams(*q, evict_streams(*q, keep), [&](int n, const d2c_memory_desc &part) {
+        return evict(&part, key, value, table + n * q->table_stride, lengths + n, seen + n, usage, positions, keep, recent, ws, (hipStream_t)stream);
+    });
 }
