@@ -111,7 +111,8 @@ class AttentionDesc(ctypes.Structure):
 
 class PackedAttentionDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("sequences", "Hq", "Hkv", "D", "dtype", "causal", "frame")] + [("scale", ctypes.c_float)] + [
-        (n, ctypes.c_int64) for n in ("queries", "keys")] + [(n, ctypes.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride")]
+        (n, ctypes.c_int64) for n in ("queries", "keys")] + [(n, ctypes.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride")] + [
+        ("part_limit", ctypes.c_int64)]
 
 
 class MemoryDesc(ctypes.Structure):

@@ -311,8 +311,7 @@ class _PackedAttentionFunction(torch.autograd.Function):
         lse = torch.empty((Hkv, T * (Hq // Hkv)), dtype=torch.float32, device=dev) if grad else None
         low = torch.empty_like(out) if grad and out.dtype == torch.bfloat16 else None
         with torch.cuda.device(dev):
-            nb = lib.d2c_packed_attention_forward_workspace_bytes(ctypes.byref(desc))
-            ws = _workspace(nb, dev)
+            ws, nb = _part_workspace(desc, lib.d2c_packed_attention_forward_workspace_bytes, dev)
             rc = lib.d2c_packed_attention_forward(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(starts), _ptr(key_starts), _ptr(out),
                                                   _ptr(low), _ptr(lse), _ptr(ws), nb, _stream(dev))
         _lib.check(rc, "packed_attention forward")
@@ -326,13 +325,13 @@ class _PackedAttentionFunction(torch.autograd.Function):
         lib = _lib.load()
         q, k, v, starts, key_starts, out, low, lse = ctx.saved_tensors
         desc, dev, need = ctx.desc, q.device, ctx.needs_input_grad
+        desc.part_limit = 0
         q, k, v = (_heads_contiguous(t) for t in (q, k, v))
         desc.q_stride, desc.k_stride, desc.v_stride = (_long2(*t.stride()[:2]) for t in (q, k, v))
         g = grad_out.to(q.dtype).contiguous()
         gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((q, k, v), need))
         with torch.cuda.device(dev):
-            nb = lib.d2c_packed_attention_backward_workspace_bytes(ctypes.byref(desc))
-            ws = _workspace(nb, dev)
+            ws, nb = _part_workspace(desc, lib.d2c_packed_attention_backward_workspace_bytes, dev)
             rc = lib.d2c_packed_attention_backward(ctypes.byref(desc), _ptr(g), _ptr(q), _ptr(k), _ptr(v), _ptr(starts), _ptr(key_starts),
                                                    _ptr(out), _ptr(low), _ptr(lse), _ptr(gq), _ptr(gk), _ptr(gv), _ptr(ws), nb, _stream(dev))
         _lib.check(rc, "packed_attention backward")
@@ -348,7 +347,8 @@ def packed_attention(query, key, value, starts, key_starts=None, causal=True, fr
     the same for its keys where these are others (default: starts), whose last tokens then are the queries.  `causal`: query i of Lq
     is token p = Lk - Lq + i and reads the keys up to its own, or, with `frame` tokens to a frame, up to the end of its frame; what it
     does not read has no influence on it whatever it holds.  Otherwise all keys of its sequence.  A query without keys, or of no sequence, is 0 and has gradients of
-    0.  Any strides with the channels adjacent are read in place.  Sums in an order that sizes, strides, starts and GPU determine.
+    0.  Any strides with the channels adjacent are read in place.  Sums in an order that sizes, strides, starts and GPU determine, unless the
+    GPU's memory has no room for the partial sums of long walks (256 MB at most), which then are not cut.
     (Starts that do not rise have results of no meaning, and touch nothing else.)"""
     out = _try_native("packed_attention", query, key, value, starts, key_starts, causal, frame, scale)
     if out is not None:

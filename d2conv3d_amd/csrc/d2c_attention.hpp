@@ -346,7 +346,7 @@ inline Walks plan_walks(long units, long steps, long places, double step_us, dou
     if (w.splits == 1) { w.whole += w.shared; w.shared = 0; }
     return w;
 }
-inline double part_limit(const d2c_attention_desc &q) { return q.part_limit == 0 ? (double)D2C_ATTENTION_PART_BYTES : (double)q.part_limit; }
+template <typename Desc> double part_limit(const Desc &q) { return q.part_limit == 0 ? (double)D2C_ATTENTION_PART_BYTES : (double)q.part_limit; }
 inline unsigned workgroups(const Walks &w) { return (unsigned)(w.whole + w.shared * w.splits); }
 // Workgroups of a kernel that a compute unit holds
 int resident(const void *kernel, int lds);

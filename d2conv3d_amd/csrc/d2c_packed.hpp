@@ -287,7 +287,7 @@ inline Split split_walks(const d2c_packed_attention_desc &q, long units, long pl
     // pieces of 4, 121 of 6 or 8, 145 of 12)
     const long chunk = std::max((long)(each * 0.3), units * (longest / 4 + 1) * (q.causal ? 1 : 2) <= 2 * places ? 4L : 8L);
     long s = std::min((longest + chunk - 1) / chunk, 16L);
-    while (s > 1 && (double)s * (double)units * unit_bytes > (double)D2C_ATTENTION_PART_BYTES) s--;
+    while (s > 1 && (double)s * (double)units * unit_bytes > part_limit(q)) s--;
     return {(int)s, s > 1 ? (int)chunk : 1 << 30};
 }
 

@@ -756,7 +756,7 @@ void strides(d2c_attention_desc &q, const Tensor &query, const Tensor &key, cons
 
 // The workspace of an attention call, from the allocator, and its size: without room for partial sums (D2C_ATTENTION_PART_BYTES at most, tens of megabytes as a
 // rule) where there is none
-Tensor part_workspace(d2c_attention_desc &q, size_t (*size)(const d2c_attention_desc *), size_t &bytes, const Tensor &like)
+template <typename Desc> Tensor part_workspace(Desc &q, size_t (*size)(const Desc *), size_t &bytes, const Tensor &like)
 {
     bytes = size(&q);
     try {
@@ -901,8 +901,9 @@ struct PackedAttentionBackward : public Node {
             if (should_compute_output(0)) r[0] = no_grad_empty_like(vq);
             if (should_compute_output(1)) r[1] = no_grad_empty_like(vk);
             if (should_compute_output(2)) r[2] = no_grad_empty_like(vv);
-            const size_t nb = d2c_packed_attention_backward_workspace_bytes(&q);
-            const Tensor ws = small_workspace(nb, vq);
+            size_t nb = 0;
+            q.part_limit = 0;
+            const Tensor ws = part_workspace(q, d2c_packed_attention_backward_workspace_bytes, nb, vq);
             check(d2c_packed_attention_backward(&q, ptr(g), ptr(vq), ptr(vk), ptr(vv), (const int32_t *)ptr(vs), (const int32_t *)ptr(vks), ptr(vo), ptr(vlow),
                                                 (const float *)ptr(vl), ptr(r[0]), ptr(r[1]), ptr(r[2]), ptr(ws), nb, st),
                   "packed_attention backward");
@@ -948,8 +949,8 @@ py::object packed_attention(const Tensor &query, const Tensor &key, const Tensor
     Tensor out = at::empty(query.sizes(), opt), low, lse;
     if (grad && dt == D2C_BF16) low = at::empty(query.sizes(), opt);
     if (grad) lse = at::empty({q.Hkv, q.queries * (q.Hq / q.Hkv)}, opt.dtype(at::kFloat));
-    const size_t nb = d2c_packed_attention_forward_workspace_bytes(&q);
-    const Tensor ws = small_workspace(nb, query);
+    size_t nb = 0;
+    const Tensor ws = part_workspace(q, d2c_packed_attention_forward_workspace_bytes, nb, query);
     check(d2c_packed_attention_forward(&q, ptr(query), ptr(key), ptr(value), (const int32_t *)ptr(starts), (const int32_t *)ptr(other), ptr(out), ptr(low), (float *)ptr(lse),
                                        ptr(ws), nb, stream_of(query)),
           "packed_attention forward");

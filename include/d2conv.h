@@ -556,13 +556,15 @@ int d2c_attention_backward(const d2c_attention_desc *desc, const void *grad_out,
  * a query does not read have no influence on it whatever they hold.  A query without keys is 0, as are queries of no sequence; so are their
  * gradients and those of keys that nobody reads.  out, grad_out and the gradients are contiguous.  `lse` [Hkv, queries * Hq / Hkv] and, bfloat16,
  * `out_low` (as out) are for the backward call (see d2c_attention_forward).
- * Sums are made in an order that sizes, strides, starts and GPU determine.  Starts that do not rise: results of no meaning, but nothing outside
+ * Sums are made in an order that sizes, strides, starts, GPU and part_limit determine; part_limit: bytes of partial sums at most, as in
+ * d2c_attention_desc (0: D2C_ATTENTION_PART_BYTES; negative: none).  Starts that do not rise: results of no meaning, but nothing outside
  * the tensors is read or written. */
 typedef struct d2c_packed_attention_desc {
     int32_t sequences, Hq, Hkv, D, dtype, causal, frame;
     float scale;
     int64_t queries, keys;
     int64_t q_stride[2], k_stride[2], v_stride[2];
+    int64_t part_limit;
 } d2c_packed_attention_desc;
 size_t d2c_packed_attention_forward_workspace_bytes(const d2c_packed_attention_desc *desc);
 int d2c_packed_attention_forward(const d2c_packed_attention_desc *desc, const void *query, const void *key, const void *value,
