@@ -90,7 +90,7 @@ D2C_DEV int first_row(const PackedArgs &a, const PackedUnit &u, int key) { retur
 
 // Kernels of one term of the weights (bfloat16, see kWeightTerms) take two for tiles that have sums of 64 terms or fewer, which do not average out: a tile of rows whose first reads no more
 // keys, a tile of keys whose last is read by no more rows.  So results whose sums are as short, a short sequence's and those of a long one's first and last tokens, have two whatever they are
-// packed with.  Such tiles' walks are short, as limits go by token or frame: forward and backward, 8 heads of 64, 500 sequences of 100 take 366 us (350 with one term everywhere), 200 of 200 279 (271);
+// packed with.  Such tiles' walks are short, as limits go by token or frame: forward and backward, 8 heads of 64, 500 sequences of 100 take 364 us (350 with one term everywhere), 200 of 200 281 (273);
 // the longer the sequences, the fewer such tiles.  Rows of 2 to 4 keys are off by up to 0.0068 of sum p |v| with one term, by 0.0039, the result's own rounding, with two.
 D2C_DEV bool few_keys(const PackedArgs &a, const PackedUnit &u) { return limit_of_row(a, u, u.tile * kRows) <= kExactKeys; }
 D2C_DEV bool few_rows(const PackedArgs &a, const PackedUnit &u) { return u.rows - first_row(a, u, min(u.tile * kRows + kRows, u.lk) - 1) <= kExactKeys; }
