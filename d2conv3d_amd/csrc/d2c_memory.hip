@@ -758,7 +758,9 @@ D2C_DEV uint32_t rank_of(float usage, bool stays)
 // lanes meet in), then the slots that go before `keep` and those that stay behind it, each in rising order.  A wavefront has neighbouring slots, 64 at a time, whose
 // truth values are one word each: counted by a lane to a word.
 // Bound: a compute unit's instructions and the latency of its chain (counts, pages, usage, three histograms).  64 units of up to 25920 slots 35 us (33 with the ranks in LDS, as far as they have
-// room there; 44 with a request for each page after the other; 51 with ranks in registers and loops unrolled, whose instructions every launch fetches anew), 4 units of 3240 slots 10.5.
+// room there; 44 with a request for each page after the other; 51 with ranks in registers and loops unrolled, whose instructions every launch fetches anew), 4 units of 3240 slots 10.5.  Where all
+// usages are equal (a memory that was read without them being added up) lanes wait for one bin and one count: whole passes, 64 units of up to 25920 slots 100 us instead of 72, one of 64800 191
+// instead of 75.
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
 __global__ void __launch_bounds__(kEvictThreads) mem_rank_kernel(EvictArgs a)
 {

@@ -20,8 +20,8 @@ template <typename T, int DP, bool WHOLE> struct FwdShape {
 // One pass over the keys with the running maximum and sum of a softmax, as attn_fwd_kernel; the weights go from one product's accumulator into the next one's operand in registers.
 // Only tiles in which some row has a key that it does not read look at limits, and clean the values that others read from infinities and NaN (take_in brings them back).  Registers: what three
 // workgroups of a compute unit have room for at 64 channels.  Bound: matrix instructions and the exponentials, maxima, sums and roundings between them.
-// Measured, bfloat16: 16 pieces of up to 4096 queries on up to 12288 keys, 16 heads of 128 that share 4, 1.94 ms (0.96 PFLOP/s; a library product of 8192 cubed 1.22); one sequence of 25920, 8
-// heads of 64 that share 2, 0.79 ms (0.87); six of up to 12960 in frames of 1620, 8 heads of 64, 0.73 ms (0.79).  float32: three of up to 1417, 6 heads of 40, 32 us and the join 5.8.
+// Measured, bfloat16: 16 pieces of up to 4096 queries on up to 12288 keys, 16 heads of 128 that share 4, 1.93 ms (0.97 PFLOP/s; a library product of 8192 cubed 1.22); one sequence of 25920, 8
+// heads of 64 that share 2, 0.80 ms (0.86); six of up to 12960 in frames of 1620, 8 heads of 64, 0.73 ms (0.79).  float32: three of up to 1417, 6 heads of 40, 32 us and the join 5.1.
 template <typename T, int DP, int NP, bool WHOLE, int PW> D2C_DEV void fwd_rows(const PackedArgs &a, const PackedUnit &u)
 {
     using Shape = FwdShape<T, DP, WHOLE>;
@@ -186,7 +186,7 @@ template <typename T, int DP, int NP, bool WHOLE> __global__ void __launch_bound
 }
 
 // The partial results of the workgroups that shared a walk: a workgroup to 16 rows of a tile, a thread to four columns and those 64 further on, four splits
-// requested at a time.  Bound: latency (3.4 to 5.8 us).
+// requested at a time.  Bound: latency (3.1 to 5.4 us).
 template <typename T> __global__ void __launch_bounds__(256) packed_join_kernel(PackedArgs a)
 {
     const PackedUnit u = unit_of<false>(a, blockIdx.x / 8);

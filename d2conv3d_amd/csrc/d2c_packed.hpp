@@ -33,7 +33,7 @@ D2C_DEV void region_of(const int32_t *starts, int S, int T, int i, int &first, i
     count = max((i > S ? T : bound_of(starts, S, T, i + 1)) - first, 0);
 }
 // The region of tile `at` of the line, which of its tiles that is, its first token and how many it has.  `group`: rows to a token.  63 regions to a vote, three votes to 250000; the last has the
-// region's bounds as well.  6480 sequences of 8 tokens, 8 heads of 64, bfloat16: 440 us (448 with the bounds asked for afterwards, 1466 with regions taken 64 after 64)
+// region's bounds as well.  6480 sequences of 8 tokens, 8 heads of 64, bfloat16: 436 us (448 with the bounds asked for afterwards, 1466 with regions taken 64 after 64)
 D2C_DEV void find_tile(const int32_t *starts, int S, int T, int group, int at, int &region, int &tile, int &first, int &count)
 {
     const int lane = threadIdx.x & 63;
@@ -276,7 +276,8 @@ D2C_DEV Walk key_walk(const PackedArgs &a, const PackedUnit &u)
 }
 // On the host, where only the average length is known: the longest walk is taken to be twice that of a sequence of the average length, or that of the only sequence.  Pieces cost a second
 // launch and their sums' way through memory, so walks are cut where one is longer than what every place gets anyway, into pieces of a third of that: one sequence of 25920, forward and backward,
-// 3.44 ms (4.99 whole, 3.95 in pieces of three quarters, 3.67 of a fifth); six of up to 12960 2.98 whole, 3.07 to 3.16 in pieces.
+// 3.37 ms (when this was chosen 3.44; 4.99 whole, 3.95 in pieces of three quarters, 3.67 of a fifth); six of up to 12960 2.95 (then 2.98; 3.07 to 3.16 in pieces).  One long sequence beside many short
+// ones, whose average says nothing of it, is not cut.
 struct Split { int splits, chunk; };
 inline Split split_walks(const d2c_packed_attention_desc &q, long units, long places, long along, long step, double unit_bytes)
 {

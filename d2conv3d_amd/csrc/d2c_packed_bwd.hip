@@ -19,8 +19,8 @@ template <typename T, int DP, bool WHOLE> struct QShape {
 
 // s and dp of a tile of keys, then dq += ds k.  As attn_bwd_q_kernel: rows along the lanes, ds into the last product's operand in registers, K and V through LDS (K read
 // twice, by rows and by columns; where it holds infinities or NaN and some rows do not read all of the tile, it is cleaned in LDS between the two).  Bound: matrix instructions (3 products to
-// one exponential).  Measured, bfloat16: one sequence of 25920, 8 heads of 64 that share 2, 1.06 ms (0.98 PFLOP/s); six of up to 12960 in frames, 8 heads of 64, 0.97 ms (0.90).  float32: three of up to
-// 1417, 6 heads of 40, 35 us and the join 4.9.
+// one exponential).  Measured, bfloat16: one sequence of 25920, 8 heads of 64 that share 2, 1.07 ms (0.96 PFLOP/s); six of up to 12960 in frames, 8 heads of 64, 0.98 ms (0.89).  float32: three of up to
+// 1417, 6 heads of 40, 34 us and the join 4.8.
 template <typename T, int DP, int NP, bool WHOLE, int PW> D2C_DEV void bwd_rows(const PackedArgs &a, const PackedUnit &u)
 {
     using Shape = QShape<T, DP, WHOLE>;
@@ -180,8 +180,8 @@ template <typename T, int DP, bool WHOLE> struct KvShape {
 
 // Keys along the lanes, their K and V in registers from first to last; queries and grad_out of a tile of rows through LDS, each read by rows (s, dp) and by columns
 // (dk, dv).  dp starts from -delta.  As attn_bwd_kv_kernel; the walk begins with the first row that reads a key of the tile.  Bound: matrix instructions (4 products to one exponential), behind
-// them LDS.  Measured, bfloat16: one sequence of 25920, 8 heads of 64 that share 2, 1.54 ms and the join 24 us (0.90 PFLOP/s; 3.1 ms before walks were cut in pieces, the first keys' being as long
-// as the whole sequence); six of up to 12960 in frames, 8 heads of 64, 1.25 ms (0.93).  float32: three of up to 1417, 6 heads of 40, 45 us and the join 5.7.
+// them LDS.  Measured, bfloat16: one sequence of 25920, 8 heads of 64 that share 2, 1.49 ms and the join 23 us (0.93 PFLOP/s; 3.1 ms before walks were cut in pieces, the first keys' being as long
+// as the whole sequence); six of up to 12960 in frames, 8 heads of 64, 1.21 ms (0.96).  float32: three of up to 1417, 6 heads of 40, 42 us and the join 5.4.
 template <typename T, int DP, int NP, bool WHOLE, int PW> D2C_DEV void bwd_keys(const PackedArgs &a, const PackedUnit &u)
 {
     using Shape = KvShape<T, DP, WHOLE>;

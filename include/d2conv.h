@@ -557,7 +557,7 @@ int d2c_attention_backward(const d2c_attention_desc *desc, const void *grad_out,
  * gradients and those of keys that nobody reads.  out, grad_out and the gradients are contiguous.  `lse` [Hkv, queries * Hq / Hkv] and, bfloat16,
  * `out_low` (as out) are for the backward call (see d2c_attention_forward).
  * Sums are made in an order that sizes, strides, starts, GPU and part_limit determine; part_limit: bytes of partial sums at most, as in
- * d2c_attention_desc (0: D2C_ATTENTION_PART_BYTES; negative: none).  Starts that do not rise: results of no meaning, but nothing outside
+ * d2c_attention_desc: 0 is D2C_ATTENTION_PART_BYTES, a negative number none.  Starts that do not rise: results of no meaning, but nothing outside
  * the tensors is read or written. */
 typedef struct d2c_packed_attention_desc {
     int32_t sequences, Hq, Hkv, D, dtype, causal, frame;
